@@ -40,6 +40,9 @@ extern "C" {
 /* element types of logits / probability inputs */
 #define PLH_F32 0
 #define PLH_F64 1
+/* element types of activations and weights (plh_fp8_*), beside PLH_F32 */
+#define PLH_BF16 2
+#define PLH_F16 3
 
 /* plh_sample flags */
 #define PLH_SAMPLE_ROWWISE 1 /* one workgroup per row (the general kernel) */
@@ -248,6 +251,110 @@ int plh_append_ids(plh_ctx* ctx, int32_t* slab, const int64_t* pos, const int32_
  */
 int plh_rmsnorm_lm_head(plh_ctx* ctx, const float* h, int64_t ldh, int N, int D, const float* norm, double eps,
                         const float* W, int64_t ldw, int V, float* out, int64_t ldo);
+
+/*
+ * Biases, penalties and grammar masks on a batch's logits, for requests that
+ * ask for more than the reference's repetition penalty
+ * (src/pagellm/engine/sampling.py:52-62, which plh_penalize and plh_sample
+ * apply).  Of row b, in this order:
+ *   v = x + bias        tokens of the row's bias list
+ *   v = v > 0 ? v / r : v * r      tokens of the row's history
+ *   v = v - (f * n + p)  tokens that occur n > 0 times among the row's outputs
+ *   v = -inf             tokens whose bit in the row's mask is clear, whatever
+ *                        stood there (NaN and infinities too)
+ * A token that the first three lines touch is computed in float64 and rounded
+ * once to `dtype`; every other one keeps its bits.
+ *   logits      [B, ld] of `dtype` (PLH_F32 / PLH_F64), aligned to its element
+ *   hist_ids    int32 token ids of the rows' histories (prompt, then outputs),
+ *   hist_off    int64 [B+1] offsets into them, or with PLH_SAMPLE_HIST_SPANS in
+ *               flags [2B] (start, end) pairs; both NULL: no histories.  Ids
+ *               outside [0, V) count for no token
+ *   out_start   int64 [B]: the outputs of row b start this far into its
+ *               history; NULL: every token of a history is an output
+ *   rep_penalty, frequency, presence   float64 [B] r, f and p; NULL: 1, 0, 0
+ *   bias_ids    int32 token ids with a bias, in any order; ids outside [0, V)
+ *   bias        are passed over, and of an id listed twice the last counts;
+ *   bias_off    float64 biases; int64 [B+1] offsets into both (all NULL: none)
+ *   mask        uint32 [mask_rows, mask_ld]: bit v % 32 of word v / 32 is set
+ *               where token v is allowed; NULL: no masks
+ *   mask_row    int32 [B]: row b's row of mask, and no mask where that is not
+ *               in [0, mask_rows) (-1); rows may share one.  NULL: row b of mask
+ *               (mask_rows >= B)
+ *   out         [B, out_ld] of `dtype`: logits itself with out_ld = ld (then
+ *               only what changes is written), or rows that meet no row of it
+ * Any V.  Uses no workspace; a call may be captured into a graph.
+ */
+int plh_process_logits(plh_ctx* ctx, const void* logits, int dtype, int64_t ld, int B, int V,
+                       const int32_t* hist_ids, const int64_t* hist_off, const int64_t* out_start,
+                       const double* rep_penalty, const double* frequency, const double* presence,
+                       const int32_t* bias_ids, const double* bias, const int64_t* bias_off, const uint32_t* mask,
+                       int64_t mask_ld, int mask_rows, const int32_t* mask_row, void* out, int64_t out_ld, int flags);
+
+/*
+ * Log probabilities of logits rows: the chosen token's, its rank, and the
+ * n_top best tokens with theirs (the reference returns none; a server's
+ * `logprobs`, and the scores of a prompt's tokens).
+ *   lse = m + log(sum_v exp(x[b, v] - m)), m = max_v x[b, v]
+ *   out_lp[b]    x[b, ids[b]] - lse
+ *   out_rank[b]  1 + the tokens before ids[b] in the order of logits
+ *                descending, then of ids ascending
+ *   top_ids      int32 [B, n_top], the first n_top of that order
+ *   top_lp       [B, n_top], theirs
+ * out_lp and top_lp are of `dtype`, computed in float64 (float32 rows: from
+ * float32 exponentials) and rounded once.  NaN stands before +inf in the order,
+ * -0 and 0 are alike; a row that holds NaN or +inf has only NaN log
+ * probabilities, and one of -inf only has only -inf.  An id outside [0, V) gives
+ * NaN and rank 0.  ids NULL: out_lp and out_rank are not written (and may be
+ * NULL); 0 <= n_top <= min(V, PLH_MAX_TOP).  Where a row is shared out over several
+ * workgroups the call uses the context's workspace (such a call may allocate,
+ * and is ordered with the context's other workspace calls); under graph capture
+ * it uses none.
+ */
+#define PLH_MAX_TOP 64
+int plh_logprobs(plh_ctx* ctx, const void* logits, int dtype, int64_t ld, int B, int V, const int32_t* ids,
+                 void* out_lp, int32_t* out_rank, int n_top, int32_t* top_ids, void* top_lp);
+
+/*
+ * Products with 8-bit weights: e4m3 codes (OCP, no infinities, largest value
+ * 448) of a [V, D] matrix with one float32 scale for each block of 128 x 128 of
+ * it.  The library keeps such a matrix in its own layout, made once:
+ *   codes   plh_fp8_codes_bytes(V, D) bytes, 16-byte aligned
+ *   scales  float32 [ceil(V / 128), ceil(D / 128)]
+ * plh_fp8_pack lays out the codes [V, ldc] and scales [ceil(V / 128), lds] of a
+ * checkpoint.  plh_fp8_quantize rounds a matrix of `dtype` (PLH_F32, PLH_BF16,
+ * PLH_F16) whose element (v, d) is W[v * stride_v + d * stride_d] (the
+ * reference's [D, V] lm_head has stride_v 1): a block's scale is the smallest
+ * power of two s >= 2^-126 with max|w| <= 448 s, its codes the e4m3 values
+ * nearest to w / s, ties to even; NaN and infinities become NaN.
+ */
+int64_t plh_fp8_codes_bytes(int V, int D);
+int plh_fp8_pack(plh_ctx* ctx, const uint8_t* codes, int64_t ldc, const float* scales, int64_t lds, int V, int D,
+                 uint8_t* out_codes, float* out_scales);
+int plh_fp8_quantize(plh_ctx* ctx, const void* W, int dtype, int64_t stride_v, int64_t stride_d, int V, int D,
+                     uint8_t* out_codes, float* out_scales);
+
+/*
+ * out[n, v] = sum_d a[n, d] w[v, d] in float32, w the matrix above and a the
+ * rows y rounded to e4m3 in blocks of 128 of a row, by the rule of
+ * plh_fp8_quantize:
+ *   y = x                                    with norm NULL, else
+ *   y = x / sqrt(mean_d(x[n, d]^2) + eps) * norm   (in float64, rounded once to
+ *       float32; src/pagellm/model/transformer.py:79-82, :271)
+ * Products of rounded values are exact (bf16 matrix cores); their sums over a
+ * block, scaled, and the sum of the blocks are float32.  A row that holds NaN or an
+ * infinity gives NaN; rounded values of 2^128 and more are infinite, and steps below
+ * 2^-126 may be lost.
+ * The order of a sum depends on (N, V, D) and the device: equal calls give equal
+ * bits.
+ * x [N, ldx] of `dtype` (PLH_F32, PLH_BF16, PLH_F16); norm float32 [D]; out
+ * float32 [N, ldo], 4-byte aligned; ws: plh_fp8_ws_bytes(ctx, N, V, D) bytes,
+ * 256-byte aligned, the caller's, free again when the call's kernels have ended
+ * (so that calls on several streams, and graphs, share none).
+ */
+int64_t plh_fp8_ws_bytes(plh_ctx* ctx, int N, int V, int D);
+int plh_fp8_linear(plh_ctx* ctx, const void* x, int dtype, int64_t ldx, int N, int D, const float* norm, double eps,
+                   const uint8_t* codes, const float* scales, int V, float* out, int64_t ldo, void* ws,
+                   int64_t ws_bytes);
 
 #ifdef __cplusplus
 }

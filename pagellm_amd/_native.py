@@ -24,6 +24,9 @@ PLH_ERR_UNSUPPORTED = -4
 PLH_ERR_NO_DEVICE = -5
 PLH_F32 = 0
 PLH_F64 = 1
+PLH_BF16 = 2
+PLH_F16 = 3
+PLH_MAX_TOP = 64
 PLH_SAMPLE_ROWWISE = 1
 PLH_SAMPLE_HIST_SPANS = 2
 PLH_SAMPLE_NUCLEUS = 4
@@ -70,6 +73,20 @@ SIGNATURES = {
     "plh_rmsnorm_lm_head": (
         _c_int,
         [_vp, _vp, _c_i64, _c_int, _c_int, _vp, ctypes.c_double, _vp, _c_i64, _c_int, _vp, _c_i64],
+    ),
+    "plh_process_logits": (
+        _c_int,
+        [_vp, _vp, _c_int, _c_i64, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_int,
+         _vp, _vp, _c_i64, _c_int],
+    ),
+    "plh_logprobs": (_c_int, [_vp, _vp, _c_int, _c_i64, _c_int, _c_int, _vp, _vp, _vp, _c_int, _vp, _vp]),
+    "plh_fp8_codes_bytes": (_c_i64, [_c_int, _c_int]),
+    "plh_fp8_pack": (_c_int, [_vp, _vp, _c_i64, _vp, _c_i64, _c_int, _c_int, _vp, _vp]),
+    "plh_fp8_quantize": (_c_int, [_vp, _vp, _c_int, _c_i64, _c_i64, _c_int, _c_int, _vp, _vp]),
+    "plh_fp8_ws_bytes": (_c_i64, [_vp, _c_int, _c_int, _c_int]),
+    "plh_fp8_linear": (
+        _c_int,
+        [_vp, _vp, _c_int, _c_i64, _c_int, _c_int, _vp, ctypes.c_double, _vp, _vp, _c_int, _vp, _c_i64, _vp, _c_i64],
     ),
 }
 
@@ -345,6 +362,36 @@ class Context:
     def rmsnorm_lm_head(self, h_ptr, ldh, N, D, norm_ptr, eps, w_ptr, ldw, V, out_ptr, ldo) -> None:
         self._check(self.lib.plh_rmsnorm_lm_head(self.handle, h_ptr, ldh, N, D, norm_ptr, eps, w_ptr, ldw, V,
                                                  out_ptr, ldo))
+
+    def process_logits(self, logits_ptr, dtype_code, ld, B, V, hist_ids, hist_off, out_start, rep_penalty, frequency,
+                       presence, bias_ids, bias, bias_off, mask, mask_ld, mask_rows, mask_row, out_ptr, out_ld,
+                       flags=0) -> None:
+        self._check(
+            self.lib.plh_process_logits(
+                self.handle, logits_ptr, dtype_code, ld, B, V, hist_ids, hist_off, out_start, rep_penalty, frequency,
+                presence, bias_ids, bias, bias_off, mask, mask_ld, mask_rows, mask_row, out_ptr, out_ld, flags,
+            )
+        )
+
+    def logprobs(self, logits_ptr, dtype_code, ld, B, V, ids, out_lp, out_rank, n_top=0, top_ids=None,
+                 top_lp=None) -> None:
+        self._check(self.lib.plh_logprobs(self.handle, logits_ptr, dtype_code, ld, B, V, ids, out_lp, out_rank, n_top,
+                                          top_ids, top_lp))
+
+    def fp8_pack(self, codes_ptr, ldc, scales_ptr, lds, V, D, out_codes, out_scales) -> None:
+        self._check(self.lib.plh_fp8_pack(self.handle, codes_ptr, ldc, scales_ptr, lds, V, D, out_codes, out_scales))
+
+    def fp8_quantize(self, w_ptr, dtype_code, stride_v, stride_d, V, D, out_codes, out_scales) -> None:
+        self._check(self.lib.plh_fp8_quantize(self.handle, w_ptr, dtype_code, stride_v, stride_d, V, D, out_codes,
+                                              out_scales))
+
+    def fp8_ws_bytes(self, N, V, D) -> int:
+        return int(self.lib.plh_fp8_ws_bytes(self.handle, N, V, D))
+
+    def fp8_linear(self, x_ptr, dtype_code, ldx, N, D, norm_ptr, eps, codes, scales, V, out_ptr, ldo, ws,
+                   ws_bytes) -> None:
+        self._check(self.lib.plh_fp8_linear(self.handle, x_ptr, dtype_code, ldx, N, D, norm_ptr, eps, codes, scales, V,
+                                            out_ptr, ldo, ws, ws_bytes))
 
     def append_ids(self, slab_ptr, pos_ptr, ids_ptr, n) -> None:
         self._check(self.lib.plh_append_ids(self.handle, slab_ptr, pos_ptr, ids_ptr, int(n)))

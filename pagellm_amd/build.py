@@ -19,7 +19,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OUT = PKG / "libpagellm_hip.so"
 BUILD = PKG / "_build"
-SOURCES = ["plh_sample.hip", "plh_small.hip", "plh_probs.hip", "plh_draw.hip", "plh_verify.hip", "plh_head.hip", "plh_api.hip"]
+SOURCES = ["plh_sample.hip", "plh_small.hip", "plh_probs.hip", "plh_draw.hip", "plh_verify.hip", "plh_head.hip", "plh_logits.hip", "plh_logprobs.hip",
+           "plh_fp8.hip", "plh_api.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = os.environ.get("PLH_OFFLOAD_ARCH", "gfx950")

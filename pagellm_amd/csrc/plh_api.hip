@@ -46,6 +46,7 @@ struct plh_ctx {
 namespace {
 
 constexpr int kMaxVBitmap = 262144;
+constexpr size_t kMostCodes = size_t(1) << 40;  // of a matrix in e4m3 (its pieces and blocks fit a grid)
 
 int fail(plh_ctx* c, int code, const char* fmt, const char* detail = nullptr) {
   if (c != nullptr) {
@@ -119,6 +120,25 @@ int timing_begin(plh_ctx* c, std::array<hipEvent_t, 3>& ev) {
   c->ev_pending.push_back(ev);
   PLH_HIP(c, hipEventRecord(ev[0], c->stream), "hipEventRecord");
   return PLH_OK;
+}
+
+// Whether some row of x [B, ld] and some row of out [B, out_ld], V elements of
+// es bytes each, share memory.
+bool rows_overlap(const void* x, int64_t ld, const void* out, int64_t out_ld, int B, int V, size_t es) {
+  const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), o0 = reinterpret_cast<uintptr_t>(out);
+  const uintptr_t x1 = x0 + ((size_t)(B - 1) * (size_t)ld + (size_t)V) * es;
+  const uintptr_t o1 = o0 + ((size_t)(B - 1) * (size_t)out_ld + (size_t)V) * es;
+  if (!(x0 < o1 && o0 < x1)) return false;
+  if (ld != out_ld) return true;
+  // interleaved rows (x = buf[:, :V], out = buf[:, V:2V]) never touch:
+  // row b' of out meets row b of x iff |d + (b' - b) * L| < V * es, with
+  // d = o0 - x0 and L the row pitch; only the two m = b' - b nearest
+  // -d / L can satisfy it
+  const int64_t d = (int64_t)(o0 - x0), L = ld * (int64_t)es, w = (int64_t)V * (int64_t)es;
+  const int64_t q = d >= 0 ? -(d / L) - 1 : (-d) / L;  // floor(-d / L) or one below it
+  for (int64_t m = q - 1; m <= q + 2; ++m)
+    if (m > -(int64_t)B && m < (int64_t)B && d + m * L < w && d + m * L > -w) return true;
+  return false;
 }
 
 constexpr size_t kScratchBytes = size_t(64) << 20;  // the no-allocation entry point's workspace, per GPU
@@ -495,27 +515,10 @@ int plh_penalize(plh_ctx* c, const void* x, int dtype, int64_t ld, int B, int V,
     return fail(c, PLH_ERR_INVALID_ARG, "null device pointer%s");
   if (hist_off != nullptr && hist_ids == nullptr)
     return fail(c, PLH_ERR_INVALID_ARG, "hist_off given without hist_ids%s");
-  {
-    // the kernel copies x to out and then penalises out from x: in place, a
-    // repeated id could read a value another thread has already penalised
-    const size_t es = dtype == PLH_F64 ? 8 : 4;
-    const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), o0 = reinterpret_cast<uintptr_t>(out);
-    const uintptr_t x1 = x0 + ((size_t)(B - 1) * (size_t)ld + (size_t)V) * es;
-    const uintptr_t o1 = o0 + ((size_t)(B - 1) * (size_t)out_ld + (size_t)V) * es;
-    bool overlap = x0 < o1 && o0 < x1;
-    if (overlap && ld == out_ld) {
-      // interleaved rows (x = buf[:, :V], out = buf[:, V:2V]) never touch:
-      // row b' of out meets row b of x iff |d + (b' - b) * L| < V * es, with
-      // d = o0 - x0 and L the row pitch; only the two m = b' - b nearest
-      // -d / L can satisfy it
-      const int64_t d = (int64_t)(o0 - x0), L = ld * (int64_t)es, w = (int64_t)V * (int64_t)es;
-      const int64_t q = d >= 0 ? -(d / L) - 1 : (-d) / L;  // floor(-d / L) or one below it
-      overlap = false;
-      for (int64_t m = q - 1; m <= q + 2; ++m)
-        if (m > -(int64_t)B && m < (int64_t)B && d + m * L < w && d + m * L > -w) overlap = true;
-    }
-    if (overlap) return fail(c, PLH_ERR_INVALID_ARG, "out must not overlap x (the penalty works on a copy)%s");
-  }
+  // the kernel copies x to out and then penalises out from x: in place, a
+  // repeated id could read a value another thread has already penalised
+  if (rows_overlap(x, ld, out, out_ld, B, V, dtype == PLH_F64 ? 8 : 4))
+    return fail(c, PLH_ERR_INVALID_ARG, "out must not overlap x (the penalty works on a copy)%s");
   int rc = use_device(c);
   if (rc != PLH_OK) return rc;
   plh::PenalizeArgs a{x, ld, out, out_ld, B, V, hist_ids, hist_off, rep_penalty};
@@ -647,6 +650,190 @@ int plh_rmsnorm_lm_head(plh_ctx* c, const float* h, int64_t ldh, int N, int D, c
   if (e != hipSuccess) return hip_fail(c, e, "plh_rmsnorm_lm_head launch");
   c->ws_stream = c->stream;
   c->ws_open = true;
+  return PLH_OK;
+}
+
+int plh_process_logits(plh_ctx* c, const void* logits, int dtype, int64_t ld, int B, int V, const int32_t* hist_ids,
+                       const int64_t* hist_off, const int64_t* out_start, const double* rep_penalty,
+                       const double* frequency, const double* presence, const int32_t* bias_ids, const double* bias,
+                       const int64_t* bias_off, const uint32_t* mask, int64_t mask_ld, int mask_rows,
+                       const int32_t* mask_row, void* out, int64_t out_ld, int flags) {
+  if (c == nullptr) return PLH_ERR_INVALID_ARG;
+  if (B < 0 || V < 1) return fail(c, PLH_ERR_INVALID_ARG, "need B >= 0 and V >= 1%s");
+  if (B == 0) return PLH_OK;
+  if (dtype != PLH_F32 && dtype != PLH_F64) return fail(c, PLH_ERR_INVALID_ARG, "dtype must be PLH_F32 or PLH_F64%s");
+  if (ld < V || out_ld < V) return fail(c, PLH_ERR_INVALID_ARG, "ld and out_ld must be >= V%s");
+  if (logits == nullptr || out == nullptr) return fail(c, PLH_ERR_INVALID_ARG, "null device pointer%s");
+  if (flags & ~PLH_SAMPLE_HIST_SPANS) return fail(c, PLH_ERR_INVALID_ARG, "unknown flag%s");
+  if (hist_off != nullptr && hist_ids == nullptr)
+    return fail(c, PLH_ERR_INVALID_ARG, "hist_off given without hist_ids%s");
+  if (bias_off != nullptr && (bias_ids == nullptr || bias == nullptr))
+    return fail(c, PLH_ERR_INVALID_ARG, "bias_off given without bias_ids and bias%s");
+  if (mask != nullptr && (mask_ld < ((int64_t)V + 31) / 32 || mask_rows < (mask_row != nullptr ? 0 : B)))
+    return fail(c, PLH_ERR_INVALID_ARG, "need mask_ld >= ceil(V / 32), and without mask_row mask_rows >= B%s");
+  const size_t es = dtype == PLH_F64 ? 8 : 4;
+  if (reinterpret_cast<uintptr_t>(logits) % es != 0 || reinterpret_cast<uintptr_t>(out) % es != 0)
+    return fail(c, PLH_ERR_INVALID_ARG, "logits and out must be aligned to their element size%s");
+  if (logits == out ? ld != out_ld : rows_overlap(logits, ld, out, out_ld, B, V, es))
+    return fail(c, PLH_ERR_INVALID_ARG, "out must be logits itself (out_ld = ld) or rows that meet none of it%s");
+  int rc = use_device(c);
+  if (rc != PLH_OK) return rc;
+  plh::ProcessArgs a{};
+  a.x = logits;
+  a.ld = ld;
+  a.out = out;
+  a.out_ld = out_ld;
+  a.B = B;
+  a.V = V;
+  a.hist_ids = hist_ids;
+  a.hist_off = hist_off;
+  a.hist_spans = (flags & PLH_SAMPLE_HIST_SPANS) ? 1 : 0;
+  a.out_start = out_start;
+  a.rep = rep_penalty;
+  a.freq = frequency;
+  a.pres = presence;
+  a.bias_ids = bias_ids;
+  a.bias = bias;
+  a.bias_off = bias_off;
+  a.mask = mask;
+  a.mask_ld = mask_ld;
+  a.mask_rows = mask_rows;
+  a.mask_row = mask_row;
+  const hipError_t e = plh::launch_process(a, dtype == PLH_F64, c->stream);
+  if (e != hipSuccess) return hip_fail(c, e, "plh_process_logits launch");
+  return PLH_OK;
+}
+
+int plh_logprobs(plh_ctx* c, const void* logits, int dtype, int64_t ld, int B, int V, const int32_t* ids, void* out_lp,
+                 int32_t* out_rank, int n_top, int32_t* top_ids, void* top_lp) {
+  if (c == nullptr) return PLH_ERR_INVALID_ARG;
+  if (B < 0 || V < 1) return fail(c, PLH_ERR_INVALID_ARG, "need B >= 0 and V >= 1%s");
+  if (n_top < 0 || n_top > PLH_MAX_TOP || n_top > V)
+    return fail(c, PLH_ERR_INVALID_ARG, "need 0 <= n_top <= min(V, 64)%s");
+  if (B == 0) return PLH_OK;
+  if (dtype != PLH_F32 && dtype != PLH_F64) return fail(c, PLH_ERR_INVALID_ARG, "dtype must be PLH_F32 or PLH_F64%s");
+  if (ld < V) return fail(c, PLH_ERR_INVALID_ARG, "ld must be >= V%s");
+  if (logits == nullptr || (ids != nullptr && (out_lp == nullptr || out_rank == nullptr)) ||
+      (n_top > 0 && (top_ids == nullptr || top_lp == nullptr)))
+    return fail(c, PLH_ERR_INVALID_ARG, "null device pointer%s");
+  const size_t es = dtype == PLH_F64 ? 8 : 4;
+  if (reinterpret_cast<uintptr_t>(logits) % es != 0)
+    return fail(c, PLH_ERR_INVALID_ARG, "logits must be aligned to their element size%s");
+  if (ids == nullptr && n_top == 0) return PLH_OK;
+  int rc = use_device(c);
+  if (rc != PLH_OK) return rc;
+  plh::LogprobsArgs a{};
+  a.x = logits;
+  a.ld = ld;
+  a.B = B;
+  a.V = V;
+  a.ids = ids;
+  a.lp = out_lp;
+  a.rank = out_rank;
+  a.n = n_top;
+  a.top_ids = top_ids;
+  a.top_lp = top_lp;
+  // the one-launch form needs no workspace: it serves calls under graph
+  // capture, which must not allocate or wait for another stream
+  size_t need = plh::plan_logprobs(a, dtype == PLH_F64, c->num_cu, false);
+  if (need > 0) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    PLH_HIP(c, hipStreamIsCapturing(c->stream, &st), "hipStreamIsCapturing");
+    if (st != hipStreamCaptureStatusNone) need = plh::plan_logprobs(a, dtype == PLH_F64, c->num_cu, true);
+  }
+  if (need > 0) {
+    rc = reserve_ws(c, need);
+    if (rc != PLH_OK) return rc;
+    a.ws = c->ws;
+    c->ws_stream = c->stream;
+    c->ws_open = true;
+  }
+  const hipError_t e = plh::launch_logprobs(a, dtype == PLH_F64, c->stream);
+  if (e != hipSuccess) return hip_fail(c, e, "plh_logprobs launch");
+  return PLH_OK;
+}
+
+int64_t plh_fp8_codes_bytes(int V, int D) {
+  return V < 1 || D < 1 ? PLH_ERR_INVALID_ARG : (int64_t)plh::fp8_codes_bytes(V, D);
+}
+
+int plh_fp8_pack(plh_ctx* c, const uint8_t* codes, int64_t ldc, const float* scales, int64_t lds, int V, int D,
+                 uint8_t* out_codes, float* out_scales) {
+  if (c == nullptr) return PLH_ERR_INVALID_ARG;
+  if (V < 1 || D < 1) return fail(c, PLH_ERR_INVALID_ARG, "need V >= 1 and D >= 1%s");
+  if (ldc < D || lds < ((int64_t)D + 127) / 128)
+    return fail(c, PLH_ERR_INVALID_ARG, "need ldc >= D and lds >= ceil(D / 128)%s");
+  if (codes == nullptr || scales == nullptr || out_codes == nullptr || out_scales == nullptr)
+    return fail(c, PLH_ERR_INVALID_ARG, "null device pointer%s");
+  if (!aligned16(out_codes)) return fail(c, PLH_ERR_INVALID_ARG, "out_codes must be 16-byte aligned%s");
+  if (plh::fp8_codes_bytes(V, D) > kMostCodes) return fail(c, PLH_ERR_UNSUPPORTED, "more than 2^40 codes%s");
+  int rc = use_device(c);
+  if (rc != PLH_OK) return rc;
+  const hipError_t e = plh::launch_fp8_pack(codes, ldc, scales, lds, V, D, out_codes, out_scales, c->stream);
+  if (e != hipSuccess) return hip_fail(c, e, "plh_fp8_pack launch");
+  return PLH_OK;
+}
+
+int plh_fp8_quantize(plh_ctx* c, const void* W, int dtype, int64_t stride_v, int64_t stride_d, int V, int D,
+                     uint8_t* out_codes, float* out_scales) {
+  if (c == nullptr) return PLH_ERR_INVALID_ARG;
+  if (V < 1 || D < 1) return fail(c, PLH_ERR_INVALID_ARG, "need V >= 1 and D >= 1%s");
+  if (dtype != PLH_F32 && dtype != PLH_BF16 && dtype != PLH_F16)
+    return fail(c, PLH_ERR_INVALID_ARG, "dtype must be PLH_F32, PLH_BF16 or PLH_F16%s");
+  if (stride_v < 0 || stride_d < 0) return fail(c, PLH_ERR_INVALID_ARG, "strides must be >= 0%s");
+  if (W == nullptr || out_codes == nullptr || out_scales == nullptr)
+    return fail(c, PLH_ERR_INVALID_ARG, "null device pointer%s");
+  if (!aligned16(out_codes)) return fail(c, PLH_ERR_INVALID_ARG, "out_codes must be 16-byte aligned%s");
+  if (plh::fp8_codes_bytes(V, D) > kMostCodes) return fail(c, PLH_ERR_UNSUPPORTED, "more than 2^40 codes%s");
+  int rc = use_device(c);
+  if (rc != PLH_OK) return rc;
+  const hipError_t e =
+      plh::launch_fp8_quantize(W, dtype, stride_v, stride_d, V, D, out_codes, out_scales, c->stream);
+  if (e != hipSuccess) return hip_fail(c, e, "plh_fp8_quantize launch");
+  return PLH_OK;
+}
+
+int64_t plh_fp8_ws_bytes(plh_ctx* c, int N, int V, int D) {
+  if (c == nullptr || N < 0 || V < 1 || D < 1) return PLH_ERR_INVALID_ARG;
+  return (int64_t)plh::fp8_ws_bytes(N, V, D, c->num_cu);
+}
+
+int plh_fp8_linear(plh_ctx* c, const void* x, int dtype, int64_t ldx, int N, int D, const float* norm, double eps,
+                   const uint8_t* codes, const float* scales, int V, float* out, int64_t ldo, void* ws,
+                   int64_t ws_bytes) {
+  if (c == nullptr) return PLH_ERR_INVALID_ARG;
+  if (N < 0 || D < 1 || V < 1) return fail(c, PLH_ERR_INVALID_ARG, "need N >= 0, D >= 1 and V >= 1%s");
+  if (N == 0) return PLH_OK;
+  if (dtype != PLH_F32 && dtype != PLH_BF16 && dtype != PLH_F16)
+    return fail(c, PLH_ERR_INVALID_ARG, "dtype must be PLH_F32, PLH_BF16 or PLH_F16%s");
+  if (ldx < D || ldo < V) return fail(c, PLH_ERR_INVALID_ARG, "need ldx >= D and ldo >= V%s");
+  if (x == nullptr || codes == nullptr || scales == nullptr || out == nullptr || ws == nullptr)
+    return fail(c, PLH_ERR_INVALID_ARG, "null device pointer%s");
+  if (norm != nullptr && (!(eps >= 0.0) || !std::isfinite(eps)))
+    return fail(c, PLH_ERR_INVALID_ARG, "eps must be finite and >= 0%s");
+  if (!aligned16(codes) || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0)
+    return fail(c, PLH_ERR_INVALID_ARG, "codes must be 16-byte and ws 256-byte aligned%s");
+  if (reinterpret_cast<uintptr_t>(x) % (dtype == PLH_F32 ? 4 : 2) != 0 || reinterpret_cast<uintptr_t>(out) % 4 != 0)
+    return fail(c, PLH_ERR_INVALID_ARG, "x and out must be aligned to their element size%s");
+  if (plh::fp8_codes_bytes(V, D) > kMostCodes) return fail(c, PLH_ERR_UNSUPPORTED, "more than 2^40 codes%s");
+  if (ws_bytes < (int64_t)plh::fp8_ws_bytes(N, V, D, c->num_cu))
+    return fail(c, PLH_ERR_INVALID_ARG, "ws is smaller than plh_fp8_ws_bytes%s");
+  int rc = use_device(c);
+  if (rc != PLH_OK) return rc;
+  plh::Fp8Args a{};
+  a.x = x;
+  a.ldx = ldx;
+  a.norm = norm;
+  a.eps = eps;
+  a.codes = codes;
+  a.scales = scales;
+  a.out = out;
+  a.ldo = ldo;
+  a.N = N;
+  a.D = D;
+  a.V = V;
+  const hipError_t e = plh::launch_fp8_linear(a, dtype, ws, c->num_cu, c->stream);
+  if (e != hipSuccess) return hip_fail(c, e, "plh_fp8_linear launch");
   return PLH_OK;
 }
 

@@ -1,0 +1,408 @@
+// gfx950 kernels for products with e4m3 weights and a scale for each block of
+// 128 (plh_fp8_*): out[n, v] = sum_b t[v / 128, b] sum_{k in b} a[n, k] w[v, k], a
+// the rows' rounded values.
+//
+//   k_fp8_act       rows -> RMSNorm -> rounded to e4m3 by blocks -> bf16
+//   k_fp8_skinny    at most 32 rows: bound by one read of the codes
+//   k_fp8_tiles     more rows
+//   k_fp8_pack, k_fp8_quantize   the weights' layout, once
+//
+// The products run on the bf16 matrix cores.  The 8-bit ones align a sum's
+// products to the largest with 14 bits below it: a block's sum comes out 1.5e-5
+// (relative, normal operands) from its exact value, and 4.6e-5 with operands of
+// mixed sizes, where bf16 operands give 9e-9 and 8e-8, as float32 sums do.  An
+// e4m3 value is a bf16 value, and so is one times its row's scale, a power of two:
+// the activations are stored as bf16 with their scales applied, the weights stay
+// 8-bit in memory and are widened in registers (one instruction for two), and only
+// the weights' scale, the same for a block's 128 x 128, is left for the
+// accumulators: one float32 multiply-add for each output and block.
+//
+// The weights are the matrix instruction's rows and the activations its columns: a
+// lane then holds four consecutive v of one n, and the logits leave in 16-byte
+// stores.
+//
+// Layout of the codes: tiles of 32 rows x 128 k, all blocks of 32 rows one after
+// the other, each tile 4 KB in the order in which a wave reads it for the 32 x 32
+// x 16 instruction: 16-byte piece (q, h, r) of row r and k = 32 q + 16 h + 0 .. 15
+// at 1024 q + 512 h + 16 r.  A wave's load is 1 KB of consecutive bytes and 32
+// rows are one stream.  (An instruction sums over its k, so any order of k that
+// both operands share is right: its two steps of a piece take 8 codes each.)
+#include "plh_device.h"
+#include "plh_kernels.h"
+
+#include "pagellm_hip.h"
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include <algorithm>
+
+namespace plh {
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4e __attribute__((ext_vector_type(4))) __attribute__((aligned(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kBlock = 128;
+constexpr int kTileRows = 32;                     // rows of a tile of codes
+constexpr int kTileBytes = kTileRows * kBlock;    // its size
+constexpr float kE4m3Max = 448.0f;
+
+__host__ __device__ constexpr int blocks_of(int n) { return (n + kBlock - 1) / kBlock; }
+__host__ __device__ constexpr int tiles_of(int n, int rows = kTileRows) { return (n + rows - 1) / rows; }
+
+// Where the 16 codes of row r and k = 16 p .. 16 p + 15 lie, in a matrix of kb
+// blocks a row.
+__device__ __forceinline__ size_t code_at(int64_t r, int p, int kb) {
+  return ((size_t)(r / kTileRows) * kb + p / 8) * kTileBytes + (p % 8) * (kTileRows * 16) + (r % kTileRows) * 16;
+}
+
+// Where the 8 rounded values of row n and k = 8 p .. 8 p + 7 lie (16-byte units)
+// among the rows' tiles of R rows x 128 k, R that of the matrix instruction: its
+// step's operand is 64 lanes x 16 bytes.  p's bits of a block are (q, h, j) as
+// above: with R = 32 step (q, j) holds (h, row) in lane 32 h + row, with R = 16 a
+// step holds two of the q: step (q / 2, j), lane 16 (2 (q % 2) + h) + row.
+template <int R>
+__device__ __forceinline__ size_t act_at(int64_t n, int p, int kb) {
+  const int q = (p >> 2) & 3, h = (p >> 1) & 1, j = p & 1, r = (int)(n % R);
+  const int in = R == 32 ? (2 * q + j) * 64 + 32 * h + r : ((q & 2) + j) * 64 + 16 * (2 * (q & 1) + h) + r;
+  return ((size_t)(n / R) * kb + p / 16) * (R * 16) + in;
+}
+
+// The smallest power of two s >= 2^-126 with amax <= 448 s (448 = 1.75 * 2^8);
+// 1 where amax is not finite.  1 / s is a power of two too, so y / s is exact.
+__device__ __forceinline__ float block_scale(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  if (u >= 0x7f800000u) return 1.0f;
+  const int e = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return __uint_as_float((uint32_t)max(e, 1) << 23);
+}
+
+__device__ __forceinline__ float inverse_pow2(float s) { return __uint_as_float(0x7f000000u - __float_as_uint(s)); }
+
+// Four values, |x| <= 448 or NaN for what is not finite, as e4m3 codes.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+
+__device__ __forceinline__ float code_input(float y, float inv) {
+  const float t = y * inv;
+  return fabsf(t) <= kE4m3Max ? t : NAN;
+}
+
+template <typename T>
+__device__ __forceinline__ float widen(T v) { return (float)v; }
+
+// ------------------------------------------------------------ activations
+
+constexpr int kRun = 16;                   // k values of a thread at a time: one 16-byte piece of codes
+constexpr int kSweep = kRun * kThreads;    // k values of a workgroup at a time
+
+template <typename TX>
+__device__ __forceinline__ void load_run(const TX* x, int k0, int D, float (&v)[kRun]) {
+#pragma unroll
+  for (int j = 0; j < kRun; ++j) v[j] = k0 + j < D ? widen(x[k0 + j]) : 0.0f;
+}
+
+// e4m3 codes back to the values they stand for, times the power of two s, as
+// bf16 (exact: four significant bits).
+__device__ __forceinline__ uint32_t rounded2(uint32_t codes, bool hi, float s) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 v = hi ? __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false);
+  return (__float_as_uint(v[0] * s) >> 16) | (__float_as_uint(v[1] * s) & 0xffff0000u);
+}
+
+// One workgroup per row.
+template <typename TX, int R>
+__global__ __launch_bounds__(kThreads) void k_fp8_act(Fp8Args a) {
+  __shared__ double red[kWaves];
+  const int n = blockIdx.x;
+  const TX* x = static_cast<const TX*>(a.x) + (int64_t)n * a.ldx;
+  float v[kRun];
+  double r = 1.0;
+  if (a.norm != nullptr) {
+    double s = 0.0;
+    for (int k0 = threadIdx.x * kRun; k0 < a.D; k0 += kSweep) {
+      load_run(x, k0, a.D, v);
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) s += (double)v[j] * (double)v[j];
+    }
+    s = block_sum(s, red);
+    r = 1.0 / sqrt(s / (double)a.D + a.eps);
+  }
+  for (int k0 = threadIdx.x * kRun; k0 < a.kb * kBlock; k0 += kSweep) {
+    load_run(x, k0, a.D, v);
+    float amax = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      if (a.norm != nullptr) v[j] = k0 + j < a.D ? (float)((double)v[j] * r * (double)a.norm[k0 + j]) : 0.0f;
+      amax = fmaxf(amax, fabsf(v[j]));
+    }
+    // the block's eight threads are lanes 8 i .. 8 i + 7
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) amax = fmaxf(amax, __shfl_xor(amax, d));
+    const float s = block_scale(amax), inv = inverse_pow2(s);
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t c = codes4(code_input(v[4 * j], inv), code_input(v[4 * j + 1], inv), code_input(v[4 * j + 2], inv),
+                                code_input(v[4 * j + 3], inv));
+      w[2 * j] = rounded2(c, false, s);
+      w[2 * j + 1] = rounded2(c, true, s);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      a.act[act_at<R>(n, k0 / 8 + j, a.kb)] = uint4{w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]};
+  }
+}
+
+// ----------------------------------------------------------------- product
+
+// Eight codes as the matrix instruction's operand.
+__device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+__device__ __forceinline__ bf16x8 as_bf16(u32x4 v) { return __builtin_bit_cast(bf16x8, v); }
+
+// The matrix instruction with R rows of weights and R of activations, and its
+// operands of one tile and block.
+template <int R>
+struct Mma;
+template <>
+struct Mma<32> {
+  typedef f32x16 Acc;
+  static constexpr int kSteps = 8;    // per block of 128
+  static constexpr int kPieces = 4;   // 16-byte pieces of codes a lane holds
+  static __device__ __forceinline__ size_t piece(int i) { return (size_t)i * 1024 + lane() * 16; }
+  static __device__ __forceinline__ Acc mma(bf16x8 w, bf16x8 x, Acc c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, x, c, 0, 0, 0);
+  }
+  // accumulator registers 4 g .. 4 g + 3 hold rows row(g) .. + 3 of column lane() % 32
+  static __device__ __forceinline__ int row(int g) { return 8 * g + 4 * (lane() >> 5); }
+};
+template <>
+struct Mma<16> {
+  typedef f32x4 Acc;
+  static constexpr int kSteps = 4;
+  static constexpr int kPieces = 2;
+  // of 16 rows of a tile, the others 256 bytes further on: lane group g reads
+  // (q, h) = (2 i + g / 2, g % 2)
+  static __device__ __forceinline__ size_t piece(int i) {
+    const int g = lane() >> 4;
+    return (size_t)(2 * i + (g >> 1)) * 1024 + (g & 1) * 512 + (lane() & 15) * 16;
+  }
+  static __device__ __forceinline__ Acc mma(bf16x8 w, bf16x8 x, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ int row(int g) { return 4 * (lane() >> 4); }
+};
+
+// Four consecutive logits of row n, those inside the vocabulary.
+__device__ __forceinline__ void store4(const Fp8Args& a, int n, int v, f32x4 t) {
+  if (n >= a.N || v >= a.V) return;
+  float* o = a.out + (int64_t)n * a.ldo + v;
+  if (v + 4 <= a.V) {
+    *reinterpret_cast<f32x4e*>(o) = t;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (v + e < a.V) o[e] = t[e];
+  }
+}
+
+// --------------------------------------------------------------- few rows
+
+constexpr int kSkinnyCols = 64;  // columns of the logits of a workgroup: half a scale block
+
+// R rows x 64 columns per workgroup.  The 8 waves share them and take every
+// eighth block of k each, codes and activations straight from memory into
+// registers; their sums meet in LDS at the end, in a fixed order.
+template <int R>
+__global__ __launch_bounds__(kThreads) void k_fp8_skinny(Fp8Args a) {
+  using M = Mma<R>;
+  constexpr int kVT = kSkinnyCols / R, kRegs = R * R / 64, kQuads = kVT * kRegs / 4;
+  __shared__ f32x4 sm[kWaves][kQuads][kWave];
+  const int v0 = blockIdx.x * kSkinnyCols, nt = blockIdx.y;
+  typename M::Acc acc[kVT];
+#pragma unroll
+  for (int i = 0; i < kVT; ++i) acc[i] = typename M::Acc{};
+  const uint8_t* w[kVT];
+  // rows past the last read as the last ones, and are not stored
+#pragma unroll
+  for (int i = 0; i < kVT; ++i) {
+    const int v = min(v0 + i * R, tiles_of(a.V) * kTileRows - R);
+    w[i] = a.codes + (size_t)(v / kTileRows) * a.kb * kTileBytes + (v % kTileRows) * 16;
+  }
+  const u32x4* act = reinterpret_cast<const u32x4*>(a.act) + (size_t)nt * a.kb * (R * 16) + lane();
+  const float* ts = a.scales + (size_t)(v0 / kBlock) * a.kb;
+  for (int b = wave(); b < a.kb; b += kWaves) {
+    u32x4 x[M::kSteps], c[kVT][M::kPieces];
+#pragma unroll
+    for (int i = 0; i < kVT; ++i)
+#pragma unroll
+      for (int q = 0; q < M::kPieces; ++q)
+        c[i][q] = *reinterpret_cast<const u32x4*>(w[i] + (size_t)b * kTileBytes + M::piece(q));
+#pragma unroll
+    for (int s = 0; s < M::kSteps; ++s) x[s] = act[(size_t)b * (R * 16) + s * kWave];
+    const float t = ts[b];
+#pragma unroll
+    for (int i = 0; i < kVT; ++i) {
+      typename M::Acc p{};
+#pragma unroll
+      for (int q = 0; q < M::kPieces; ++q) {
+        p = M::mma(widen8(c[i][q][0], c[i][q][1]), as_bf16(x[2 * q]), p);
+        p = M::mma(widen8(c[i][q][2], c[i][q][3]), as_bf16(x[2 * q + 1]), p);
+      }
+#pragma unroll
+      for (int e = 0; e < kRegs; ++e) acc[i][e] = fmaf(p[e], t, acc[i][e]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kVT; ++i)
+#pragma unroll
+    for (int g = 0; g < kRegs / 4; ++g)
+      sm[wave()][i * (kRegs / 4) + g][lane()] =
+          f32x4{acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]};
+  wg_barrier();
+  for (int u = wave(); u < kQuads; u += kWaves) {
+    f32x4 t = sm[0][u][lane()];
+#pragma unroll
+    for (int k = 1; k < kWaves; ++k) t += sm[k][u][lane()];
+    store4(a, nt * R + lane() % R, v0 + u / (kRegs / 4) * R + M::row(u % (kRegs / 4)), t);
+  }
+}
+
+// ---------------------------------------------------------------- weights
+
+// One thread per 16 codes of the layout.
+__global__ __launch_bounds__(256) void k_fp8_pack(const uint8_t* codes, int64_t ldc, const float* scales, int64_t lds,
+                                                  int V, int D, uint8_t* out, float* out_scales) {
+  const int kb = blocks_of(D);
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, pieces = (int64_t)tiles_of(V) * kTileRows * kb * 8;
+  if (i < pieces) {
+    const int64_t r = i / (kb * 8);
+    const int q = (int)(i % (kb * 8));
+    __align__(16) uint8_t c[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) c[j] = r < V && q * 16 + j < D ? codes[r * ldc + q * 16 + j] : 0;
+    *reinterpret_cast<uint4*>(out + code_at(r, q, kb)) = *reinterpret_cast<const uint4*>(c);
+  }
+  if (i < (int64_t)blocks_of(V) * kb) out_scales[i] = scales[i / kb * lds + i % kb];
+}
+
+// One workgroup of 256 threads per block of 128 x 128.  `along_v`: neighbouring threads take neighbouring rows (W is
+// contiguous along v).
+template <typename TW>
+__global__ __launch_bounds__(256) void k_fp8_quantize(const TW* W, int64_t sv, int64_t sd, int V, int D, uint8_t* out,
+                                                      float* out_scales) {
+  __shared__ float tile[kBlock][kBlock + 1];
+  __shared__ float red[4];
+  const int kb = blocks_of(D), b = blockIdx.x % kb, vb = blockIdx.x / kb;
+  const bool along_v = sv < sd;
+  float amax = 0.0f;
+  for (int i = threadIdx.x; i < kBlock * kBlock; i += 256) {
+    const int r = along_v ? i % kBlock : i / kBlock, k = along_v ? i / kBlock : i % kBlock;
+    const int64_t v = (int64_t)vb * kBlock + r;
+    const int d = b * kBlock + k;
+    const float x = v < V && d < D ? widen(W[v * sv + d * sd]) : 0.0f;
+    tile[r][k] = x;
+    if (fabsf(x) < INFINITY) amax = fmaxf(amax, fabsf(x));
+  }
+  amax = wave_max(amax);
+  if (lane() == 0) red[wave()] = amax;
+  __syncthreads();
+  const float s = block_scale(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]))), inv = inverse_pow2(s);
+  if (threadIdx.x == 0) out_scales[(size_t)vb * kb + b] = s;
+  for (int i = threadIdx.x; i < kBlock * 8; i += 256) {
+    const int r = i % kBlock, q = i / kBlock;
+    if (vb * kBlock + r >= tiles_of(V) * kTileRows) continue;
+    uint32_t c[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float* t = &tile[r][q * 16 + 4 * j];
+      c[j] = codes4(code_input(t[0], inv), code_input(t[1], inv), code_input(t[2], inv), code_input(t[3], inv));
+    }
+    *reinterpret_cast<uint4*>(out + code_at((int64_t)vb * kBlock + r, b * 8 + q, kb)) = uint4{c[0], c[1], c[2], c[3]};
+  }
+}
+
+}  // namespace
+
+size_t fp8_codes_bytes(int V, int D) { return (size_t)tiles_of(V) * blocks_of(D) * kTileBytes; }
+
+namespace {
+// Rows of the matrix instruction: 16 where that holds all rows, else 32.
+int rows_of(int N) { return N <= 16 ? 16 : 32; }
+
+template <int R>
+hipError_t launch_act(const Fp8Args& a, int dtype, hipStream_t s) {
+  if (dtype == PLH_BF16) hipLaunchKernelGGL((k_fp8_act<__hip_bfloat16, R>), dim3(a.N), dim3(kThreads), 0, s, a);
+  else if (dtype == PLH_F16) hipLaunchKernelGGL((k_fp8_act<__half, R>), dim3(a.N), dim3(kThreads), 0, s, a);
+  else hipLaunchKernelGGL((k_fp8_act<float, R>), dim3(a.N), dim3(kThreads), 0, s, a);
+  return hipGetLastError();
+}
+}  // namespace
+
+size_t fp8_ws_bytes(int N, int V, int D, int num_cu) {
+  const int R = rows_of(N);
+  return (size_t)tiles_of(N, R) * R * blocks_of(D) * kBlock * 2;
+}
+
+hipError_t launch_fp8_pack(const uint8_t* codes, int64_t ldc, const float* scales, int64_t lds, int V, int D,
+                           uint8_t* out_codes, float* out_scales, hipStream_t s) {
+  const int64_t pieces = (int64_t)tiles_of(V) * kTileRows * blocks_of(D) * 8;
+  hipLaunchKernelGGL(k_fp8_pack, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, codes, ldc, scales, lds, V, D,
+                     out_codes, out_scales);
+  return hipGetLastError();
+}
+
+hipError_t launch_fp8_quantize(const void* w, int dtype, int64_t sv, int64_t sd, int V, int D, uint8_t* out_codes,
+                               float* out_scales, hipStream_t s) {
+  const dim3 grid((unsigned)(blocks_of(V) * (int64_t)blocks_of(D)));
+  if (dtype == PLH_BF16)
+    hipLaunchKernelGGL((k_fp8_quantize<__hip_bfloat16>), grid, dim3(256), 0, s, static_cast<const __hip_bfloat16*>(w),
+                       sv, sd, V, D, out_codes, out_scales);
+  else if (dtype == PLH_F16)
+    hipLaunchKernelGGL((k_fp8_quantize<__half>), grid, dim3(256), 0, s, static_cast<const __half*>(w), sv, sd, V, D,
+                       out_codes, out_scales);
+  else
+    hipLaunchKernelGGL((k_fp8_quantize<float>), grid, dim3(256), 0, s, static_cast<const float*>(w), sv, sd, V, D,
+                       out_codes, out_scales);
+  return hipGetLastError();
+}
+
+hipError_t launch_fp8_linear(Fp8Args a, int dtype, void* ws, int num_cu, hipStream_t s) {
+  a.kb = blocks_of(a.D);
+  a.act = static_cast<uint4*>(ws);
+  const int R = rows_of(a.N);
+  hipError_t e = R == 16 ? launch_act<16>(a, dtype, s) : launch_act<32>(a, dtype, s);
+  if (e != hipSuccess) return e;
+  const unsigned gx = (a.V + kSkinnyCols - 1) / kSkinnyCols;
+  // the grid's y holds 65 535 row tiles
+  const int step = 65535 * R;
+  for (int64_t n0 = 0; n0 < a.N; n0 += step) {
+    Fp8Args c = a;
+    c.N = (int)std::min<int64_t>(step, a.N - n0);
+    c.out = a.out + n0 * a.ldo;
+    c.act = a.act + n0 / R * a.kb * (R * 16);
+    const dim3 grid(gx, tiles_of(c.N, R));
+    if (R == 16) hipLaunchKernelGGL((k_fp8_skinny<16>), grid, dim3(kThreads), 0, s, c);
+    else hipLaunchKernelGGL((k_fp8_skinny<32>), grid, dim3(kThreads), 0, s, c);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace plh

@@ -152,6 +152,58 @@ struct HeadArgs {
   int N, D, V;
 };
 
+struct ProcessArgs {
+  const void* x;
+  int64_t ld;
+  void* out;
+  int64_t out_ld;
+  int B, V;
+  const int32_t* hist_ids;
+  const int64_t* hist_off;   // B+1 offsets, or B (start, end) pairs
+  int hist_spans;            // 1: hist_off holds (start, end) pairs
+  const int64_t* out_start;  // [B] or null (0)
+  const double* rep;         // [B] each, or null (1, 0, 0)
+  const double* freq;
+  const double* pres;
+  const int32_t* bias_ids;
+  const double* bias;
+  const int64_t* bias_off;   // [B+1] or null
+  const uint32_t* mask;      // [mask_rows, mask_ld] or null
+  int64_t mask_ld;
+  int mask_rows;
+  const int32_t* mask_row;   // [B] or null (row b)
+};
+
+struct LogprobsArgs {
+  const void* x;
+  int64_t ld;
+  int B, V;
+  const int32_t* ids;  // [B] or null
+  void* lp;            // [B]
+  int32_t* rank;       // [B]
+  int n;               // top tokens, at most kMaxTop
+  int32_t* top_ids;    // [B, n]
+  void* top_lp;        // [B, n]
+  int segs;            // segments per row, a workgroup each
+  int seg_chunks;      // chunks per segment
+  void* ws;            // the segments' partials (segs > 1)
+};
+constexpr int kMaxTop = 64;
+
+struct Fp8Args {
+  const void* x;       // [N, ldx] rows
+  int64_t ldx;
+  const float* norm;   // [D] or null
+  double eps;
+  const uint8_t* codes;  // the weights in the library's layout
+  const float* scales;   // [ceil(V/128), kb]
+  float* out;          // [N, ldo]
+  int64_t ldo;
+  uint4* act;          // workspace: the rows, rounded, as bf16 in the product's operand layout
+  int N, D, V;
+  int kb;              // blocks of 128 in a row: ceil(D / 128)
+};
+
 // Rows of at most kSmallV tokens: the whole call in one launch, no workspace.
 // `between` (when not null) is recorded after it.
 constexpr int kSmallV = 1024;
@@ -193,6 +245,19 @@ hipError_t launch_verify(const VerifyArgs& a, const VerifyWs& ws, bool f64, hipS
 // the partial sums, and with slices their sum).
 size_t head_ws_bytes(int N, int D, int V, int64_t ldw, int num_cu);
 hipError_t launch_head(HeadArgs a, int num_cu, hipStream_t s);
+// Biases, penalties and masks; log probabilities (plan_logprobs sets segs and
+// seg_chunks and returns the workspace's bytes, 0 with one segment).
+hipError_t launch_process(const ProcessArgs& a, bool f64, hipStream_t s);
+size_t plan_logprobs(LogprobsArgs& a, bool f64, int num_cu, bool one_launch);
+hipError_t launch_logprobs(const LogprobsArgs& a, bool f64, hipStream_t s);
+// Products with e4m3 weights: dtype is a PLH_* code of the rows or the matrix.
+size_t fp8_codes_bytes(int V, int D);
+size_t fp8_ws_bytes(int N, int V, int D, int num_cu);
+hipError_t launch_fp8_pack(const uint8_t* codes, int64_t ldc, const float* scales, int64_t lds, int V, int D,
+                           uint8_t* out_codes, float* out_scales, hipStream_t s);
+hipError_t launch_fp8_quantize(const void* w, int dtype, int64_t stride_v, int64_t stride_d, int V, int D,
+                               uint8_t* out_codes, float* out_scales, hipStream_t s);
+hipError_t launch_fp8_linear(Fp8Args a, int dtype, void* ws, int num_cu, hipStream_t s);
 hipError_t launch_append(int32_t* slab, const int64_t* pos, const int32_t* ids, int n, hipStream_t s);
 
 }  // namespace plh

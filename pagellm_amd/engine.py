@@ -14,7 +14,8 @@ step:
 * each sequence keeps its own numpy ``Generator`` on the host: one
   ``rng.random()`` per non-greedy row, none for greedy rows, in row order,
   exactly as the per-row loop consumes them (``sampling.py:98``, ``:102-106``);
-* only the token ids come back to the host.
+* only the token ids come back to the host, with their log probabilities where
+  a step asks for them.
 
 Forked sequences (``SamplingParams.n > 1``, ``llm_engine.py:259-278``) join
 with the parent's token list at the time of the fork, so each child samples
@@ -28,6 +29,7 @@ from typing import Hashable, Sequence
 import numpy as np
 
 from . import _native
+from .logits import DeviceLogprobs, _check_mask, _expand_rules, _pack_rules
 from .sampling import _draw_uniforms, _expand_params, _history_ids, _is_torch_cuda, _nucleus_hint, _pack_params
 
 __all__ = ["BatchSampler", "DeviceHistories"]
@@ -52,6 +54,7 @@ class DeviceHistories:
         self._free = list(range(self.max_seqs - 1, -1, -1))
         self._slot: dict[Hashable, int] = {}
         self._len: dict[Hashable, int] = {}
+        self._prompt: dict[Hashable, int] = {}  # where each sequence's outputs begin
 
     def __contains__(self, key) -> bool:
         return key in self._slot
@@ -62,13 +65,17 @@ class DeviceHistories:
     def length(self, key) -> int:
         return self._len[key]
 
-    def add(self, key, tokens) -> None:
-        """A new sequence (or a fork) with its current token list."""
+    def add(self, key, tokens, prompt_len: int | None = None) -> None:
+        """A new sequence (or a fork) with its current token list, the first
+        ``prompt_len`` of which (None: all) are its prompt: frequency and
+        presence penalties count the tokens after them."""
         if key in self._slot:
             raise ValueError(f"sequence {key!r} already has a history")
         ids = _history_ids(tokens, self.V)
         if ids.size > self.max_len:
             raise ValueError(f"history of {ids.size} tokens exceeds max_len {self.max_len}")
+        if prompt_len is not None and not 0 <= prompt_len <= ids.size:
+            raise ValueError(f"prompt_len must be in [0, {ids.size}]")
         if not self._free:
             raise RuntimeError(f"all {self.max_seqs} history slots are in use")
         slot = self._free.pop()
@@ -77,11 +84,13 @@ class DeviceHistories:
             c._check(c.lib.plh_h2d(c.handle, self.slab.ptr + 4 * slot * self.max_len, ids.ctypes.data, ids.nbytes))
         self._slot[key] = slot
         self._len[key] = int(ids.size)
+        self._prompt[key] = int(ids.size if prompt_len is None else prompt_len)
 
     def remove(self, key) -> None:
         """A finished or aborted sequence gives its slot back."""
         slot = self._slot.pop(key)
         del self._len[key]
+        del self._prompt[key]
         self._free.append(slot)
 
     def download(self, key) -> np.ndarray:
@@ -130,6 +139,10 @@ class DeviceHistories:
             raise RuntimeError(f"history of {key!r} is full ({self.max_len} tokens)")
         return slots * self.max_len + lens
 
+    def output_starts(self, keys: Sequence) -> np.ndarray:
+        """int64 [B]: where in its history each row's outputs begin."""
+        return np.fromiter(map(self._prompt.__getitem__, keys), dtype=np.int64, count=len(keys))
+
     def advance(self, keys: Sequence) -> None:
         for key in keys:
             self._len[key] += 1
@@ -146,7 +159,8 @@ class BatchSampler:
         # SamplingParams objects (so that equal ids mean the same objects)
         self._packed = None
 
-    def sample(self, logits, params, rngs: Sequence | None, keys: Sequence, *, uniforms=None) -> np.ndarray:
+    def sample(self, logits, params, rngs: Sequence | None, keys: Sequence, *, uniforms=None, rules=None, masks=None,
+               mask_rows=None, logprobs: int | None = None):
         """Samples one token per row and appends it to the row's history.
 
         ``logits`` is [B, V] (numpy, or a torch CUDA tensor read in place on
@@ -154,11 +168,30 @@ class BatchSampler:
         row; ``rngs[b]`` row b's Generator (None allowed for greedy rows);
         ``keys[b]`` the sequence of row b, which must be in the histories.
         Returns int64 ids [B].
+
+        ``rules`` (one :class:`pagellm_amd.logits.LogitRules`, or one or None per
+        row) and ``masks`` with ``mask_rows`` (as ``process_logits`` takes them)
+        are applied to a copy of the logits first: biases, then the repetition
+        penalty, then frequency and presence penalties over the row's outputs
+        (``DeviceHistories.add``'s ``prompt_len``), then the mask.  Rows without
+        rules keep the sampler's own repetition penalty, and so their ids,
+        whatever rows stand beside them.  With ``logprobs`` = n the call returns
+        (ids, :class:`pagellm_amd.logits.Logprobs`): the sampled tokens' log
+        probabilities and ranks and the n best tokens under the logits as given.
         """
         c = self.ctx
         B = len(keys)
+        n_top = 0 if logprobs is None else int(logprobs)
+        if not 0 <= n_top <= min(self.hist.V, _native.PLH_MAX_TOP):
+            raise ValueError(f"logprobs must be in [0, {min(self.hist.V, _native.PLH_MAX_TOP)}]")
+        masks, mask_rows = _check_mask(masks, mask_rows, B, self.hist.V, c.device)
+        rules = _expand_rules(rules, B)
+        # refused here, before a Generator moves
+        f, pr, bias_ids, bias, bias_off = _pack_rules(rules, self.hist.V)
+        ruled = np.array([not rule.neutral for rule in rules], dtype=bool)
         if B == 0:
-            return np.zeros(0, dtype=np.int64)
+            ids = np.zeros(0, dtype=np.int64)
+            return ids if logprobs is None else (ids, DeviceLogprobs(c, 0, n_top, np.float32).download())
         if _is_torch_cuda(logits):
             import torch
 
@@ -192,24 +225,51 @@ class BatchSampler:
         else:
             t, k, p, r = _pack_params(params)
             self._packed = (ids, list(params), (t, k, p, r))
+        process = masks is not None or bool(ruled.any())
         # sampling.py:56: only rows whose penalty is active read their history
-        spans, pos = self.hist.spans_and_positions(keys, r != 1.0)
+        # (for rows with rules the processing applies it, ahead of the sampler)
+        own_r = np.where(ruled, 1.0, r) if process else r
+        spans, pos = self.hist.spans_and_positions(keys, own_r != 1.0)
         # every per-row array in one page-locked host buffer, one queued copy
         # to the device (the download of the ids below waits for it)
-        parts = [t, p, r, u, spans, pos, k]
-        offs = np.cumsum([0] + [a.nbytes for a in parts])
+        parts = [t, p, own_r, u, spans, pos, k]
+        if process:
+            rule_spans = self.hist.spans(keys, ruled & ((r != 1.0) | (f != 0.0) | (pr != 0.0)))
+            host = [np.where(ruled, r, 1.0), f, pr, rule_spans, self.hist.output_starts(keys), bias, bias_off,
+                    bias_ids, mask_rows, masks if isinstance(masks, np.ndarray) else None]
+            parts += [a for a in host if a is not None]
+        offs = np.cumsum([0] + [(a.nbytes + 7) & ~7 for a in parts])
         stage = c.pinned("eng_stage", int(offs[-1]))
         for a, o in zip(parts, offs[:-1]):
-            stage[o:o + a.nbytes] = np.ascontiguousarray(a).view(np.uint8)
+            stage[o:o + a.nbytes] = np.ascontiguousarray(a).reshape(-1).view(np.uint8)
         d = c.scratch("eng_stage", (int(offs[-1]),), np.uint8)
         c.h2d_async(d.ptr, stage[:int(offs[-1])])
-        d_t, d_p, d_r, d_u, d_sp, d_pos, d_k = (d.ptr + int(o) for o in offs[:-1])
+        d_t, d_p, d_r, d_u, d_sp, d_pos, d_k = (d.ptr + int(o) for o in offs[:7])
+        given, given_ld = ptr, ld
+        if process:
+            rest = iter(d.ptr + int(o) for o in offs[7:-1])
+            h_r, h_f, h_p, h_sp, h_st, h_b, h_bo, h_bi, h_mr, h_m = (next(rest) if a is not None else None for a in host)
+            mask_ld = n_masks = 0
+            if masks is not None:
+                n_masks, mask_ld = int(masks.shape[0]), int(masks.shape[1])
+                if not isinstance(masks, np.ndarray):
+                    h_m, mask_ld = masks.data_ptr(), int(masks.stride(0)) if n_masks > 1 else mask_ld
+                if n_masks == 0:
+                    h_m = None
+            es = 8 if code == _native.PLH_F64 else 4
+            ld = -(-V * es // 16) * 16 // es
+            work = c.scratch("eng_processed", (B, ld), np.float64 if es == 8 else np.float32)
+            ptr = work.ptr
+            c.process_logits(given, code, given_ld, B, V, self.hist.slab.ptr, h_sp, h_st, h_r, h_f, h_p, h_bi, h_b,
+                             h_bo, h_m, mask_ld, n_masks, h_mr, ptr, ld, _native.PLH_SAMPLE_HIST_SPANS)
         out = c.scratch("eng_out", (B,), np.int32)
         c.sample(ptr, code, ld, B, V, self.hist.slab.ptr, d_sp, d_t, d_k, d_p, d_r, d_u,
                  out.ptr, None, _native.PLH_SAMPLE_HIST_SPANS | _nucleus_hint(t, k, p, V))
         # llm_engine.py:284: the token joins the history, on the device
         c.append_ids(self.hist.slab.ptr, d_pos, out.ptr, B)
+        if logprobs is not None:
+            res = DeviceLogprobs(c, B, n_top, np.float64 if code == _native.PLH_F64 else np.float32)
+            c.logprobs(given, code, given_ld, B, V, out.ptr, *res.pointers())
         ids = out.download().astype(np.int64)
         self.hist.advance(keys)
-        return ids
-
+        return ids if logprobs is None else (ids, res.download())

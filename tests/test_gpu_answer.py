@@ -1,0 +1,97 @@
+"""The way from hidden states to an answer, as a serving loop runs it: e4m3
+logits, rules and grammar masks, sampling, log probabilities, through
+``BatchSampler`` with histories on the device (needs an MI355X)."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import oracle
+from oracle import logits as O
+from pagellm_amd.engine import BatchSampler, DeviceHistories
+from pagellm_amd.fp8 import Fp8LogitsHead
+from pagellm_amd.logits import LogitRules, pack_mask
+from pagellm_amd.params import SamplingParams, make_rng
+
+pytestmark = pytest.mark.gpu
+
+V, D = 3000, 256
+ROWS = [  # (params, rules, prompt length, under a grammar)
+    (SamplingParams(temperature=0.0), None, 5, False),
+    (SamplingParams(temperature=0.0, repetition_penalty=1.3), LogitRules(0.4, 0.2), 9, False),
+    (SamplingParams(temperature=0.8, top_k=20), LogitRules(logit_bias={7: 12.0, 8: -np.inf}), 7, True),
+    (SamplingParams(temperature=1.0, top_p=0.9, repetition_penalty=1.2), None, 12, True),
+    (SamplingParams(temperature=0.0), LogitRules(0.0, 3.0), 3, True),
+]
+
+
+@pytest.mark.parametrize("on_gpu", [True, False])
+def test_steps_match_the_oracle(on_gpu):
+    g = np.random.default_rng(3)
+    norm = (1 + 0.1 * g.standard_normal(D)).astype(np.float32)
+    head = Fp8LogitsHead(norm, (0.1 * g.standard_normal((D, V))).astype(np.float32))
+    hist = DeviceHistories(V, max_seqs=8, max_len=64)
+    sampler = BatchSampler(hist)
+    keys = list("abcde")
+    tokens = {k: [int(t) for t in g.integers(0, V, row[2])] for k, row in zip(keys, ROWS)}
+    for k in keys:
+        hist.add(k, tokens[k])
+    rngs, ref_rngs = ([make_rng(i, 0) for i in range(5)] for _ in range(2))
+    for step in range(6):
+        logits = head(g.standard_normal((5, D)).astype(np.float32))
+        x = logits.cpu().numpy()
+        masks = np.stack([pack_mask(g.random(V) < 0.3, V), pack_mask([5, 7, 8, 11], V)])
+        at = [None, None, 1, 0, 1 if step % 2 else 0]
+        ids, lps = sampler.sample(logits if on_gpu else x, [r[0] for r in ROWS], rngs, keys, rules=[r[1] for r in ROWS],
+                                  masks=masks, mask_rows=at, logprobs=5)
+        assert np.array_equal(logits.cpu().numpy(), x)  # the caller's logits stay as they were
+        for b, (k, (params, rule, plen, _)) in enumerate(zip(keys, ROWS)):
+            rule = rule or LogitRules()
+            ruled = not rule.neutral
+            y = O.process_row(x[b], history=tokens[k], out_start=plen, rep=params.repetition_penalty if ruled else 1.0,
+                              freq=rule.frequency_penalty, pres=rule.presence_penalty,
+                              bias=list(rule.logit_bias.items()), mask=masks[at[b]] if at[b] is not None else None)
+            y = y.astype(np.float32)
+            rest = SamplingParams(temperature=params.temperature, top_k=params.top_k, top_p=params.top_p,
+                                  repetition_penalty=1.0 if ruled else params.repetition_penalty)
+            u = None if params.greedy else ref_rngs[b].random()
+            want = oracle.sample(y, rest, u, tokens[k])
+            assert ids[b] == want, (step, k)
+            order = O.order(x[b])
+            assert lps.rank[b] == 1 + int(np.flatnonzero(order == want)[0])
+            assert np.array_equal(lps.top_ids[b], order[:5])
+            lp = O.logprobs_row(x[b])
+            tol = O.logprobs_error(x[b]) + 2.0 ** -24 * 50
+            assert abs(lps.logprob[b] - lp[want]) <= tol
+            assert np.all(np.abs(lps.top_logprobs[b] - lp[order[:5]]) <= tol)
+            tokens[k].append(int(want))
+            assert np.array_equal(hist.download(k), tokens[k])
+    for a, b in zip(rngs, ref_rngs):
+        assert a.random() == b.random()
+
+
+def test_rows_without_rules_keep_their_ids_and_errors_change_nothing():
+    g = np.random.default_rng(0)
+    x = g.normal(0, 2, (2, V)).astype(np.float32)
+    params = SamplingParams(temperature=1.0, repetition_penalty=1.2, top_p=0.9)
+    ids = []
+    for rules in (None, [None, LogitRules(0.5)]):
+        hist = DeviceHistories(V, max_seqs=2, max_len=8)
+        hist.add(0, [1, 2, 3], prompt_len=1)
+        hist.add(1, [4, 5, 6])
+        sampler = BatchSampler(hist)
+        rngs = [make_rng(1, 0), make_rng(2, 0)]
+        with pytest.raises(IndexError):
+            sampler.sample(x, params, rngs, [0, 1], rules=LogitRules(logit_bias={V: 1.0}))
+        with pytest.raises(ValueError):
+            sampler.sample(x, params, rngs, [0, 1], masks=np.zeros((1, 94), np.uint32))
+        with pytest.raises(ValueError):
+            sampler.sample(x, params, rngs, [0, 1], logprobs=65)
+        ids.append(sampler.sample(x, params, rngs, [0, 1], rules=rules))
+        assert list(hist.output_starts([0, 1])) == [1, 3]
+    assert ids[0][0] == ids[1][0]
+    with pytest.raises(ValueError):
+        hist.remove(0)
+        hist.add(0, [1, 2], prompt_len=3)
+    assert sampler.sample(x[:0], [], [], [], logprobs=2)[1].top_ids.shape == (0, 2)

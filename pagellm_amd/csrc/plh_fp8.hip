@@ -4,7 +4,7 @@
 //
 //   k_fp8_act       rows -> RMSNorm -> rounded to e4m3 by blocks -> bf16
 //   k_fp8_skinny    at most 32 rows: bound by one read of the codes
-//   k_fp8_tiles     more rows
+//   k_fp8_tiles     more rows (k_fp8_sum: where k is cut into slices)
 //   k_fp8_pack, k_fp8_quantize   the weights' layout, once
 //
 // The products run on the bf16 matrix cores.  The 8-bit ones align a sum's
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(kThreads) void k_fp8_skinny(Fp8Args a) {
   using M = Mma<R>;
   constexpr int kVT = kSkinnyCols / R, kRegs = R * R / 64, kQuads = kVT * kRegs / 4;
   __shared__ f32x4 sm[kWaves][kQuads][kWave];
-  const int v0 = blockIdx.x * kSkinnyCols, nt = blockIdx.y;
+  const int v0 = blockIdx.x * kSkinnyCols;
   typename M::Acc acc[kVT];
 #pragma unroll
   for (int i = 0; i < kVT; ++i) acc[i] = typename M::Acc{};
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(kThreads) void k_fp8_skinny(Fp8Args a) {
     const int v = min(v0 + i * R, tiles_of(a.V) * kTileRows - R);
     w[i] = a.codes + (size_t)(v / kTileRows) * a.kb * kTileBytes + (v % kTileRows) * 16;
   }
-  const u32x4* act = reinterpret_cast<const u32x4*>(a.act) + (size_t)nt * a.kb * (R * 16) + lane();
+  const u32x4* act = reinterpret_cast<const u32x4*>(a.act) + lane();
   const float* ts = a.scales + (size_t)(v0 / kBlock) * a.kb;
   for (int b = wave(); b < a.kb; b += kWaves) {
     u32x4 x[M::kSteps], c[kVT][M::kPieces];
@@ -279,8 +279,128 @@ __global__ __launch_bounds__(kThreads) void k_fp8_skinny(Fp8Args a) {
     f32x4 t = sm[0][u][lane()];
 #pragma unroll
     for (int k = 1; k < kWaves; ++k) t += sm[k][u][lane()];
-    store4(a, nt * R + lane() % R, v0 + u / (kRegs / 4) * R + M::row(u % (kRegs / 4)), t);
+    store4(a, lane() % R, v0 + u / (kRegs / 4) * R + M::row(u % (kRegs / 4)), t);
   }
+}
+
+// -------------------------------------------------------------- more rows
+
+// The tile of a workgroup: workgroups of one XCD (every eighth) get one
+// contiguous range of tiles, so that they share codes and activations in its L2;
+// in that order kGroup row tiles run under one column tile, then the next.
+constexpr int kXcds = 8, kGroup = 8;
+__device__ __forceinline__ void tile_of_group(int vtiles, int ntiles, int& vt, int& nt) {
+  const int total = vtiles * ntiles, x = blockIdx.x % kXcds, slot = blockIdx.x / kXcds;
+  const int idx = x * (total / kXcds) + min(x, total % kXcds) + slot;
+  const int g = idx / (kGroup * vtiles), in = idx % (kGroup * vtiles), rows = min(kGroup, ntiles - g * kGroup);
+  vt = in / rows;
+  nt = g * kGroup + in % rows;
+}
+
+// A workgroup's 8 waves lie WN along the rows; each forms VI x 2 tiles of 32
+// columns x 32 rows.  Codes go from memory into registers, one block ahead,
+// activations through LDS, double-buffered, staged in registers one block ahead:
+// a wave reads 64 rows' activations from LDS for VI * 32 columns, and only the WN
+// waves side by side widen the same codes.  Block sums are their own registers, so
+// that a block's scale meets its sum: as many again as the accumulators, which
+// keeps a wave's tile at 64 x 64.
+template <int VI, int WN>
+struct Tiles {
+  static constexpr int kCols = kWaves / WN * VI * 32;  // of a workgroup
+  static constexpr int kRows = WN * 64;
+  static constexpr int kStage = kRows / 32;            // 32-row tiles of activations in LDS
+};
+
+template <int VI, int WN>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(VI == 2 ? 2 : 4, VI == 2 ? 2 : 4))) void
+k_fp8_tiles(Fp8Args a) {
+  using G = Tiles<VI, WN>;
+  using M = Mma<32>;
+  constexpr int kUnit = kTileRows * 16;  // 16-byte units of a tile of activations and block
+  __shared__ u32x4 sm[2][G::kStage * kUnit];
+  int vt, nt;
+  tile_of_group(tiles_of(a.V, G::kCols), tiles_of(a.N, G::kRows), vt, nt);
+  const int w = uniform(wave()), l = lane();
+  const int v0 = vt * G::kCols + w / WN * (VI * 32), n0 = nt * G::kRows, nw = w % WN * 64;
+  const int b0 = (int)((int64_t)a.kb * blockIdx.z / gridDim.z), b1 = (int)((int64_t)a.kb * (blockIdx.z + 1) / gridDim.z);
+  // tiles past the last read as the last, and are not stored
+  const uint8_t* codes[VI];
+#pragma unroll
+  for (int i = 0; i < VI; ++i)
+    codes[i] = a.codes + (size_t)min(v0 / kTileRows + i, tiles_of(a.V) - 1) * a.kb * kTileBytes;
+  const u32x4* act[G::kStage];
+#pragma unroll
+  for (int r = 0; r < G::kStage; ++r)
+    act[r] = reinterpret_cast<const u32x4*>(a.act) +
+             (size_t)min(n0 / kTileRows + r, tiles_of(a.N) - 1) * a.kb * kUnit + threadIdx.x;
+  const float* ts = a.scales + (size_t)min(v0 / kBlock, blocks_of(a.V) - 1) * a.kb;
+
+  u32x4 c[VI][M::kPieces], st[G::kStage];
+  f32x16 acc[VI][2];
+#pragma unroll
+  for (int i = 0; i < VI; ++i) {
+    acc[i][0] = f32x16{};
+    acc[i][1] = f32x16{};
+#pragma unroll
+    for (int q = 0; q < M::kPieces; ++q)
+      c[i][q] = *reinterpret_cast<const u32x4*>(codes[i] + (size_t)b0 * kTileBytes + M::piece(q));
+  }
+#pragma unroll
+  for (int r = 0; r < G::kStage; ++r) sm[0][r * kUnit + (int)threadIdx.x] = act[r][(size_t)b0 * kUnit];
+  wg_barrier();
+  for (int b = b0; b < b1; ++b) {
+    const int buf = (b - b0) & 1, next = min(b + 1, b1 - 1);
+    const float t = ts[b];
+#pragma unroll
+    for (int r = 0; r < G::kStage; ++r) st[r] = act[r][(size_t)next * kUnit];
+    f32x16 p[VI][2];
+#pragma unroll
+    for (int i = 0; i < VI; ++i) p[i][0] = f32x16{}, p[i][1] = f32x16{};
+#pragma unroll
+    for (int s = 0; s < M::kSteps; ++s) {
+      bf16x8 x[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) x[j] = as_bf16(sm[buf][(nw / 32 + j) * kUnit + s * kWave + l]);
+#pragma unroll
+      for (int i = 0; i < VI; ++i) {
+        const bf16x8 wt = widen8(c[i][s / 2][s % 2 * 2], c[i][s / 2][s % 2 * 2 + 1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) p[i][j] = M::mma(wt, x[j], p[i][j]);
+        if (s % 2 == 1)
+          c[i][s / 2] = *reinterpret_cast<const u32x4*>(codes[i] + (size_t)next * kTileBytes + M::piece(s / 2));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VI; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(p[i][j][e], t, acc[i][j][e]);
+#pragma unroll
+    for (int r = 0; r < G::kStage; ++r) sm[buf ^ 1][r * kUnit + (int)threadIdx.x] = st[r];
+    wg_barrier();
+  }
+  if (gridDim.z > 1) {
+    a.out = a.part + (size_t)blockIdx.z * a.N * a.V;
+    a.ldo = a.V;
+  }
+#pragma unroll
+  for (int i = 0; i < VI; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        store4(a, n0 + nw + 32 * j + l % 32, v0 + 32 * i + M::row(g),
+               f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]});
+}
+
+// The slices' partial sums, in order.
+__global__ __launch_bounds__(256) void k_fp8_sum(Fp8Args a, int slices) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)a.N * a.V;
+  if (i >= n) return;
+  float t = a.part[i];
+  for (int z = 1; z < slices; ++z) t += a.part[z * n + i];
+  a.out[i / a.V * a.ldo + i % a.V] = t;
 }
 
 // ---------------------------------------------------------------- weights
@@ -354,9 +474,35 @@ hipError_t launch_act(const Fp8Args& a, int dtype, hipStream_t s) {
 }
 }  // namespace
 
-size_t fp8_ws_bytes(int N, int V, int D, int num_cu) {
+namespace {
+size_t act_bytes(int N, int D) {
   const int R = rows_of(N);
   return (size_t)tiles_of(N, R) * R * blocks_of(D) * kBlock * 2;
+}
+
+// How a product of more than 32 rows runs: 64 or 128 rows a workgroup, and the
+// slices that k is cut into where the tiles do not fill the chip.
+struct Plan {
+  bool wide;
+  int tiles, slices;
+};
+
+Plan plan_of(int N, int V, int D, int num_cu) {
+  Plan p;
+  p.wide = N > 64;
+  const int64_t t = p.wide ? (int64_t)tiles_of(V, Tiles<2, 2>::kCols) * tiles_of(N, Tiles<2, 2>::kRows)
+                           : (int64_t)tiles_of(V, Tiles<1, 1>::kCols) * tiles_of(N, Tiles<1, 1>::kRows);
+  p.tiles = (int)t;
+  // at least four blocks a slice
+  p.slices = (int)std::max<int64_t>(1, std::min<int64_t>({num_cu / t, blocks_of(D) / 4, 16}));
+  return p;
+}
+}  // namespace
+
+size_t fp8_ws_bytes(int N, int V, int D, int num_cu) {
+  if (N <= 32) return act_bytes(N, D);
+  const Plan p = plan_of(N, V, D, num_cu);
+  return act_bytes(N, D) + (p.slices > 1 ? (size_t)p.slices * N * V * sizeof(float) : 0);
 }
 
 hipError_t launch_fp8_pack(const uint8_t* codes, int64_t ldc, const float* scales, int64_t lds, int V, int D,
@@ -388,21 +534,21 @@ hipError_t launch_fp8_linear(Fp8Args a, int dtype, void* ws, int num_cu, hipStre
   const int R = rows_of(a.N);
   hipError_t e = R == 16 ? launch_act<16>(a, dtype, s) : launch_act<32>(a, dtype, s);
   if (e != hipSuccess) return e;
-  const unsigned gx = (a.V + kSkinnyCols - 1) / kSkinnyCols;
-  // the grid's y holds 65 535 row tiles
-  const int step = 65535 * R;
-  for (int64_t n0 = 0; n0 < a.N; n0 += step) {
-    Fp8Args c = a;
-    c.N = (int)std::min<int64_t>(step, a.N - n0);
-    c.out = a.out + n0 * a.ldo;
-    c.act = a.act + n0 / R * a.kb * (R * 16);
-    const dim3 grid(gx, tiles_of(c.N, R));
-    if (R == 16) hipLaunchKernelGGL((k_fp8_skinny<16>), grid, dim3(kThreads), 0, s, c);
-    else hipLaunchKernelGGL((k_fp8_skinny<32>), grid, dim3(kThreads), 0, s, c);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
+  if (a.N <= 32) {
+    const dim3 grid((a.V + kSkinnyCols - 1) / kSkinnyCols);
+    if (R == 16) hipLaunchKernelGGL((k_fp8_skinny<16>), grid, dim3(kThreads), 0, s, a);
+    else hipLaunchKernelGGL((k_fp8_skinny<32>), grid, dim3(kThreads), 0, s, a);
+    return hipGetLastError();
   }
-  return hipSuccess;
+  const Plan p = plan_of(a.N, a.V, a.D, num_cu);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + act_bytes(a.N, a.D));
+  const dim3 grid(p.tiles, 1, p.slices);
+  if (p.wide) hipLaunchKernelGGL((k_fp8_tiles<2, 2>), grid, dim3(kThreads), 0, s, a);
+  else hipLaunchKernelGGL((k_fp8_tiles<1, 1>), grid, dim3(kThreads), 0, s, a);
+  e = hipGetLastError();
+  if (e != hipSuccess || p.slices == 1) return e;
+  hipLaunchKernelGGL(k_fp8_sum, dim3((unsigned)(((int64_t)a.N * a.V + 255) / 256)), dim3(256), 0, s, a, p.slices);
+  return hipGetLastError();
 }
 
 }  // namespace plh

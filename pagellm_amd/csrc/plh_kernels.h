@@ -200,6 +200,7 @@ struct Fp8Args {
   float* out;          // [N, ldo]
   int64_t ldo;
   uint4* act;          // workspace: the rows, rounded, as bf16 in the product's operand layout
+  float* part;         // workspace: [slices, N, V] partial sums, with several slices of k
   int N, D, V;
   int kb;              // blocks of 128 in a row: ceil(D / 128)
 };

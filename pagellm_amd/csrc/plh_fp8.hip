@@ -336,11 +336,11 @@ k_fp8_tiles(Fp8Args a) {
   const float* ts = a.scales + (size_t)min(v0 / kBlock, blocks_of(a.V) - 1) * a.kb;
 
   u32x4 c[VI][M::kPieces], st[G::kStage];
-  f32x16 acc[VI][2];
+  f32x16 acc[VI][2], p[VI][2];
 #pragma unroll
   for (int i = 0; i < VI; ++i) {
-    acc[i][0] = f32x16{};
-    acc[i][1] = f32x16{};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{}, p[i][j] = f32x16{};
 #pragma unroll
     for (int q = 0; q < M::kPieces; ++q)
       c[i][q] = *reinterpret_cast<const u32x4*>(codes[i] + (size_t)b0 * kTileBytes + M::piece(q));
@@ -348,38 +348,60 @@ k_fp8_tiles(Fp8Args a) {
 #pragma unroll
   for (int r = 0; r < G::kStage; ++r) sm[0][r * kUnit + (int)threadIdx.x] = act[r][(size_t)b0 * kUnit];
   wg_barrier();
+  float t = 0.0f;  // the scale of the block before
   for (int b = b0; b < b1; ++b) {
     const int buf = (b - b0) & 1, next = min(b + 1, b1 - 1);
-    const float t = ts[b];
+    const float tb = ts[b];
 #pragma unroll
     for (int r = 0; r < G::kStage; ++r) st[r] = act[r][(size_t)next * kUnit];
-    f32x16 p[VI][2];
+    const u32x4* xs = &sm[buf][nw / 32 * kUnit + l];
+    bf16x8 x[2][2], wt[2][VI];
 #pragma unroll
-    for (int i = 0; i < VI; ++i) p[i][0] = f32x16{}, p[i][1] = f32x16{};
+    for (int j = 0; j < 2; ++j) x[0][j] = as_bf16(xs[j * kUnit]);
+#pragma unroll
+    for (int i = 0; i < VI; ++i) wt[0][i] = widen8(c[i][0][0], c[i][0][1]);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int s = 0; s < M::kSteps; ++s) {
-      bf16x8 x[2];
+      // the next step's operands, and the next block's codes into registers that
+      // have been widened
+      const int n = s + 1;
+      if (n < M::kSteps) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) x[j] = as_bf16(sm[buf][(nw / 32 + j) * kUnit + s * kWave + l]);
+        for (int j = 0; j < 2; ++j) x[n & 1][j] = as_bf16(xs[j * kUnit + n * kWave]);
 #pragma unroll
-      for (int i = 0; i < VI; ++i) {
-        const bf16x8 wt = widen8(c[i][s / 2][s % 2 * 2], c[i][s / 2][s % 2 * 2 + 1]);
+        for (int i = 0; i < VI; ++i) wt[n & 1][i] = widen8(c[i][n / 2][n % 2 * 2], c[i][n / 2][n % 2 * 2 + 1]);
+      }
+      if (s % 2 == 1) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) p[i][j] = M::mma(wt, x[j], p[i][j]);
-        if (s % 2 == 1)
+        for (int i = 0; i < VI; ++i)
           c[i][s / 2] = *reinterpret_cast<const u32x4*>(codes[i] + (size_t)next * kTileBytes + M::piece(s / 2));
       }
+#pragma unroll
+      for (int i = 0; i < VI; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (s == 0) {
+            // the block before meets its scale among this one's first products
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(p[i][j][e], t, acc[i][j][e]);
+            p[i][j] = f32x16{};
+          }
+          p[i][j] = M::mma(wt[s & 1][i], x[s & 1][j], p[i][j]);
+        }
+      __builtin_amdgcn_sched_barrier(0);
     }
-#pragma unroll
-    for (int i = 0; i < VI; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(p[i][j][e], t, acc[i][j][e]);
+    t = tb;
 #pragma unroll
     for (int r = 0; r < G::kStage; ++r) sm[buf ^ 1][r * kUnit + (int)threadIdx.x] = st[r];
     wg_barrier();
   }
+#pragma unroll
+  for (int i = 0; i < VI; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(p[i][j][e], t, acc[i][j][e]);
   if (gridDim.z > 1) {
     a.out = a.part + (size_t)blockIdx.z * a.N * a.V;
     a.ldo = a.V;

@@ -289,6 +289,8 @@ __global__ __launch_bounds__(kThreads) void k_fp8_skinny(Fp8Args a) {
 // contiguous range of tiles, so that they share codes and activations in its L2;
 // in that order kGroup row tiles run under one column tile, then the next.
 constexpr int kXcds = 8, kGroup = 8;
+// instruction classes of __builtin_amdgcn_sched_group_barrier
+constexpr int kVector = 0x002, kMatrix = 0x008, kDsRead = 0x100;
 __device__ __forceinline__ void tile_of_group(int vtiles, int ntiles, int& vt, int& nt) {
   const int total = vtiles * ntiles, x = blockIdx.x % kXcds, slot = blockIdx.x / kXcds;
   const int idx = x * (total / kXcds) + min(x, total % kXcds) + slot;
@@ -304,19 +306,21 @@ __device__ __forceinline__ void tile_of_group(int vtiles, int ntiles, int& vt, i
 // waves side by side widen the same codes.  Block sums are their own registers, so
 // that a block's scale meets its sum: as many again as the accumulators, which
 // keeps a wave's tile at 64 x 64.
-template <int VI, int WN>
+template <int VI, int WN, int NW>
 struct Tiles {
-  static constexpr int kCols = kWaves / WN * VI * 32;  // of a workgroup
+  static constexpr int kCols = NW / WN * VI * 32;  // of a workgroup
   static constexpr int kRows = WN * 64;
-  static constexpr int kStage = kRows / 32;            // 32-row tiles of activations in LDS
+  static constexpr int kStage = kRows / 32;        // 32-row tiles of activations in LDS
+  static constexpr int kUnit = kTileRows * 16;     // 16-byte units of such a tile and block
+  static constexpr int kLoads = kStage * kUnit / (NW * kWave);  // of a thread
 };
 
-template <int VI, int WN>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(VI == 2 ? 2 : 4, VI == 2 ? 2 : 4))) void
+template <int VI, int WN, int NW>
+__global__ __launch_bounds__(NW * kWave) __attribute__((amdgpu_waves_per_eu(VI == 2 ? 2 : 4, VI == 2 ? 2 : 4))) void
 k_fp8_tiles(Fp8Args a) {
-  using G = Tiles<VI, WN>;
+  using G = Tiles<VI, WN, NW>;
   using M = Mma<32>;
-  constexpr int kUnit = kTileRows * 16;  // 16-byte units of a tile of activations and block
+  constexpr int kUnit = G::kUnit, kN = NW * kWave;
   __shared__ u32x4 sm[2][G::kStage * kUnit];
   int vt, nt;
   tile_of_group(tiles_of(a.V, G::kCols), tiles_of(a.N, G::kRows), vt, nt);
@@ -328,14 +332,16 @@ k_fp8_tiles(Fp8Args a) {
 #pragma unroll
   for (int i = 0; i < VI; ++i)
     codes[i] = a.codes + (size_t)min(v0 / kTileRows + i, tiles_of(a.V) - 1) * a.kb * kTileBytes;
-  const u32x4* act[G::kStage];
+  const u32x4* act[G::kLoads];
 #pragma unroll
-  for (int r = 0; r < G::kStage; ++r)
+  for (int r = 0; r < G::kLoads; ++r) {
+    const int at = r * kN + (int)threadIdx.x;
     act[r] = reinterpret_cast<const u32x4*>(a.act) +
-             (size_t)min(n0 / kTileRows + r, tiles_of(a.N) - 1) * a.kb * kUnit + threadIdx.x;
+             (size_t)min(n0 / kTileRows + at / kUnit, tiles_of(a.N) - 1) * a.kb * kUnit + at % kUnit;
+  }
   const float* ts = a.scales + (size_t)min(v0 / kBlock, blocks_of(a.V) - 1) * a.kb;
 
-  u32x4 c[VI][M::kPieces], st[G::kStage];
+  u32x4 c[VI][M::kPieces], st[G::kLoads];
   f32x16 acc[VI][2], p[VI][2];
 #pragma unroll
   for (int i = 0; i < VI; ++i) {
@@ -346,21 +352,20 @@ k_fp8_tiles(Fp8Args a) {
       c[i][q] = *reinterpret_cast<const u32x4*>(codes[i] + (size_t)b0 * kTileBytes + M::piece(q));
   }
 #pragma unroll
-  for (int r = 0; r < G::kStage; ++r) sm[0][r * kUnit + (int)threadIdx.x] = act[r][(size_t)b0 * kUnit];
+  for (int r = 0; r < G::kLoads; ++r) sm[0][r * kN + (int)threadIdx.x] = act[r][(size_t)b0 * kUnit];
   wg_barrier();
   float t = 0.0f;  // the scale of the block before
   for (int b = b0; b < b1; ++b) {
     const int buf = (b - b0) & 1, next = min(b + 1, b1 - 1);
     const float tb = ts[b];
 #pragma unroll
-    for (int r = 0; r < G::kStage; ++r) st[r] = act[r][(size_t)next * kUnit];
+    for (int r = 0; r < G::kLoads; ++r) st[r] = act[r][(size_t)next * kUnit];
     const u32x4* xs = &sm[buf][nw / 32 * kUnit + l];
     bf16x8 x[2][2], wt[2][VI];
 #pragma unroll
     for (int j = 0; j < 2; ++j) x[0][j] = as_bf16(xs[j * kUnit]);
 #pragma unroll
     for (int i = 0; i < VI; ++i) wt[0][i] = widen8(c[i][0][0], c[i][0][1]);
-    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int s = 0; s < M::kSteps; ++s) {
       // the next step's operands, and the next block's codes into registers that
@@ -389,11 +394,21 @@ k_fp8_tiles(Fp8Args a) {
           }
           p[i][j] = M::mma(wt[s & 1][i], x[s & 1][j], p[i][j]);
         }
+      // LDS reads first, then the vector instructions among the products
+      if (s == 0) __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
+      else if (n < M::kSteps) __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
+#pragma unroll
+      for (int m = 0; m < 2 * VI; ++m) {
+        if (s == 0 && m == 0) __builtin_amdgcn_sched_group_barrier(kVector, 16 + 4 * VI, 0);
+        else if (s == 0) __builtin_amdgcn_sched_group_barrier(kVector, 16, 0);
+        __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+        if (n < M::kSteps) __builtin_amdgcn_sched_group_barrier(kVector, 2, 0);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     t = tb;
 #pragma unroll
-    for (int r = 0; r < G::kStage; ++r) sm[buf ^ 1][r * kUnit + (int)threadIdx.x] = st[r];
+    for (int r = 0; r < G::kLoads; ++r) sm[buf ^ 1][r * kN + (int)threadIdx.x] = st[r];
     wg_barrier();
   }
 #pragma unroll
@@ -504,6 +519,8 @@ size_t act_bytes(int N, int D) {
 
 // How a product of more than 32 rows runs: 64 or 128 rows a workgroup, and the
 // slices that k is cut into where the tiles do not fill the chip.
+using WideTiles = Tiles<2, 2, 8>;
+using NarrowTiles = Tiles<1, 1, 8>;
 struct Plan {
   bool wide;
   int tiles, slices;
@@ -512,8 +529,8 @@ struct Plan {
 Plan plan_of(int N, int V, int D, int num_cu) {
   Plan p;
   p.wide = N > 64;
-  const int64_t t = p.wide ? (int64_t)tiles_of(V, Tiles<2, 2>::kCols) * tiles_of(N, Tiles<2, 2>::kRows)
-                           : (int64_t)tiles_of(V, Tiles<1, 1>::kCols) * tiles_of(N, Tiles<1, 1>::kRows);
+  const int64_t t = p.wide ? (int64_t)tiles_of(V, WideTiles::kCols) * tiles_of(N, WideTiles::kRows)
+                           : (int64_t)tiles_of(V, NarrowTiles::kCols) * tiles_of(N, NarrowTiles::kRows);
   p.tiles = (int)t;
   // at least four blocks a slice
   p.slices = (int)std::max<int64_t>(1, std::min<int64_t>({num_cu / t, blocks_of(D) / 4, 16}));
@@ -565,8 +582,8 @@ hipError_t launch_fp8_linear(Fp8Args a, int dtype, void* ws, int num_cu, hipStre
   const Plan p = plan_of(a.N, a.V, a.D, num_cu);
   a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + act_bytes(a.N, a.D));
   const dim3 grid(p.tiles, 1, p.slices);
-  if (p.wide) hipLaunchKernelGGL((k_fp8_tiles<2, 2>), grid, dim3(kThreads), 0, s, a);
-  else hipLaunchKernelGGL((k_fp8_tiles<1, 1>), grid, dim3(kThreads), 0, s, a);
+  if (p.wide) hipLaunchKernelGGL((k_fp8_tiles<2, 2, 8>), grid, dim3(kThreads), 0, s, a);
+  else hipLaunchKernelGGL((k_fp8_tiles<1, 1, 8>), grid, dim3(kThreads), 0, s, a);
   e = hipGetLastError();
   if (e != hipSuccess || p.slices == 1) return e;
   hipLaunchKernelGGL(k_fp8_sum, dim3((unsigned)(((int64_t)a.N * a.V + 255) / 256)), dim3(256), 0, s, a, p.slices);

@@ -313,6 +313,7 @@ struct Tiles {
   static constexpr int kStage = kRows / 32;        // 32-row tiles of activations in LDS
   static constexpr int kUnit = kTileRows * 16;     // 16-byte units of such a tile and block
   static constexpr int kLoads = kStage * kUnit / (NW * kWave);  // of a thread
+  static_assert(kLoads <= Mma<32>::kSteps / 2, "a step of every two stores one");
 };
 
 template <int VI, int WN, int NW>
@@ -321,7 +322,7 @@ k_fp8_tiles(Fp8Args a) {
   using G = Tiles<VI, WN, NW>;
   using M = Mma<32>;
   constexpr int kUnit = G::kUnit, kN = NW * kWave;
-  __shared__ u32x4 sm[2][G::kStage * kUnit];
+  __shared__ u32x4 sm[3][G::kStage * kUnit];
   int vt, nt;
   tile_of_group(tiles_of(a.V, G::kCols), tiles_of(a.N, G::kRows), vt, nt);
   const int w = uniform(wave()), l = lane();
@@ -351,36 +352,46 @@ k_fp8_tiles(Fp8Args a) {
     for (int q = 0; q < M::kPieces; ++q)
       c[i][q] = *reinterpret_cast<const u32x4*>(codes[i] + (size_t)b0 * kTileBytes + M::piece(q));
   }
+  // activations of block b in buffer (b - b0) % 3: two blocks ahead when the loop
+  // is at one, and a third in registers
+  auto load = [&](int b, int r) { return act[r][(size_t)min(b, b1 - 1) * kUnit]; };
 #pragma unroll
-  for (int r = 0; r < G::kLoads; ++r) sm[0][r * kN + (int)threadIdx.x] = act[r][(size_t)b0 * kUnit];
+  for (int r = 0; r < G::kLoads; ++r) sm[0][r * kN + (int)threadIdx.x] = load(b0, r);
+#pragma unroll
+  for (int r = 0; r < G::kLoads; ++r) sm[1][r * kN + (int)threadIdx.x] = load(b0 + 1, r);
+#pragma unroll
+  for (int r = 0; r < G::kLoads; ++r) st[r] = load(b0 + 2, r);
   wg_barrier();
+  const int x0 = nw / 32 * kUnit + l;
   float t = 0.0f;  // the scale of the block before
+  bf16x8 x[2][2], wt[2][VI];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) x[0][j] = as_bf16(sm[0][x0 + j * kUnit]);
+#pragma unroll
+  for (int i = 0; i < VI; ++i) wt[0][i] = widen8(c[i][0][0], c[i][0][1]);
+  int at = 0;  // this block's buffer
   for (int b = b0; b < b1; ++b) {
-    const int buf = (b - b0) & 1, next = min(b + 1, b1 - 1);
+    const int next = min(b + 1, b1 - 1), after = at == 2 ? 0 : at + 1, last = at == 0 ? 2 : at - 1;
     const float tb = ts[b];
-#pragma unroll
-    for (int r = 0; r < G::kLoads; ++r) st[r] = act[r][(size_t)next * kUnit];
-    const u32x4* xs = &sm[buf][nw / 32 * kUnit + l];
-    bf16x8 x[2][2], wt[2][VI];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) x[0][j] = as_bf16(xs[j * kUnit]);
-#pragma unroll
-    for (int i = 0; i < VI; ++i) wt[0][i] = widen8(c[i][0][0], c[i][0][1]);
 #pragma unroll
     for (int s = 0; s < M::kSteps; ++s) {
       // the next step's operands, and the next block's codes into registers that
       // have been widened
-      const int n = s + 1;
-      if (n < M::kSteps) {
+      const int n = (s + 1) % M::kSteps;
+      const u32x4* xs = &sm[n == 0 ? after : at][x0 + n * kWave];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) x[n & 1][j] = as_bf16(xs[j * kUnit + n * kWave]);
+      for (int j = 0; j < 2; ++j) x[n & 1][j] = as_bf16(xs[j * kUnit]);
 #pragma unroll
-        for (int i = 0; i < VI; ++i) wt[n & 1][i] = widen8(c[i][n / 2][n % 2 * 2], c[i][n / 2][n % 2 * 2 + 1]);
-      }
-      if (s % 2 == 1) {
+      for (int i = 0; i < VI; ++i) wt[n & 1][i] = widen8(c[i][n / 2][n % 2 * 2], c[i][n / 2][n % 2 * 2 + 1]);
+      if (s % 2 == 0) {
 #pragma unroll
         for (int i = 0; i < VI; ++i)
           c[i][s / 2] = *reinterpret_cast<const u32x4*>(codes[i] + (size_t)next * kTileBytes + M::piece(s / 2));
+      }
+      // the block two ahead into the buffer that was read last
+      if (s % 2 == 1 && s / 2 < G::kLoads) {
+        sm[last][s / 2 * kN + (int)threadIdx.x] = st[s / 2];
+        st[s / 2] = load(b + 3, s / 2);
       }
 #pragma unroll
       for (int i = 0; i < VI; ++i)
@@ -395,20 +406,17 @@ k_fp8_tiles(Fp8Args a) {
           p[i][j] = M::mma(wt[s & 1][i], x[s & 1][j], p[i][j]);
         }
       // LDS reads first, then the vector instructions among the products
-      if (s == 0) __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
-      else if (n < M::kSteps) __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
 #pragma unroll
       for (int m = 0; m < 2 * VI; ++m) {
-        if (s == 0 && m == 0) __builtin_amdgcn_sched_group_barrier(kVector, 16 + 4 * VI, 0);
-        else if (s == 0) __builtin_amdgcn_sched_group_barrier(kVector, 16, 0);
+        if (s == 0) __builtin_amdgcn_sched_group_barrier(kVector, 16, 0);
         __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
-        if (n < M::kSteps) __builtin_amdgcn_sched_group_barrier(kVector, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kVector, 2, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
     t = tb;
-#pragma unroll
-    for (int r = 0; r < G::kLoads; ++r) sm[buf ^ 1][r * kN + (int)threadIdx.x] = st[r];
+    at = after;
     wg_barrier();
   }
 #pragma unroll

@@ -429,14 +429,29 @@ k_fp8_tiles(Fp8Args a) {
     a.out = a.part + (size_t)blockIdx.z * a.N * a.V;
     a.ldo = a.V;
   }
+  // 32 rows at a time through the wave's part of LDS (the last barrier has
+  // passed: nobody reads activations there), so that a store writes whole runs of
+  // the logits' rows
+  constexpr int kRun4 = VI * 8, kPitch = kRun4 + 1;  // 16-byte units of a row, and its pitch
+  u32x4* own = &sm[0][0] + w * 32 * kPitch;
+  static_assert(NW * 32 * kPitch <= 3 * G::kStage * kUnit, "the waves' parts lie in LDS");
 #pragma unroll
-  for (int i = 0; i < VI; ++i)
+  for (int j = 0; j < 2; ++j) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int i = 0; i < VI; ++i)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        store4(a, n0 + nw + 32 * j + l % 32, v0 + 32 * i + M::row(g),
-               f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]});
+        own[l % 32 * kPitch + 8 * i + M::row(g) / 4] = __builtin_bit_cast(
+            u32x4, f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]});
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < 32 * kRun4 / kWave; ++r) {
+      const int at = r * kWave + l;
+      store4(a, n0 + nw + 32 * j + at / kRun4, v0 + at % kRun4 * 4,
+             __builtin_bit_cast(f32x4, own[at / kRun4 * kPitch + at % kRun4]));
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
 }
 
 // The slices' partial sums, in order.

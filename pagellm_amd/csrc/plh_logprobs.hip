@@ -3,7 +3,7 @@
 // and the n best tokens.
 //
 // One pass over the logits.  A workgroup walks one segment of a row in chunks of
-// kLpChunk tokens, the next chunk's loads in flight while it works on one.  In
+// 32 KB (8192 float32 tokens), the next chunk's loads in flight while it works on one.  In
 // the walk every thread keeps its own running maximum and (float64) sum, and
 // every wave its own list of candidates for the n best with a threshold that n
 // tokens of the list reach, so that the walk has no barrier: a chunk of a wave
@@ -18,7 +18,7 @@
 // -inf).  All counts are integers and all sums have a fixed order.
 //
 // Bound by the read of the logits.
-#include "plh_device.h"
+#include "plh_fast.h"
 #include "plh_kernels.h"
 
 #include <algorithm>
@@ -27,8 +27,11 @@ namespace plh {
 
 namespace {
 
-constexpr int kLpChunk = 8192;
-constexpr int kVals = kLpChunk / kThreads;  // tokens of a chunk per thread, in groups of four
+// Tokens of a chunk per thread, in groups of four: 64 bytes.
+template <typename T>
+constexpr int kValsOf = 64 / sizeof(T);
+template <typename T>
+constexpr int kChunkOf = kValsOf<T> * kThreads;
 constexpr int kList = 256;                  // candidate slots of a wave
 constexpr int kMergeList = 1024;            // candidates that the second launch ranks in LDS
 
@@ -57,31 +60,58 @@ struct Order<double> {
   static __device__ __forceinline__ double value(K k) { return k == ~0ull ? (double)NAN : val_of_key(k); }
 };
 
-__device__ __forceinline__ double exp_term(float d) {
+// exp(d) for d <= 0 as a term of a row's sum; NaN for what is not (a NaN, or
+// inf - inf).
+__device__ __forceinline__ double exp_term(float d, const double*) {
   return (double)__builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
 }
-__device__ __forceinline__ double exp_term(double d) { return exp(d); }
+__device__ __forceinline__ double exp_term(double d, const double* tab) {
+  return d <= 0.0 ? exp_neg_term(d, tab) : (double)NAN;
+}
+
+// The factor that takes a sum from the maximum m to M >= m.
+__device__ __forceinline__ double rescale(double m, double M, const double* tab) {
+  return m < M ? exp_neg_term(m - M, tab) : 1.0;
+}
 
 template <typename K>
 __device__ __forceinline__ bool before(K ka, int ia, K kb, int ib) {
   return ka > kb || (ka == kb && ia < ib);
 }
 
-// The largest t that at least n of the wave's keys reach (n of them do), or some
-// t that exactly n reach.
-template <typename T, int R>
-__device__ __forceinline__ typename Order<T>::K nth_key(const typename Order<T>::K (&k)[R], int n) {
-  typedef typename Order<T>::K K;
-  K t = 0;
-  for (int b = Order<T>::kBits - 1; b >= 0; --b) {
-    const K trial = t | ((K)1 << b);
-    int c = 0;
+template <typename K, int R>
+__device__ __forceinline__ int count_ge(const K (&k)[R], K t) {
+  int c = 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r) c += __popcll(__ballot(k[r] >= trial));
-    if (c >= n) t = trial;
-    if (c == n) break;
+  for (int r = 0; r < R; ++r) c += __popcll(__ballot(k[r] >= t));
+  return c;
+}
+
+// The largest t that at least n of the wave's keys reach (n of them do), or some
+// t that n to `most` of them reach.  Down from the largest key in growing steps (the
+// first about a twelfth of a value), then by halves.
+template <typename T, int R>
+__device__ __forceinline__ typename Order<T>::K nth_key(const typename Order<T>::K (&k)[R], int n, int most) {
+  typedef typename Order<T>::K K;
+  K top = k[0];
+#pragma unroll
+  for (int r = 1; r < R; ++r) top = k[r] > top ? k[r] : top;
+  top = wave_max(top);
+  K lo = top, step = (K)1 << (Order<T>::kBits == 32 ? 20 : 49);
+  int c = count_ge<K, R>(k, lo);
+  while (c < n) {
+    top = lo;
+    lo = step != 0 && lo > step ? lo - step : 0;  // all keys reach 0
+    step <<= 1;
+    c = count_ge<K, R>(k, lo);
   }
-  return t;
+  while (c > most && top - lo > 1) {
+    const K mid = lo + (top - lo) / 2;
+    const int m = count_ge<K, R>(k, mid);
+    if (m >= n) lo = mid, c = m;
+    else top = mid;
+  }
+  return lo;
 }
 
 // A wave's candidate list in LDS.
@@ -94,7 +124,7 @@ struct List {
 // Cuts a list of len >= n entries to its n first in the order; returns the
 // threshold that exactly these reach among themselves.
 template <typename T>
-__device__ typename Order<T>::K prune(const List<T>& l, int len, int n) {
+__device__ __forceinline__ typename Order<T>::K prune(const List<T>& l, int len, int n) {
   typedef typename Order<T>::K K;
   constexpr int R = kList / kWave;
   K k[R];
@@ -105,7 +135,7 @@ __device__ typename Order<T>::K prune(const List<T>& l, int len, int n) {
     k[r] = i < len ? l.key[i] : 0;
     id[r] = i < len ? l.id[i] : INT_MAX;
   }
-  const K t = nth_key<T, R>(k, n);
+  const K t = nth_key<T, R>(k, n, n);
   int above = 0, reach = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -139,6 +169,24 @@ __device__ typename Order<T>::K prune(const List<T>& l, int len, int n) {
   return t;
 }
 
+// Calls f(rank, key, id) for each of the count entries (in LDS), a thread or a
+// group of threads of the workgroup each: 8 up to 64 entries, 4 up to 128, ...
+template <typename K, class F>
+__device__ __forceinline__ void rank_list(const K* key, const int* id, int count, const F& f) {
+  int each = 8;
+  while (each > 1 && count * each > kThreads) each >>= 1;
+  const int part = (int)threadIdx.x & (each - 1);
+  for (int i = (int)threadIdx.x / each; i < count; i += kThreads / each) {
+    const K k = key[i];
+    const int t = id[i];
+    int r = 0;
+#pragma unroll 4
+    for (int j = part; j < count; j += each) r += before<K>(key[j], id[j], k, t);
+    for (int d = 1; d < each; d <<= 1) r += __shfl_xor(r, d);
+    if (part == 0) f(r, k, t);
+  }
+}
+
 // What a segment leaves for the second launch, before its n candidates' keys and
 // ids.
 struct Part {
@@ -169,7 +217,7 @@ __device__ __forceinline__ PartView<T> part_of(const LogprobsArgs& a, int row, i
 // The log probability of x under a row of maximum m and sum s.
 template <typename T>
 __device__ __forceinline__ T log_prob(double x, double m, double s) {
-  if (m == -INFINITY && s == 0.0) return (T)-INFINITY;  // nothing but -inf in the row
+  if (m == -INFINITY && s == s) return (T)-INFINITY;  // nothing but -inf in the row
   return (T)((x - m) - log(s));
 }
 
@@ -219,30 +267,46 @@ __device__ __forceinline__ void load4(const double* p, double* v) {
 // The thread's tokens of the chunk at c0: group g holds tokens c0 + 4 (g *
 // kThreads + thread) .. + 3; those past the row's end read as -inf.
 template <typename T>
-__device__ __forceinline__ void load_chunk(const T* x, int64_t c0, int V, T (&v)[kVals]) {
+__device__ __forceinline__ void load_chunk(const T* x, int64_t c0, int V, T (&v)[kValsOf<T>]) {
+  constexpr int kVals = kValsOf<T>, kLpChunk = kChunkOf<T>;
+  const T* p = x + c0;  // uniform
+  const int t = 4 * (int)threadIdx.x, left = (int)min((int64_t)kLpChunk, V - c0);
+  if (left == kLpChunk) {
 #pragma unroll
-  for (int g = 0; g < kVals / 4; ++g) {
-    const int64_t t = c0 + 4 * (g * kThreads + (int)threadIdx.x);
-    if (t + 4 <= V) {
-      load4(x + t, &v[4 * g]);
-    } else {
+    for (int g = 0; g < kVals / 4; ++g) load4(p + 4 * g * kThreads + t, &v[4 * g]);
+  } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * g + e] = t + e < V ? x[t + e] : (T)-INFINITY;
+    for (int g = 0; g < kVals / 4; ++g) {
+      if (t + 4 * g * kThreads + 4 <= left) {
+        load4(p + 4 * g * kThreads + t, &v[4 * g]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = t + 4 * g * kThreads + e;
+          v[4 * g + e] = i < left ? p[i] : (T)-INFINITY;
+        }
+      }
     }
   }
 }
 
 // TOP: n > 0.
 template <typename T, bool TOP>
-__global__ __launch_bounds__(kThreads) void k_logprobs(LogprobsArgs a) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) void
+k_logprobs(LogprobsArgs a) {
   typedef Order<T> O;
   typedef typename O::K K;
+  constexpr int kVals = kValsOf<T>, kLpChunk = kChunkOf<T>;
   __shared__ K lkey[TOP ? kWaves * kList : 1];
   __shared__ int lid[TOP ? kWaves * kList : 1];
   __shared__ double redd[kWaves];
   __shared__ int redi[kWaves];
   __shared__ K wthr[kWaves];
   __shared__ int wlen[kWaves];
+  __shared__ int fill;
+  __shared__ double tabs[kWaves * kWave];
+  double* tab = tabs + wave() * kWave;
+  init_exp_table_wave(tab);
   const int seg = blockIdx.x;
   for (int row = blockIdx.y; row < a.B; row += gridDim.y) {
     const T* x = static_cast<const T*>(a.x) + (int64_t)row * a.ld;
@@ -257,6 +321,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(LogprobsArgs a) {
       if ((unsigned)chosen < (unsigned)a.V) ck = O::key(x[chosen]);
       else chosen = -1;
     }
+    const T cv = chosen >= 0 ? O::value(ck) : (T)0;
     T m = (T)-INFINITY;
     double s = 0.0;
     int above = 0, len = 0;
@@ -271,101 +336,180 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(LogprobsArgs a) {
       for (int i = 1; i < kVals; ++i) mt = fmax(mt, v[i]);
       const T mn = fmax(m, mt);
       const T M = mn == (T)-INFINITY ? (T)0 : mn;  // -inf - M is -inf
-      if (!(mn == m)) s *= exp((double)m - (double)M);
+      s *= rescale((double)m, (double)M, tab);
       m = mn;
 #pragma unroll
-      for (int i = 0; i < kVals; ++i) s += exp_term(v[i] - M);
-      K k[kVals], km = 0;
+      for (int g = 0; g < kVals; g += 4) {
 #pragma unroll
-      for (int i = 0; i < kVals; ++i) {
-        k[i] = O::key(v[i]);
-        km = k[i] > km ? k[i] : km;
+        for (int i = g; i < g + 4; ++i) s += exp_term(v[i] - M, tab);
+        __builtin_amdgcn_sched_barrier(0);  // four terms at a time in registers
       }
-      const int64_t t0 = c0 + 4 * (int)threadIdx.x;
-      if (chosen >= 0) {
+      const uint32_t t0 = (uint32_t)c0 + 4 * threadIdx.x;
+      const auto token = [&](int i) { return t0 + 4 * (i / 4) * kThreads + i % 4; };
+      // a NaN, which the maxima pass over, shows in the sum from then on
+      const bool nan = s != s;
+      if (chosen >= 0 && __ballot(!(mt < cv) || nan) != 0) {
 #pragma unroll
         for (int i = 0; i < kVals; ++i) {
-          const int64_t t = t0 + 4 * (i / 4) * kThreads + i % 4;
-          above += k[i] > ck || (k[i] == ck && t < chosen);
+          const K k = O::key(v[i]);
+          above += k > ck || (k == ck && token(i) < (uint32_t)chosen);
         }
       }
       if constexpr (TOP) {
-        const int lanes = __popcll(__ballot(km > thr));
-        if (lanes == 0) continue;
-        // at least n tokens of the chunk reach the n-th of the lane maxima
-        const bool enough = lanes >= a.n;
-        K reach = thr + 1;  // thr is below some key here
-        if (enough) {
-          const K one[1] = {km};
-          reach = nth_key<T, 1>(one, a.n);
-        }
-        bool cut = enough;
+        const bool start = c0 == first;  // uniform
+        // the start's threshold holds n tokens of the first two chunks, so that only
+        // from the third on a like one is behind them
+        const K pass = c0 - first <= kLpChunk && thr > O::kNegInf ? thr : thr + 1;
+        if (!start && __ballot(O::key(mt) >= pass || nan) == 0) continue;
+        K k[kVals], one[1] = {0};
 #pragma unroll
         for (int i = 0; i < kVals; ++i) {
-          uint64_t in = __ballot(k[i] >= reach);
-          if (in == 0) continue;
-          if (len + __popcll(in) > kList) {
-            reach = prune(list, len, a.n);
-            len = a.n;
-            cut = true;
-            in = __ballot(k[i] >= reach);
+          k[i] = O::key(v[i]);
+          one[0] = k[i] > one[0] ? k[i] : one[0];
+        }
+        K reach;
+        if (start) {
+          // n tokens reach about the n-th of the threads' maxima over this chunk and
+          // the next
+          K km = one[0];
+          if (c0 + kLpChunk < end) {
+#pragma unroll
+            for (int i = 0; i < kVals; ++i) {
+              const K q = O::key(next[i]);
+              km = q > km ? q : km;
+            }
           }
+          lkey[threadIdx.x] = km;
+          wg_barrier();
+          if (wave() == 0) {
+            K all[kWaves];
+            int c = 0;
+#pragma unroll
+            for (int r = 0; r < kWaves; ++r) {
+              all[r] = lkey[r * kWave + lane()];
+              c += __popcll(__ballot(all[r] > O::kNegInf));
+            }
+            const K t = c >= a.n ? nth_key<T, kWaves>(all, a.n, a.n + a.n / 4) : O::kNegInf;
+            if (lane() == 0) wthr[0] = t;
+          }
+          wg_barrier();
+          thr = wthr[0];
+          reach = thr > O::kNegInf ? thr : thr + 1;
+          if (__ballot(one[0] >= reach) == 0) continue;
+        } else {
+          const int lanes = __popcll(__ballot(one[0] >= pass));
+          if (lanes == 0 || pass == 0) continue;  // (0: behind n NaNs)
+          reach = pass;
+          if (lanes >= a.n) {
+            // the same for a wave, where a row rises
+            reach = nth_key<T, 1>(one, a.n, a.n);
+            thr = reach;
+          }
+        }
+        if (len + count_ge<K, kVals>(k, reach) > kList) {
+          if (len >= a.n) {
+            const K t = prune(list, len, a.n);
+            len = a.n;
+            if (t >= reach) {
+              thr = t;
+              if (t == ~(K)0) continue;
+              reach = t + 1;
+            }
+          }
+          if (len + count_ge<K, kVals>(k, reach) > kList) {
+            // many like values, or a chunk that rises: exactly n of it, of like ones
+            // the first (n are there: else they would fit)
+            reach = nth_key<T, kVals>(k, a.n, a.n);
+            thr = reach;
+            uint32_t last = UINT_MAX;
+            const auto count = [&](uint32_t id) {
+              int c = 0;
+#pragma unroll
+              for (int i = 0; i < kVals; ++i) c += __popcll(__ballot(k[i] > reach || (k[i] == reach && token(i) <= id)));
+              return c;
+            };
+            for (int b = 31; b >= 0; --b) {
+              const uint32_t trial = last & ~(1u << b);
+              if (count(trial) >= a.n) last = trial;
+            }
+#pragma unroll
+            for (int i = 0; i < kVals; ++i) k[i] = k[i] == reach && token(i) > last ? 0 : k[i];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kVals; ++i) {
+          const uint64_t in = __ballot(k[i] >= reach);
+          if (in == 0) continue;
           if (k[i] >= reach) {
             const int p = len + __popcll(in & ((1ull << lane()) - 1));
             list.key[p] = k[i];
-            list.id[p] = (int)(t0 + 4 * (i / 4) * kThreads + i % 4);
+            list.id[p] = (int)token(i);
           }
           len += __popcll(in);
         }
-        if (cut) thr = reach;  // n listed tokens reach it, with lower ids than any that follow
       }
     }
     // the segment's maximum and sum
     const double mb = block_max((double)m, redd);
     const double Mb = mb == -INFINITY ? 0.0 : mb;
-    const double sb = block_sum(s * exp((double)m - Mb), redd);
+    const double sb = block_sum(s * rescale((double)m, Mb, tab), redd);
     const int ab = block_sum(above, redi);
     const PartView<T> pv = part_of<T>(a, row, seg);
     if (a.segs == 1) write_chosen<T>(a, row, mb, sb, ab);
     int count = 0;
     if constexpr (TOP) {
-      if (len >= a.n) {
-        thr = prune(list, len, a.n);
-        len = a.n;
-      } else {
-        thr = 0;
-      }
+      if (threadIdx.x == 0) fill = 0;
       if (lane() == 0) {
         wthr[wave()] = thr;
         wlen[wave()] = len;
       }
       wg_barrier();
-      K best = 0;
+      K best = 0;  // n listed tokens reach it
+      int listed = 0;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) best = wthr[w] > best ? wthr[w] : best;
-      // one entry per thread (len <= n <= 64); those below `best` are not among the n
-      const bool in = lane() < len && list.key[lane()] >= best;
-      const K k = in ? list.key[lane()] : 0;
-      const int id = in ? list.id[lane()] : 0;
-      wg_barrier();
-      const int at = block_excl_scan<int>(in ? 1 : 0, redi, &count);
-      if (in) {
-        lkey[at] = k;
-        lid[at] = id;
+      for (int w = 0; w < kWaves; ++w) {
+        best = wthr[w] > best ? wthr[w] : best;
+        listed += wlen[w];
+      }
+      if (listed > kThreads) {
+        // more than a thread each: the waves' first n
+        if (len >= a.n) prune(list, len, a.n);
+        len = min(len, a.n);
+      }
+      // those below `best` are not among the n: at most one entry per thread is left
+      K k[kList / kWave];
+      int id[kList / kWave];
+#pragma unroll
+      for (int r = 0; r < kList / kWave; ++r) {
+        const int i = r * kWave + lane();
+        k[r] = i < len ? list.key[i] : 0;
+        id[r] = i < len ? list.id[i] : 0;
       }
       wg_barrier();
-      if (in) {
-        int r = 0;
-        for (int j = 0; j < count; ++j) r += before<K>(lkey[j], lid[j], k, id);
-        if (r < a.n) {
-          if (a.segs == 1) {
-            write_top<T>(a, row, r, k, id, mb, sb);
-          } else {
-            pv.key[r] = k;
-            pv.id[r] = id;
-          }
+#pragma unroll
+      for (int r = 0; r < kList / kWave; ++r) {
+        if (r * kWave >= len) break;
+        const bool in = k[r] >= best && k[r] > 0;
+        const uint64_t m = __ballot(in);
+        int at = 0;
+        if (lane() == 0) at = lds_fetch_add(&fill, __popcll(m));
+        at = uniform(at) + __popcll(m & ((1ull << lane()) - 1));
+        if (in) {
+          lkey[at] = k[r];
+          lid[at] = id[r];
         }
       }
+      wg_barrier();
+      count = fill;
+      rank_list<K>(lkey, lid, count, [&](int r, K key, int tok) {
+        if (r >= a.n) return;
+        if (a.segs == 1) {
+          write_top<T>(a, row, r, key, tok, mb, sb);
+        } else {
+          pv.key[r] = key;
+          pv.id[r] = tok;
+        }
+      });
       if (a.segs == 1 && count < a.n) fill_top<T>(a, row, lid, count, mb, sb, redi);
       wg_barrier();  // the lists are read before the next row writes them
     }
@@ -384,16 +528,30 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_merge(LogprobsArgs a) {
   __shared__ int redi[kWaves];
   __shared__ K redk[kWaves];
   __shared__ int fill;
+  __shared__ double tabs[kWaves * kWave];
+  double* tab = tabs + wave() * kWave;
+  init_exp_table_wave(tab);
   for (int row = blockIdx.x; row < a.B; row += gridDim.x) {
     if (threadIdx.x == 0) fill = 0;
     double m = -INFINITY, s = 0.0;
     int above = 0, have = 0;
     K best = 0;
+    // a thread's first entry, loaded beside the partials
+    const int64_t entries = (int64_t)a.segs * a.n;
+    K ek = 0;
+    int eid = 0, ecount = 0, ej = 0;
+    if ((int64_t)threadIdx.x < entries) {
+      const PartView<T> pv = part_of<T>(a, row, (int)threadIdx.x / a.n);
+      ej = (int)threadIdx.x % a.n;
+      ek = pv.key[ej];
+      eid = pv.id[ej];
+      ecount = pv.part->count;
+    }
     for (int g = threadIdx.x; g < a.segs; g += kThreads) {
       const PartView<T> pv = part_of<T>(a, row, g);
       const Part p = *pv.part;
       const double mn = fmax(m, p.m), M = mn == -INFINITY ? 0.0 : mn;
-      s = s * exp(m - M) + p.s * exp(p.m - M);
+      s = s * rescale(m, M, tab) + p.s * rescale(p.m, M, tab);
       m = mn;
       above += p.above;
       have += p.count;
@@ -404,14 +562,18 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_merge(LogprobsArgs a) {
     }
     const double mb = block_max(m, redd);
     const double Mb = mb == -INFINITY ? 0.0 : mb;
-    const double sb = block_sum(s * exp(m - Mb), redd);
+    const double sb = block_sum(s * rescale(m, Mb, tab), redd);
     above = block_sum(above, redi);
     write_chosen<T>(a, row, mb, sb, above);
     if (a.n == 0) continue;
     have = min(block_sum(have, redi), a.n);
     best = block_max(best, redk);
-    const int64_t entries = (int64_t)a.segs * a.n;
-    for (int64_t e = threadIdx.x; e < entries; e += kThreads) {
+    if (ej < ecount && ek >= best) {
+      const int p = lds_fetch_add(&fill, 1);  // fits: a thread each
+      lkey[p] = ek;
+      lid[p] = eid;
+    }
+    for (int64_t e = threadIdx.x + kThreads; e < entries; e += kThreads) {
       const PartView<T> pv = part_of<T>(a, row, (int)(e / a.n));
       const int j = (int)(e % a.n);
       if (j < pv.part->count && pv.key[j] >= best) {
@@ -425,11 +587,9 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_merge(LogprobsArgs a) {
     wg_barrier();
     const int count = fill;
     if (count <= kMergeList) {
-      for (int i = threadIdx.x; i < count; i += kThreads) {
-        int r = 0;
-        for (int j = 0; j < count; ++j) r += before<K>(lkey[j], lid[j], lkey[i], lid[i]);
-        if (r < a.n) write_top<T>(a, row, r, lkey[i], lid[i], mb, sb);
-      }
+      rank_list<K>(lkey, lid, count, [&](int r, K key, int tok) {
+        if (r < a.n) write_top<T>(a, row, r, key, tok, mb, sb);
+      });
       if (have < a.n) fill_top<T>(a, row, lid, have, mb, sb, redi);
     } else {
       // very many like values over very many segments: the n first one by one
@@ -469,10 +629,11 @@ hipError_t launch_t(const LogprobsArgs& a, hipStream_t s) {
 
 }  // namespace
 
-// Segments: as many workgroups as four per compute unit, a whole chunk or more
-// each.
+// Segments: as many workgroups as fit the chip at once, two per compute unit, a
+// whole chunk or more each.
 size_t plan_logprobs(LogprobsArgs& a, bool f64, int num_cu, bool one_launch) {
-  const int64_t chunks = ((int64_t)a.V + kLpChunk - 1) / kLpChunk, target = 4 * (int64_t)num_cu;
+  const int chunk = f64 ? kChunkOf<double> : kChunkOf<float>;
+  const int64_t chunks = ((int64_t)a.V + chunk - 1) / chunk, target = 2 * (int64_t)num_cu;
   const int64_t each = one_launch ? chunks : std::min(chunks, (a.B * chunks + target - 1) / target);
   a.seg_chunks = (int)each;
   a.segs = (int)((chunks + each - 1) / each);

@@ -323,6 +323,27 @@ def test_logprobs_match_oracle(V, dt):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("V", [4000, 40000])
+@pytest.mark.parametrize("B", [1, 600])  # several segments, and one of all chunks
+def test_logprobs_many_nan_and_like_values(B, V, dt):
+    """More NaNs, or more tokens of one value, than are asked for, in one chunk or
+    another, or each chunk with larger values than the one before."""
+    g = np.random.default_rng(V)
+    x = g.normal(0, 1, (8, V))
+    for b, at in enumerate([slice(0, 70), slice(V - 70, V), slice(V // 2, V // 2 + 64), slice(0, V, V // 65)]):
+        x[b, at] = np.nan
+    x[4, V // 2:] = 9.0
+    x[5] = np.floor(np.arange(V) / 100)
+    x[6, ::2] = 3.0
+    x[7] = np.arange(V) // 4096 + g.random(V)
+    x = x.astype(dt)
+    for n in (1, 20, 64):
+        print(f"[logprobs] like values B={B} V={V} {dt.__name__} n={n}", flush=True)
+        res = token_logprobs(np.tile(x, (-(-B // 8), 1))[:max(B, 8)], None, n)
+        _check_logprobs(type(res)(None, None, *(a[:8] for a in res[2:])), x, None, n)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("B,V", [(300, 20000), (2100, 8300), (1, 300000)])
 def test_logprobs_row_shares(B, V, dt):
     """Batches whose rows are shared out differently over workgroups: several

@@ -23,7 +23,8 @@ namespace plh {
 
 namespace {
 
-constexpr int kProcChunk = 8192;
+constexpr int kProcChunk = 4096;
+constexpr int kAhead = 4;
 constexpr int kQuads = kProcChunk / (4 * kThreads);  // groups of four tokens per thread
 
 // Four consecutive tokens, aligned to their element only: rows of an odd
@@ -99,7 +100,7 @@ __device__ __forceinline__ T touched(T x, uint32_t w, uint32_t s, const RowRules
 
 // INPLACE: out is x, and only quads that change are read and written.
 template <typename T, bool INPLACE>
-__global__ __launch_bounds__(kThreads) void k_process(ProcessArgs a) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 8 : 6))) void k_process(ProcessArgs a) {
   __shared__ __align__(16) uint32_t words[kProcChunk];  // history words (touched())
   __shared__ __align__(16) uint32_t slots[kProcChunk];  // bias slots
   const int c0 = blockIdx.x * kProcChunk;
@@ -147,11 +148,18 @@ __global__ __launch_bounds__(kThreads) void k_process(ProcessArgs a) {
       }
       wg_barrier();
       if (pen) {
-        for (int64_t h = h0 + threadIdx.x; h < h1; h += kThreads) {
-          const uint32_t t = (uint32_t)a.hist_ids[h] - (uint32_t)c0;
-          if (t < (uint32_t)ntok) {
-            if (h >= out0) lds_add(&words[t], 2u);
-            else lds_or(&words[t], 1u);
+        // kAhead loads in flight (past the end: the last token again, not counted)
+        for (int64_t h = h0 + threadIdx.x; h < h1; h += kAhead * kThreads) {
+          uint32_t id[kAhead];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) id[u] = (uint32_t)a.hist_ids[min(h + u * kThreads, h1 - 1)];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            const uint32_t t = id[u] - (uint32_t)c0;
+            if (t < (uint32_t)ntok && h + u * kThreads < h1) {
+              if (h + u * kThreads >= out0) lds_add(&words[t], 2u);
+              else lds_or(&words[t], 1u);
+            }
           }
         }
       }

@@ -101,13 +101,24 @@ __device__ __forceinline__ float widen(T v) { return (float)v; }
 
 // ------------------------------------------------------------ activations
 
-constexpr int kRun = 16;                   // k values of a thread at a time: one 16-byte piece of codes
+constexpr int kRun = 8;                    // k values of a thread at a time: one 16-byte piece of the operand
 constexpr int kSweep = kRun * kThreads;    // k values of a workgroup at a time
+constexpr int kKept = 2;                   // sweeps that stay in registers between the two passes
 
+// Eight values from k0 on, zeros from D on.  Rows start anywhere.
 template <typename TX>
 __device__ __forceinline__ void load_run(const TX* x, int k0, int D, float (&v)[kRun]) {
+  struct __attribute__((packed, aligned(sizeof(TX)))) Run {
+    TX e[kRun];
+  };
+  if (k0 + kRun <= D) {
+    const Run r = *reinterpret_cast<const Run*>(x + k0);
 #pragma unroll
-  for (int j = 0; j < kRun; ++j) v[j] = k0 + j < D ? widen(x[k0 + j]) : 0.0f;
+    for (int j = 0; j < kRun; ++j) v[j] = widen(r.e[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) v[j] = k0 + j < D ? widen(x[k0 + j]) : 0.0f;
+  }
 }
 
 // e4m3 codes back to the values they stand for, times the power of two s, as
@@ -118,47 +129,67 @@ __device__ __forceinline__ uint32_t rounded2(uint32_t codes, bool hi, float s) {
   return (__float_as_uint(v[0] * s) >> 16) | (__float_as_uint(v[1] * s) & 0xffff0000u);
 }
 
-// One workgroup per row.
+// The largest of a row of 16 lanes, in all of them (rotations within the row).
+__device__ __forceinline__ float row16_max(float v) {
+  v = fmaxf(v, dpp<0x128, 0xf>(v, v));
+  v = fmaxf(v, dpp<0x124, 0xf>(v, v));
+  v = fmaxf(v, dpp<0x122, 0xf>(v, v));
+  return fmaxf(v, dpp<0x121, 0xf>(v, v));
+}
+
+// One workgroup per row; a block's 16 threads are one row of 16 lanes.
 template <typename TX, int R>
 __global__ __launch_bounds__(kThreads) void k_fp8_act(Fp8Args a) {
   __shared__ double red[kWaves];
-  const int n = blockIdx.x;
+  const int n = blockIdx.x, kt = threadIdx.x * kRun;
   const TX* x = static_cast<const TX*>(a.x) + (int64_t)n * a.ldx;
-  float v[kRun];
+  float v[kKept][kRun], w[kKept][kRun];
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) {
+    load_run(x, kt + i * kSweep, a.D, v[i]);
+    if (a.norm != nullptr) load_run(a.norm, kt + i * kSweep, a.D, w[i]);
+  }
   double r = 1.0;
   if (a.norm != nullptr) {
     double s = 0.0;
-    for (int k0 = threadIdx.x * kRun; k0 < a.D; k0 += kSweep) {
-      load_run(x, k0, a.D, v);
 #pragma unroll
-      for (int j = 0; j < kRun; ++j) s += (double)v[j] * (double)v[j];
+    for (int i = 0; i < kKept; ++i)
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) s += (double)v[i][j] * (double)v[i][j];
+    for (int k0 = kt + kKept * kSweep; k0 < a.D; k0 += kSweep) {
+      float u[kRun];
+      load_run(x, k0, a.D, u);
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) s += (double)u[j] * (double)u[j];
     }
     s = block_sum(s, red);
     r = 1.0 / sqrt(s / (double)a.D + a.eps);
   }
-  for (int k0 = threadIdx.x * kRun; k0 < a.kb * kBlock; k0 += kSweep) {
-    load_run(x, k0, a.D, v);
+  const auto emit = [&](int k0, float (&y)[kRun], const float (&g)[kRun]) {
     float amax = 0.0f;
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
-      if (a.norm != nullptr) v[j] = k0 + j < a.D ? (float)((double)v[j] * r * (double)a.norm[k0 + j]) : 0.0f;
-      amax = fmaxf(amax, fabsf(v[j]));
+      if (a.norm != nullptr) y[j] = k0 + j < a.D ? (float)((double)y[j] * r * (double)g[j]) : 0.0f;
+      amax = fmaxf(amax, fabsf(y[j]));
     }
-    // the block's eight threads are lanes 8 i .. 8 i + 7
+    const float s = block_scale(row16_max(amax)), inv = inverse_pow2(s);
+    uint32_t o[4];
 #pragma unroll
-    for (int d = 1; d < 8; d <<= 1) amax = fmaxf(amax, __shfl_xor(amax, d));
-    const float s = block_scale(amax), inv = inverse_pow2(s);
-    uint32_t w[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t c = codes4(code_input(v[4 * j], inv), code_input(v[4 * j + 1], inv), code_input(v[4 * j + 2], inv),
-                                code_input(v[4 * j + 3], inv));
-      w[2 * j] = rounded2(c, false, s);
-      w[2 * j + 1] = rounded2(c, true, s);
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t c = codes4(code_input(y[4 * j], inv), code_input(y[4 * j + 1], inv), code_input(y[4 * j + 2], inv),
+                                code_input(y[4 * j + 3], inv));
+      o[2 * j] = rounded2(c, false, s);
+      o[2 * j + 1] = rounded2(c, true, s);
     }
+    a.act[act_at<R>(n, k0 / kRun, a.kb)] = uint4{o[0], o[1], o[2], o[3]};
+  };
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-      a.act[act_at<R>(n, k0 / 8 + j, a.kb)] = uint4{w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]};
+  for (int i = 0; i < kKept; ++i)
+    if (kt + i * kSweep < a.kb * kBlock) emit(kt + i * kSweep, v[i], w[i]);
+  for (int k0 = kt + kKept * kSweep; k0 < a.kb * kBlock; k0 += kSweep) {
+    load_run(x, k0, a.D, v[0]);
+    if (a.norm != nullptr) load_run(a.norm, k0, a.D, w[0]);
+    emit(k0, v[0], w[0]);
   }
 }
 

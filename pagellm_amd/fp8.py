@@ -21,7 +21,7 @@ from __future__ import annotations
 import numpy as np
 
 from . import _native
-from .sampling import _is_torch_cuda
+from .sampling import _is_torch_cuda, _stream_of
 
 __all__ = ["Fp8LogitsHead", "Fp8Weights", "fp8_linear"]
 
@@ -90,7 +90,7 @@ class Fp8Weights:
             raise TypeError("the matrix must be float32, bfloat16 or float16")
         code = _float_code(w, "the matrix")
         out = cls(w.shape[0], w.shape[1], c)
-        c.set_stream(torch.cuda.current_stream(w.device).cuda_stream)
+        c.set_stream(_stream_of(w))
         c.fp8_quantize(w.data_ptr(), code, int(w.stride(0)), int(w.stride(1)), out.V, out.D, out.codes.data_ptr(),
                        out.scales.data_ptr())
         return out
@@ -114,7 +114,7 @@ class Fp8Weights:
             raise ValueError(f"scales must be {list(out.scales.shape)} for codes {list(q.shape)}, got {list(s.shape)}")
         q = q if q.stride(1) == 1 and q.stride(0) >= out.D else q.contiguous()
         s = s.contiguous()
-        c.set_stream(torch.cuda.current_stream(q.device).cuda_stream)
+        c.set_stream(_stream_of(q))
         c.fp8_pack(q.data_ptr(), max(int(q.stride(0)), out.D), s.data_ptr(), int(s.shape[1]), out.V, out.D,
                    out.codes.data_ptr(), out.scales.data_ptr())
         return out
@@ -166,7 +166,7 @@ def fp8_linear(x, weights: Fp8Weights, *, norm=None, eps: float = 1e-5, out=None
             raise ValueError("rows of out must not overlap")
     if N == 0:
         return out
-    c.set_stream(torch.cuda.current_stream(x.device).cuda_stream)
+    c.set_stream(_stream_of(x))
     nbytes = c.fp8_ws_bytes(N, V, weights.D)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)  # torch's allocator orders its reuse on the stream
     ldx = int(x.stride(0)) if N > 1 else weights.D

@@ -22,7 +22,7 @@ from typing import Iterable, Mapping, NamedTuple, Sequence
 import numpy as np
 
 from . import _native
-from .sampling import _as_float_rows, _ctx, _expand_params, _history_ids, _int64_row, _is_torch_cuda
+from .sampling import _as_float_rows, _ctx, _expand_params, _history_ids, _int64_row, _is_torch_cuda, _stream_of
 
 __all__ = ["LogitRules", "Logprobs", "pack_mask", "process_logits", "token_logprobs"]
 
@@ -253,7 +253,7 @@ def process_logits(
     buf, offs = _pack([r, f, p, bias, bias_off, hist_off, start, bias_ids, hist_ids, mask_rows, host_masks])
     code = _native.PLH_F64 if "float64" in str(logits.dtype) else _native.PLH_F32
     if on_gpu:
-        c.set_stream(torch.cuda.current_stream(logits.device).cuda_stream)
+        c.set_stream(_stream_of(logits))
         keep = torch.from_numpy(buf).to(logits.device)  # torch's allocator orders its reuse on the stream
         base = keep.data_ptr()
         x, ld = logits.data_ptr(), int(logits.stride(0)) if B > 1 else V
@@ -330,7 +330,7 @@ def token_logprobs(logits, ids=None, n_top: int = 0, *, ctx: _native.Context | N
                        new((B, n), torch.int32), new((B, n), logits.dtype))
         if B == 0:
             return res
-        c.set_stream(torch.cuda.current_stream(logits.device).cuda_stream)
+        c.set_stream(_stream_of(logits))
         code = _native.PLH_F64 if logits.dtype == torch.float64 else _native.PLH_F32
         ptr = lambda t: t.data_ptr() if t is not None and t.numel() else None  # noqa: E731
         c.logprobs(logits.data_ptr(), code, int(logits.stride(0)) if B > 1 else V, B, V, ptr(ids), ptr(res.logprob),

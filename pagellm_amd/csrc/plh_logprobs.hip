@@ -299,7 +299,7 @@ k_logprobs(LogprobsArgs a) {
   constexpr int kVals = kValsOf<T>, kLpChunk = kChunkOf<T>;
   __shared__ K lkey[TOP ? kWaves * kList : 1];
   __shared__ int lid[TOP ? kWaves * kList : 1];
-  __shared__ double redd[kWaves];
+  __shared__ double redm[kWaves], redd[kWaves];
   __shared__ int redi[kWaves];
   __shared__ K wthr[kWaves];
   __shared__ int wlen[kWaves];
@@ -449,43 +449,59 @@ k_logprobs(LogprobsArgs a) {
         }
       }
     }
-    // the segment's maximum and sum
-    const double mb = block_max((double)m, redd);
-    const double Mb = mb == -INFINITY ? 0.0 : mb;
-    const double sb = block_sum(s * rescale((double)m, Mb, tab), redd);
-    const int ab = block_sum(above, redi);
-    const PartView<T> pv = part_of<T>(a, row, seg);
-    if (a.segs == 1) write_chosen<T>(a, row, mb, sb, ab);
-    int count = 0;
-    if constexpr (TOP) {
-      if (threadIdx.x == 0) fill = 0;
-      if (lane() == 0) {
-        wthr[wave()] = thr;
-        wlen[wave()] = len;
-      }
-      wg_barrier();
-      K best = 0;  // n listed tokens reach it
-      int listed = 0;
+    // the segment's maximum, sum and rank count, and what its waves' lists hold: two
+    // rounds through LDS
+    const double mw = wave_max((double)m);
+    if (threadIdx.x == 0) fill = 0;
+    if (lane() == 0) {
+      redm[wave()] = mw;
+      wthr[wave()] = thr;
+      wlen[wave()] = len;
+    }
+    wg_barrier();
+    double mb = redm[0];
+    K best = wthr[0];  // n listed tokens reach it
+    int listed = wlen[0];
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        best = wthr[w] > best ? wthr[w] : best;
-        listed += wlen[w];
-      }
+    for (int w = 1; w < kWaves; ++w) {
+      mb = fmax(mb, redm[w]);
+      best = wthr[w] > best ? wthr[w] : best;
+      listed += wlen[w];
+    }
+    const double sw = wave_sum(s * rescale((double)m, mb == -INFINITY ? 0.0 : mb, tab));
+    const int aw = wave_sum(above);
+    if (lane() == 0) {
+      redd[wave()] = sw;
+      redi[wave()] = aw;
+    }
+    K k[kList / kWave];
+    int id[kList / kWave];
+    if constexpr (TOP) {
       if (listed > kThreads) {
         // more than a thread each: the waves' first n
         if (len >= a.n) prune(list, len, a.n);
         len = min(len, a.n);
       }
-      // those below `best` are not among the n: at most one entry per thread is left
-      K k[kList / kWave];
-      int id[kList / kWave];
 #pragma unroll
       for (int r = 0; r < kList / kWave; ++r) {
         const int i = r * kWave + lane();
         k[r] = i < len ? list.key[i] : 0;
         id[r] = i < len ? list.id[i] : 0;
       }
-      wg_barrier();
+    }
+    wg_barrier();
+    double sb = redd[0];
+    int ab = redi[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) {
+      sb += redd[w];
+      ab += redi[w];
+    }
+    const PartView<T> pv = part_of<T>(a, row, seg);
+    if (a.segs == 1) write_chosen<T>(a, row, mb, sb, ab);
+    int count = 0;
+    if constexpr (TOP) {
+      // those below `best` are not among the n: at most one entry per thread is left
 #pragma unroll
       for (int r = 0; r < kList / kWave; ++r) {
         if (r * kWave >= len) break;
@@ -511,8 +527,8 @@ k_logprobs(LogprobsArgs a) {
         }
       });
       if (a.segs == 1 && count < a.n) fill_top<T>(a, row, lid, count, mb, sb, redi);
-      wg_barrier();  // the lists are read before the next row writes them
     }
+    wg_barrier();  // what lies in LDS is read before the next row writes it
     if (a.segs > 1 && threadIdx.x == 0) *pv.part = Part{mb, sb, ab, min(count, a.n)};
   }
 }

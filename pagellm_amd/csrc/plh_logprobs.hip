@@ -646,11 +646,14 @@ hipError_t launch_t(const LogprobsArgs& a, hipStream_t s) {
 }  // namespace
 
 // Segments: as many workgroups as fit the chip at once, two per compute unit, a
-// whole chunk or more each.
+// whole chunk or more each (256 x 128256, 20 best: 49 us, with four 57 us).  Rows of
+// up to three chunks take one: a second launch costs more than the chunks behind one
+// another (64 rows of two chunks 10.3 -> 7.8 us, with 20 best 17.8 -> 14.4 us; three:
+// 10.4 -> 9.4, 18.2 -> 17.0 us; four: 10.4 -> 10.3, 19.0 -> 19.5 us).
 size_t plan_logprobs(LogprobsArgs& a, bool f64, int num_cu, bool one_launch) {
   const int chunk = f64 ? kChunkOf<double> : kChunkOf<float>;
   const int64_t chunks = ((int64_t)a.V + chunk - 1) / chunk, target = 2 * (int64_t)num_cu;
-  const int64_t each = one_launch ? chunks : std::min(chunks, (a.B * chunks + target - 1) / target);
+  const int64_t each = one_launch || chunks <= 3 ? chunks : std::min(chunks, (a.B * chunks + target - 1) / target);
   a.seg_chunks = (int)each;
   a.segs = (int)((chunks + each - 1) / each);
   return a.segs == 1 ? 0 : (size_t)a.B * a.segs * (f64 ? part_bytes<double>(a.n) : part_bytes<float>(a.n));

@@ -130,6 +130,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
     }
     if (INPLACE && !pen && !bias && mask == nullptr) continue;
 
+    // the first tokens of the history and of the bias list ahead of the logits: loads
+    // return in order, and the tables are built while the logits are on their way
+    // (past the end: the last token again, not counted)
+    uint32_t id[kAhead], bid = 0;
+    if (pen) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) id[u] = (uint32_t)a.hist_ids[min(h0 + threadIdx.x + u * kThreads, h1 - 1)];
+    }
+    if (bias) bid = (uint32_t)a.bias_ids[min(b0 + threadIdx.x, b1 - 1)];
+    __builtin_amdgcn_sched_barrier(0);
     Quad<T> v[kQuads];
     uint32_t allow[kQuads];
 #pragma unroll
@@ -148,11 +158,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
       }
       wg_barrier();
       if (pen) {
-        // kAhead loads in flight (past the end: the last token again, not counted)
-        for (int64_t h = h0 + threadIdx.x; h < h1; h += kAhead * kThreads) {
-          uint32_t id[kAhead];
-#pragma unroll
-          for (int u = 0; u < kAhead; ++u) id[u] = (uint32_t)a.hist_ids[min(h + u * kThreads, h1 - 1)];
+        for (int64_t h = h0 + threadIdx.x;;) {
 #pragma unroll
           for (int u = 0; u < kAhead; ++u) {
             const uint32_t t = id[u] - (uint32_t)c0;
@@ -161,11 +167,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
               else lds_or(&words[t], 1u);
             }
           }
+          h += kAhead * kThreads;
+          if (h >= h1) break;
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) id[u] = (uint32_t)a.hist_ids[min(h + u * kThreads, h1 - 1)];
         }
       }
       if (bias) {
         for (int64_t j = b0 + threadIdx.x; j < b1; j += kThreads) {
-          const uint32_t t = (uint32_t)a.bias_ids[j] - (uint32_t)c0;
+          const uint32_t t = (j < b0 + kThreads ? bid : (uint32_t)a.bias_ids[j]) - (uint32_t)c0;
           if (t < (uint32_t)ntok) lds_max(reinterpret_cast<int*>(&slots[t]), (int)(j - b0) + 1);  // the last counts
         }
       }

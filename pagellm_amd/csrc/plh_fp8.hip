@@ -316,19 +316,25 @@ __global__ __launch_bounds__(kThreads) void k_fp8_skinny(Fp8Args a) {
 
 // -------------------------------------------------------------- more rows
 
-// The tile of a workgroup: workgroups of one XCD (every eighth) get one
-// contiguous range of tiles, so that they share codes and activations in its L2;
-// in that order kGroup row tiles run under one column tile, then the next.
+// The tile of a workgroup.  kGroup row tiles run under one column tile, then the
+// next.  With `ranges`, the workgroups of one XCD (every eighth) get one contiguous
+// range of that order, so that they share codes and activations in its L2 (50 257
+// columns: 256 rows of 4096 119 -> 113 us, 1024 rows 433 -> 419 us); without, the
+// whole chip writes neighbouring tiles of the logits, which counts for more where a
+// tile's sums are short and the rows many (2048 rows of 512: 217 -> 199 us, of 1000
+// 297 -> 278 us, of 1536 375 -> 365 us, of 2048 458 us either way).
 constexpr int kXcds = 8, kGroup = 8;
-// instruction classes of __builtin_amdgcn_sched_group_barrier
-constexpr int kVector = 0x002, kMatrix = 0x008, kDsRead = 0x100;
-__device__ __forceinline__ void tile_of_group(int vtiles, int ntiles, int& vt, int& nt) {
+constexpr int kPlainRows = 1024, kPlainBlocks = 16;
+__device__ __forceinline__ void tile_of_group(int vtiles, int ntiles, bool ranges, int& vt, int& nt) {
   const int total = vtiles * ntiles, x = blockIdx.x % kXcds, slot = blockIdx.x / kXcds;
-  const int idx = x * (total / kXcds) + min(x, total % kXcds) + slot;
+  const int idx = ranges ? x * (total / kXcds) + min(x, total % kXcds) + slot : (int)blockIdx.x;
   const int g = idx / (kGroup * vtiles), in = idx % (kGroup * vtiles), rows = min(kGroup, ntiles - g * kGroup);
   vt = in / rows;
   nt = g * kGroup + in % rows;
 }
+
+// instruction classes of __builtin_amdgcn_sched_group_barrier
+constexpr int kVector = 0x002, kMatrix = 0x008, kDsRead = 0x100;
 
 // A workgroup's 8 waves lie WN along the rows; each forms VI x 2 tiles of 32
 // columns x 32 rows.  Codes go from memory into registers, one block ahead,
@@ -355,7 +361,7 @@ k_fp8_tiles(Fp8Args a) {
   constexpr int kUnit = G::kUnit, kN = NW * kWave;
   __shared__ u32x4 sm[3][G::kStage * kUnit];
   int vt, nt;
-  tile_of_group(tiles_of(a.V, G::kCols), tiles_of(a.N, G::kRows), vt, nt);
+  tile_of_group(tiles_of(a.V, G::kCols), tiles_of(a.N, G::kRows), a.N <= kPlainRows || a.kb >= kPlainBlocks, vt, nt);
   const int w = uniform(wave()), l = lane();
   const int v0 = vt * G::kCols + w / WN * (VI * 32), n0 = nt * G::kRows, nw = w % WN * 64;
   const int b0 = (int)((int64_t)a.kb * blockIdx.z / gridDim.z), b1 = (int)((int64_t)a.kb * (blockIdx.z + 1) / gridDim.z);

@@ -301,7 +301,7 @@ k_logprobs(LogprobsArgs a) {
   __shared__ int lid[TOP ? kWaves * kList : 1];
   __shared__ double redm[kWaves], redd[kWaves];
   __shared__ int redi[kWaves];
-  __shared__ K wthr[kWaves];
+  __shared__ K wthr[kWaves], sthr;
   __shared__ int wlen[kWaves];
   __shared__ int fill;
   __shared__ double tabs[kWaves * kWave];
@@ -390,10 +390,10 @@ k_logprobs(LogprobsArgs a) {
               c += __popcll(__ballot(all[r] > O::kNegInf));
             }
             const K t = c >= a.n ? nth_key<T, kWaves>(all, a.n, a.n + a.n / 4) : O::kNegInf;
-            if (lane() == 0) wthr[0] = t;
+            if (lane() == 0) sthr = t;
           }
           wg_barrier();
-          thr = wthr[0];
+          thr = sthr;
           reach = thr > O::kNegInf ? thr : thr + 1;
           if (__ballot(one[0] >= reach) == 0) continue;
         } else {

@@ -184,7 +184,7 @@ class BatchSampler:
         n_top = 0 if logprobs is None else int(logprobs)
         if not 0 <= n_top <= min(self.hist.V, _native.PLH_MAX_TOP):
             raise ValueError(f"logprobs must be in [0, {min(self.hist.V, _native.PLH_MAX_TOP)}]")
-        masks, mask_rows = _check_mask(masks, mask_rows, B, self.hist.V, c.device)
+        masks, mask_rows = _check_mask(masks, mask_rows, B, self.hist.V, c.device, _is_torch_cuda(logits))
         rules = _expand_rules(rules, B)
         # refused here, before a Generator moves
         f, pr, bias_ids, bias, bias_off = _pack_rules(rules, self.hist.V)

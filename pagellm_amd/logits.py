@@ -38,7 +38,7 @@ class LogitRules:
 
     frequency_penalty: float = 0.0
     presence_penalty: float = 0.0
-    logit_bias: Mapping[int, float] = field(default_factory=dict)
+    logit_bias: Mapping[int, float] = field(default_factory=dict, hash=False)
 
     def __post_init__(self) -> None:
         if not math.isfinite(self.frequency_penalty):
@@ -122,7 +122,7 @@ def _pack_rules(rules: Sequence[LogitRules], V: int):
     return f, p, np.concatenate([r._ids for r in rules]), np.concatenate([r._values for r in rules]), off
 
 
-def _check_mask(masks, mask_rows, B: int, V: int, device: int):
+def _check_mask(masks, mask_rows, B: int, V: int, device: int, logits_on_gpu: bool):
     """(masks, per-row int32 mask rows or None) of a call; masks as a CUDA
     tensor or a contiguous uint32 array."""
     if masks is None:
@@ -132,6 +132,8 @@ def _check_mask(masks, mask_rows, B: int, V: int, device: int):
     if _is_torch_cuda(masks):
         import torch
 
+        if not logits_on_gpu:  # these are processed on the context's stream, not on torch's
+            raise TypeError("CUDA masks need CUDA logits")
         if masks.dtype not in (torch.int32, getattr(torch, "uint32", torch.int32)):
             raise TypeError("masks must be int32 or uint32 words")
         if masks.device.index != device:
@@ -225,7 +227,7 @@ def process_logits(
         raise ValueError("empty vocabulary")
     rules = _expand_rules(rules, B)
     params = _expand_params(params, B) if params is not None else None
-    masks, mask_rows = _check_mask(masks, mask_rows, B, V, c.device)
+    masks, mask_rows = _check_mask(masks, mask_rows, B, V, c.device, on_gpu)
     f, p, bias_ids, bias, bias_off = _pack_rules(rules, V)
     r = np.array([sp.repetition_penalty for sp in params], dtype=np.float64) if params is not None else None
     hist_ids = hist_off = start = None

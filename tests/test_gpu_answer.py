@@ -72,6 +72,8 @@ def test_steps_match_the_oracle(on_gpu):
 
 
 def test_rows_without_rules_keep_their_ids_and_errors_change_nothing():
+    import torch
+
     g = np.random.default_rng(0)
     x = g.normal(0, 2, (2, V)).astype(np.float32)
     params = SamplingParams(temperature=1.0, repetition_penalty=1.2, top_p=0.9)
@@ -88,6 +90,8 @@ def test_rows_without_rules_keep_their_ids_and_errors_change_nothing():
             sampler.sample(x, params, rngs, [0, 1], masks=np.zeros((1, 94), np.uint32))
         with pytest.raises(ValueError):
             sampler.sample(x, params, rngs, [0, 1], logprobs=65)
+        with pytest.raises(TypeError):  # masks on torch's stream, logits on the context's
+            sampler.sample(x, params, rngs, [0, 1], masks=torch.zeros((2, 94), dtype=torch.int32, device="cuda"))
         ids.append(sampler.sample(x, params, rngs, [0, 1], rules=rules))
         assert list(hist.output_starts([0, 1])) == [1, 3]
     assert ids[0][0] == ids[1][0]

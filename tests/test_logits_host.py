@@ -38,6 +38,7 @@ def test_rules_validate_and_pack():
     with pytest.raises(IndexError):
         _pack_rules(rules, 7)
     assert _pack_rules([LogitRules()], 8)[2:] == (None, None, None)
+    assert hash(rules[1]) == hash(LogitRules(0.5, 0.25)) and rules[1] != LogitRules(0.5, 0.25)
     # a dict given stays the caller's
     d = {1: 1.0}
     r = LogitRules(logit_bias=d)

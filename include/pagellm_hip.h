@@ -325,7 +325,8 @@ int plh_logprobs(plh_ctx* ctx, const void* logits, int dtype, int64_t ld, int B,
  * PLH_F16) whose element (v, d) is W[v * stride_v + d * stride_d] (the
  * reference's [D, V] lm_head has stride_v 1): a block's scale is the smallest
  * power of two s >= 2^-126 with max|w| <= 448 s, its codes the e4m3 values
- * nearest to w / s, ties to even; NaN and infinities become NaN.
+ * nearest to w / s, ties to even; NaN and infinities become NaN.  At most 2^35
+ * codes a matrix (PLH_ERR_UNSUPPORTED).
  */
 int64_t plh_fp8_codes_bytes(int V, int D);
 int plh_fp8_pack(plh_ctx* ctx, const uint8_t* codes, int64_t ldc, const float* scales, int64_t lds, int V, int D,

@@ -46,7 +46,7 @@ struct plh_ctx {
 namespace {
 
 constexpr int kMaxVBitmap = 262144;
-constexpr size_t kMostCodes = size_t(1) << 40;  // of a matrix in e4m3 (its pieces and blocks fit a grid)
+constexpr size_t kMostCodes = size_t(1) << 35;  // of a matrix in e4m3 (a thread for each 16 fits a grid)
 
 int fail(plh_ctx* c, int code, const char* fmt, const char* detail = nullptr) {
   if (c != nullptr) {
@@ -766,7 +766,7 @@ int plh_fp8_pack(plh_ctx* c, const uint8_t* codes, int64_t ldc, const float* sca
   if (codes == nullptr || scales == nullptr || out_codes == nullptr || out_scales == nullptr)
     return fail(c, PLH_ERR_INVALID_ARG, "null device pointer%s");
   if (!aligned16(out_codes)) return fail(c, PLH_ERR_INVALID_ARG, "out_codes must be 16-byte aligned%s");
-  if (plh::fp8_codes_bytes(V, D) > kMostCodes) return fail(c, PLH_ERR_UNSUPPORTED, "more than 2^40 codes%s");
+  if (plh::fp8_codes_bytes(V, D) > kMostCodes) return fail(c, PLH_ERR_UNSUPPORTED, "more than 2^35 codes%s");
   int rc = use_device(c);
   if (rc != PLH_OK) return rc;
   const hipError_t e = plh::launch_fp8_pack(codes, ldc, scales, lds, V, D, out_codes, out_scales, c->stream);
@@ -784,7 +784,7 @@ int plh_fp8_quantize(plh_ctx* c, const void* W, int dtype, int64_t stride_v, int
   if (W == nullptr || out_codes == nullptr || out_scales == nullptr)
     return fail(c, PLH_ERR_INVALID_ARG, "null device pointer%s");
   if (!aligned16(out_codes)) return fail(c, PLH_ERR_INVALID_ARG, "out_codes must be 16-byte aligned%s");
-  if (plh::fp8_codes_bytes(V, D) > kMostCodes) return fail(c, PLH_ERR_UNSUPPORTED, "more than 2^40 codes%s");
+  if (plh::fp8_codes_bytes(V, D) > kMostCodes) return fail(c, PLH_ERR_UNSUPPORTED, "more than 2^35 codes%s");
   int rc = use_device(c);
   if (rc != PLH_OK) return rc;
   const hipError_t e =
@@ -815,7 +815,7 @@ int plh_fp8_linear(plh_ctx* c, const void* x, int dtype, int64_t ldx, int N, int
     return fail(c, PLH_ERR_INVALID_ARG, "codes must be 16-byte and ws 256-byte aligned%s");
   if (reinterpret_cast<uintptr_t>(x) % (dtype == PLH_F32 ? 4 : 2) != 0 || reinterpret_cast<uintptr_t>(out) % 4 != 0)
     return fail(c, PLH_ERR_INVALID_ARG, "x and out must be aligned to their element size%s");
-  if (plh::fp8_codes_bytes(V, D) > kMostCodes) return fail(c, PLH_ERR_UNSUPPORTED, "more than 2^40 codes%s");
+  if (plh::fp8_codes_bytes(V, D) > kMostCodes) return fail(c, PLH_ERR_UNSUPPORTED, "more than 2^35 codes%s");
   if (ws_bytes < (int64_t)plh::fp8_ws_bytes(N, V, D, c->num_cu))
     return fail(c, PLH_ERR_INVALID_ARG, "ws is smaller than plh_fp8_ws_bytes%s");
   int rc = use_device(c);

@@ -137,62 +137,64 @@ __device__ __forceinline__ float row16_max(float v) {
   return fmaxf(v, dpp<0x121, 0xf>(v, v));
 }
 
-// One workgroup per row; a block's 16 threads are one row of 16 lanes.  The norm is
-// computed in float64: a last bit of y next to a border between two codes would
-// change the code.  8 x 4096 float32 4.8 us (its chain of loads and sums), 2048 x
+// One workgroup per row, more than 2^20 rows in turn (a grid holds 2^32 threads); a
+// block's 16 threads are one row of 16 lanes.  The norm is computed in float64: a last
+// bit of y next to a border between two codes would change the code.  8 x 4096 float32 4.8 us (its chain of loads and sums), 2048 x
 // 4096 bf16 22 us (the 16-byte stores of the operand's layout).
 template <typename TX, int R>
 __global__ __launch_bounds__(kThreads) void k_fp8_act(Fp8Args a) {
   __shared__ double red[kWaves];
-  const int n = blockIdx.x, kt = threadIdx.x * kRun;
-  const TX* x = static_cast<const TX*>(a.x) + (int64_t)n * a.ldx;
-  float v[kKept][kRun], w[kKept][kRun];
+  const int kt = threadIdx.x * kRun;
+  for (int64_t n = blockIdx.x; n < a.N; n += gridDim.x) {
+    const TX* x = static_cast<const TX*>(a.x) + n * a.ldx;
+    float v[kKept][kRun], w[kKept][kRun];
 #pragma unroll
-  for (int i = 0; i < kKept; ++i) {
-    load_run(x, kt + i * kSweep, a.D, v[i]);
-    if (a.norm != nullptr) load_run(a.norm, kt + i * kSweep, a.D, w[i]);
-  }
-  double r = 1.0;
-  if (a.norm != nullptr) {
-    double s = 0.0;
+    for (int i = 0; i < kKept; ++i) {
+      load_run(x, kt + i * kSweep, a.D, v[i]);
+      if (a.norm != nullptr) load_run(a.norm, kt + i * kSweep, a.D, w[i]);
+    }
+    double r = 1.0;
+    if (a.norm != nullptr) {
+      double s = 0.0;
+#pragma unroll
+      for (int i = 0; i < kKept; ++i)
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) s += (double)v[i][j] * (double)v[i][j];
+      for (int k0 = kt + kKept * kSweep; k0 < a.D; k0 += kSweep) {
+        float u[kRun];
+        load_run(x, k0, a.D, u);
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) s += (double)u[j] * (double)u[j];
+      }
+      s = block_sum(s, red);
+      r = 1.0 / sqrt(s / (double)a.D + a.eps);
+    }
+    const auto emit = [&](int k0, float (&y)[kRun], const float (&g)[kRun]) {
+      float amax = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        if (a.norm != nullptr) y[j] = k0 + j < a.D ? (float)((double)y[j] * r * (double)g[j]) : 0.0f;
+        amax = fmaxf(amax, fabsf(y[j]));
+      }
+      const float s = block_scale(row16_max(amax)), inv = inverse_pow2(s);
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t c = codes4(code_input(y[4 * j], inv), code_input(y[4 * j + 1], inv), code_input(y[4 * j + 2], inv),
+                                  code_input(y[4 * j + 3], inv));
+        o[2 * j] = rounded2(c, false, s);
+        o[2 * j + 1] = rounded2(c, true, s);
+      }
+      a.act[act_at<R>(n, k0 / kRun, a.kb)] = uint4{o[0], o[1], o[2], o[3]};
+    };
 #pragma unroll
     for (int i = 0; i < kKept; ++i)
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) s += (double)v[i][j] * (double)v[i][j];
-    for (int k0 = kt + kKept * kSweep; k0 < a.D; k0 += kSweep) {
-      float u[kRun];
-      load_run(x, k0, a.D, u);
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) s += (double)u[j] * (double)u[j];
+      if (kt + i * kSweep < a.kb * kBlock) emit(kt + i * kSweep, v[i], w[i]);
+    for (int k0 = kt + kKept * kSweep; k0 < a.kb * kBlock; k0 += kSweep) {
+      load_run(x, k0, a.D, v[0]);
+      if (a.norm != nullptr) load_run(a.norm, k0, a.D, w[0]);
+      emit(k0, v[0], w[0]);
     }
-    s = block_sum(s, red);
-    r = 1.0 / sqrt(s / (double)a.D + a.eps);
-  }
-  const auto emit = [&](int k0, float (&y)[kRun], const float (&g)[kRun]) {
-    float amax = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      if (a.norm != nullptr) y[j] = k0 + j < a.D ? (float)((double)y[j] * r * (double)g[j]) : 0.0f;
-      amax = fmaxf(amax, fabsf(y[j]));
-    }
-    const float s = block_scale(row16_max(amax)), inv = inverse_pow2(s);
-    uint32_t o[4];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint32_t c = codes4(code_input(y[4 * j], inv), code_input(y[4 * j + 1], inv), code_input(y[4 * j + 2], inv),
-                                code_input(y[4 * j + 3], inv));
-      o[2 * j] = rounded2(c, false, s);
-      o[2 * j + 1] = rounded2(c, true, s);
-    }
-    a.act[act_at<R>(n, k0 / kRun, a.kb)] = uint4{o[0], o[1], o[2], o[3]};
-  };
-#pragma unroll
-  for (int i = 0; i < kKept; ++i)
-    if (kt + i * kSweep < a.kb * kBlock) emit(kt + i * kSweep, v[i], w[i]);
-  for (int k0 = kt + kKept * kSweep; k0 < a.kb * kBlock; k0 += kSweep) {
-    load_run(x, k0, a.D, v[0]);
-    if (a.norm != nullptr) load_run(a.norm, k0, a.D, w[0]);
-    emit(k0, v[0], w[0]);
   }
 }
 
@@ -578,9 +580,10 @@ int rows_of(int N) { return N <= 16 ? 16 : 32; }
 
 template <int R>
 hipError_t launch_act(const Fp8Args& a, int dtype, hipStream_t s) {
-  if (dtype == PLH_BF16) hipLaunchKernelGGL((k_fp8_act<__hip_bfloat16, R>), dim3(a.N), dim3(kThreads), 0, s, a);
-  else if (dtype == PLH_F16) hipLaunchKernelGGL((k_fp8_act<__half, R>), dim3(a.N), dim3(kThreads), 0, s, a);
-  else hipLaunchKernelGGL((k_fp8_act<float, R>), dim3(a.N), dim3(kThreads), 0, s, a);
+  const dim3 grid(std::min(a.N, 1 << 20));
+  if (dtype == PLH_BF16) hipLaunchKernelGGL((k_fp8_act<__hip_bfloat16, R>), grid, dim3(kThreads), 0, s, a);
+  else if (dtype == PLH_F16) hipLaunchKernelGGL((k_fp8_act<__half, R>), grid, dim3(kThreads), 0, s, a);
+  else hipLaunchKernelGGL((k_fp8_act<float, R>), grid, dim3(kThreads), 0, s, a);
   return hipGetLastError();
 }
 }  // namespace

@@ -34,7 +34,8 @@ template <typename T>
 constexpr int kValsOf = 64 / sizeof(T);
 template <typename T>
 constexpr int kChunkOf = kValsOf<T> * kThreads;
-constexpr int kList = 256;                  // candidate slots of a wave
+constexpr int kList = 128;                  // candidate slots of a wave: twice the most that are asked for
+static_assert(kList >= 2 * kMaxTop && kWaves * kList >= kThreads, "n listed and n of a chunk; a key per thread");
 constexpr int kMergeList = 1024;            // candidates that the second launch ranks in LDS
 
 // Order keys: larger value, larger key; -0 and 0 alike, every NaN the largest.

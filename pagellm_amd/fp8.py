@@ -184,6 +184,8 @@ class Fp8LogitsHead:
     def __init__(self, norm, lm_head, eps: float = 1e-5, *, ctx: _native.Context | None = None):
         """``lm_head`` is the reference's [D, V] (``transformer.py:184-197``)."""
         c = _ctx(ctx)
+        if isinstance(lm_head, np.ndarray) and lm_head.dtype == np.float64:
+            lm_head = lm_head.astype(np.float32)  # as LogitsHead takes it
         w = _on_device(lm_head, c)
         if w.dim() != 2:
             raise ValueError("lm_head must be [D, V]")

@@ -350,3 +350,27 @@ def test_offsets_past_32_bits():
     fp8_linear(x[:3], w, out=far)
     ref, bound = O.linear(x[:3].double().cpu().numpy(), w.dequantize().double().cpu().numpy())
     _check(far, ref, bound, D)
+
+
+def test_very_many_rows():
+    """More rows than a grid has threads for, 512 each."""
+    import torch
+
+    N, D = 8_500_001, 16
+    print("[fp8] 8500001 rows", flush=True)
+    w = Fp8Weights.from_codes(_cuda(np.full((2, D), 0x38, dtype=np.uint8)), _cuda(np.array([[0.5]], dtype=np.float32)))
+    x = torch.randn((N, D), device="cuda", dtype=torch.bfloat16)
+    out = fp8_linear(x, w)
+    rows = [0, (1 << 20) - 1, 1 << 20, 1 << 23, N - 1]
+    ref, bound = O.linear(x[rows].double().cpu().numpy(), np.full((2, D), 0.5))
+    _check(out[rows], ref, bound, D)
+    # the rest: within e4m3's rounding of the float32 sums
+    full = 0.5 * x.float().sum(1)
+    assert bool(((out[:, 0] - full).abs() <= 0.5 * (2.0 ** -4 + 2.0 ** -9) * x.float().abs().sum(1) + 1e-6).all())
+
+
+def test_refuses_more_codes_than_a_grid_holds():
+    c = _native.Context(0)
+    with pytest.raises(NotImplementedError):
+        c.fp8_pack(256, 1 << 20, 256, 1 << 13, 1 << 16, 1 << 20, 256, 256)
+    c.close()

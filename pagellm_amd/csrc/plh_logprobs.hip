@@ -224,14 +224,14 @@ __device__ __forceinline__ T log_prob(double x, double m, double s) {
   return (T)((x - m) - log(s));
 }
 
+// The chosen token's answers, x its logit (read ahead of the sums), id -1 for an id
+// outside the vocabulary.
 template <typename T>
-__device__ __forceinline__ void write_chosen(const LogprobsArgs& a, int row, double m, double s, int above) {
+__device__ __forceinline__ void write_chosen(const LogprobsArgs& a, int row, int id, T x, double m, double s,
+                                             int above) {
   if (a.ids == nullptr || threadIdx.x != 0) return;
-  const int id = a.ids[row];
-  const bool ok = (unsigned)id < (unsigned)a.V;
-  static_cast<T*>(a.lp)[row] =
-      ok ? log_prob<T>((double)static_cast<const T*>(a.x)[(int64_t)row * a.ld + id], m, s) : (T)NAN;
-  a.rank[row] = ok ? above + 1 : 0;
+  static_cast<T*>(a.lp)[row] = id >= 0 ? log_prob<T>((double)x, m, s) : (T)NAN;
+  a.rank[row] = id >= 0 ? above + 1 : 0;
 }
 
 template <typename T>
@@ -513,7 +513,7 @@ k_logprobs(LogprobsArgs a) {
       ab += redi[w];
     }
     const PartView<T> pv = part_of<T>(a, row, seg);
-    if (a.segs == 1) write_chosen<T>(a, row, mb, sb, ab);
+    if (a.segs == 1) write_chosen<T>(a, row, chosen, cv, mb, sb, ab);
     int count = 0;
     if constexpr (TOP) {
       // those below `best` are not among the n: at most one entry per thread is left
@@ -555,7 +555,6 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_merge(LogprobsArgs a) {
   typedef typename O::K K;
   __shared__ K lkey[kMergeList];
   __shared__ int lid[kMergeList];
-  __shared__ double redd[kWaves];
   __shared__ int redi[kWaves];
   __shared__ K redk[kWaves];
   __shared__ int fill;
@@ -567,6 +566,9 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_merge(LogprobsArgs a) {
     double m = -INFINITY, s = 0.0;
     int above = 0, have = 0;
     K best = 0;
+    int chosen = a.ids != nullptr ? a.ids[row] : -1;
+    if ((unsigned)chosen >= (unsigned)a.V) chosen = -1;
+    const T cv = chosen >= 0 ? static_cast<const T*>(a.x)[(int64_t)row * a.ld + chosen] : (T)0;
     // a thread's first entry, loaded beside the partials
     const int64_t entries = (int64_t)a.segs * a.n;
     K ek = 0;
@@ -578,7 +580,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_merge(LogprobsArgs a) {
       eid = pv.id[ej];
       ecount = pv.part->count;
     }
-    for (int g = threadIdx.x; g < a.segs; g += kThreads) {
+    // every wave joins all partials for itself: no barrier
+    for (int g = lane(); g < a.segs; g += kWave) {
       const PartView<T> pv = part_of<T>(a, row, g);
       const Part p = *pv.part;
       const double mn = fmax(m, p.m), M = mn == -INFINITY ? 0.0 : mn;
@@ -591,14 +594,14 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_merge(LogprobsArgs a) {
         best = k > best ? k : best;
       }
     }
-    const double mb = block_max(m, redd);
-    const double Mb = mb == -INFINITY ? 0.0 : mb;
-    const double sb = block_sum(s * rescale(m, Mb, tab), redd);
-    above = block_sum(above, redi);
-    write_chosen<T>(a, row, mb, sb, above);
+    const double mb = wave_max(m);
+    const double sb = wave_sum(s * rescale(m, mb == -INFINITY ? 0.0 : mb, tab));
+    above = wave_sum(above);
+    write_chosen<T>(a, row, chosen, cv, mb, sb, above);
     if (a.n == 0) continue;
-    have = min(block_sum(have, redi), a.n);
-    best = block_max(best, redk);
+    have = min(wave_sum(have), a.n);
+    best = wave_max(best);
+    wg_barrier();  // fill is 0
     if (ej < ecount && ek >= best) {
       const int p = lds_fetch_add(&fill, 1);  // fits: a thread each
       lkey[p] = ek;

@@ -594,24 +594,28 @@ size_t act_bytes(int N, int D) {
   return (size_t)tiles_of(N, R) * R * blocks_of(D) * kBlock * 2;
 }
 
-// How a product of more than 32 rows runs: 64 or 128 rows a workgroup, and the
-// slices that k is cut into where the tiles do not fill the chip.
+// How a product of more than 32 rows runs: 128 rows a workgroup where such tiles
+// (nearly) fill the chip, one each CU, else 64, two each CU; and the slices that k is
+// cut into where the tiles are fewer than the CUs.  (Rows x 4096 x columns, 128 / 64 rows a
+// workgroup, us: 1000 x 4000, 128 tiles, 58 / 48; 100 x 16 000, 63 tiles, 37 / 33; 300 x
+// 16 000, 189 tiles, 62 / 63; 2048 x 4000, 256 tiles, 80 / 84; 2048 x 16 000 254 /
+// 263.  In slices / in one: 100 x 4096 x 4000 23 / 35 us, 100 x 1000 x 16 000 23 /
+// 16: a sum of few blocks is done before a second launch could add slices up.)
 using WideTiles = Tiles<2, 2, 8>;
 using NarrowTiles = Tiles<1, 1, 8>;
+constexpr int kSliceFrom = 12;  // blocks of a sum that is cut into slices, of at least four
 struct Plan {
   bool wide;
   int tiles, slices;
 };
 
 Plan plan_of(int N, int V, int D, int num_cu) {
-  Plan p;
-  p.wide = N > 64;
-  const int64_t t = p.wide ? (int64_t)tiles_of(V, WideTiles::kCols) * tiles_of(N, WideTiles::kRows)
-                           : (int64_t)tiles_of(V, NarrowTiles::kCols) * tiles_of(N, NarrowTiles::kRows);
-  p.tiles = (int)t;
-  // at least four blocks a slice
-  p.slices = (int)std::max<int64_t>(1, std::min<int64_t>({num_cu / t, blocks_of(D) / 4, 16}));
-  return p;
+  const int64_t w = (int64_t)tiles_of(V, WideTiles::kCols) * tiles_of(N, WideTiles::kRows);
+  const bool wide = N > 64 && 4 * w >= 3 * (int64_t)num_cu;
+  const int64_t t = wide ? w : (int64_t)tiles_of(V, NarrowTiles::kCols) * tiles_of(N, NarrowTiles::kRows);
+  const int blocks = blocks_of(D);
+  const int64_t s = blocks < kSliceFrom ? 1 : std::min<int64_t>({num_cu / t, blocks / 4, 16});
+  return Plan{wide, (int)t, (int)std::max<int64_t>(1, s)};
 }
 }  // namespace
 

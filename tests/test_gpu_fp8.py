@@ -133,6 +133,17 @@ def test_product_matches_oracle(N, V, D):
     _check(fp8_linear(_cuda(x), w, norm=_cuda(norm), eps=1e-5), ref, bound, D)
 
 
+@pytest.mark.parametrize("N,V,D", [
+    (300, 20011, 200),   # tiles of 128 rows, everything ragged
+    (129, 50001, 130),
+    (1100, 6007, 1537),  # more rows than run in ranges, k of 13 blocks
+    (40, 2000, 1536),    # slices of k
+    (200, 1000, 4000),
+])
+def test_tiles_and_slices(N, V, D):
+    test_product_matches_oracle(N, V, D)
+
+
 @pytest.mark.parametrize("N", [8, 40, 300])
 @pytest.mark.parametrize("V,D", [(333, 200), (1024, 384)])
 def test_strided_rows_and_outputs(N, V, D):

@@ -5,13 +5,14 @@
 // One pass over the logits.  A workgroup walks one segment of a row in chunks of
 // 32 KB (8192 float32 tokens), the next chunk's loads in flight while it works on one.  In
 // the walk every thread keeps its own running maximum and (float64) sum, and
-// every wave its own list of candidates for the n best with a threshold that n
-// tokens of the list reach, so that the walk has no barrier: a chunk of a wave
-// (1024 tokens) whose 64 lane maxima all lie at or below the threshold costs one
-// ballot; where n of them lie above it, the n-th largest is the new threshold.
-// At the end the waves cut their lists to n and the workgroup ranks what reaches
-// the best of the waves' thresholds.  Rows shared out over several segments leave
-// (m, sum, rank count, n candidates) each for a second launch.
+// every wave its own list of candidates for the n best, with a threshold that n
+// listed tokens reach.  The threads' maxima over the first two chunks give the
+// first threshold (about their n-th largest); from there on the walk has no barrier: a
+// chunk of a wave (1024 float32 tokens) whose 64 lane maxima all lie at or below the
+// threshold costs one ballot, and where n of them lie above it, the n-th largest is
+// the new one.  At the end the workgroup ranks what reaches the best of the waves'
+// thresholds.  Rows shared out over several segments leave (m, sum, rank count, n
+// candidates) each for a second launch.
 //
 // Tokens of -inf never enter a list: a row with fewer than n others fills up with
 // its lowest tokens that are not listed (under a grammar's mask most tokens are
@@ -19,7 +20,8 @@
 //
 // Bound by the read of the logits, where there is no list: 2048 x 32 000 58 us, 4.5
 // TB/s.  The n best cost the chains at the start and end of each segment and the
-// second launch: 256 x 128 256 33 us without, 46 us with 20 of them.
+// second launch: 256 x 128 256 33 us without, 45 us with 20 of them
+// (97 us with a threshold searched by every wave in every chunk).
 #include "plh_fast.h"
 #include "plh_kernels.h"
 

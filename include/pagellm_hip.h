@@ -291,6 +291,15 @@ int plh_process_logits(plh_ctx* ctx, const void* logits, int dtype, int64_t ld, 
                        int64_t mask_ld, int mask_rows, const int32_t* mask_row, void* out, int64_t out_ld, int flags);
 
 /*
+ * out[b] = logits[b, ids[b]], of `dtype` (NaN for an id outside [0, V)).  Of
+ * processed rows and the ids plh_sample took from them it tells the rows that
+ * rules and masks leave nothing of: those whose token stands at -inf.  (No
+ * counterpart in the reference, whose rows always keep a token.)  Uses no workspace.
+ */
+int plh_token_logits(plh_ctx* ctx, const void* logits, int dtype, int64_t ld, int B, int V, const int32_t* ids,
+                     void* out);
+
+/*
  * Log probabilities of logits rows: the chosen token's, its rank, and the
  * n_top best tokens with theirs (the reference returns none; a server's
  * `logprobs`, and the scores of a prompt's tokens).

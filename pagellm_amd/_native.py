@@ -79,6 +79,7 @@ SIGNATURES = {
         [_vp, _vp, _c_int, _c_i64, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_int,
          _vp, _vp, _c_i64, _c_int],
     ),
+    "plh_token_logits": (_c_int, [_vp, _vp, _c_int, _c_i64, _c_int, _c_int, _vp, _vp]),
     "plh_logprobs": (_c_int, [_vp, _vp, _c_int, _c_i64, _c_int, _c_int, _vp, _vp, _vp, _c_int, _vp, _vp]),
     "plh_fp8_codes_bytes": (_c_i64, [_c_int, _c_int]),
     "plh_fp8_pack": (_c_int, [_vp, _vp, _c_i64, _vp, _c_i64, _c_int, _c_int, _vp, _vp]),
@@ -372,6 +373,9 @@ class Context:
                 presence, bias_ids, bias, bias_off, mask, mask_ld, mask_rows, mask_row, out_ptr, out_ld, flags,
             )
         )
+
+    def token_logits(self, logits_ptr, dtype_code, ld, B, V, ids, out) -> None:
+        self._check(self.lib.plh_token_logits(self.handle, logits_ptr, dtype_code, ld, B, V, ids, out))
 
     def logprobs(self, logits_ptr, dtype_code, ld, B, V, ids, out_lp, out_rank, n_top=0, top_ids=None,
                  top_lp=None) -> None:

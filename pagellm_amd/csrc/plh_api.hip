@@ -704,6 +704,25 @@ int plh_process_logits(plh_ctx* c, const void* logits, int dtype, int64_t ld, in
   return PLH_OK;
 }
 
+int plh_token_logits(plh_ctx* c, const void* logits, int dtype, int64_t ld, int B, int V, const int32_t* ids,
+                     void* out) {
+  if (c == nullptr) return PLH_ERR_INVALID_ARG;
+  if (B < 0 || V < 1) return fail(c, PLH_ERR_INVALID_ARG, "need B >= 0 and V >= 1%s");
+  if (B == 0) return PLH_OK;
+  if (dtype != PLH_F32 && dtype != PLH_F64) return fail(c, PLH_ERR_INVALID_ARG, "dtype must be PLH_F32 or PLH_F64%s");
+  if (ld < V) return fail(c, PLH_ERR_INVALID_ARG, "ld must be >= V%s");
+  if (logits == nullptr || ids == nullptr || out == nullptr)
+    return fail(c, PLH_ERR_INVALID_ARG, "null device pointer%s");
+  const size_t es = dtype == PLH_F64 ? 8 : 4;
+  if (reinterpret_cast<uintptr_t>(logits) % es != 0 || reinterpret_cast<uintptr_t>(out) % es != 0)
+    return fail(c, PLH_ERR_INVALID_ARG, "logits and out must be aligned to their element size%s");
+  int rc = use_device(c);
+  if (rc != PLH_OK) return rc;
+  const hipError_t e = plh::launch_token_logits(logits, dtype == PLH_F64, ld, B, V, ids, out, c->stream);
+  if (e != hipSuccess) return hip_fail(c, e, "plh_token_logits launch");
+  return PLH_OK;
+}
+
 int plh_logprobs(plh_ctx* c, const void* logits, int dtype, int64_t ld, int B, int V, const int32_t* ids, void* out_lp,
                  int32_t* out_rank, int n_top, int32_t* top_ids, void* top_lp) {
   if (c == nullptr) return PLH_ERR_INVALID_ARG;

@@ -246,9 +246,11 @@ hipError_t launch_verify(const VerifyArgs& a, const VerifyWs& ws, bool f64, hipS
 // the partial sums, and with slices their sum).
 size_t head_ws_bytes(int N, int D, int V, int64_t ldw, int num_cu);
 hipError_t launch_head(HeadArgs a, int num_cu, hipStream_t s);
-// Biases, penalties and masks; log probabilities (plan_logprobs sets segs and
+// Biases, penalties and masks; chosen tokens' logits; log probabilities (plan_logprobs sets segs and
 // seg_chunks and returns the workspace's bytes, 0 with one segment).
 hipError_t launch_process(const ProcessArgs& a, bool f64, hipStream_t s);
+hipError_t launch_token_logits(const void* x, bool f64, int64_t ld, int B, int V, const int32_t* ids, void* out,
+                               hipStream_t s);
 size_t plan_logprobs(LogprobsArgs& a, bool f64, int num_cu, bool one_launch);
 hipError_t launch_logprobs(const LogprobsArgs& a, bool f64, hipStream_t s);
 // Products with e4m3 weights: dtype is a PLH_* code of the rows or the matrix.

@@ -4,6 +4,7 @@
 //   v = v > 0 ? v / r : v * r       tokens of the history
 //   v = v - (f * n + p)             tokens that occur n > 0 times among the outputs
 //   v = -inf                        tokens the mask rules out
+// and for the chosen tokens' processed logits (plh_token_logits).
 //
 // One workgroup per row and chunk of kProcChunk tokens.  The history and the
 // bias list are sparse and unsorted, the logits dense: the workgroup counts the
@@ -214,7 +215,28 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
   }
 }
 
+// A thread per row: one load behind another, B of them.
+template <typename T>
+__global__ __launch_bounds__(256) void k_token_logits(const T* x, int64_t ld, int B, int V, const int32_t* ids, T* out) {
+  const int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (b >= B) return;
+  const int id = ids[b];
+  out[b] = (unsigned)id < (unsigned)V ? x[b * ld + id] : (T)NAN;
+}
+
 }  // namespace
+
+hipError_t launch_token_logits(const void* x, bool f64, int64_t ld, int B, int V, const int32_t* ids, void* out,
+                               hipStream_t s) {
+  const dim3 grid((unsigned)(((int64_t)B + 255) / 256));
+  if (f64)
+    hipLaunchKernelGGL(k_token_logits<double>, grid, dim3(256), 0, s, static_cast<const double*>(x), ld, B, V, ids,
+                       static_cast<double*>(out));
+  else
+    hipLaunchKernelGGL(k_token_logits<float>, grid, dim3(256), 0, s, static_cast<const float*>(x), ld, B, V, ids,
+                       static_cast<float*>(out));
+  return hipGetLastError();
+}
 
 hipError_t launch_process(const ProcessArgs& a, bool f64, hipStream_t s) {
   const dim3 grid((a.V + kProcChunk - 1) / kProcChunk, std::min(a.B, 65535));

@@ -175,9 +175,12 @@ class BatchSampler:
         penalty, then frequency and presence penalties over the row's outputs
         (``DeviceHistories.add``'s ``prompt_len``), then the mask.  Rows without
         rules keep the sampler's own repetition penalty, and so their ids,
-        whatever rows stand beside them.  With ``logprobs`` = n the call returns
-        (ids, :class:`pagellm_amd.logits.Logprobs`): the sampled tokens' log
-        probabilities and ranks and the n best tokens under the logits as given.
+        whatever rows stand beside them.  A row whose rules and mask leave no
+        token (-inf everywhere) gives the id -1 and joins no history; its
+        Generator has moved like any other row's.  With ``logprobs`` = n the call
+        returns (ids, :class:`pagellm_amd.logits.Logprobs`): the sampled tokens'
+        log probabilities and ranks (NaN and 0 for an id of -1) and the n best
+        tokens under the logits as given.
         """
         c = self.ctx
         B = len(keys)
@@ -192,6 +195,9 @@ class BatchSampler:
             f, pr, bias_ids, bias, bias_off = _pack_rules(rules, self.hist.V)
             ruled = np.array([not rule.neutral for rule in rules], dtype=bool)
             process = masks is not None or bool(ruled.any())
+            # the rows whose tokens may all be ruled out
+            masked = masks is not None if mask_rows is None else mask_rows >= 0
+            closed = ruled | masked
         if B == 0:
             ids = np.zeros(0, dtype=np.int64)
             return ids if logprobs is None else (ids, DeviceLogprobs(c, 0, n_top, np.float32).download())
@@ -266,14 +272,30 @@ class BatchSampler:
             ptr = work.ptr
             c.process_logits(given, code, given_ld, B, V, self.hist.slab.ptr, h_sp, h_st, h_r, h_f, h_p, h_bi, h_b,
                              h_bo, h_m, mask_ld, n_masks, h_mr, ptr, ld, _native.PLH_SAMPLE_HIST_SPANS)
-        out = c.scratch("eng_out", (B,), np.int32)
+        # the ids and, with rules, behind them their processed logits
+        at = (4 * B + 7) & ~7
+        value = np.dtype(np.float64 if code == _native.PLH_F64 else np.float32)
+        out = c.scratch("eng_out", (at + value.itemsize * B if process else 4 * B,), np.uint8)
         c.sample(ptr, code, ld, B, V, self.hist.slab.ptr, d_sp, d_t, d_k, d_p, d_r, d_u,
                  out.ptr, None, _native.PLH_SAMPLE_HIST_SPANS | _nucleus_hint(t, k, p, V))
         # llm_engine.py:284: the token joins the history, on the device
         c.append_ids(self.hist.slab.ptr, d_pos, out.ptr, B)
+        if process:
+            c.token_logits(ptr, code, ld, B, V, out.ptr, out.ptr + at)
         if logprobs is not None:
-            res = DeviceLogprobs(c, B, n_top, np.float64 if code == _native.PLH_F64 else np.float32)
+            res = DeviceLogprobs(c, B, n_top, value)
             c.logprobs(given, code, given_ld, B, V, out.ptr, *res.pointers())
-        ids = out.download().astype(np.int64)
+        raw = out.download()
+        ids = raw[:4 * B].view(np.int32).astype(np.int64)
+        lps = res.download() if logprobs is not None else None
+        if process:
+            # the sampler takes a token at -inf only where there is no other
+            none = closed & np.isneginf(raw[at:].view(value))
+            if none.any():
+                ids[none] = -1
+                if lps is not None:
+                    lps.logprob[none] = np.nan
+                    lps.rank[none] = 0
+                keys = [key for key, left in zip(keys, ~none) if left]
         self.hist.advance(keys)
-        return ids if logprobs is None else (ids, res.download())
+        return ids if logprobs is None else (ids, lps)

@@ -99,3 +99,62 @@ def test_rows_without_rules_keep_their_ids_and_errors_change_nothing():
         hist.remove(0)
         hist.add(0, [1, 2], prompt_len=3)
     assert sampler.sample(x[:0], [], [], [], logprobs=2)[1].top_ids.shape == (0, 2)
+
+
+@pytest.mark.parametrize("dt", [np.float32, np.float64])
+@pytest.mark.parametrize("on_gpu", [True, False])
+@pytest.mark.parametrize("n", [65, 3000, 50257])
+def test_rows_of_which_rules_and_masks_leave_nothing(n, on_gpu, dt):
+    """Such a row gives -1, joins nothing and has no log probability, greedy or
+    sampled, whatever rows stand beside it; its sequence goes on in a later step."""
+    import torch
+
+    print(f"[answer] nothing left V={n} {dt.__name__} on_gpu={on_gpu}", flush=True)
+    g = np.random.default_rng(n)
+    x = g.normal(0, 2, (8, n)).astype(dt)
+    x[7] = -np.inf  # the model's own: no rule and no mask of this row's did it
+    greedy, drawn = SamplingParams(temperature=0.0, repetition_penalty=1.3), SamplingParams(temperature=0.9, top_p=0.9)
+    params = [greedy, drawn, drawn, greedy, drawn, drawn, greedy, greedy]
+    rules = [None] * 8
+    rules[3] = LogitRules(logit_bias={7: -np.inf, 9: -np.inf})  # all that the mask allows
+    rules[6] = LogitRules(0.5, 0.1)
+    masks = np.zeros((4, (n + 31) // 32), dtype=np.uint32)
+    masks[1] = pack_mask([7, 9], n)
+    masks[2] = pack_mask([3, 7, 9], n)
+    masks[3, -1] = (0xFFFFFFFF << (n % 32)) & 0xFFFFFFFF if n % 32 else 0  # bits past the vocabulary
+    at = [0, 0, 2, 1, None, 3, None, None]
+    hist = DeviceHistories(n, max_seqs=8, max_len=16)
+    sampler = BatchSampler(hist)
+    keys = list("abcdefgh")
+    tokens = {k: [3, 7, 9, b] for b, k in enumerate(keys)}
+    for k in keys:
+        hist.add(k, tokens[k], prompt_len=2)
+    rngs, ref_rngs = ([make_rng(i, 0) for i in range(8)] for _ in range(2))
+    logits = torch.from_numpy(x).cuda() if on_gpu else x
+    words = torch.from_numpy(masks.view(np.int32)).cuda() if on_gpu else masks
+    for given_masks in (words, None):  # a step under the masks, and one without
+        ids, lps = sampler.sample(logits, params, rngs, keys, rules=rules if given_masks is not None else None,
+                                  masks=given_masks, mask_rows=at if given_masks is not None else None, logprobs=3)
+        for b, k in enumerate(keys):
+            rule = rules[b] if given_masks is not None and rules[b] is not None else LogitRules()
+            mask = masks[at[b]] if given_masks is not None and at[b] is not None else None
+            rep = params[b].repetition_penalty
+            y = O.process_row(x[b], history=tokens[k], out_start=2, rep=1.0 if rule.neutral else rep,
+                              freq=rule.frequency_penalty, pres=rule.presence_penalty,
+                              bias=list(rule.logit_bias.items()), mask=mask).astype(dt)
+            rest = SamplingParams(temperature=params[b].temperature, top_p=params[b].top_p,
+                                  repetition_penalty=rep if rule.neutral else 1.0)
+            u = None if params[b].greedy else ref_rngs[b].random()  # drawn whether or not something is left
+            order = O.order(x[b])
+            assert np.array_equal(lps.top_ids[b], order[:3])
+            if given_masks is not None and b in (0, 1, 3, 5):
+                assert ids[b] == -1 and np.isnan(lps.logprob[b]) and lps.rank[b] == 0
+            else:
+                want = oracle.sample(y, rest, u, tokens[k])
+                assert ids[b] == want, (b, ids[b], want)
+                assert lps.rank[b] == 1 + int(np.flatnonzero(order == want)[0])
+                tokens[k].append(int(want))
+            assert hist.length(k) == len(tokens[k])
+            assert np.array_equal(hist.download(k), tokens[k])
+    for a, b in zip(rngs, ref_rngs):
+        assert a.random() == b.random()

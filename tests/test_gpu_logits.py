@@ -507,3 +507,31 @@ def test_offsets_past_32_bits_and_very_many_rows():
     assert np.array_equal(x[rows].cpu().numpy(), want)
     zero = x[1000]
     assert float(zero[3]) == -1.0 and float(zero[6]) == -0.5 and float(zero.sum()) == -1.5
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_token_logits(dt):
+    """The chosen tokens' logits, NaN for ids outside the vocabulary; rows of a wider
+    buffer; refusals."""
+    import torch
+
+    B, V, ld = 300, 1001, 1010
+    x = torch.randn((B, ld), device="cuda", dtype=getattr(torch, np.dtype(dt).name))
+    ids = torch.randint(0, V, (B,), device="cuda").to(torch.int32)
+    ids[[0, 1, 299]] = torch.tensor([-1, V, V - 1], dtype=torch.int32, device="cuda")
+    out = torch.zeros(B + 1, device="cuda", dtype=x.dtype)
+    code = _native.dtype_code(dt)
+    c = _native.Context(0)
+    c.set_stream(torch.cuda.current_stream().cuda_stream)
+    p, i, o = x.data_ptr(), ids.data_ptr(), out.data_ptr()
+    c.token_logits(p, code, ld, B, V, i, o)
+    got = out.cpu().numpy()
+    assert np.isnan(got[:2]).all() and got[B] == 0
+    assert np.array_equal(got[2:B], x.gather(1, ids.long().clamp(0, V - 1)[:, None])[2:, 0].cpu().numpy())
+    c.token_logits(None, code, ld, 0, V, None, None)
+    for args in [(None, code, ld, B, V, i, o), (p, code, ld, B, V, None, o), (p, code, ld, B, V, i, None),
+                 (p, 2, ld, B, V, i, o), (p, code, V - 1, B, V, i, o), (p, code, ld, -1, V, i, o),
+                 (p, code, ld, B, 0, i, o), (p + 2, code, ld, 1, V, i, o), (p, code, ld, B, V, i, o + 2)]:
+        with pytest.raises(ValueError):
+            c.token_logits(*args)
+    c.close()

@@ -144,3 +144,8 @@ def test_null_contexts_and_sizes():
     header = (_native.LIB_PATH.parents[1] / "include" / "pagellm_hip.h").read_text()
     for name in ("PLH_BF16", "PLH_F16", "PLH_MAX_TOP"):
         assert f"#define {name} {getattr(_native, name)}\n" in header
+
+
+def test_token_logits_without_a_context():
+    lib = _native.load_library()
+    assert lib.plh_token_logits(None, None, 0, 1, 1, 1, None, None) == -1

@@ -8,9 +8,10 @@
 
 Logits may be numpy arrays (uploaded, and the results downloaded) or torch CUDA
 tensors (read and written in place on torch's current stream; results stay on
-the GPU and nothing waits for them).  :class:`pagellm_amd.engine.BatchSampler`
-takes the same rules and masks and returns the same log probabilities for an
-engine's step.
+the GPU and the host waits for nothing: rules, masks and ids that are on the host
+go over in a queued copy, which a graph cannot capture).
+:class:`pagellm_amd.engine.BatchSampler` takes the same rules and masks and returns
+the same log probabilities for an engine's step.
 """
 
 from __future__ import annotations
@@ -161,15 +162,29 @@ def _check_mask(masks, mask_rows, B: int, V: int, device: int, logits_on_gpu: bo
     return masks, rows.astype(np.int32)
 
 
-def _pack(parts) -> tuple[np.ndarray, list[int | None]]:
+def _pinned(n: int, dtype, device):
+    """A page-locked host tensor for one queued copy to the device on torch's
+    current stream: torch's allocator hands its memory out again only when the
+    stream has passed the copy.  A graph would replay the copy from memory that is
+    another call's by then, so under capture there is none."""
+    import torch
+
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("host arguments cannot be captured into a graph: give device tensors, or capture "
+                               "Context.process_logits / Context.logprobs on device arrays")
+        return torch.empty(n, dtype=dtype, pin_memory=True)
+
+
+def _pack(parts, empty=lambda n: np.empty(n, dtype=np.uint8)) -> tuple[np.ndarray, list[int | None]]:
     """The host arrays in parts (None allowed) in one buffer, each 16-byte
-    aligned, and their offsets."""
+    aligned, and their offsets; the buffer is empty(its bytes)."""
     arrs = [None if a is None else np.ascontiguousarray(a) for a in parts]
     offs, n = [], 0
     for a in arrs:
         offs.append(None if a is None else n)
         n += 0 if a is None else (a.nbytes + 15) & ~15
-    buf = np.empty(max(n, 16), dtype=np.uint8)
+    buf = empty(max(n, 16))
     for a, o in zip(arrs, offs):
         if a is not None:
             buf[o:o + a.nbytes] = a.reshape(-1).view(np.uint8)
@@ -252,15 +267,28 @@ def process_logits(
     if B == 0:
         return out if on_gpu else logits
     host_masks = masks if masks is not None and not _is_torch_cuda(masks) else None
-    buf, offs = _pack([r, f, p, bias, bias_off, hist_off, start, bias_ids, hist_ids, mask_rows, host_masks])
+    f, p = (a if a.any() else None for a in (f, p))
+    r = r if r is not None and (r != 1.0).any() else None
+    parts = [r, f, p, bias, bias_off, hist_off, start, bias_ids, hist_ids, mask_rows, host_masks]
     code = _native.PLH_F64 if "float64" in str(logits.dtype) else _native.PLH_F32
     if on_gpu:
+        base, offs = 0, [None] * len(parts)
+        if any(a is not None for a in parts):
+            stage = None
+
+            def empty(n):
+                nonlocal stage
+                stage = _pinned(n, torch.uint8, logits.device)
+                return stage.numpy()
+
+            _, offs = _pack(parts, empty)
+            keep = stage.to(logits.device, non_blocking=True)  # torch's allocator orders its reuse on the stream
+            base = keep.data_ptr()
         c.set_stream(_stream_of(logits))
-        keep = torch.from_numpy(buf).to(logits.device)  # torch's allocator orders its reuse on the stream
-        base = keep.data_ptr()
         x, ld = logits.data_ptr(), int(logits.stride(0)) if B > 1 else V
         o, ldo = out.data_ptr(), int(out.stride(0)) if B > 1 else V
     else:
+        buf, offs = _pack(parts)
         c.set_stream(None)
         base = c.scratch_upload("process_in", buf).ptr
         dev, ld = c.upload_rows("process_x", logits)
@@ -323,6 +351,9 @@ def token_logprobs(logits, ids=None, n_top: int = 0, *, ctx: _native.Context | N
             ids = torch.as_tensor(ids)
             if ids.is_floating_point():
                 raise TypeError("ids must be integers")
+            if not ids.is_cuda:
+                stage = _pinned(B, torch.int32, logits.device)
+                ids = stage.copy_(ids).to(logits.device, non_blocking=True)
             # ids past int32 stay outside every vocabulary
             ids = ids.clamp(-1, 2**31 - 1) if ids.dtype == torch.int64 else ids
             ids = ids.to(device=logits.device, dtype=torch.int32).contiguous()

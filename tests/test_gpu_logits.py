@@ -535,3 +535,80 @@ def test_token_logits(dt):
         with pytest.raises(ValueError):
             c.token_logits(*args)
     c.close()
+
+
+def test_calls_on_cuda_tensors_wait_for_nothing():
+    """Calls with host rules, masks and ids return while their logits' producer runs,
+    and many of them in flight keep their own arguments."""
+    import torch
+
+    V, B = 5000, 4
+    g = np.random.default_rng(11)
+    a = torch.randn((8192, 8192), device="cuda", dtype=torch.bfloat16)
+    b = torch.empty_like(a)
+    src = torch.randn((B, V), device="cuda")
+    x = torch.zeros_like(src)
+    hosts = [(LogitRules(0.5, 0.25, {int(t): float(v) for t, v in zip(g.integers(0, V, 9), g.normal(0, 2, 9))}),
+              [g.integers(0, V, 30).tolist() for _ in range(B)], pack_mask(g.random(V) < 0.5, V)[None],
+              g.integers(0, V, B)) for _ in range(16)]
+
+    def calls():
+        got = []
+        for rule, hist, mask, ids in hosts:
+            y = process_logits(x, rule, contexts=hist, masks=mask, mask_rows=[0] * B)
+            got.append((y, token_logprobs(x, ids, 5)))
+        return got
+
+    def produce():
+        for _ in range(60):  # tens of milliseconds
+            torch.mm(a, a, out=b)
+        x.copy_(src)
+        e = torch.cuda.Event()
+        e.record()
+        return e
+
+    produce()
+    calls()  # the allocators' first time
+    torch.cuda.synchronize()
+    x.zero_()
+    done = produce()
+    got = calls()
+    assert not done.query(), "a call waited for the logits' producer"
+    torch.cuda.synchronize()
+    host = src.cpu().numpy()
+    for (rule, hist, mask, ids), (y, lp) in zip(hosts, got):
+        rows = [(1.0, rule, 30, 0, None)] * B
+        _check(y.cpu().numpy(), host, rows, [np.asarray(h) for h in hist], [mask[0]] * B)
+        _check_logprobs(type(lp)(*(t.cpu().numpy() for t in lp)), host, ids, 5)
+    assert token_logprobs(x[:0], [], 3).rank.shape == (0,)
+
+
+def test_calls_under_capture():
+    """Calls whose arguments are all on the device are captured; host arguments are
+    refused, and the capture goes on."""
+    import torch
+
+    V, B = 5000, 4
+    x = torch.randn((B, V), device="cuda")
+    masks = torch.randint(-2**31, 2**31 - 1, (B, -(-V // 32)), device="cuda").to(torch.int32)
+    ids = torch.tensor([1, 2, 3, 4], dtype=torch.int32, device="cuda")
+    process_logits(x, masks=masks)
+    token_logprobs(x, ids, 5)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="captured"):
+            process_logits(x, LogitRules(logit_bias={3: 1.0}))
+        with pytest.raises(RuntimeError, match="captured"):
+            token_logprobs(x, [1, 2, 3, 4])
+        y = process_logits(x, masks=masks)
+        plain = process_logits(x, LogitRules(), SamplingParams(), [[1, 2]] * B)
+        lp = token_logprobs(x, ids, 5)
+    for i in range(3):
+        x.normal_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, process_logits(x, masks=masks)) and torch.equal(plain, x)
+        _check_logprobs(type(lp)(*(t.cpu().numpy() for t in lp)), x.cpu().numpy(), ids.cpu().numpy(), 5)
+    _native.default_context().set_stream(None)

@@ -239,7 +239,7 @@ hipError_t launch_token_logits(const void* x, bool f64, int64_t ld, int B, int V
 }
 
 hipError_t launch_process(const ProcessArgs& a, bool f64, hipStream_t s) {
-  const dim3 grid((a.V + kProcChunk - 1) / kProcChunk, std::min(a.B, 65535));
+  const dim3 grid((unsigned)(((int64_t)a.V + kProcChunk - 1) / kProcChunk), std::min(a.B, 65535));
   const bool inplace = a.x == a.out;
   if (f64) {
     if (inplace) hipLaunchKernelGGL((k_process<double, true>), grid, dim3(kThreads), 0, s, a);

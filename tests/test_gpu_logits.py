@@ -612,3 +612,38 @@ def test_calls_under_capture():
         assert torch.equal(y, process_logits(x, masks=masks)) and torch.equal(plain, x)
         _check_logprobs(type(lp)(*(t.cpu().numpy() for t in lp)), x.cpu().numpy(), ids.cpu().numpy(), 5)
     _native.default_context().set_stream(None)
+
+
+def test_the_longest_row():
+    """V = 2^31 - 1, the most that the entry points take: the last chunk's bounds."""
+    import torch
+
+    V = 2**31 - 1
+    print("[logits] one row of 2^31 - 1", flush=True)
+    x = torch.zeros((1, V), device="cuda")
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    at = [0, 4095, 4096, V - 4096, V - 2, V - 1]
+    bias_ids, bias = i32(at), torch.arange(1.0, 7.0, dtype=torch.float64, device="cuda")
+    hist, off = i32([V - 1, 5, V - 1]), torch.tensor([0, 3], device="cuda")
+    f = torch.full((1,), 0.25, dtype=torch.float64, device="cuda")
+    b_off = torch.tensor([0, 6], device="cuda")
+    mask = torch.full((1, (V + 31) // 32), -1, dtype=torch.int32, device="cuda")
+    mask[0, -1] = 0x7FFFFFFF & ~(1 << 29)  # token V - 2
+    out = torch.full((1, V + 1), 7.0, device="cuda")  # and nothing past the row
+    c = _native.default_context()
+    c.set_stream(torch.cuda.current_stream().cuda_stream)
+    for o in (out, x):  # out of place, then in place
+        c.process_logits(x.data_ptr(), _native.PLH_F32, V, 1, V, hist.data_ptr(), off.data_ptr(), None, None, f.data_ptr(),
+                         None, bias_ids.data_ptr(), bias.data_ptr(), b_off.data_ptr(), mask.data_ptr(), mask.shape[1], 1,
+                         None, o.data_ptr(), V)
+        y = o[0, :V]
+        assert y[at].tolist() == [1.0, 2.0, 3.0, 4.0, -np.inf, 5.5] and float(y[5]) == -0.25
+        assert int((y != 0).sum()) == 7
+    assert float(out[0, V]) == 7.0
+    del out
+    res = token_logprobs(x, torch.tensor([V - 1], device="cuda"), 5)
+    assert res.top_ids.tolist() == [[V - 1, V - 4096, 4096, 4095, 0]] and res.rank.tolist() == [1]
+    e = np.exp(np.array([5.5, 4.0, 3.0, 2.0, 1.0, -0.25]))
+    lse = np.log(e.sum() + V - 7)
+    # the float32 terms (2^-23 of each), their float64 sum and one rounding
+    assert np.allclose(res.top_logprobs.cpu().numpy()[0], np.array([5.5, 4, 3, 2, 1]) - lse, rtol=2.0 ** -24, atol=2.0 ** -22)

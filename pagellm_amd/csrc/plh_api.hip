@@ -814,6 +814,7 @@ int plh_fp8_quantize(plh_ctx* c, const void* W, int dtype, int64_t stride_v, int
 
 int64_t plh_fp8_ws_bytes(plh_ctx* c, int N, int V, int D) {
   if (c == nullptr || N < 0 || V < 1 || D < 1) return PLH_ERR_INVALID_ARG;
+  if (plh::fp8_codes_bytes(V, D) > kMostCodes) return fail(c, PLH_ERR_UNSUPPORTED, "more than 2^35 codes%s");
   return (int64_t)plh::fp8_ws_bytes(N, V, D, c->num_cu);
 }
 

@@ -53,8 +53,11 @@ constexpr int kTileRows = 32;                     // rows of a tile of codes
 constexpr int kTileBytes = kTileRows * kBlock;    // its size
 constexpr float kE4m3Max = 448.0f;
 
-__host__ __device__ constexpr int blocks_of(int n) { return (n + kBlock - 1) / kBlock; }
-__host__ __device__ constexpr int tiles_of(int n, int rows = kTileRows) { return (n + rows - 1) / rows; }
+// n up to 2^31 - 1: the sums would pass an int
+__host__ __device__ constexpr int blocks_of(int n) { return (int)(((unsigned)n + kBlock - 1) / kBlock); }
+__host__ __device__ constexpr int tiles_of(int n, int rows = kTileRows) {
+  return (int)(((unsigned)n + (unsigned)rows - 1) / (unsigned)rows);
+}
 
 // Where the 16 codes of row r and k = 16 p .. 16 p + 15 lie, in a matrix of kb
 // blocks a row.

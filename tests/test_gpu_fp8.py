@@ -385,3 +385,17 @@ def test_refuses_more_codes_than_a_grid_holds():
     with pytest.raises(NotImplementedError):
         c.fp8_pack(256, 1 << 20, 256, 1 << 13, 1 << 16, 1 << 20, 256, 256)
     c.close()
+
+
+def test_workspaces_of_very_many_rows():
+    """The bytes of rows near 2^31 (nothing of that size is allocated), which no smaller
+    workspace passes for; matrices past 2^35 codes are refused."""
+    c = _native.Context(0)
+    for N in (2**31 - 1, 2**31 - 31, 2**31 - 32, 2**31 - 200):
+        assert c.fp8_ws_bytes(N, 1, 1) == -(-N // 32) * 32 * 128 * 2, N
+        with pytest.raises(ValueError):  # before anything is launched: the pointers are never read
+            c.fp8_linear(256, _native.PLH_BF16, 1, N, 1, None, 0.0, 256, 256, 1, 256, 1, 256, 1 << 38)
+    assert c.fp8_ws_bytes(2**31 - 1, 32, 2**30) == 2**62
+    assert c.fp8_ws_bytes(1, 2**31 - 1, 2**31 - 1) == _native.PLH_ERR_UNSUPPORTED
+    assert c.fp8_ws_bytes(1, 2**29, 128) == _native.PLH_ERR_UNSUPPORTED
+    c.close()

@@ -141,6 +141,8 @@ def _check_mask(masks, mask_rows, B: int, V: int, device: int, logits_on_gpu: bo
             raise ValueError(f"masks are on GPU {masks.device.index}, the context on GPU {device}")
         if masks.dim() != 2 or masks.stride(1) != 1 and masks.shape[1] > 1:
             raise ValueError("masks must be [rows, words] with unit stride")
+        if masks.shape[0] > 1 and masks.stride(0) < mask_words(V):
+            raise ValueError("rows of masks must not overlap (let rows share one by mask_rows)")
     else:
         masks = np.asarray(masks)
         if masks.dtype not in (np.dtype(np.uint32), np.dtype(np.int32)):

@@ -11,7 +11,7 @@ import oracle
 from oracle import logits as O
 from pagellm_amd.engine import BatchSampler, DeviceHistories
 from pagellm_amd.fp8 import Fp8LogitsHead
-from pagellm_amd.logits import LogitRules, pack_mask
+from pagellm_amd.logits import LogitRules, pack_mask, process_logits
 from pagellm_amd.params import SamplingParams, make_rng
 
 pytestmark = pytest.mark.gpu
@@ -158,3 +158,24 @@ def test_rows_of_which_rules_and_masks_leave_nothing(n, on_gpu, dt):
             assert np.array_equal(hist.download(k), tokens[k])
     for a, b in zip(rngs, ref_rngs):
         assert a.random() == b.random()
+
+
+def test_masks_whose_rows_overlap_are_refused_before_a_generator_moves():
+    import torch
+
+    x = torch.randn((3, V), device="cuda")
+    hist = DeviceHistories(V, max_seqs=3, max_len=8)
+    for k in range(3):
+        hist.add(k, [1, 2])
+    rngs = [make_rng(k, 0) for k in range(3)]
+    words = torch.from_numpy(pack_mask([4, 5], V).view(np.int32)).cuda()
+    sampler = BatchSampler(hist)
+    for masks in (words[None].expand(3, -1), torch.zeros(94 * 3, dtype=torch.int32, device="cuda").as_strided((3, 94), (93, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            sampler.sample(x, SamplingParams(), rngs, [0, 1, 2], masks=masks)
+        with pytest.raises(ValueError, match="overlap"):
+            process_logits(x, masks=masks)
+    assert [r.random() for r in rngs] == [make_rng(k, 0).random() for k in range(3)]
+    # what is meant: one row of masks for all
+    ids = sampler.sample(x, SamplingParams(), rngs, [0, 1, 2], masks=words[None].expand(1, -1), mask_rows=[0, 0, 0])
+    assert set(ids) <= {4, 5}

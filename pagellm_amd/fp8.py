@@ -70,6 +70,8 @@ class Fp8Weights:
         self.ctx, self.V, self.D = ctx, int(V), int(D)
         if self.V < 1 or self.D < 1:
             raise ValueError("the matrix must be [V, D] with V, D >= 1")
+        if max(self.V, self.D) > 2**31 - 1:  # ctypes would wrap them
+            raise ValueError("at most 2^31 - 1 rows and columns")
         dev = torch.device("cuda", ctx.device)
         nbytes = int(ctx.lib.plh_fp8_codes_bytes(self.V, self.D))
         self.codes = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -146,6 +148,8 @@ def fp8_linear(x, weights: Fp8Weights, *, norm=None, eps: float = 1e-5, out=None
     if x.dim() != 2 or int(x.shape[1]) != weights.D:
         raise ValueError(f"x must be [N, {weights.D}]")
     N, V = int(x.shape[0]), weights.V
+    if N > 2**31 - 1:  # ctypes would wrap it
+        raise ValueError("at most 2^31 - 1 rows")
     if x.numel() and x.stride(1) != 1 and weights.D > 1:
         raise ValueError("x must have unit stride in its last dimension")
     if norm is not None:

@@ -123,6 +123,13 @@ def _pack_rules(rules: Sequence[LogitRules], V: int):
     return f, p, np.concatenate([r._ids for r in rules]), np.concatenate([r._values for r in rules]), off
 
 
+def _check_sizes(B: int, V: int) -> None:
+    if V == 0:
+        raise ValueError("empty vocabulary")
+    if max(B, V) > 2**31 - 1:  # ctypes would wrap them
+        raise ValueError("at most 2^31 - 1 rows and tokens")
+
+
 def _check_mask(masks, mask_rows, B: int, V: int, device: int, logits_on_gpu: bool):
     """(masks, per-row int32 mask rows or None) of a call; masks as a CUDA
     tensor or a contiguous uint32 array."""
@@ -240,8 +247,7 @@ def process_logits(
         if logits.ndim != 2:
             raise ValueError("logits must be [B, V]")
     B, V = int(logits.shape[0]), int(logits.shape[1])
-    if V == 0:
-        raise ValueError("empty vocabulary")
+    _check_sizes(B, V)
     rules = _expand_rules(rules, B)
     params = _expand_params(params, B) if params is not None else None
     masks, mask_rows = _check_mask(masks, mask_rows, B, V, c.device, on_gpu)
@@ -336,8 +342,7 @@ def token_logprobs(logits, ids=None, n_top: int = 0, *, ctx: _native.Context | N
         if logits.ndim != 2:
             raise ValueError("logits must be [B, V]")
     B, V = int(logits.shape[0]), int(logits.shape[1])
-    if V == 0:
-        raise ValueError("empty vocabulary")
+    _check_sizes(B, V)
     n = int(n_top)
     if not 0 <= n <= min(V, _native.PLH_MAX_TOP):
         raise ValueError(f"n_top must be in [0, {min(V, _native.PLH_MAX_TOP)}]")

@@ -399,3 +399,17 @@ def test_workspaces_of_very_many_rows():
     assert c.fp8_ws_bytes(1, 2**31 - 1, 2**31 - 1) == _native.PLH_ERR_UNSUPPORTED
     assert c.fp8_ws_bytes(1, 2**29, 128) == _native.PLH_ERR_UNSUPPORTED
     c.close()
+
+
+def test_sizes_past_int32_are_refused():
+    """Not taken modulo 2^32 (nothing but the allocation happens at these sizes)."""
+    import torch
+
+    w = Fp8Weights.from_codes(np.zeros((1, 1), np.uint8), np.ones((1, 1), np.float32))
+    print("[fp8] 2^32 + 10 rows", flush=True)
+    x = torch.empty(2**32 + 10, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="2\\^31"):
+        fp8_linear(x[:, None], w, out=torch.empty(1, device="cuda").expand(2**32 + 10, 1))
+    for m in (x[:, None], x[None]):
+        with pytest.raises(ValueError, match="2\\^31"):
+            Fp8Weights.quantize(m)

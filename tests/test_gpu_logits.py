@@ -647,3 +647,16 @@ def test_the_longest_row():
     lse = np.log(e.sum() + V - 7)
     # the float32 terms (2^-23 of each), their float64 sum and one rounding
     assert np.allclose(res.top_logprobs.cpu().numpy()[0], np.array([5.5, 4, 3, 2, 1]) - lse, rtol=2.0 ** -24, atol=2.0 ** -22)
+
+
+def test_sizes_past_int32_are_refused():
+    """Not taken modulo 2^32 (nothing but the allocation happens at these sizes)."""
+    import torch
+
+    print("[logits] 2^32 + 10 tokens", flush=True)
+    x = torch.empty(2**32 + 10, device="cuda")
+    for t in (x[None], x[:, None]):
+        with pytest.raises(ValueError, match="2\\^31"):
+            process_logits(t, out=t)
+        with pytest.raises(ValueError, match="2\\^31"):
+            token_logprobs(t, None, 1)

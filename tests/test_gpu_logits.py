@@ -660,3 +660,62 @@ def test_sizes_past_int32_are_refused():
             process_logits(t, out=t)
         with pytest.raises(ValueError, match="2\\^31"):
             token_logprobs(t, None, 1)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("V", [4063, 4064, 4095, 4096, 4097, 4100, 8191, 8195, 12287, 12289])
+def test_process_around_its_chunks(V, dt):
+    """k_process takes 4096 tokens a workgroup: rows that end just before, at and behind
+    a chunk, in place and not."""
+    import torch
+
+    print(f"[process] chunks V={V} {dt.__name__}", flush=True)
+    x, rows, hist, masks = _case(V, 7, V, dt)
+    got = _run_numpy(x, rows, hist, masks)
+    _check(got, x, rows, hist, masks)
+    t = torch.from_numpy(x).cuda()
+    words = np.stack([m if m is not None else pack_mask(np.ones(V, bool), V) for m in masks])
+    process_logits(t, [k[1] for k in rows], [SamplingParams(repetition_penalty=k[0]) for k in rows], hist,
+                   prompt_lens=[k[3] for k in rows], masks=words, out=t)
+    assert np.array_equal(t.cpu().numpy(), got)
+
+
+def _shares(B, V, dt, cus):
+    """(segments, chunks of one) of rows: at most two workgroups a CU, whole chunks of
+    8192 float32 or 4096 float64 tokens each, one segment up to three chunks."""
+    chunks = -(-V // (8192 if dt == np.float32 else 4096))
+    each = chunks if chunks <= 3 else min(chunks, -(-B * chunks // (2 * cus)))
+    return -(-chunks // each), each
+
+
+@pytest.mark.parametrize("n", [0, 20, 64])
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("B,V", [(256, 128256), (200, 70000), (100, 152064), (140, 41000), (190, 41000)])
+def test_logprobs_segments_of_many_chunks(B, V, dt, n):
+    """Rows cut into several segments of several chunks each: a segment's own threshold
+    from its third chunk on, away from the row's start, and the second launch's join."""
+    import torch
+
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    segs, each = _shares(B, V, dt, cus)
+    assert segs >= 2 and each >= (2 if B == 140 else 3), (segs, each)  # 140 float32 rows: segments of two
+    g = np.random.default_rng(V + n)
+    kinds = np.concatenate([_hard_rows(g, V, dt), np.zeros((8, V), dt)])
+    more = kinds[12:]
+    more[:] = g.normal(0, 1, more.shape)
+    for b, at in enumerate([slice(0, 70), slice(V - 70, V), slice(V // 2, V // 2 + 64), slice(0, V, V // 65)]):
+        more[b, at] = np.nan
+    more[4, V // 2:] = 9.0                       # like values over whole segments
+    more[5] = np.floor(np.arange(V) / 100)       # every chunk larger than the one before
+    more[6, ::2] = 3.0
+    more[7] = np.arange(V)[::-1] // 4096 + g.random(V)  # the best at each segment's start
+    rows = np.arange(B) % 20
+    ids = g.integers(0, V, B)
+    print(f"[logprobs] segments B={B} V={V} {dt.__name__} n={n}: {segs} of {each} chunks", flush=True)
+    res = token_logprobs(torch.from_numpy(kinds).cuda()[torch.from_numpy(rows).cuda()], ids, n)
+    res = type(res)(*(t.cpu().numpy() for t in res))
+    _check_logprobs(type(res)(*(a[B - 20:] for a in res)), kinds[rows[B - 20:]], ids[B - 20:], n)
+    # like rows, like answers
+    for k in range(20):
+        same = res.top_ids[rows == k]
+        assert (same == same[0]).all()

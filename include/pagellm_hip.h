@@ -112,6 +112,15 @@ int plh_d2h(plh_ctx* ctx, void* dst, const void* src, size_t bytes);
 int plh_host_alloc(plh_ctx* ctx, void** out, size_t bytes);
 int plh_host_free(plh_ctx* ctx, void* ptr);
 int plh_h2d_async(plh_ctx* ctx, void* dst, const void* src, size_t bytes);
+/* The same for callers that wait for nothing.  plh_stage gives `bytes` of
+ * page-locked memory to fill, the context's; plh_stage_h2d queues the copy of
+ * what stands there to dst and takes the memory back (bytes 0: takes it back
+ * alone).  It is given out again when the stream has passed the copy; while
+ * copies are under way there is more of it.  Not under graph capture, where a
+ * replay would copy what stands there by then (PLH_ERR_UNSUPPORTED).  No
+ * reference counterpart. */
+int plh_stage(plh_ctx* ctx, void** out, size_t bytes);
+int plh_stage_h2d(plh_ctx* ctx, void* dst, const void* src, size_t bytes);
 int plh_sync(plh_ctx* ctx);
 
 /*

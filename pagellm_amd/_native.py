@@ -53,6 +53,8 @@ SIGNATURES = {
     "plh_host_alloc": (_c_int, [_vp, ctypes.POINTER(_vp), _c_sz]),
     "plh_host_free": (_c_int, [_vp, _vp]),
     "plh_h2d_async": (_c_int, [_vp, _vp, _vp, _c_sz]),
+    "plh_stage": (_c_int, [_vp, _vp, _c_sz]),
+    "plh_stage_h2d": (_c_int, [_vp, _vp, _vp, _c_sz]),
     "plh_sync": (_c_int, [_vp]),
     "plh_sample": (
         _c_int,
@@ -288,6 +290,17 @@ class Context:
         the context's stream; src must stay unchanged until the stream has
         passed it (the next download or sync)."""
         self._check(self.lib.plh_h2d_async(self.handle, dst_ptr, src.ctypes.data, src.nbytes))
+
+    def stage(self, nbytes: int) -> np.ndarray:
+        """Page-locked memory (uint8) to fill for one stage_h2d, which must follow."""
+        ptr = _vp()
+        self._check(self.lib.plh_stage(self.handle, ctypes.byref(ptr), nbytes))
+        return np.ctypeslib.as_array((ctypes.c_uint8 * nbytes).from_address(ptr.value))
+
+    def stage_h2d(self, dst_ptr: int, src: np.ndarray) -> None:
+        """Queues the copy of src (from stage()) on the context's stream and gives
+        src back: it must not be touched any more."""
+        self._check(self.lib.plh_stage_h2d(self.handle, dst_ptr, src.ctypes.data, src.nbytes))
 
     def stage_upload(self, name: str, parts) -> list[int]:
         """Copy the host arrays in parts to one device buffer with a single

@@ -40,6 +40,15 @@ struct plh_ctx {
   bool timing = false;
   std::vector<hipEvent_t> ev_free;
   std::vector<std::array<hipEvent_t, 3>> ev_pending;
+  // plh_stage: page-locked buffers; `done` closes the last copy from one
+  struct Stage {
+    void* host;
+    size_t bytes;
+    hipEvent_t done;
+    bool given;   // between plh_stage and plh_stage_h2d
+    bool queued;  // a copy was queued and is not known to have ended
+  };
+  std::vector<Stage> stages;
   std::string err;
 };
 
@@ -327,6 +336,11 @@ void plh_destroy(plh_ctx* c) {
   for (auto& t : c->ev_pending)
     for (hipEvent_t e : t) c->ev_free.push_back(e);
   for (hipEvent_t e : c->ev_free) (void)hipEventDestroy(e);
+  for (plh_ctx::Stage& s : c->stages) {
+    if (s.queued) (void)hipEventSynchronize(s.done);
+    (void)hipEventDestroy(s.done);
+    (void)hipHostFree(s.host);
+  }
   if (c->fallback != nullptr) (void)hipFree(c->fallback);
   if (c->own_stream != nullptr) (void)hipStreamDestroy(c->own_stream);
   delete c;
@@ -469,6 +483,74 @@ int plh_h2d_async(plh_ctx* c, void* dst, const void* src, size_t bytes) {
   if (bytes == 0) return PLH_OK;
   PLH_HIP(c, hipMemcpyAsync(dst, src, bytes, hipMemcpyHostToDevice, c->stream), "hipMemcpyAsync(H2D)");
   return PLH_OK;
+}
+
+int plh_stage(plh_ctx* c, void** out, size_t bytes) {
+  if (c == nullptr || out == nullptr) return PLH_ERR_INVALID_ARG;
+  *out = nullptr;
+  int rc = use_device(c);
+  if (rc != PLH_OK) return rc;
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  PLH_HIP(c, hipStreamIsCapturing(c->stream, &st), "hipStreamIsCapturing");
+  if (st != hipStreamCaptureStatusNone)
+    return fail(c, PLH_ERR_UNSUPPORTED, "arguments in host memory cannot be captured into a graph%s");
+  plh_ctx::Stage* fit = nullptr;
+  for (plh_ctx::Stage& s : c->stages) {
+    if (s.given || s.bytes < bytes || (fit != nullptr && fit->bytes <= s.bytes)) continue;
+    if (s.queued) {
+      const hipError_t e = hipEventQuery(s.done);
+      if (e == hipErrorNotReady) (void)hipGetLastError();  // no error: launches ask for the last one
+      if (e != hipSuccess) continue;
+      s.queued = false;
+    }
+    fit = &s;
+  }
+  if (fit == nullptr) {
+    // powers of two, so that a few buffers serve calls of all sizes
+    size_t size = 4096;
+    while (size < bytes) size *= 2;
+    plh_ctx::Stage s{nullptr, size, nullptr, false, false};
+    PLH_HIP(c, hipHostMalloc(&s.host, size, hipHostMallocDefault), "hipHostMalloc");
+    hipError_t e = hipEventCreateWithFlags(&s.done, hipEventDisableTiming);
+    if (e == hipSuccess) {
+      try {
+        c->stages.push_back(s);
+      } catch (const std::bad_alloc&) {
+        (void)hipEventDestroy(s.done);
+        e = hipErrorOutOfMemory;
+      }
+    }
+    if (e != hipSuccess) {
+      (void)hipHostFree(s.host);
+      return hip_fail(c, e, "plh_stage");
+    }
+    fit = &c->stages.back();
+  }
+  fit->given = true;
+  *out = fit->host;
+  return PLH_OK;
+}
+
+int plh_stage_h2d(plh_ctx* c, void* dst, const void* src, size_t bytes) {
+  if (c == nullptr || src == nullptr) return PLH_ERR_INVALID_ARG;
+  for (plh_ctx::Stage& s : c->stages) {
+    if (s.host != src || !s.given) continue;
+    if (bytes > s.bytes || (bytes > 0 && dst == nullptr))
+      return fail(c, PLH_ERR_INVALID_ARG, "need dst, and no more bytes than the buffer has%s");
+    s.given = false;
+    if (bytes == 0) return PLH_OK;
+    int rc = use_device(c);
+    if (rc != PLH_OK) return rc;
+    PLH_HIP(c, hipMemcpyAsync(dst, src, bytes, hipMemcpyHostToDevice, c->stream), "hipMemcpyAsync(H2D)");
+    const hipError_t e = hipEventRecord(s.done, c->stream);
+    if (e != hipSuccess) {
+      (void)hipStreamSynchronize(c->stream);  // nothing tells when the copy ends
+      return hip_fail(c, e, "hipEventRecord");
+    }
+    s.queued = true;
+    return PLH_OK;
+  }
+  return fail(c, PLH_ERR_INVALID_ARG, "src is not memory that plh_stage gave%s");
 }
 
 int plh_d2h(plh_ctx* c, void* dst, const void* src, size_t bytes) {

@@ -171,20 +171,6 @@ def _check_mask(masks, mask_rows, B: int, V: int, device: int, logits_on_gpu: bo
     return masks, rows.astype(np.int32)
 
 
-def _pinned(n: int, dtype, device):
-    """A page-locked host tensor for one queued copy to the device on torch's
-    current stream: torch's allocator hands its memory out again only when the
-    stream has passed the copy.  A graph would replay the copy from memory that is
-    another call's by then, so under capture there is none."""
-    import torch
-
-    with torch.cuda.device(device):
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("host arguments cannot be captured into a graph: give device tensors, or capture "
-                               "Context.process_logits / Context.logprobs on device arrays")
-        return torch.empty(n, dtype=dtype, pin_memory=True)
-
-
 def _pack(parts, empty=lambda n: np.empty(n, dtype=np.uint8)) -> tuple[np.ndarray, list[int | None]]:
     """The host arrays in parts (None allowed) in one buffer, each 16-byte
     aligned, and their offsets; the buffer is empty(its bytes)."""
@@ -280,19 +266,13 @@ def process_logits(
     parts = [r, f, p, bias, bias_off, hist_off, start, bias_ids, hist_ids, mask_rows, host_masks]
     code = _native.PLH_F64 if "float64" in str(logits.dtype) else _native.PLH_F32
     if on_gpu:
+        c.set_stream(_stream_of(logits))
         base, offs = 0, [None] * len(parts)
         if any(a is not None for a in parts):
-            stage = None
-
-            def empty(n):
-                nonlocal stage
-                stage = _pinned(n, torch.uint8, logits.device)
-                return stage.numpy()
-
-            _, offs = _pack(parts, empty)
-            keep = stage.to(logits.device, non_blocking=True)  # torch's allocator orders its reuse on the stream
-            base = keep.data_ptr()
-        c.set_stream(_stream_of(logits))
+            buf, offs = _pack(parts, c.stage)
+            keep = torch.empty(buf.size, dtype=torch.uint8, device=logits.device)
+            base = keep.data_ptr()  # torch's allocator orders its reuse on the stream
+            c.stage_h2d(base, buf)
         x, ld = logits.data_ptr(), int(logits.stride(0)) if B > 1 else V
         o, ldo = out.data_ptr(), int(out.stride(0)) if B > 1 else V
     else:
@@ -354,13 +334,16 @@ def token_logprobs(logits, ids=None, n_top: int = 0, *, ctx: _native.Context | N
     if ids is not None and tuple(ids.shape) != (B,):
         raise ValueError(f"expected {B} ids")
     if on_gpu:
-        if ids is not None:
-            ids = torch.as_tensor(ids)
+        c.set_stream(_stream_of(logits))
+        if isinstance(ids, np.ndarray):
+            host, ids = ids, torch.empty(B, dtype=torch.int32, device=logits.device)
+            if B:
+                buf = c.stage(host.nbytes)
+                buf[:] = host.view(np.uint8)
+                c.stage_h2d(ids.data_ptr(), buf)
+        elif ids is not None:
             if ids.is_floating_point():
                 raise TypeError("ids must be integers")
-            if not ids.is_cuda:
-                stage = _pinned(B, torch.int32, logits.device)
-                ids = stage.copy_(ids).to(logits.device, non_blocking=True)
             # ids past int32 stay outside every vocabulary
             ids = ids.clamp(-1, 2**31 - 1) if ids.dtype == torch.int64 else ids
             ids = ids.to(device=logits.device, dtype=torch.int32).contiguous()
@@ -370,7 +353,6 @@ def token_logprobs(logits, ids=None, n_top: int = 0, *, ctx: _native.Context | N
                        new((B, n), torch.int32), new((B, n), logits.dtype))
         if B == 0:
             return res
-        c.set_stream(_stream_of(logits))
         code = _native.PLH_F64 if logits.dtype == torch.float64 else _native.PLH_F32
         ptr = lambda t: t.data_ptr() if t is not None and t.numel() else None  # noqa: E731
         c.logprobs(logits.data_ptr(), code, int(logits.stride(0)) if B > 1 else V, B, V, ptr(ids), ptr(res.logprob),

@@ -719,3 +719,42 @@ def test_logprobs_segments_of_many_chunks(B, V, dt, n):
     for k in range(20):
         same = res.top_ids[rows == k]
         assert (same == same[0]).all()
+
+
+def test_staged_copies():
+    """Memory that is given out twice is two buffers, and is not given again before its
+    copy has ended; refusals leave it given."""
+    import torch
+
+    c = _native.Context(0)
+    n = 100_000
+    d = torch.zeros((40, n), dtype=torch.uint8, device="cuda")
+    side = torch.cuda.Stream()
+    a = torch.randn((4096, 4096), device="cuda")
+    for stream in (None, side):
+        with torch.cuda.stream(stream):
+            torch.cuda.synchronize()
+            for _ in range(20):
+                torch.mm(a, a)
+            c.set_stream(torch.cuda.current_stream().cuda_stream)
+            for i in range(40):
+                s = c.stage(n - i)
+                s[:] = i + 1
+                c.stage_h2d(d[i].data_ptr(), s)
+            got = d.clone()
+        torch.cuda.synchronize()
+        for i in range(40):
+            assert bool((got[i, :n - i] == i + 1).all()) and not bool(got[i, n - i:].any())
+        d.zero_()
+    s, t = c.stage(10), c.stage(10)
+    assert s.ctypes.data != t.ctypes.data
+    with pytest.raises(ValueError):
+        c.stage_h2d(d.data_ptr(), np.zeros(10, np.uint8))
+    with pytest.raises(ValueError):
+        c.stage_h2d(None, s)
+    with pytest.raises(ValueError):
+        c._check(c.lib.plh_stage_h2d(c.handle, d.data_ptr(), s.ctypes.data, 1 << 30))
+    c.stage_h2d(None, s[:0])  # given back alone
+    with pytest.raises(ValueError):
+        c.stage_h2d(d.data_ptr(), s)
+    c.close()

@@ -155,3 +155,9 @@ def test_sizes_of_very_large_matrices():
     lib = _native.load_library()
     for V, D in [(2**31 - 1, 1), (1, 2**31 - 1), (2**31 - 31, 129), (2**31 - 1, 2**31 - 1), (2**28, 128)]:
         assert lib.plh_fp8_codes_bytes(V, D) == -(-V // 32) * -(-D // 128) * 4096, (V, D)
+
+
+def test_stage_without_a_context():
+    lib = _native.load_library()
+    assert lib.plh_stage(None, None, 8) == -1
+    assert lib.plh_stage_h2d(None, None, None, 0) == -1

@@ -179,3 +179,49 @@ def test_masks_whose_rows_overlap_are_refused_before_a_generator_moves():
     # what is meant: one row of masks for all
     ids = sampler.sample(x, SamplingParams(), rngs, [0, 1, 2], masks=words[None].expand(1, -1), mask_rows=[0, 0, 0])
     assert set(ids) <= {4, 5}
+
+
+def test_the_chain_captured_behind_eager_calls():
+    """e4m3 logits, masks and log probabilities in one graph, captured while the context's
+    workspace is in use by eager calls of the default stream; replays between such calls
+    match them."""
+    import torch
+
+    from pagellm_amd.logits import token_logprobs
+
+    n, rows = 100000, 3
+    g = np.random.default_rng(2)
+    norm = np.ones(D, np.float32)
+    head = Fp8LogitsHead(norm, (0.1 * g.standard_normal((D, n))).astype(np.float32))
+    h = torch.randn((rows, D), device="cuda")
+    masks = torch.from_numpy(np.stack([pack_mask(g.random(n) < 0.4, n) for _ in range(rows)]).view(np.int32)).cuda()
+    ids = torch.tensor([5, 6, 7], dtype=torch.int32, device="cuda")
+
+    def chain():
+        logits = head(h)
+        left = process_logits(logits, masks=masks)
+        return logits, left, token_logprobs(left, ids, 20)
+
+    chain()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        chain()
+    torch.cuda.synchronize()
+    chain()  # several workgroups a row: the workspace
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain()
+    for _ in range(3):
+        h.normal_()
+        want = chain()
+        graph.replay()
+        again = chain()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(again[1], want[1])
+        assert torch.equal(got[2].top_ids, want[2].top_ids) and torch.equal(got[2].rank, want[2].rank)
+        assert torch.equal(again[2].top_logprobs, want[2].top_logprobs)
+        # one segment a row in the graph: another order of float64 sums, one rounding
+        fin = torch.isfinite(want[2].logprob)
+        assert torch.equal(fin, torch.isfinite(got[2].logprob))
+        assert float((got[2].top_logprobs - want[2].top_logprobs).abs().max()) < 2e-6
+        assert float((got[2].logprob - want[2].logprob)[fin].abs().sum()) < 6e-6

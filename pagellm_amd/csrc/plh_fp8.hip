@@ -142,8 +142,9 @@ __device__ __forceinline__ float row16_max(float v) {
 
 // One workgroup per row, more than 2^20 rows in turn (a grid holds 2^32 threads); a
 // block's 16 threads are one row of 16 lanes.  The norm is computed in float64: a last
-// bit of y next to a border between two codes would change the code.  8 x 4096 float32 4.8 us (its chain of loads and sums), 2048 x
-// 4096 bf16 22 us (the 16-byte stores of the operand's layout).
+// bit of y next to a border between two codes would change the code.  8 x 4096 float32
+// 5 us (its chain of loads and sums), 2048 x 4096 bf16 23-24 us (the 16-byte stores of the
+// operand's layout, 512 bytes apart).
 template <typename TX, int R>
 __global__ __launch_bounds__(kThreads) void k_fp8_act(Fp8Args a) {
   __shared__ double red[kWaves];
@@ -355,8 +356,9 @@ constexpr int kVector = 0x002, kMatrix = 0x008, kDsRead = 0x100;
 // keeps a wave's tile at 64 x 64.
 //
 // Bound by the matrix cores at the clock that the power limit leaves them (1.9 GHz; operands
-// of zeros run a fifth faster), 53% busy: 256 x 4096 x 128 256 266-273 us, 2048 x 4096 x
-// 32 000 497-514 us (1.05 PFLOP/s; a large bf16 matrix product reaches 1.2 here).  What it
+// of zeros run a fifth faster), 53% busy: 256 x 4096 x 128 256 263-274 us, 2048 x 4096 x
+// 32 000 493-520 us (1.03-1.09 PFLOP/s; a large bf16 matrix product reaches 1.2 here); 33,
+// 64 and 128 rows x 4096 x 128 256 109, 117 and 152 us.  What it
 // took there: loads issued where they are wanted (582 -> 540 us: the compiler sinks
 // them to their use), LDS reads and vector instructions placed among the products
 // (-> 532), three LDS buffers instead of two (256 rows: 283 -> 274), whole runs of
@@ -521,7 +523,8 @@ __global__ __launch_bounds__(256) void k_fp8_sum(Fp8Args a, int slices) {
 
 // ---------------------------------------------------------------- weights
 
-// One thread per 16 codes of the layout.
+// One thread per 16 codes of the layout, read byte by byte: rows start anywhere.  Once a
+// model: 128 256 x 4096 0.8 ms.
 __global__ __launch_bounds__(256) void k_fp8_pack(const uint8_t* codes, int64_t ldc, const float* scales, int64_t lds,
                                                   int V, int D, uint8_t* out, float* out_scales) {
   const int kb = blocks_of(D);
@@ -537,8 +540,9 @@ __global__ __launch_bounds__(256) void k_fp8_pack(const uint8_t* codes, int64_t 
   if (i < (int64_t)blocks_of(V) * kb) out_scales[i] = scales[i / kb * lds + i % kb];
 }
 
-// One workgroup of 256 threads per block of 128 x 128.  `along_v`: neighbouring threads take neighbouring rows (W is
-// contiguous along v).
+// One workgroup of 256 threads per block of 128 x 128.  `along_v`: neighbouring threads
+// take neighbouring rows (W is contiguous along v).  Once a model: 128 256 x 4096 2.1 ms from
+// float32, either way round.
 template <typename TW>
 __global__ __launch_bounds__(256) void k_fp8_quantize(const TW* W, int64_t sv, int64_t sd, int V, int D, uint8_t* out,
                                                       float* out_scales) {

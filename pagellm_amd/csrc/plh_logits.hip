@@ -15,8 +15,8 @@
 // (from L2), 4 H bytes beside the 8 * kProcChunk of its logits.
 //
 // Bound by the read and write of the logits: 256 x 128 256, half of the rows with
-// 2048-token histories and half with masks, 64 us (logits not in the caches; a copy of them
-// 50 us), 53 us where they are.  Chunks of 4096 with at most 64 registers put four
+// 2048-token histories and half with masks, 65 us (logits not in the caches; a copy of them
+// 50 us), 54 us where they are.  In place, masks that leave most quads alone 34 us.  Chunks of 4096 with at most 64 registers put four
 // workgroups on a CU (chunks of 8192, two: 60 us); four history loads in flight a thread
 // (64 x 128 256 with 32 768-token histories: 61 -> 39 us).
 #include "plh_device.h"

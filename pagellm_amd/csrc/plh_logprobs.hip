@@ -18,9 +18,9 @@
 // its lowest tokens that are not listed (under a grammar's mask most tokens are
 // -inf).  All counts are integers and all sums have a fixed order.
 //
-// Bound by the read of the logits, where there is no list: 2048 x 32 000 58 us, 4.5
+// Bound by the read of the logits, where there is no list: 2048 x 32 000 57 us, 4.6
 // TB/s.  The n best cost the chains at the start and end of each segment and the
-// second launch: 256 x 128 256 33 us without, 45 us with 20 of them
+// second launch: 256 x 128 256 33 us without, 46-47 us with 20 of them
 // (97 us with a threshold searched by every wave in every chunk).
 #include "plh_fast.h"
 #include "plh_kernels.h"
@@ -666,7 +666,8 @@ hipError_t launch_t(const LogprobsArgs& a, hipStream_t s) {
 }  // namespace
 
 // Segments: as many workgroups as fit the chip at once, two per compute unit, a
-// whole chunk or more each (256 x 128256, 20 best: 49 us, with four 57 us).  Rows of
+// whole chunk or more each (256 x 128256, 20 best, when this was chosen: 49 us, with four 57
+// us).  Rows of
 // up to three chunks take one: a second launch costs more than the chunks behind one
 // another (64 rows of two chunks 10.3 -> 7.8 us, with 20 best 17.8 -> 14.4 us; three:
 // 10.4 -> 9.4, 18.2 -> 17.0 us; four: 10.4 -> 10.3, 19.0 -> 19.5 us).

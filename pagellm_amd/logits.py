@@ -35,7 +35,8 @@ class LogitRules:
     ``frequency_penalty`` is taken off a token's logit once for each time it
     occurs among the request's outputs, ``presence_penalty`` once if it occurs
     at all; ``logit_bias`` maps token ids to what is added to their logits
-    (-inf rules a token out)."""
+    (-inf rules a token out).  The mapping is packed here: changing it later
+    changes nothing."""
 
     frequency_penalty: float = 0.0
     presence_penalty: float = 0.0

@@ -270,8 +270,14 @@ def process_logits(
         c.set_stream(_stream_of(logits))
         base, offs = 0, [None] * len(parts)
         if any(a is not None for a in parts):
-            buf, offs = _pack(parts, c.stage)
-            keep = torch.empty(buf.size, dtype=torch.uint8, device=logits.device)
+            keep = None
+
+            def empty(n):
+                nonlocal keep  # first: what fails here leaves no staged memory given
+                keep = torch.empty(n, dtype=torch.uint8, device=logits.device)
+                return c.stage(n)
+
+            buf, offs = _pack(parts, empty)
             base = keep.data_ptr()  # torch's allocator orders its reuse on the stream
             c.stage_h2d(base, buf)
         x, ld = logits.data_ptr(), int(logits.stride(0)) if B > 1 else V

@@ -375,6 +375,132 @@ int plh_fp8_linear(plh_ctx* ctx, const void* x, int dtype, int64_t ldx, int N, i
                    const uint8_t* codes, const float* scales, int V, float* out, int64_t ldo, void* ws,
                    int64_t ws_bytes);
 
+/*
+ * A cache of keys and values in pages, and speculation with trees of drafted
+ * tokens over it (the reference's cache is src/pagellm/cache/paged.py, on the
+ * host; its speculation drafts chains, src/pagellm/engine/speculative.py:97-140).
+ *
+ * One layer's keys (and its values, alike) are [num_pages, kv_heads, page_size, D]
+ * of PLH_F32, PLH_BF16 or PLH_F16, page_size a power of two from 16 to 1024.  Token
+ * t of sequence b lies in page page_table[b, t / page_size] (int32 [B, ldt]), at
+ * t % page_size.  Page numbers outside [0, num_pages) hold nothing: they are never
+ * read or written.
+ *
+ * A step's rows are the nodes of the sequences' trees, one sequence after the other:
+ * node i of sequence b is row node_off[b] + i (int32 [B+1], ascending from 0, at
+ * most max_nodes nodes each).  Node 0 is the tree's root, the last token that the
+ * target has not seen; parents come before their children.  Before a step sequence
+ * b holds lens[b] tokens; its node i goes to place lens[b] + i.  Rows past
+ * node_off[B] belong to no sequence and are left as they are.
+ *
+ * None of these calls uses the context's workspace, and all may be captured into a
+ * graph.
+ */
+
+/*
+ * Rotary positions, and a step's keys and values into their places:
+ *   (a, b) -> factor * (a cos t - b sin t, b cos t + a sin t), t = positions[n] * inv_freq[i]
+ * for pair i < pairs of each head of q and k (transformer.py's rotary positions;
+ * the angle in float64, the rest in float32, rounded once).  Pairs are (x[i],
+ * x[i + pairs]), or with `interleaved` (x[2 i], x[2 i + 1]); a head's values from
+ * 2 * pairs on, and v, stay as they are.
+ *   q       [N, ldq], q_heads heads of D values each; q_out [N, ldqo] takes it
+ *           turned: q itself (ldqo = ldq), or rows that meet none of it.  Both
+ *           NULL: no queries
+ *   k, v    [N, ldk] and [N, ldv], kv_heads heads; written to the layer's pages
+ *           at slots[n] = page * page_size + place (int64).  Rows with a slot
+ *           outside the pages write nothing; of rows with the same slot one wins,
+ *           value by value.  Both NULL: no keys and values (the arguments that
+ *           describe them are not read)
+ *   inv_freq float64 [pairs] radians a position; positions int64 [N]
+ * D <= 8192.
+ */
+int plh_rotary_append(plh_ctx* ctx, const void* q, int64_t ldq, int q_heads, void* q_out, int64_t ldqo, const void* k,
+                      int64_t ldk, const void* v, int64_t ldv, int kv_heads, int dtype, int N, int D,
+                      const int64_t* positions, const double* inv_freq, int pairs, int interleaved, double factor,
+                      void* k_pages, void* v_pages, int num_pages, int page_size, const int64_t* slots);
+
+/*
+ * Attention of a step's nodes over the cache (their own keys and values among
+ * it): for node i of sequence b and query head h, over the keys j that it sees,
+ *   out = sum_j w_j v_j / sum_j w_j, w_j = exp(scale * q . k_j); lse = log(sum_j w_j)
+ * It sees the sequence's lens[b] tokens, and of the tree node j where bit j of
+ * visible[row] is set (uint64 [N]; at most PLH_MAX_TREE_NODES nodes a tree), or with
+ * visible NULL nodes 0 .. i (a chain, or a chunk of a prompt, of any length).  A
+ * row that sees nothing gets 0 and lse -inf.  Keys and values that a row does not
+ * see never reach it, whatever they are.
+ *   q    [N, ldq], q_heads heads of D values each; head h reads key head
+ *        h / (q_heads / kv_heads)
+ *   out  [N, ldo] of q's type, may not overlap q; lse float32 [N, q_heads] or NULL
+ *   max_len  at least every lens[b] + its nodes, for the plan alone (larger ones
+ *        are right too, and slower), at most 2^30
+ *   ws   plh_tree_attention_ws_bytes of the same sizes, 256-byte aligned, the
+ *        caller's until the call's kernels have ended (may be NULL for 0 bytes)
+ * D is a multiple of 8, at most 256; pages are 16-byte aligned.  Sums and maxima are
+ * float32; for 16-bit types the weights are rounded to the type once.  The order of a
+ * sum depends on the sizes (max_len and max_nodes too) and the device: equal calls
+ * give equal bits.
+ */
+#define PLH_MAX_TREE_NODES 64
+int64_t plh_tree_attention_ws_bytes(plh_ctx* ctx, int dtype, int N, int q_heads, int kv_heads, int D, int B,
+                                    int max_nodes, int64_t max_len);
+int plh_tree_attention(plh_ctx* ctx, const void* q, int dtype, int64_t ldq, int N, int q_heads, int kv_heads, int D,
+                       const void* k_pages, const void* v_pages, int num_pages, int page_size,
+                       const int32_t* page_table, int64_t ldt, const int32_t* lens, const int32_t* node_off, int B,
+                       const uint64_t* visible, double scale, int max_nodes, int64_t max_len, void* out, int64_t ldo,
+                       float* lse, void* ws, int64_t ws_bytes);
+
+/*
+ * Batched accept/resample over trees: plh_verify's rule
+ * (src/pagellm/engine/speculative.py:38-60) applied to a node's children in turn.
+ * From the root on, the current node's children x are tested in the order of their
+ * rows against r = p[node], s = q[node], both distributions:
+ *   accept while u < min(1, r(x) / s(x)) (NaN: 1): the child is the current node now
+ *   else r = max(r - s, 0) / its sum, s = s without x / its sum, next child
+ * After a rejection a token of which nothing is left in r is never accepted.  The
+ * token after the path is drawn from the last node's r (p itself where nothing is
+ * left of it), the first whose running sum exceeds u * sum.  A test and the draw
+ * take the sequence's next uniform each: sequence b's t-th is uniforms[b, t].
+ *   p, q      [N, ld] of `dtype` (PLH_F32, PLH_F64; float64 arithmetic): row of a
+ *             node: the target's distribution after it, and the draft's that its
+ *             children were drawn from, without replacement, or with it
+ *             (`replacement`: s stays as it is).  Rows without children are not
+ *             read in q.  q NULL: each child was its draft's only choice, s(x) = 1
+ *   tokens    int32 [N] (a root's is not read), parents int32 [N] (place in the
+ *             tree; nodes whose parent is not before them are never tested)
+ *   uniforms  float64 [B, ldu], ldu >= max_nodes
+ *   out_tokens int32 [B, max_nodes]: the accepted nodes' tokens, then the drawn
+ *             one, then -1; out_path [B, max_nodes]: 0 and the accepted nodes, then
+ *             -1; out_n_acc [B]: how many were accepted; out_n_used [B]: uniforms
+ * A sequence without nodes, with more than max_nodes, or whose walk tests a token
+ * outside [0, V) gives -1 everywhere and uses no uniform.  max_nodes <= 256, V <=
+ * 524288.  A chain gives what plh_verify gives.
+ */
+int plh_verify_tree(plh_ctx* ctx, const void* p, const void* q, int dtype, int64_t ld, int N, int V,
+                    const int32_t* tokens, const int32_t* parents, const int32_t* node_off, int B, int max_nodes,
+                    const double* uniforms, int64_t ldu, int replacement, int32_t* out_tokens, int32_t* out_path,
+                    int32_t* out_n_acc, int32_t* out_n_used);
+
+/*
+ * Pages src[i] of all layers copied to dst[i] (int32 [n]), keys and values: what a
+ * forked sequence needs before it writes to a page that it shares.  Layers lie
+ * layer_bytes apart, pages page_bytes, both multiples of 16.  No dst may be
+ * another dst or any src; pairs with a page outside [0, num_pages) do nothing.
+ */
+int plh_copy_pages(plh_ctx* ctx, void* k_pages, void* v_pages, int layers, int64_t layer_bytes, int num_pages,
+                   int64_t page_bytes, const int32_t* src, const int32_t* dst, int n);
+
+/*
+ * The accepted nodes' keys and values moved behind the sequences' tokens, in all
+ * layers: node path[b, j] from place lens[b] + path[b, j] to lens[b] + j, for 1 <= j
+ * <= n_acc[b] (plh_verify_tree's out_path and out_n_acc; -1 moves nothing).  Path
+ * entries ascend; one that is not above its place stays.  row_bytes: of a token's
+ * row in one head, a multiple of 16.
+ */
+int plh_keep_nodes(plh_ctx* ctx, void* k_pages, void* v_pages, int layers, int64_t layer_bytes, int num_pages,
+                   int page_size, int kv_heads, int row_bytes, const int32_t* page_table, int64_t ldt,
+                   const int32_t* lens, const int32_t* path, int64_t ldp, const int32_t* n_acc, int B);
+
 #ifdef __cplusplus
 }
 #endif

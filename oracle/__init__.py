@@ -19,4 +19,4 @@ from .sampler import (  # noqa: F401
     verify_boundary_gap,
 )
 from .head import head_error_bound, lm_head_logits, rms_norm  # noqa: F401,E402
-from . import fp8, logits  # noqa: F401,E402
+from . import fp8, logits, tree  # noqa: F401,E402

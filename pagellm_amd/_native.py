@@ -27,6 +27,7 @@ PLH_F64 = 1
 PLH_BF16 = 2
 PLH_F16 = 3
 PLH_MAX_TOP = 64
+PLH_MAX_TREE_NODES = 64
 PLH_SAMPLE_ROWWISE = 1
 PLH_SAMPLE_HIST_SPANS = 2
 PLH_SAMPLE_NUCLEUS = 4
@@ -90,6 +91,27 @@ SIGNATURES = {
     "plh_fp8_linear": (
         _c_int,
         [_vp, _vp, _c_int, _c_i64, _c_int, _c_int, _vp, ctypes.c_double, _vp, _vp, _c_int, _vp, _c_i64, _vp, _c_i64],
+    ),
+    "plh_rotary_append": (
+        _c_int,
+        [_vp, _vp, _c_i64, _c_int, _vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_int, _c_int, _c_int, _c_int, _vp, _vp,
+         _c_int, _c_int, ctypes.c_double, _vp, _vp, _c_int, _c_int, _vp],
+    ),
+    "plh_tree_attention_ws_bytes": (_c_i64, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64]),
+    "plh_tree_attention": (
+        _c_int,
+        [_vp, _vp, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _c_int, _c_int, _vp, _c_i64, _vp, _vp,
+         _c_int, _vp, ctypes.c_double, _c_int, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64],
+    ),
+    "plh_verify_tree": (
+        _c_int,
+        [_vp, _vp, _vp, _c_int, _c_i64, _c_int, _c_int, _vp, _vp, _vp, _c_int, _c_int, _vp, _c_i64, _c_int, _vp, _vp,
+         _vp, _vp],
+    ),
+    "plh_copy_pages": (_c_int, [_vp, _vp, _vp, _c_int, _c_i64, _c_int, _c_i64, _vp, _vp, _c_int]),
+    "plh_keep_nodes": (
+        _c_int,
+        [_vp, _vp, _vp, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _vp, _c_i64, _vp, _vp, _c_i64, _vp, _c_int],
     ),
 }
 
@@ -409,6 +431,50 @@ class Context:
                    ws_bytes) -> None:
         self._check(self.lib.plh_fp8_linear(self.handle, x_ptr, dtype_code, ldx, N, D, norm_ptr, eps, codes, scales, V,
                                             out_ptr, ldo, ws, ws_bytes))
+
+    def rotary_append(self, q_ptr, ldq, q_heads, q_out_ptr, ldqo, k_ptr, ldk, v_ptr, ldv, kv_heads, dtype_code, N, D,
+                      positions, inv_freq, pairs, interleaved, factor, k_pages, v_pages, num_pages, page_size,
+                      slots) -> None:
+        self._check(
+            self.lib.plh_rotary_append(self.handle, q_ptr, ldq, q_heads, q_out_ptr, ldqo, k_ptr, ldk, v_ptr, ldv,
+                                       kv_heads, dtype_code, N, D, positions, inv_freq, pairs, interleaved, factor,
+                                       k_pages, v_pages, num_pages, page_size, slots)
+        )
+
+    def tree_attention_ws_bytes(self, dtype_code, N, q_heads, kv_heads, D, B, max_nodes, max_len) -> int:
+        n = int(self.lib.plh_tree_attention_ws_bytes(self.handle, dtype_code, N, q_heads, kv_heads, D, B, max_nodes,
+                                                     max_len))
+        if n < 0:
+            self._check(n)
+        return n
+
+    def tree_attention(self, q_ptr, dtype_code, ldq, N, q_heads, kv_heads, D, k_pages, v_pages, num_pages, page_size,
+                       table, ldt, lens, node_off, B, visible, scale, max_nodes, max_len, out_ptr, ldo, lse, ws,
+                       ws_bytes) -> None:
+        self._check(
+            self.lib.plh_tree_attention(self.handle, q_ptr, dtype_code, ldq, N, q_heads, kv_heads, D, k_pages, v_pages,
+                                        num_pages, page_size, table, ldt, lens, node_off, B, visible, scale, max_nodes,
+                                        max_len, out_ptr, ldo, lse, ws, ws_bytes)
+        )
+
+    def verify_tree(self, p_ptr, q_ptr, dtype_code, ld, N, V, tokens, parents, node_off, B, max_nodes, uniforms, ldu,
+                    replacement, out_tokens, out_path, out_n_acc, out_n_used) -> None:
+        self._check(
+            self.lib.plh_verify_tree(self.handle, p_ptr, q_ptr, dtype_code, ld, N, V, tokens, parents, node_off, B,
+                                     max_nodes, uniforms, ldu, int(replacement), out_tokens, out_path, out_n_acc,
+                                     out_n_used)
+        )
+
+    def copy_pages(self, k_ptr, v_ptr, layers, layer_bytes, num_pages, page_bytes, src, dst, n) -> None:
+        self._check(self.lib.plh_copy_pages(self.handle, k_ptr, v_ptr, layers, layer_bytes, num_pages, page_bytes, src,
+                                            dst, n))
+
+    def keep_nodes(self, k_ptr, v_ptr, layers, layer_bytes, num_pages, page_size, kv_heads, row_bytes, table, ldt, lens,
+                   path, ldp, n_acc, B) -> None:
+        self._check(
+            self.lib.plh_keep_nodes(self.handle, k_ptr, v_ptr, layers, layer_bytes, num_pages, page_size, kv_heads,
+                                    row_bytes, table, ldt, lens, path, ldp, n_acc, B)
+        )
 
     def append_ids(self, slab_ptr, pos_ptr, ids_ptr, n) -> None:
         self._check(self.lib.plh_append_ids(self.handle, slab_ptr, pos_ptr, ids_ptr, int(n)))

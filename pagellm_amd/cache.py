@@ -1,0 +1,600 @@
+"""Keys and values of live sequences in pages, in HBM.
+
+The reference keeps them on the host (``src/pagellm/cache/paged.py:47-464``:
+``PagedKVPool``, ``BlockManager``, ``PagedBatch``).  Here one layer's keys are
+[pages, kv heads, page size, head size], all layers' one tensor, and the host keeps
+which pages each sequence holds:
+
+* :class:`PagedCache`: sequences join, fork (sharing their pages until one of
+  them writes), step, keep what was accepted, shrink and leave;
+* :func:`rotary_append`: rotary positions of a step's queries and keys, keys and
+  values into their places (``plh_rotary_append``), :class:`Rotary`;
+* :func:`copy_pages`, :func:`keep_nodes`: pages copied, and the accepted nodes of
+  a tree of drafts moved together, in all layers (``plh_copy_pages``,
+  ``plh_keep_nodes``).
+
+The attention that reads the pages is in :mod:`pagellm_amd.tree`.  Tensors are torch
+CUDA tensors on the context's GPU, read and written in place on torch's current
+stream; nothing waits.  A cache's steps run on one stream, or are ordered by the
+caller.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Hashable, Mapping, Sequence
+
+import numpy as np
+
+from . import _native
+from .fp8 import _check_device, _float_code
+from .logits import _pack
+from .sampling import _ctx, _is_torch_cuda, _stream_of
+
+__all__ = ["CacheStep", "PagedCache", "Rotary", "copy_pages", "keep_nodes", "rotary_append"]
+
+
+class Rotary:
+    """Rotary positions: pair i of a head is turned by position * inv_freq[i].
+
+    ``Rotary(head_dim)`` has the usual frequencies ``base ** (-2 i / part)`` of the
+    first ``part`` values of a head (None: all).  ``layout`` names the pairs: "half"
+    (x[i], x[i + part / 2]) or "interleaved" (x[2 i], x[2 i + 1]).  ``scaling``
+    serves contexts longer than a model was trained on:
+
+        {"kind": "linear", "factor": s}     every frequency divided by s
+        {"kind": "ntk", "factor": s}        base * s ** (part / (part - 2)): the
+                                            slowest pair divided by s, the fastest kept
+        {"kind": "yarn", "factor": s, "original_len": n}
+                                            pairs of up to ``slow`` (1) turns in n
+                                            positions divided by s, those of ``fast``
+                                            (32) and more kept, a ramp between them;
+                                            turned values times 0.1 ln s + 1
+
+    ``inv_freq`` (radians a position, float64) and ``factor`` (on turned values)
+    replace what these give."""
+
+    def __init__(self, head_dim: int | None = None, *, base: float = 10000.0, part: int | None = None,
+                 layout: str = "half", scaling: Mapping | None = None, inv_freq=None, factor: float | None = None,
+                 ctx: _native.Context | None = None):
+        import torch
+
+        self.ctx = _ctx(ctx)
+        if layout not in ("half", "interleaved"):
+            raise ValueError('layout must be "half" or "interleaved"')
+        self.interleaved = layout == "interleaved"
+        scale = 1.0
+        if inv_freq is None:
+            if head_dim is None:
+                raise ValueError("need head_dim or inv_freq")
+            freq, scale = rotary_frequencies(head_dim if part is None else part, base, scaling)
+            if part is not None and part > head_dim:
+                raise ValueError(f"part must be at most head_dim ({head_dim})")
+        elif scaling is not None or part is not None:
+            raise ValueError("inv_freq stands for part and scaling")
+        else:
+            freq = inv_freq
+        self.factor = float(scale if factor is None else factor)
+        if not math.isfinite(self.factor):
+            raise ValueError("factor must be finite")
+        if not isinstance(freq, torch.Tensor):
+            freq = torch.from_numpy(np.ascontiguousarray(freq, dtype=np.float64))
+        if freq.dim() != 1 or not freq.is_floating_point():
+            raise ValueError("inv_freq must be one float64 value for each pair")
+        self.inv_freq = freq.to(device=torch.device("cuda", self.ctx.device), dtype=torch.float64).contiguous()
+        self.pairs = int(freq.numel())
+
+
+def rotary_frequencies(part: int, base: float = 10000.0, scaling: Mapping | None = None) -> tuple[np.ndarray, float]:
+    """(radians a position [part / 2] in float64, factor on turned values) of
+    :class:`Rotary`'s arguments."""
+    part = int(part)
+    if part < 2 or part % 2:
+        raise ValueError("the turned part of a head must be even and at least 2")
+    if not (base > 0.0 and math.isfinite(base)):
+        raise ValueError("base must be finite and > 0")
+    exponent = -2.0 * np.arange(part // 2) / part
+    if scaling is None:
+        return base ** exponent, 1.0
+    given = dict(scaling)
+    kind, s = given.pop("kind", None), float(given.pop("factor", 0.0))
+    if not (s >= 1.0 and math.isfinite(s)):
+        raise ValueError("scaling needs a factor >= 1")
+    if kind == "linear":
+        freq, factor = base ** exponent / s, 1.0
+    elif kind == "ntk":
+        if part < 4:
+            raise ValueError("ntk scaling needs two pairs")
+        freq, factor = (base * s ** (part / (part - 2))) ** exponent, 1.0
+    elif kind == "yarn":
+        n = float(given.pop("original_len", 0.0))
+        slow, fast = float(given.pop("slow", 1.0)), float(given.pop("fast", 32.0))
+        if not (n > 0.0 and fast > slow):
+            raise ValueError("yarn scaling needs original_len > 0 and fast > slow")
+        freq = base ** exponent
+        keep = np.clip((n * freq / (2.0 * math.pi) - slow) / (fast - slow), 0.0, 1.0)
+        freq, factor = freq * keep + freq / s * (1.0 - keep), 0.1 * math.log(s) + 1.0
+    else:
+        raise ValueError('scaling kind must be "linear", "ntk" or "yarn"')
+    if given:
+        raise ValueError(f"unknown scaling arguments: {', '.join(sorted(given))}")
+    return freq, factor
+
+
+def _rows(c, x, name: str, dim: int | None = None):
+    """(heads, D, row stride) of x [N, heads, D], whose heads lie side by side."""
+    _check_device(c, x, name)
+    if x.dim() != 3:
+        raise ValueError(f"{name} must be [N, heads, D]")
+    n, h, d = x.shape
+    if dim is not None and d != dim:
+        raise ValueError(f"{name} has heads of {d} values, the others of {dim}")
+    s = x.stride()
+    if x.numel() and ((d > 1 and s[2] != 1) or (h > 1 and s[1] != d)):
+        raise ValueError(f"the heads of a row of {name} must lie side by side")
+    if n > 1 and x.numel() and s[0] < h * d:
+        raise ValueError(f"rows of {name} must not overlap")
+    return int(h), int(d), int(s[0]) if n > 1 else int(h * d)
+
+
+def _check_pages(c, k_pages, v_pages, dims: int) -> None:
+    _check_device(c, k_pages, "k_pages")
+    _check_device(c, v_pages, "v_pages")
+    if k_pages.dim() != dims:
+        raise ValueError("k_pages must be [pages, kv heads, page size, D]" if dims == 4 else
+                         "k_pages must be [layers, pages, kv heads, page size, D]")
+    if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+        raise ValueError("v_pages must be like k_pages")
+    if dims == 4:
+        if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+            raise ValueError("pages must be contiguous")
+    elif k_pages.numel() == 0 or not (k_pages[0].is_contiguous() and v_pages[0].is_contiguous()) or \
+            k_pages.stride(0) != v_pages.stride(0):
+        raise ValueError("each layer's pages must be contiguous, the layers as far apart in both")
+
+
+def _ints(c, x, name: str, dtype, n: int | None = None):
+    """x as a contiguous CUDA tensor of one of torch's integer types on the
+    context's GPU; sequences and arrays go over in a queued copy."""
+    import torch
+
+    if not _is_torch_cuda(x):
+        if isinstance(x, torch.Tensor):
+            x = x.numpy()
+        host = np.asarray(x)
+        if host.size and host.dtype.kind not in "iu":
+            raise TypeError(f"{name} must be integers")
+        info = torch.iinfo(dtype)
+        if host.size and (int(host.min()) < info.min or int(host.max()) > info.max):
+            raise ValueError(f"{name} must fit {str(dtype).split('.')[1]}")
+        host = np.ascontiguousarray(host.astype(f"i{info.bits // 8}"))
+        x = torch.empty(host.shape, dtype=dtype, device=torch.device("cuda", c.device))
+        if host.size:
+            c.set_stream(_stream_of(x))
+            buf = c.stage(host.nbytes)
+            buf[:] = host.reshape(-1).view(np.uint8)
+            c.stage_h2d(x.data_ptr(), buf)
+    else:
+        if x.device.index != c.device:
+            raise ValueError(f"{name} is on GPU {x.device.index}, the context on GPU {c.device}")
+        if x.dtype != dtype:
+            if x.dtype not in (torch.int32, torch.int64):
+                raise TypeError(f"{name} must be int32 or int64")
+            if dtype == torch.int32:  # what does not fit stays outside every range
+                x = x.clamp(-1, 2**31 - 1)
+            x = x.to(dtype)
+        if not x.is_contiguous():
+            x = x.contiguous()
+    if n is not None and tuple(x.shape) != (n,):
+        raise ValueError(f"expected {n} {name}, got {list(x.shape)}")
+    return x
+
+
+def rotary_append(q, k, v, positions, slots, k_pages, v_pages, rotary: Rotary | None, *, q_out=None,
+                  ctx: _native.Context | None = None):
+    """Turns the queries ``q`` [N, heads, D] and keys ``k`` [N, kv heads, D] by their
+    ``positions`` [N] and writes the keys and the values ``v`` to ``slots`` [N] (page *
+    page size + place) of one layer's pages [pages, kv heads, page size, D].  Returns
+    the turned queries, in ``q_out`` (a new tensor when None; ``q`` itself turns them
+    in place).
+
+    Rows may be views of a wider buffer (one product's q, k and v).  Without ``q``
+    keys and values are written alone, without ``k`` and ``v`` queries turned alone;
+    ``rotary`` None turns nothing.  Rows with a slot outside the pages (-1) write
+    nothing; no two rows may have the same."""
+    import torch
+
+    c = _ctx(ctx)
+    if (k is None) != (v is None):
+        raise ValueError("k and v go together")
+    some = q if q is not None else k
+    if some is None:
+        raise ValueError("need q, or k and v")
+    heads = kv_heads = ldq = ldqo = ldk = ldv = pages = page_size = 0
+    dim = None
+    if q is not None:
+        heads, dim, ldq = _rows(c, q, "q")
+    elif q_out is not None:
+        raise ValueError("q_out given without q")
+    code = _float_code(some, "q" if q is not None else "k")
+    N = int(some.shape[0])
+    if N > 2**31 - 1:  # ctypes would wrap it
+        raise ValueError("at most 2^31 - 1 rows")
+    if k is not None:
+        kv_heads, dim, ldk = _rows(c, k, "k", dim)
+        v_heads, _, ldv = _rows(c, v, "v", dim)
+        if v_heads != kv_heads or k.shape[0] != N or v.shape[0] != N:
+            raise ValueError("q, k and v must have as many rows, k and v as many heads")
+        _check_pages(c, k_pages, v_pages, 4)
+        if k.dtype != some.dtype or v.dtype != some.dtype or k_pages.dtype != some.dtype:
+            raise TypeError("q, k, v and the pages must have one type")
+        pages, page_heads, page_size, page_dim = map(int, k_pages.shape)
+        if page_heads != kv_heads or page_dim != dim:
+            raise ValueError(f"the pages hold {page_heads} heads of {page_dim} values, k {kv_heads} of {dim}")
+        slots = _ints(c, slots, "slots", torch.int64, N)
+    pairs = 0
+    if rotary is not None:
+        pairs = rotary.pairs
+        if 2 * pairs > dim:
+            raise ValueError(f"{pairs} pairs do not fit heads of {dim} values")
+        _check_device(c, rotary.inv_freq, "inv_freq")
+        positions = _ints(c, positions, "positions", torch.int64, N)
+    if q is not None:
+        if q_out is None:
+            q_out = torch.empty((N, heads, dim), dtype=q.dtype, device=q.device)
+        elif q_out.dtype != q.dtype or q_out.shape != q.shape:
+            raise ValueError("q_out must be like q")
+        ldqo = _rows(c, q_out, "q_out")[2]
+    if N == 0:
+        return q_out
+    c.set_stream(_stream_of(some))
+    at = lambda x: x.data_ptr() if x is not None else None  # noqa: E731
+    kv = k is not None
+    c.rotary_append(at(q), ldq, heads, at(q_out), ldqo, at(k), ldk, at(v), ldv, kv_heads, code, N, dim,
+                    positions.data_ptr() if pairs else None, rotary.inv_freq.data_ptr() if pairs else None, pairs,
+                    int(rotary.interleaved) if pairs else 0, rotary.factor if pairs else 1.0,
+                    k_pages.data_ptr() if kv else None, v_pages.data_ptr() if kv else None, pages, page_size,
+                    slots.data_ptr() if kv else None)
+    return q_out
+
+
+def _layers(k_pool, v_pool):
+    """(layers, bytes from one to the next) of pools [layers, pages, kv heads, page size, D]."""
+    return int(k_pool.shape[0]), int(k_pool.stride(0)) * k_pool.element_size()
+
+
+def copy_pages(k_pool, v_pool, src, dst, *, ctx: _native.Context | None = None) -> None:
+    """Copies pages ``src`` [n] of all layers to ``dst`` [n], keys and values (pools
+    [layers, pages, kv heads, page size, D]).  No ``dst`` may be another ``dst`` or any
+    ``src``: sequences are checked; CUDA tensors are not, and pairs with a page
+    outside the pool do nothing."""
+    import torch
+
+    c = _ctx(ctx)
+    _check_pages(c, k_pool, v_pool, 5)
+    pages = int(k_pool.shape[1])
+    if not _is_torch_cuda(src) and not _is_torch_cuda(dst):
+        a, b = (np.asarray(x, dtype=np.int64).reshape(-1) for x in (src, dst))
+        for x, name in ((a, "src"), (b, "dst")):
+            if x.size and (x.min() < 0 or x.max() >= pages):
+                raise IndexError(f"{name} must be in [0, {pages})")
+        if np.unique(b).size != b.size or np.intersect1d(a, b).size:
+            raise ValueError("no page may be copied to twice, or to and from")
+        src, dst = a, b
+    src = _ints(c, src, "src", torch.int32)
+    dst = _ints(c, dst, "dst", torch.int32)
+    if src.dim() != 1 or src.shape != dst.shape:
+        raise ValueError("expected as many src as dst")
+    if src.numel() == 0:
+        return
+    layers, layer_bytes = _layers(k_pool, v_pool)
+    page_bytes = int(k_pool.stride(1)) * k_pool.element_size()
+    c.set_stream(_stream_of(k_pool))
+    c.copy_pages(k_pool.data_ptr(), v_pool.data_ptr(), layers, layer_bytes, pages, page_bytes, src.data_ptr(),
+                 dst.data_ptr(), int(src.numel()))
+
+
+def _table(c, page_table, B: int | None = None):
+    """(page_table, its row stride) of int32 [B, pages]."""
+    import torch
+
+    _check_device(c, page_table, "page_table")
+    if page_table.dtype != torch.int32:
+        raise TypeError("page_table must be int32")
+    if page_table.dim() != 2 or (B is not None and page_table.shape[0] != B) or page_table.shape[1] < 1 or \
+            (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError("page_table must be [sequences, pages] with unit stride")
+    if page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]:
+        raise ValueError("rows of page_table must not overlap")
+    # the kernels read no page past a row's own
+    return page_table, int(page_table.shape[1]), int(page_table.stride(0)) if page_table.shape[0] > 1 else int(page_table.shape[1])
+
+
+def keep_nodes(k_pool, v_pool, page_table, lens, path, n_acc, *, ctx: _native.Context | None = None) -> None:
+    """Moves the accepted nodes' keys and values behind their sequences' tokens, in
+    all layers of the pools [layers, pages, kv heads, page size, D]: node ``path[b, j]``
+    from place ``lens[b] + path[b, j]`` to ``lens[b] + j``, 1 <= j <= ``n_acc[b]``
+    (:func:`pagellm_amd.tree.verify_tree`'s)."""
+    import torch
+
+    c = _ctx(ctx)
+    _check_pages(c, k_pool, v_pool, 5)
+    lens = _ints(c, lens, "lens", torch.int32)
+    B = int(lens.numel())
+    n_acc = _ints(c, n_acc, "n_acc", torch.int32, B)
+    path = _ints(c, path, "path", torch.int32)
+    if lens.dim() != 1 or path.dim() != 2 or path.shape[0] != B or path.shape[1] < 1:
+        raise ValueError("lens must be [B], path [B, nodes]")
+    table, width, ldt = _table(c, page_table, B)
+    if ldt != width:
+        table, ldt = table.contiguous(), width
+    if B == 0:
+        return
+    layers, layer_bytes = _layers(k_pool, v_pool)
+    _, pages, heads, page_size, dim = map(int, k_pool.shape)
+    c.set_stream(_stream_of(k_pool))
+    c.keep_nodes(k_pool.data_ptr(), v_pool.data_ptr(), layers, layer_bytes, pages, page_size, heads,
+                 dim * k_pool.element_size(), table.data_ptr(), ldt, lens.data_ptr(), path.data_ptr(),
+                 int(path.shape[1]), n_acc.data_ptr(), B)
+
+
+class CacheStep:
+    """One step of a batch over a :class:`PagedCache`: each sequence's nodes, where
+    their keys and values go and what they see, on the device.
+
+    ``tokens``, ``parents`` int32 [N], ``positions``, ``slots`` int64 [N], ``visible``
+    int64 [N] (None: all are chains), ``node_off`` int32 [B + 1], ``lens`` int32 [B] and
+    ``page_table`` int32 [B, pages]; ``max_nodes`` and ``max_len`` bound them."""
+
+    def __init__(self, cache: "PagedCache", keys, trees, host_lens):
+        self.cache, self.keys, self.trees, self.host_lens = cache, list(keys), list(trees), host_lens
+        self.open = True
+
+    def attend(self, layer: int, q, k, v, rotary: Rotary | None = None, *, scale: float | None = None, out=None):
+        """Layer ``layer``'s attention of the step's nodes: q and k turned, k and v
+        written, every node over the tokens and nodes that it sees.  q [N, heads, D],
+        k, v [N, kv heads, D]; returns [N, heads, D]."""
+        from .tree import tree_attention
+
+        if not self.open:
+            raise RuntimeError("the step has been committed")
+        cache = self.cache
+        q = rotary_append(q, k, v, self.positions, self.slots, cache.k[layer], cache.v[layer], rotary, ctx=cache.ctx)
+        return tree_attention(q, cache.k[layer], cache.v[layer], self.page_table, self.lens, self.node_off, self.visible,
+                              max_nodes=self.max_nodes, max_len=self.max_len, scale=scale, out=out, ctx=cache.ctx)
+
+
+class PagedCache:
+    """Keys and values of up to ``pages`` * ``page_size`` tokens of all layers.
+
+        cache.add(key)                                   # a new sequence, empty
+        step = cache.step(keys, trees)                   # pages for the step's nodes
+        o = step.attend(layer, q, k, v, rotary)          # in every layer
+        cache.commit(step, path, n_acc)                  # the accepted nodes stay
+        cache.fork(key, child); cache.truncate(key, n); cache.remove(key)
+
+    Forked sequences share their pages; the first that writes to a shared page gets
+    its own copy (``step`` copies all of a batch's in one launch)."""
+
+    def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: str = "bfloat16", *,
+                 ctx: _native.Context | None = None):
+        import torch
+
+        if min(layers, pages, kv_heads) < 1 or pages > 2**31 - 1:
+            raise ValueError("layers, pages and kv_heads must be >= 1")
+        if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+            raise ValueError("page_size must be a power of two from 16 to 1024")
+        if head_dim < 8 or head_dim > 256 or head_dim % 8:
+            raise ValueError("head_dim must be a multiple of 8 up to 256")
+        types = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
+        if dtype not in types:
+            raise TypeError("dtype must be float32, bfloat16 or float16")
+        self.ctx = _ctx(ctx)
+        self.page_size = int(page_size)
+        shape = (int(layers), int(pages), int(kv_heads), self.page_size, int(head_dim))
+        device = torch.device("cuda", self.ctx.device)
+        self.k = torch.empty(shape, dtype=types[dtype], device=device)
+        self.v = torch.empty(shape, dtype=types[dtype], device=device)
+        self._book = _PageBook(int(pages), self.page_size)
+
+    def __contains__(self, key) -> bool:
+        return key in self._book.held
+
+    def __len__(self) -> int:
+        return len(self._book.held)
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._book.free)
+
+    def length(self, key) -> int:
+        return self._book.length[key]
+
+    def add(self, key) -> None:
+        """A new sequence without tokens."""
+        self._book.add(key)
+
+    def fork(self, key, child) -> None:
+        """``child`` joins with the tokens of ``key`` (``llm_engine.py:259-278``)."""
+        self._book.fork(key, child)
+
+    def truncate(self, key, n: int) -> None:
+        """The sequence keeps its first ``n`` tokens."""
+        self._book.truncate(key, n)
+
+    def remove(self, key) -> None:
+        """A finished or aborted sequence gives its pages back."""
+        self._book.remove(key)
+
+    def step(self, keys: Sequence[Hashable], trees: Sequence) -> CacheStep:
+        """Room for a step of ``trees[b]`` (:class:`pagellm_amd.tree.DraftTree`) behind
+        the tokens of sequence ``keys[b]``.  Raises RuntimeError, and changes nothing,
+        where the pages do not suffice."""
+        import torch
+
+        keys, trees = list(keys), list(trees)
+        if len(keys) != len(trees) or not keys:
+            raise ValueError("expected a tree for each of at least one sequence")
+        counts = [len(t.tokens) for t in trees]
+        chains = all(t.chain for t in trees)
+        if not chains and max(counts) > _native.PLH_MAX_TREE_NODES:
+            raise ValueError(f"trees have at most {_native.PLH_MAX_TREE_NODES} nodes (chains have any number)")
+        copies = self._book.reserve(keys, counts)
+        c = self.ctx
+        if copies:
+            copy_pages(self.k, self.v, [a for a, _ in copies], [b for _, b in copies], ctx=c)
+        lens = [self._book.length[key] for key in keys]
+        step = CacheStep(self, keys, trees, lens)
+        held = [self._book.held[key] for key in keys]
+        table = np.zeros((len(keys), max(map(len, held))), dtype=np.int32)
+        for b, pages in enumerate(held):
+            table[b, : len(pages)] = pages
+        off = np.cumsum([0] + counts, dtype=np.int64)
+        seq = np.repeat(np.arange(len(keys)), counts)
+        place = np.asarray(lens, dtype=np.int64)[seq] + np.arange(off[-1]) - off[seq]
+        slots = table[seq, place // self.page_size].astype(np.int64) * self.page_size + place % self.page_size
+        depths = np.concatenate([t.depths for t in trees])
+        parts = [slots, np.asarray(lens, dtype=np.int64)[seq] + depths,
+                 None if chains else np.concatenate([t.visible for t in trees]), np.concatenate([t.tokens for t in trees]),
+                 np.concatenate([t.parents for t in trees]), off.astype(np.int32), np.asarray(lens, dtype=np.int32), table]
+        mem = None
+
+        def empty(n):
+            nonlocal mem  # first: what fails here leaves no staged memory given
+            mem = torch.empty(n, dtype=torch.uint8, device=self.k.device)
+            c.set_stream(_stream_of(self.k))
+            return c.stage(n)
+
+        buf, offs = _pack(parts, empty)
+        c.stage_h2d(mem.data_ptr(), buf)
+        views = []
+        for a, o in zip(parts, offs):
+            if a is None:
+                views.append(None)
+                continue
+            t = torch.int64 if a.dtype.itemsize == 8 else torch.int32
+            views.append(mem[o:o + a.nbytes].view(t).view(a.shape))
+        (step.slots, step.positions, step.visible, step.tokens, step.parents, step.node_off, step.lens,
+         step.page_table) = views
+        step.max_nodes, step.max_len = max(counts), max(n + t for n, t in zip(lens, counts))
+        return step
+
+    def commit(self, step: CacheStep, path=None, n_acc=None, *, accepted: Sequence[int] | None = None) -> None:
+        """Sequence b keeps its tree's root and ``n_acc[b]`` accepted nodes, those of
+        ``path`` (:func:`pagellm_amd.tree.verify_tree`'s, on the GPU), and gives the
+        pages behind them back; ``accepted`` is ``n_acc`` where the host has it (else
+        it is downloaded).  -1 keeps nothing.  Without ``path`` every node stays."""
+        if not step.open or step.cache is not self:
+            raise RuntimeError("not an open step of this cache")
+        if any(self._book.length.get(key) != n for key, n in zip(step.keys, step.host_lens)):
+            raise RuntimeError("a sequence of the step has changed since")
+        if path is None:
+            kept = [len(t.tokens) for t in step.trees]
+        else:
+            if n_acc is None:
+                raise ValueError("path needs n_acc")
+            if accepted is None:
+                accepted = n_acc.tolist()
+            kept = [int(n) + 1 for n in accepted]
+            if len(kept) != len(step.keys) or any(not 0 <= n <= len(t.tokens) for n, t in zip(kept, step.trees)):
+                raise ValueError("n_acc must be in [-1, nodes) for each sequence")
+            keep_nodes(self.k, self.v, step.page_table, step.lens, path, n_acc, ctx=self.ctx)
+        step.open = False
+        for key, n, m in zip(step.keys, step.host_lens, kept):
+            self._book.set_length(key, n + m)
+
+    def download(self, key, layer: int):
+        """(keys, values) [kv heads, tokens, D] of a sequence as the device holds them
+        (for checks)."""
+        import torch
+
+        pages = torch.tensor(self._book.held[key], dtype=torch.int64, device=self.k.device)
+        n = self._book.length[key]
+        return tuple(x[layer][pages].transpose(0, 1).flatten(1, 2)[:, :n].cpu() for x in (self.k, self.v))
+
+
+class _PageBook:
+    """Which pages each sequence holds, and how many hold each page (host only)."""
+
+    def __init__(self, pages: int, page_size: int):
+        self.page_size = page_size
+        self.free = list(range(pages - 1, -1, -1))
+        self.refs = [0] * pages
+        self.held: dict[Hashable, list[int]] = {}
+        self.length: dict[Hashable, int] = {}
+
+    def add(self, key) -> None:
+        if key in self.held:
+            raise ValueError(f"sequence {key!r} is in the cache already")
+        self.held[key], self.length[key] = [], 0
+
+    def fork(self, key, child) -> None:
+        pages, n = self.held[key], self.length[key]
+        self.add(child)
+        self.held[child] = pages[: -(-n // self.page_size)]
+        self.length[child] = n
+        for p in self.held[child]:
+            self.refs[p] += 1
+
+    def _drop(self, pages) -> None:
+        for p in reversed(pages):
+            self.refs[p] -= 1
+            if self.refs[p] == 0:
+                self.free.append(p)
+
+    def set_length(self, key, n: int) -> None:
+        keep = -(-n // self.page_size)
+        pages = self.held[key]
+        self._drop(pages[keep:])
+        del pages[keep:]
+        self.length[key] = n
+
+    def truncate(self, key, n: int) -> None:
+        if not 0 <= n <= self.length[key]:
+            raise ValueError(f"{key!r} has {self.length[key]} tokens")
+        self.set_length(key, n)
+
+    def remove(self, key) -> None:
+        self._drop(self.held.pop(key))
+        del self.length[key]
+
+    def reserve(self, keys, counts) -> list[tuple[int, int]]:
+        """Pages of their own for ``counts[b]`` more tokens of each sequence; the
+        (shared, new) pages to copy.  All or nothing."""
+        if len(set(keys)) != len(keys):
+            raise ValueError("a sequence may step once")
+        for key in keys:
+            if key not in self.held:
+                raise KeyError(key)
+        ps, left, plan, need = self.page_size, {}, [], 0
+        for key, count in zip(keys, counts):
+            if count < 1:
+                raise ValueError("a step has at least one token a sequence")
+            n, pages = self.length[key], self.held[key]
+            shared = []  # places of pages that it writes to and others hold
+            for i in range(n // ps, len(pages)):
+                refs = left.get(pages[i], self.refs[pages[i]])
+                if refs > 1:
+                    left[pages[i]] = refs - 1
+                    shared.append(i)
+            more = max(0, -(-(n + count) // ps) - len(pages))
+            plan.append((key, shared, more))
+            need += len(shared) + more
+        if need > len(self.free):
+            raise RuntimeError(f"the step needs {need} pages, {len(self.free)} are free")
+        copies = []
+        for key, shared, more in plan:
+            pages = self.held[key]
+            for i in shared:
+                new = self.free.pop()
+                self.refs[pages[i]] -= 1
+                self.refs[new] = 1
+                # a page behind the sequence's tokens holds nothing yet
+                if i * ps < self.length[key]:
+                    copies.append((pages[i], new))
+                pages[i] = new
+            for _ in range(more):
+                new = self.free.pop()
+                self.refs[new] = 1
+                pages.append(new)
+        return copies

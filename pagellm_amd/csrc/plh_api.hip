@@ -150,6 +150,39 @@ bool rows_overlap(const void* x, int64_t ld, const void* out, int64_t out_ld, in
   return false;
 }
 
+int page_shift_of(int page_size) { return __builtin_ctz((unsigned)page_size); }
+
+int check_page_size(plh_ctx* c, int page_size) {
+  if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0)
+    return fail(c, PLH_ERR_INVALID_ARG, "page_size must be a power of two from 16 to 1024%s");
+  return PLH_OK;
+}
+
+// The sizes of a tree attention call, checked, in the plan's arguments.
+int attend_sizes(plh_ctx* c, plh::AttendArgs& a, int dtype, int N, int q_heads, int kv_heads, int D, int B,
+                 int max_nodes, int64_t max_len) {
+  if (dtype != PLH_F32 && dtype != PLH_BF16 && dtype != PLH_F16)
+    return fail(c, PLH_ERR_INVALID_ARG, "dtype must be PLH_F32, PLH_BF16 or PLH_F16%s");
+  if (N < 0 || B < 0 || B > 65535 || max_nodes < 0 || max_len < 0 || max_len > (1 << 30))
+    return fail(c, PLH_ERR_INVALID_ARG, "need N >= 0, 0 <= B <= 65535, max_nodes >= 0 and 0 <= max_len <= 2^30%s");
+  if (kv_heads < 1 || q_heads < 1 || q_heads % kv_heads != 0)
+    return fail(c, PLH_ERR_INVALID_ARG, "q_heads must be a multiple of kv_heads%s");
+  if (D < 8 || D > 256 || D % 8 != 0)
+    return fail(c, PLH_ERR_INVALID_ARG, "D must be a multiple of 8 up to 256%s");
+  a.N = N;
+  a.heads = q_heads;
+  a.kv_heads = kv_heads;
+  a.group = q_heads / kv_heads;
+  a.D = D;
+  a.B = B;
+  a.max_nodes = max_nodes < N ? max_nodes : N;
+  a.max_len = max_len > 0 ? max_len : 1;
+  // rows, workgroups and the workspace's floats are counted in 64 bits up to here
+  if ((int64_t)N * q_heads > INT32_MAX || (int64_t)B * kv_heads * (((int64_t)a.max_nodes * a.group + 15) / 16) > INT32_MAX / 16)
+    return fail(c, PLH_ERR_UNSUPPORTED, "more rows than a grid holds%s");
+  return PLH_OK;
+}
+
 constexpr size_t kScratchBytes = size_t(64) << 20;  // the no-allocation entry point's workspace, per GPU
 
 }  // namespace
@@ -936,6 +969,234 @@ int plh_fp8_linear(plh_ctx* c, const void* x, int dtype, int64_t ldx, int N, int
   a.V = V;
   const hipError_t e = plh::launch_fp8_linear(a, dtype, ws, c->num_cu, c->stream);
   if (e != hipSuccess) return hip_fail(c, e, "plh_fp8_linear launch");
+  return PLH_OK;
+}
+
+int64_t plh_tree_attention_ws_bytes(plh_ctx* c, int dtype, int N, int q_heads, int kv_heads, int D, int B, int max_nodes,
+                                    int64_t max_len) {
+  if (c == nullptr) return PLH_ERR_INVALID_ARG;
+  plh::AttendArgs a{};
+  const int rc = attend_sizes(c, a, dtype, N, q_heads, kv_heads, D, B, max_nodes, max_len);
+  return rc != PLH_OK ? rc : (int64_t)plh::plan_attend(a, dtype, c->num_cu);
+}
+
+int plh_tree_attention(plh_ctx* c, const void* q, int dtype, int64_t ldq, int N, int q_heads, int kv_heads, int D,
+                       const void* k_pages, const void* v_pages, int num_pages, int page_size,
+                       const int32_t* page_table, int64_t ldt, const int32_t* lens, const int32_t* node_off, int B,
+                       const uint64_t* visible, double scale, int max_nodes, int64_t max_len, void* out, int64_t ldo,
+                       float* lse, void* ws, int64_t ws_bytes) {
+  if (c == nullptr) return PLH_ERR_INVALID_ARG;
+  plh::AttendArgs a{};
+  int rc = attend_sizes(c, a, dtype, N, q_heads, kv_heads, D, B, max_nodes, max_len);
+  if (rc != PLH_OK) return rc;
+  rc = check_page_size(c, page_size);
+  if (rc != PLH_OK) return rc;
+  const int64_t width = (int64_t)q_heads * D;
+  if (ldq < width || ldo < width) return fail(c, PLH_ERR_INVALID_ARG, "need ldq and ldo >= q_heads * D%s");
+  if (num_pages < 1 || ldt < 1 || ldt > INT32_MAX)
+    return fail(c, PLH_ERR_INVALID_ARG, "need num_pages >= 1 and 1 <= ldt < 2^31%s");
+  if (visible != nullptr && max_nodes > PLH_MAX_TREE_NODES)
+    return fail(c, PLH_ERR_UNSUPPORTED, "masks hold trees of at most 64 nodes%s");
+  if (!(scale > 0.0) || !std::isfinite((float)scale))
+    return fail(c, PLH_ERR_INVALID_ARG, "scale must be finite and > 0%s");
+  if (N == 0 || B == 0 || max_nodes == 0) return PLH_OK;
+  if (q == nullptr || k_pages == nullptr || v_pages == nullptr || page_table == nullptr || lens == nullptr ||
+      node_off == nullptr || out == nullptr)
+    return fail(c, PLH_ERR_INVALID_ARG, "null device pointer%s");
+  if (!aligned16(k_pages) || !aligned16(v_pages))
+    return fail(c, PLH_ERR_INVALID_ARG, "k_pages and v_pages must be 16-byte aligned%s");
+  const size_t es = dtype == PLH_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(q) % es != 0 || reinterpret_cast<uintptr_t>(out) % es != 0)
+    return fail(c, PLH_ERR_INVALID_ARG, "q and out must be aligned to their element size%s");
+  if (rows_overlap(q, ldq, out, ldo, N, (int)width, es))
+    return fail(c, PLH_ERR_INVALID_ARG, "out must not overlap q%s");
+  rc = use_device(c);
+  if (rc != PLH_OK) return rc;
+  const size_t need = plh::plan_attend(a, dtype, c->num_cu);
+  if (need > 0 && (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0 || ws_bytes < (int64_t)need))
+    return fail(c, PLH_ERR_INVALID_ARG, "ws must be 256-byte aligned and hold plh_tree_attention_ws_bytes%s");
+  a.q = q;
+  a.ldq = ldq;
+  a.k = k_pages;
+  a.v = v_pages;
+  a.out = out;
+  a.ldo = ldo;
+  a.lse = lse;
+  a.table = page_table;
+  a.ldt = (int)ldt;
+  a.lens = lens;
+  a.node_off = node_off;
+  a.visible = visible;
+  a.scale = (float)(scale * 1.4426950408889634074);  // exponentials to base 2
+  a.num_pages = num_pages;
+  a.page_shift = page_shift_of(page_size);
+  const hipError_t e = plh::launch_attend(a, dtype, ws, c->stream);
+  if (e != hipSuccess) return hip_fail(c, e, "plh_tree_attention launch");
+  return PLH_OK;
+}
+
+int plh_rotary_append(plh_ctx* c, const void* q, int64_t ldq, int q_heads, void* q_out, int64_t ldqo, const void* k,
+                      int64_t ldk, const void* v, int64_t ldv, int kv_heads, int dtype, int N, int D,
+                      const int64_t* positions, const double* inv_freq, int pairs, int interleaved, double factor,
+                      void* k_pages, void* v_pages, int num_pages, int page_size, const int64_t* slots) {
+  if (c == nullptr) return PLH_ERR_INVALID_ARG;
+  if (dtype != PLH_F32 && dtype != PLH_BF16 && dtype != PLH_F16)
+    return fail(c, PLH_ERR_INVALID_ARG, "dtype must be PLH_F32, PLH_BF16 or PLH_F16%s");
+  if (N < 0 || D < 1 || D > 8192 || pairs < 0 || 2 * (int64_t)pairs > D)
+    return fail(c, PLH_ERR_INVALID_ARG, "need N >= 0, 1 <= D <= 8192 and 0 <= 2 * pairs <= D%s");
+  const bool has_q = q != nullptr || q_out != nullptr, has_kv = k != nullptr || v != nullptr;
+  if (has_q && (q_heads < 1 || (int64_t)q_heads * D > INT32_MAX))
+    return fail(c, PLH_ERR_INVALID_ARG, "need q_heads >= 1%s");
+  if (has_kv && (kv_heads < 1 || (int64_t)kv_heads * D > INT32_MAX / 4))
+    return fail(c, PLH_ERR_INVALID_ARG, "need kv_heads >= 1%s");
+  if (has_q && has_kv && ((int64_t)q_heads + 2 * (int64_t)kv_heads) * D > INT32_MAX)
+    return fail(c, PLH_ERR_INVALID_ARG, "rows of more than 2^31 - 1 values%s");
+  if (!std::isfinite((float)factor)) return fail(c, PLH_ERR_INVALID_ARG, "factor must be finite%s");
+  if (has_kv) {
+    const int rc = check_page_size(c, page_size);
+    if (rc != PLH_OK) return rc;
+    if (num_pages < 1) return fail(c, PLH_ERR_INVALID_ARG, "need num_pages >= 1%s");
+    if (ldk < (int64_t)kv_heads * D || ldv < (int64_t)kv_heads * D)
+      return fail(c, PLH_ERR_INVALID_ARG, "need ldk and ldv >= kv_heads * D%s");
+  }
+  if (has_q && (ldq < (int64_t)q_heads * D || ldqo < (int64_t)q_heads * D))
+    return fail(c, PLH_ERR_INVALID_ARG, "need ldq and ldqo >= q_heads * D%s");
+  if (N == 0 || (!has_q && !has_kv)) return PLH_OK;
+  if ((has_q && (q == nullptr || q_out == nullptr)) ||
+      (has_kv && (k == nullptr || v == nullptr || k_pages == nullptr || v_pages == nullptr || slots == nullptr)) ||
+      (pairs > 0 && (positions == nullptr || inv_freq == nullptr)))
+    return fail(c, PLH_ERR_INVALID_ARG, "null device pointer%s");
+  const size_t es = dtype == PLH_F32 ? 4 : 2;
+  for (const void* p : {q, (const void*)q_out, k, v, (const void*)k_pages, (const void*)v_pages})
+    if (reinterpret_cast<uintptr_t>(p) % es != 0)
+      return fail(c, PLH_ERR_INVALID_ARG, "rows and pages must be aligned to their element size%s");
+  if (has_q && (q == q_out ? ldq != ldqo : rows_overlap(q, ldq, q_out, ldqo, N, q_heads * D, es)))
+    return fail(c, PLH_ERR_INVALID_ARG, "q_out must be q itself (ldqo = ldq) or rows that meet none of it%s");
+  int rc = use_device(c);
+  if (rc != PLH_OK) return rc;
+  plh::RotaryArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_out = q_out;
+  a.k_pages = k_pages;
+  a.v_pages = v_pages;
+  a.pos = positions;
+  a.slots = slots;
+  a.freq = inv_freq;
+  a.ldq = ldq;
+  a.ldk = ldk;
+  a.ldv = ldv;
+  a.ldqo = ldqo;
+  a.factor = (float)factor;
+  a.N = N;
+  a.q_heads = q_heads;
+  a.kv_heads = kv_heads;
+  a.D = D;
+  a.pairs = pairs;
+  a.interleaved = interleaved ? 1 : 0;
+  if (has_kv) {
+    a.page_shift = page_shift_of(page_size);
+    a.num_slots = (int64_t)num_pages * page_size;
+  }
+  const hipError_t e = plh::launch_rotary(a, dtype, c->stream);
+  if (e != hipSuccess) return hip_fail(c, e, "plh_rotary_append launch");
+  return PLH_OK;
+}
+
+int plh_copy_pages(plh_ctx* c, void* k_pages, void* v_pages, int layers, int64_t layer_bytes, int num_pages,
+                   int64_t page_bytes, const int32_t* src, const int32_t* dst, int n) {
+  if (c == nullptr) return PLH_ERR_INVALID_ARG;
+  if (n < 0 || layers < 1 || layers > 65535 || num_pages < 1 || page_bytes < 16)
+    return fail(c, PLH_ERR_INVALID_ARG, "need n >= 0, 1 <= layers <= 65535, num_pages >= 1 and page_bytes >= 16%s");
+  if (page_bytes % 16 != 0 || layer_bytes % 16 != 0 || page_bytes > INT32_MAX ||
+      (layers > 1 && layer_bytes < (int64_t)num_pages * page_bytes))
+    return fail(c, PLH_ERR_INVALID_ARG,
+                "page_bytes (< 2^31) and layer_bytes must be multiples of 16, and layers must not overlap%s");
+  if (n > 0 && (int64_t)n * ((page_bytes + 16383) / 16384) > INT32_MAX)
+    return fail(c, PLH_ERR_UNSUPPORTED, "more pages than a grid holds%s");
+  if (n == 0) return PLH_OK;
+  if (k_pages == nullptr || v_pages == nullptr || src == nullptr || dst == nullptr)
+    return fail(c, PLH_ERR_INVALID_ARG, "null device pointer%s");
+  if (!aligned16(k_pages) || !aligned16(v_pages))
+    return fail(c, PLH_ERR_INVALID_ARG, "k_pages and v_pages must be 16-byte aligned%s");
+  int rc = use_device(c);
+  if (rc != PLH_OK) return rc;
+  const hipError_t e =
+      plh::launch_copy_pages(plh::CopyArgs{k_pages, v_pages, src, dst, layer_bytes, page_bytes, layers, num_pages, 0}, n, c->stream);
+  if (e != hipSuccess) return hip_fail(c, e, "plh_copy_pages launch");
+  return PLH_OK;
+}
+
+int plh_keep_nodes(plh_ctx* c, void* k_pages, void* v_pages, int layers, int64_t layer_bytes, int num_pages,
+                   int page_size, int kv_heads, int row_bytes, const int32_t* page_table, int64_t ldt,
+                   const int32_t* lens, const int32_t* path, int64_t ldp, const int32_t* n_acc, int B) {
+  if (c == nullptr) return PLH_ERR_INVALID_ARG;
+  if (B < 0 || B > 65535 || layers < 1 || num_pages < 1 || kv_heads < 1 || row_bytes < 16 || row_bytes % 16 != 0)
+    return fail(c, PLH_ERR_INVALID_ARG,
+                "need 0 <= B <= 65535, layers, num_pages and kv_heads >= 1, row_bytes a multiple of 16%s");
+  int rc = check_page_size(c, page_size);
+  if (rc != PLH_OK) return rc;
+  const int64_t page_rows = (int64_t)kv_heads * page_size;
+  if (layer_bytes % 16 != 0 || page_rows > INT32_MAX ||
+      (layers > 1 && (layer_bytes < 0 || (double)layer_bytes < (double)num_pages * page_rows * row_bytes)))
+    return fail(c, PLH_ERR_INVALID_ARG, "layer_bytes must be a multiple of 16, and layers must not overlap%s");
+  if (2 * (int64_t)layers * kv_heads > INT32_MAX / (row_bytes / 16))
+    return fail(c, PLH_ERR_UNSUPPORTED, "more rows than a grid holds%s");
+  if (ldt < 1 || ldt > INT32_MAX || ldp < 1 || ldp > INT32_MAX)
+    return fail(c, PLH_ERR_INVALID_ARG, "need 1 <= ldt, ldp < 2^31%s");
+  if (B == 0) return PLH_OK;
+  if (k_pages == nullptr || v_pages == nullptr || page_table == nullptr || lens == nullptr || path == nullptr ||
+      n_acc == nullptr)
+    return fail(c, PLH_ERR_INVALID_ARG, "null device pointer%s");
+  if (!aligned16(k_pages) || !aligned16(v_pages))
+    return fail(c, PLH_ERR_INVALID_ARG, "k_pages and v_pages must be 16-byte aligned%s");
+  rc = use_device(c);
+  if (rc != PLH_OK) return rc;
+  plh::KeepArgs a{};
+  a.k = k_pages;
+  a.v = v_pages;
+  a.layer_bytes = layer_bytes;
+  a.table = page_table;
+  a.lens = lens;
+  a.path = path;
+  a.n_acc = n_acc;
+  a.layers = layers;
+  a.num_pages = num_pages;
+  a.kv_heads = kv_heads;
+  a.page_shift = page_shift_of(page_size);
+  a.ldt = (int)ldt;
+  a.ldp = (int)ldp;
+  a.pieces = row_bytes / 16;
+  const hipError_t e = plh::launch_keep(a, B, c->stream);
+  if (e != hipSuccess) return hip_fail(c, e, "plh_keep_nodes launch");
+  return PLH_OK;
+}
+
+int plh_verify_tree(plh_ctx* c, const void* p, const void* q, int dtype, int64_t ld, int N, int V,
+                    const int32_t* tokens, const int32_t* parents, const int32_t* node_off, int B, int max_nodes,
+                    const double* uniforms, int64_t ldu, int replacement, int32_t* out_tokens, int32_t* out_path,
+                    int32_t* out_n_acc, int32_t* out_n_used) {
+  if (c == nullptr) return PLH_ERR_INVALID_ARG;
+  if (B < 0 || N < 0 || V < 1 || max_nodes < 1)
+    return fail(c, PLH_ERR_INVALID_ARG, "need B >= 0, N >= 0, V >= 1 and max_nodes >= 1%s");
+  if (dtype != PLH_F32 && dtype != PLH_F64) return fail(c, PLH_ERR_INVALID_ARG, "dtype must be PLH_F32 or PLH_F64%s");
+  if (ld < V || ldu < max_nodes) return fail(c, PLH_ERR_INVALID_ARG, "need ld >= V and ldu >= max_nodes%s");
+  if (max_nodes > plh::kTreeNodes) return fail(c, PLH_ERR_UNSUPPORTED, "trees of more than 256 nodes%s");
+  if (V > plh::kTreeV) return fail(c, PLH_ERR_UNSUPPORTED, "rows of more than 524288 tokens%s");
+  if (B == 0) return PLH_OK;
+  if (p == nullptr || tokens == nullptr || parents == nullptr || node_off == nullptr || uniforms == nullptr ||
+      out_tokens == nullptr || out_path == nullptr || out_n_acc == nullptr || out_n_used == nullptr)
+    return fail(c, PLH_ERR_INVALID_ARG, "null device pointer%s");
+  const size_t es = dtype == PLH_F64 ? 8 : 4;
+  if (reinterpret_cast<uintptr_t>(p) % es != 0 || reinterpret_cast<uintptr_t>(q) % es != 0)
+    return fail(c, PLH_ERR_INVALID_ARG, "p and q must be aligned to their element size%s");
+  int rc = use_device(c);
+  if (rc != PLH_OK) return rc;
+  plh::TreeArgs a{p,  q,     ld, tokens, parents,   node_off,    uniforms,            ldu,       N,
+                  B,  V,     max_nodes,  replacement ? 1 : 0, out_tokens, out_path, out_n_acc, out_n_used};
+  const hipError_t e = plh::launch_verify_tree(a, dtype == PLH_F64, c->stream);
+  if (e != hipSuccess) return hip_fail(c, e, "plh_verify_tree launch");
   return PLH_OK;
 }
 

@@ -205,6 +205,83 @@ struct Fp8Args {
   int kb;              // blocks of 128 in a row: ceil(D / 128)
 };
 
+struct AttendArgs {
+  const void* q;           // [N, ldq]: heads x D of a row
+  int64_t ldq;
+  const void* k;           // [num_pages, kv_heads, page size, D]
+  const void* v;
+  void* out;               // [N, ldo]
+  int64_t ldo;
+  float* lse;              // [N, heads] or null
+  const int32_t* table;    // [B, ldt] pages of each sequence
+  const int32_t* lens;     // [B] keys ahead of the nodes
+  const int32_t* node_off; // [B + 1]
+  const uint64_t* visible; // [N] or null (a chain)
+  float* part_o;           // workspace, with several chunks: [chunks, N, heads, D]
+  float* part_ml;          // [chunks, N, heads, 2]
+  float scale;             // of the scores, times log2(e)
+  int ldt, num_pages, page_shift;
+  int B, N, heads, kv_heads, group, D;
+  int max_nodes;
+  int64_t max_len;
+  int row_tiles, row_blocks, chunk, chunks;  // plan_attend
+};
+
+struct RotaryArgs {
+  const void* q;      // [N, ldq] or null
+  const void* k;      // [N, ldk] or null (v then too)
+  const void* v;
+  void* q_out;        // [N, ldqo]
+  void* k_pages;
+  void* v_pages;
+  const int64_t* pos;   // [N]
+  const int64_t* slots; // [N]
+  const double* freq;   // [pairs]
+  int64_t ldq, ldk, ldv, ldqo, num_slots;
+  float factor;
+  int N, q_heads, kv_heads, D, pairs, interleaved, page_shift;
+};
+
+struct CopyArgs {
+  void* k;
+  void* v;
+  const int32_t* src;
+  const int32_t* dst;
+  int64_t layer_bytes, page_bytes;
+  int layers, num_pages;
+  int slices;  // launch_copy_pages
+};
+
+struct KeepArgs {
+  void* k;
+  void* v;
+  int64_t layer_bytes;
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* path;   // [B, ldp]
+  const int32_t* n_acc;  // [B]
+  int layers, num_pages, kv_heads, page_shift, ldt, ldp;
+  int pieces;            // of 16 bytes in a token's row of a head
+};
+
+struct TreeArgs {
+  const void* p;   // [N, ld]
+  const void* q;   // [N, ld] or null: each child is its draft's only token
+  int64_t ld;
+  const int32_t* tokens;
+  const int32_t* parents;
+  const int32_t* node_off;
+  const double* u;  // [B, ldu]
+  int64_t ldu;
+  int N, B, V, max_nodes, replacement;
+  int32_t* out_tokens;  // [B, max_nodes]
+  int32_t* out_path;    // [B, max_nodes]
+  int32_t* out_n_acc;
+  int32_t* out_n_used;
+};
+constexpr int kTreeNodes = 256;     // of one sequence's tree
+constexpr int kTreeV = 1 << 19;     // tokens of a row: their pieces' sums lie in LDS
+
 // Rows of at most kSmallV tokens: the whole call in one launch, no workspace.
 // `between` (when not null) is recorded after it.
 constexpr int kSmallV = 1024;
@@ -261,6 +338,13 @@ hipError_t launch_fp8_pack(const uint8_t* codes, int64_t ldc, const float* scale
 hipError_t launch_fp8_quantize(const void* w, int dtype, int64_t stride_v, int64_t stride_d, int V, int D,
                                uint8_t* out_codes, float* out_scales, hipStream_t s);
 hipError_t launch_fp8_linear(Fp8Args a, int dtype, void* ws, int num_cu, hipStream_t s);
+// Attention of tree nodes over pages: plan_attend fills in the plan and returns the workspace's bytes.
+size_t plan_attend(AttendArgs& a, int dtype, int num_cu);
+hipError_t launch_attend(AttendArgs a, int dtype, void* ws, hipStream_t s);
+hipError_t launch_rotary(const RotaryArgs& a, int dtype, hipStream_t s);
+hipError_t launch_copy_pages(CopyArgs a, int n, hipStream_t s);
+hipError_t launch_keep(const KeepArgs& a, int B, hipStream_t s);
+hipError_t launch_verify_tree(const TreeArgs& a, bool f64, hipStream_t s);
 hipError_t launch_append(int32_t* slab, const int64_t* pos, const int32_t* ids, int n, hipStream_t s);
 
 }  // namespace plh

@@ -1,0 +1,409 @@
+"""Speculation with trees of drafted tokens, batched over sequences.
+
+The reference drafts a chain a sequence (``SpeculativeDecoder.generate``,
+``src/pagellm/engine/speculative.py:97-140``), and :mod:`pagellm_amd.speculative`
+verifies chains in batches.  A tree has several candidates for a position, and one
+target forward verifies all of them:
+
+* :class:`DraftTree`: one sequence's tree, its root the last token that the target
+  has not seen;
+* :func:`tree_attention`: attention of a step's nodes over a paged cache
+  (``plh_tree_attention``), for :class:`pagellm_amd.cache.CacheStep`;
+* :func:`verify_tree`: the accepted path of each tree and the token after it, from
+  given uniforms (``plh_verify_tree``);
+* :func:`verify_tree_step`: the target's side of a round, from its logits and each
+  sequence's Generator;
+* :class:`TreeDecoder`: rounds of a batch over a cache.
+"""
+
+from __future__ import annotations
+
+from typing import Callable, NamedTuple, Sequence
+
+import numpy as np
+
+from . import _native
+from .cache import CacheStep, PagedCache, _check_pages, _ints, _rows, _table
+from .fp8 import _check_device, _float_code
+from .logits import _pack
+from .sampling import _as_float_rows, _ctx, _expand_params, _history_ids, _is_torch_cuda, _pack_params, _stream_of
+
+__all__ = ["DraftTree", "TreeDecoder", "TreeRound", "TreeVerdict", "tree_attention", "verify_tree", "verify_tree_step"]
+
+
+class DraftTree:
+    """``tokens[0]`` is the root, ``tokens[i]`` a draft for the place after node
+    ``parents[i]`` (-1 for the root, else a node before i).  Siblings are tested in
+    their order.  ``depths`` and ``visible`` (bit j of node i's: i sees node j, its
+    ancestor or itself; None past 64 nodes, which only a chain may have) follow."""
+
+    def __init__(self, tokens: Sequence[int], parents: Sequence[int] | None = None):
+        t = np.asarray(tokens, dtype=np.int64).reshape(-1)
+        if t.size < 1:
+            raise ValueError("a tree has at least its root")
+        if t.min() < 0 or t.max() > 2**31 - 1:
+            raise ValueError("tokens must be in [0, 2^31)")
+        p = np.arange(-1, t.size - 1) if parents is None else np.asarray(parents, dtype=np.int64).reshape(-1)
+        if p.size != t.size:
+            raise ValueError(f"expected {t.size} parents, got {p.size}")
+        if p[0] != -1 or np.any(p[1:] < 0) or np.any(p >= np.arange(t.size)):
+            raise ValueError("parents must be -1 for the root and an earlier node for every other one")
+        self.tokens, self.parents = t.astype(np.int32), p.astype(np.int32)
+        self.chain = bool(np.array_equal(p, np.arange(-1, t.size - 1)))
+        if not self.chain and t.size > _native.PLH_MAX_TREE_NODES:
+            raise ValueError(f"a tree has at most {_native.PLH_MAX_TREE_NODES} nodes")
+        depths, bits = [], []
+        for i, up in enumerate(p.tolist()):
+            depths.append(depths[up] + 1 if i else 0)
+            bits.append((bits[up] if i else 0) | 1 << i)
+        self.depths = np.asarray(depths, dtype=np.int64)
+        self.visible = np.array(bits, dtype=np.uint64) if t.size <= 64 else None
+
+    def __len__(self) -> int:
+        return int(self.tokens.size)
+
+    def path_to(self, node: int) -> list[int]:
+        """The tokens after the root on the way to ``node``."""
+        out = []
+        while node > 0:
+            out.append(int(self.tokens[node]))
+            node = int(self.parents[node])
+        return out[::-1]
+
+
+def tree_attention(q, k_pages, v_pages, page_table, lens, node_off, visible=None, *, max_nodes: int, max_len: int,
+                   scale: float | None = None, out=None, lse=None, ctx: _native.Context | None = None):
+    """Attention of a step's rows over one layer's pages [pages, kv heads, page size, D].
+
+    ``q`` [N, heads, D] holds the nodes of the sequences one after the other, those of
+    b from ``node_off[b]`` (int32 [B + 1]); sequence b's first ``lens[b]`` (int32 [B])
+    tokens lie in its pages ``page_table[b]`` (int32 [B, pages]), its nodes' keys and
+    values behind them.  A row sees the tokens, and of its tree the nodes whose bits
+    are set in ``visible`` (int64 or uint64 [N]; at most 64 nodes), or without
+    ``visible`` the nodes up to itself.  ``max_nodes`` and ``max_len`` are at least the
+    nodes and the tokens with nodes of every sequence.  ``scale`` is D ** -0.5 when
+    None.  Returns ``out`` [N, heads, D] (a new tensor when None); ``lse`` (float32
+    [N, heads]) takes the logarithms of the rows' sums.  Rows past node_off[B] are left
+    as they are."""
+    import torch
+
+    c = _ctx(ctx)
+    heads, dim, ldq = _rows(c, q, "q")
+    code = _float_code(q, "q")
+    _check_pages(c, k_pages, v_pages, 4)
+    if k_pages.dtype != q.dtype:
+        raise TypeError("q and the pages must have one type")
+    N, (pages, kv_heads, page_size, page_dim) = int(q.shape[0]), k_pages.shape
+    if page_dim != dim:
+        raise ValueError(f"the pages hold heads of {page_dim} values, q of {dim}")
+    for x, name in ((lens, "lens"), (node_off, "node_off")):
+        _check_device(c, x, name)
+        if x.dtype != torch.int32 or x.dim() != 1 or not x.is_contiguous():
+            raise TypeError(f"{name} must be contiguous int32, one for each sequence")
+    B = int(lens.shape[0])
+    if node_off.shape[0] != B + 1:
+        raise ValueError(f"node_off must have {B + 1} entries")
+    page_table, width, ldt = _table(c, page_table, B)
+    if ldt != width:  # a row's stride would count as its length
+        page_table, ldt = page_table.contiguous(), width
+    bits = None
+    if visible is not None:
+        _check_device(c, visible, "visible")
+        if visible.dtype not in (torch.int64, torch.uint64) or tuple(visible.shape) != (N,) or not visible.is_contiguous():
+            raise TypeError(f"visible must be contiguous int64 or uint64 [{N}]")
+        bits = visible.data_ptr()
+    max_nodes, max_len = int(max_nodes), int(max_len)
+    if not (0 <= max_nodes <= 2**31 - 1 and 0 <= max_len <= 2**30 and N <= 2**31 - 1):  # ctypes would wrap them
+        raise ValueError("need 0 <= max_nodes < 2^31, 0 <= max_len <= 2^30 and less than 2^31 rows")
+    if out is None:
+        out = torch.empty((N, heads, dim), dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape:
+        raise ValueError("out must be like q")
+    ldo = _rows(c, out, "out")[2]
+    if lse is not None:
+        _check_device(c, lse, "lse")
+        if lse.dtype != torch.float32 or tuple(lse.shape) != (N, heads) or not lse.is_contiguous():
+            raise TypeError(f"lse must be contiguous float32 [{N}, {heads}]")
+    if N == 0 or B == 0:
+        return out
+    c.set_stream(_stream_of(q))
+    nbytes = c.tree_attention_ws_bytes(code, N, heads, kv_heads, dim, B, max_nodes, max_len)
+    # torch's allocator orders its reuse on the stream
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    c.tree_attention(q.data_ptr(), code, ldq, N, heads, kv_heads, dim, k_pages.data_ptr(), v_pages.data_ptr(), pages,
+                     page_size, page_table.data_ptr(), ldt, lens.data_ptr(), node_off.data_ptr(), B, bits,
+                     dim ** -0.5 if scale is None else float(scale), max_nodes, max_len, out.data_ptr(), ldo,
+                     lse.data_ptr() if lse is not None else None, ws.data_ptr() if nbytes else None, nbytes)
+    return out
+
+
+class TreeVerdict(NamedTuple):
+    """Of each sequence: ``tokens`` [B, max_nodes], the accepted nodes' and the one
+    after them, then -1; ``path`` [B, max_nodes], 0 and the accepted nodes, then -1;
+    ``n_acc`` [B], how many were accepted; ``n_used`` [B], the uniforms that took."""
+
+    tokens: object
+    path: object
+    n_acc: object
+    n_used: object
+
+
+def verify_tree(p, q, tokens, parents, node_off, uniforms, *, max_nodes: int | None = None, replacement: bool = False,
+                ctx: _native.Context | None = None) -> TreeVerdict:
+    """Accept/resample over trees (``speculative.py:38-60`` over siblings in turn).
+
+    ``p`` [N, V] are the target's distributions after the nodes, ``q`` [N, V] the
+    draft's that their children were drawn from, without replacement unless
+    ``replacement`` (None: each child was its draft's only choice), float32 or
+    float64.  ``tokens`` and ``parents`` [N] (a node's place in its own tree),
+    ``node_off`` [B + 1], ``uniforms`` [B, >= max_nodes] float64, of which a sequence
+    uses one for each test and one for the draw.  Numpy arrays give numpy arrays
+    (int64); CUDA tensors (of p, q and uniforms; ``max_nodes`` must be given) give
+    CUDA tensors (int32), not waited for."""
+    import torch
+
+    c = _ctx(ctx)
+    on_gpu = _is_torch_cuda(p)
+    if not on_gpu:
+        p = _as_float_rows(p)
+        q = None if q is None else _as_float_rows(q)
+        dt = p.dtype if q is None else np.result_type(p.dtype, q.dtype)
+        off = np.asarray(node_off, dtype=np.int64).reshape(-1)
+        if p.ndim != 2 or p.shape[1] < 1:
+            raise ValueError("p must be [N, V]")
+        N, V = p.shape
+        if off.size < 1 or off[0] != 0 or off[-1] > N or np.any(np.diff(off) < 1):
+            raise ValueError("node_off must ascend from 0 to at most N")
+        tok, par = (np.asarray(x, dtype=np.int64).reshape(-1) for x in (tokens, parents))
+        if tok.size != N or par.size != N:
+            raise ValueError(f"expected {N} tokens and parents")
+        inner = np.ones(N, dtype=bool)
+        inner[off[:-1]] = False
+        inner[off[-1]:] = False
+        if np.any((tok[inner] < 0) | (tok[inner] >= V)):
+            raise IndexError(f"tokens must be in [0, {V})")
+        place = np.arange(N) - off[np.clip(np.searchsorted(off, np.arange(N), side="right") - 1, 0, max(off.size - 2, 0))]
+        if np.any((par[inner] < 0) | (par[inner] >= place[inner])):
+            raise ValueError("parents must be earlier nodes of the same tree")
+        most = int(np.diff(off).max(initial=1))
+        if max_nodes is not None and max_nodes < most:
+            raise ValueError(f"a tree has {most} nodes, max_nodes is {max_nodes}")
+        u = np.asarray(uniforms, dtype=np.float64)
+        dev = torch.device("cuda", c.device)
+        up = lambda x: torch.from_numpy(np.ascontiguousarray(x)).to(dev)  # noqa: E731
+        got = verify_tree(up(p.astype(dt, copy=False)), None if q is None else up(q.astype(dt, copy=False)), up(tok), up(par),
+                          up(off), up(u), max_nodes=max_nodes or most, replacement=replacement, ctx=c)
+        return TreeVerdict(*(x.cpu().numpy().astype(np.int64) for x in got))
+    _check_device(c, p, "p")
+    if p.dtype not in (torch.float32, torch.float64):
+        raise TypeError("p must be float32 or float64")
+    if p.dim() != 2 or p.shape[1] < 1 or (p.shape[1] > 1 and p.stride(1) != 1):
+        raise ValueError("p must be [N, V] with unit stride in the vocabulary dimension")
+    N, V = int(p.shape[0]), int(p.shape[1])
+    if q is not None:
+        _check_device(c, q, "q")
+        if q.dtype != p.dtype or q.shape != p.shape or (V > 1 and q.stride(1) != 1):
+            raise ValueError("q must be like p")
+        if N > 1 and q.stride(0) != p.stride(0):
+            raise ValueError("rows of p and q must lie as far apart")
+    if max_nodes is None:
+        raise ValueError("CUDA tensors need max_nodes")
+    ld = int(p.stride(0)) if N > 1 else V
+    max_nodes = int(max_nodes)
+    if max(N, V, max_nodes) > 2**31 - 1:  # ctypes would wrap them
+        raise ValueError("at most 2^31 - 1 rows, tokens and nodes")
+    tokens = _ints(c, tokens, "tokens", torch.int32, N)
+    parents = _ints(c, parents, "parents", torch.int32, N)
+    node_off = _ints(c, node_off, "node_off", torch.int32)
+    if node_off.dim() != 1 or node_off.shape[0] < 1:
+        raise ValueError("node_off must be [B + 1]")
+    B = int(node_off.shape[0]) - 1
+    _check_device(c, uniforms, "uniforms")
+    if uniforms.dtype != torch.float64 or uniforms.dim() != 2 or uniforms.shape[0] != B or uniforms.shape[1] < max_nodes or \
+            (uniforms.shape[1] > 1 and uniforms.stride(1) != 1):
+        raise ValueError(f"uniforms must be float64 [{B}, >= {max_nodes}] with unit stride")
+    ldu = int(uniforms.stride(0)) if B > 1 else int(uniforms.shape[1])
+    if B > 1 and ldu < max_nodes:
+        uniforms, ldu = uniforms.contiguous(), int(uniforms.shape[1])
+    out = torch.empty(B * (2 * max_nodes + 2), dtype=torch.int32, device=p.device)
+    n = B * max_nodes
+    res = TreeVerdict(out[:n].view(B, max_nodes), out[n:2 * n].view(B, max_nodes), out[2 * n:2 * n + B], out[2 * n + B:])
+    if B == 0:
+        return res
+    c.set_stream(_stream_of(p))
+    at = out.data_ptr()
+    c.verify_tree(p.data_ptr(), q.data_ptr() if q is not None else None,
+                  _native.PLH_F64 if p.dtype == torch.float64 else _native.PLH_F32, ld, N, V, tokens.data_ptr(),
+                  parents.data_ptr(), node_off.data_ptr(), B, max_nodes, uniforms.data_ptr(), ldu, replacement, at,
+                  at + 4 * n, at + 8 * n, at + 8 * n + 4 * B)
+    return res
+
+
+class TreeRound(NamedTuple):
+    """``emitted`` [B] token lists (the accepted drafts and the token after them) and
+    ``n_acc`` int64 [B]; ``verdict``: :class:`TreeVerdict` on the GPU."""
+
+    emitted: list
+    n_acc: np.ndarray
+    verdict: TreeVerdict
+
+
+def _tree_histories(contexts, params, trees, V: int):
+    """Histories of the nodes' rows as (ids, offsets): a sequence's context (the root
+    its last token) and the drafts on the way to the node; empty where the penalty is
+    off.  (None, None) when no row reads one."""
+    parts, sizes = [], [0]
+    for ctx, prm, tree in zip(contexts, params, trees):
+        off = prm.repetition_penalty == 1.0
+        ids = None if off else _history_ids(ctx if ctx is not None else (), V)
+        for i in range(len(tree)):
+            if off:
+                sizes.append(0)
+                continue
+            way = np.asarray(tree.path_to(i), dtype=np.int32)
+            parts += [ids, way]
+            sizes.append(ids.size + way.size)
+    offs = np.cumsum(sizes, dtype=np.int64)
+    if offs[-1] == 0:
+        return None, None
+    return np.concatenate(parts).astype(np.int32, copy=False), offs
+
+
+def verify_tree_step(target_logits, q_rows, trees: Sequence[DraftTree], params, rngs, contexts=None, *,
+                     replacement: bool = False, ctx: _native.Context | None = None) -> TreeRound:
+    """The target's side of one round for B sequences with a tree each, as
+    :func:`pagellm_amd.speculative.verify_step` is for chains: ``p[n] =
+    probs(target_logits[n], params_b, contexts[b] + the drafts on the way to n)``
+    (``speculative.py:125-127``; contexts end with the roots), then
+    :func:`verify_tree` with the uniforms of ``rngs[b]``, which ends where a loop that
+    draws one for each test and one for the token leaves it.
+
+    ``target_logits`` [N, V] are the rows of the trees one after the other, numpy or a
+    CUDA tensor (read in place on torch's current stream); ``q_rows`` float64 [N, V],
+    of the same kind, or None for drafts that are their draft's only choice."""
+    import torch
+
+    c = _ctx(ctx)
+    trees = list(trees)
+    B, counts = len(trees), [len(t) for t in trees]
+    params = _expand_params(params, B)
+    contexts = [()] * B if contexts is None else contexts
+    if len(contexts) != B or len(rngs) != B:
+        raise ValueError(f"expected {B} contexts and Generators")
+    dev = torch.device("cuda", c.device)
+    x = target_logits
+    if not _is_torch_cuda(x):
+        x = torch.from_numpy(_as_float_rows(x)).to(dev)
+    _check_device(c, x, "target_logits")
+    if x.dtype not in (torch.float32, torch.float64):
+        raise TypeError("target_logits must be float32 or float64")
+    if x.dim() != 2 or x.shape[0] != sum(counts) or x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError(f"target_logits must be [{sum(counts)}, V] with unit stride in the vocabulary dimension")
+    N, V = int(x.shape[0]), int(x.shape[1])
+    if N > 1 and x.stride(0) < V:
+        raise ValueError("rows of target_logits must not overlap")
+    if q_rows is not None:
+        if not _is_torch_cuda(q_rows):
+            q_rows = torch.from_numpy(np.ascontiguousarray(q_rows, dtype=np.float64)).to(dev)
+        if q_rows.dtype != torch.float64 or tuple(q_rows.shape) != (N, V):
+            raise ValueError(f"q_rows must be float64 [{N}, {V}]")
+        q_rows = q_rows.contiguous()
+    for t in trees:
+        if int(t.tokens[1:].max(initial=0)) >= V:
+            raise IndexError(f"drafts must be in [0, {V})")
+    if B == 0:
+        empty = torch.empty((0, 0), dtype=torch.int32, device=dev)
+        return TreeRound([], np.zeros(0, dtype=np.int64), TreeVerdict(empty, empty, empty[:, 0:0].reshape(-1), empty.reshape(-1)))
+    most = max(counts)
+    if most > 256:
+        raise NotImplementedError("trees of more than 256 nodes")
+    ids, offs = _tree_histories(contexts, params, trees, V)
+    states = [g.bit_generator.state for g in rngs]
+    u = np.zeros((B, most))
+    for b, n in enumerate(counts):
+        u[b, :n] = rngs[b].random(n)
+        rngs[b].bit_generator.state = states[b]
+    t, k, p, r = (np.repeat(a, counts) for a in _pack_params(params))
+    parts = [t, p, r, np.zeros(N), u, offs, k, np.concatenate([x.tokens for x in trees]),
+             np.concatenate([x.parents for x in trees]), np.cumsum([0] + counts).astype(np.int32), ids]
+    mem = None
+
+    def empty(n):
+        nonlocal mem  # first: what fails here leaves no staged memory given
+        mem = torch.empty(n, dtype=torch.uint8, device=dev)
+        c.set_stream(_stream_of(x))
+        return c.stage(n)
+
+    buf, at = _pack(parts, empty)
+    base = mem.data_ptr()
+    c.stage_h2d(base, buf)
+    d_t, d_p, d_r, d_0, d_u, d_off, d_k, d_tok, d_par, d_node, d_ids = (None if o is None else base + o for o in at)
+    probs = torch.empty((N, V), dtype=torch.float64, device=dev)
+    picks = torch.empty(N, dtype=torch.int32, device=dev)
+    c.sample(x.data_ptr(), _native.PLH_F64 if x.dtype == torch.float64 else _native.PLH_F32,
+             int(x.stride(0)) if N > 1 else V, N, V, d_ids, d_off, d_t, d_k, d_p, d_r, d_0, picks.data_ptr(),
+             probs.data_ptr(), 0)
+    out = torch.empty(B * (2 * most + 2), dtype=torch.int32, device=dev)
+    n = B * most
+    c.verify_tree(probs.data_ptr(), None if q_rows is None else q_rows.data_ptr(), _native.PLH_F64, V, N, V, d_tok, d_par,
+                  d_node, B, most, d_u, most, replacement, out.data_ptr(), out.data_ptr() + 4 * n, out.data_ptr() + 8 * n,
+                  out.data_ptr() + 8 * n + 4 * B)
+    verdict = TreeVerdict(out[:n].view(B, most), out[n:2 * n].view(B, most), out[2 * n:2 * n + B], out[2 * n + B:])
+    host = out.cpu().numpy().astype(np.int64)
+    toks, n_acc, used = host[:n].reshape(B, most), host[2 * n:2 * n + B], host[2 * n + B:]
+    emitted = []
+    for b in range(B):
+        rngs[b].random(int(used[b]))
+        emitted.append([int(v) for v in toks[b, : n_acc[b] + 1]])
+    return TreeRound(emitted, n_acc.copy(), verdict)
+
+
+class TreeDecoder:
+    """Rounds of speculation for a batch, the target's keys and values in a
+    :class:`pagellm_amd.cache.PagedCache`.
+
+    ``forward(step)`` is the target: it computes the logits [N, V] (a CUDA tensor)
+    of the step's nodes from ``step.tokens`` and calls ``step.attend(layer, q, k, v,
+    rotary)`` in each layer, as the reference's ``Transformer.forward`` calls its cache
+    (``src/pagellm/model/transformer.py:235-271``).
+
+        decoder.prefill(keys, prompts)
+        emitted, n_acc, _ = decoder.round(keys, trees, params, rngs, contexts)
+
+    A round takes each sequence's tree (its root the last token of its context), runs
+    the target once, accepts a path and moves its keys and values together; the
+    emitted tokens join the context, and the last of them is the next root."""
+
+    def __init__(self, cache: PagedCache, forward: Callable[[CacheStep], object]):
+        self.cache, self.forward = cache, forward
+
+    def prefill(self, keys: Sequence, prompts: Sequence[Sequence[int]]) -> None:
+        """New sequences whose prompts but their last tokens go into the cache."""
+        keys, prompts = list(keys), [list(p) for p in prompts]
+        if len(keys) != len(prompts) or any(len(p) < 1 for p in prompts):
+            raise ValueError("expected a prompt of at least one token for each sequence")
+        for key in keys:
+            if key in self.cache:
+                raise ValueError(f"sequence {key!r} is in the cache already")
+        for key in keys:
+            self.cache.add(key)
+        some = [(key, p) for key, p in zip(keys, prompts) if len(p) > 1]
+        if some:
+            try:
+                step = self.cache.step([key for key, _ in some], [DraftTree(p[:-1]) for _, p in some])
+            except Exception:
+                for key in keys:
+                    self.cache.remove(key)
+                raise
+            self.forward(step)
+            self.cache.commit(step)
+
+    def round(self, keys: Sequence, trees: Sequence[DraftTree], params, rngs, contexts=None, *, q_rows=None,
+              replacement: bool = False) -> TreeRound:
+        """One round; ``q_rows`` and ``replacement`` as :func:`verify_tree_step`."""
+        step = self.cache.step(keys, trees)
+        logits = self.forward(step)
+        res = verify_tree_step(logits, q_rows, step.trees, params, rngs, contexts, replacement=replacement,
+                               ctx=self.cache.ctx)
+        self.cache.commit(step, res.verdict.path, res.verdict.n_acc, accepted=res.n_acc)
+        return res

@@ -1,0 +1,370 @@
+"""Attention of tree nodes over a paged cache (``plh_tree_attention``) against the
+float64 oracle (needs an MI355X).
+
+Tolerance of a row.  A score is a float32 sum of D products (of D steps of 2^-24 of
+sum |q| |k|) times a factor rounded once more, and its exponential takes an argument
+rounded at up to 2^-24 of the score (and of the distance to the maximum, which at the
+distances that count is below 2^6) and is right to 2^-22: a weight is off by at most
+e = (D + 4) 2^-24 * scale * sum |q| |k| + 2^-17 of itself.  The weights are rounded to
+the cache's type for the second product (u = 0, 2^-8 or 2^-11) and enter both sums, each
+added in float32 (L + 64 roundings, chunks and waves joined among them), and the result
+is rounded to the type:
+  |out - exact| <= (2 e + u + 2 (L + 64) 2^-24) * sum w |v| / sum w + u |exact|
+  |lse - exact| <= e + (L + 64) 2^-24 + 2^-22 (1 + |exact|)"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from oracle import tree as O
+from pagellm_amd.tree import DraftTree, tree_attention
+
+pytestmark = pytest.mark.gpu
+
+U = {"float32": 0.0, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}
+
+
+def _tree(g, n, width):
+    return DraftTree(np.zeros(n), [-1] + [int(g.integers(max(0, i - width), i)) for i in range(1, n)])
+
+
+class Case:
+    """A batch's pages, filled with NaN where no token lies, and its rows."""
+
+    def __init__(self, seed, lens, trees, heads, kv_heads, dim, ps, dtype, extra_pages=3, spare_rows=0):
+        import torch
+
+        g = np.random.default_rng(seed)
+        dt = getattr(torch, dtype)
+        self.lens, self.trees, self.heads, self.kv_heads, self.dim, self.ps, self.dtype = lens, trees, heads, kv_heads, dim, ps, dtype
+        counts = [len(t) if t is not None else 0 for t in trees]
+        self.counts = counts
+        need = [-(-(n + t) // ps) for n, t in zip(lens, counts)]
+        pages = sum(need) + extra_pages
+        order = g.permutation(pages)
+        table = g.integers(-5, pages + 5, (len(lens), max(max(need), 1))).astype(np.int32)
+        self.k = np.full((pages, kv_heads, ps, dim), np.nan)
+        self.v = np.full((pages, kv_heads, ps, dim), np.nan)
+        self.keys, self.values, at = [], [], 0
+        rnd = lambda *s: torch.from_numpy(g.standard_normal(s)).to(dt).double().numpy()  # noqa: E731
+        for b, (n, t) in enumerate(zip(lens, counts)):
+            mine = order[at:at + need[b]]
+            at += need[b]
+            table[b, :need[b]] = mine
+            k, v = rnd(n + t, kv_heads, dim), rnd(n + t, kv_heads, dim)
+            self.keys.append(k)
+            self.values.append(v)
+            for x in range(n + t):
+                self.k[mine[x // ps], :, x % ps] = k[x]
+                self.v[mine[x // ps], :, x % ps] = v[x]
+        self.off = np.cumsum([0] + counts)
+        self.N = int(self.off[-1]) + spare_rows
+        self.q = 1.5 * rnd(self.N, heads, dim)
+        self.q = torch.from_numpy(self.q).to(dt).double().numpy()
+        self.table = table
+        chain = all(t is None or t.chain for t in trees)
+        self.visible = None if chain else np.concatenate(
+            [t.visible for t in trees if t is not None] + [np.zeros(spare_rows, np.uint64)]).view(np.int64)
+
+    def device(self):
+        import torch
+
+        dt = getattr(torch, self.dtype)
+        up = lambda x, t: torch.from_numpy(np.ascontiguousarray(x)).to("cuda", t)  # noqa: E731
+        d = dict(q=up(self.q, dt), k_pages=up(self.k, dt), v_pages=up(self.v, dt), page_table=up(self.table, torch.int32),
+                 lens=up(np.asarray(self.lens, dtype=np.int64), torch.int32), node_off=up(self.off, torch.int32))
+        d["visible"] = None if self.visible is None else up(self.visible, torch.int64)
+        d["max_nodes"] = max(self.counts + [1])
+        d["max_len"] = max([n + t for n, t in zip(self.lens, self.counts)] + [1])
+        return d
+
+    def check(self, out, lse, scale=None):
+        out, lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
+        scale = self.dim ** -0.5 if scale is None else scale
+        u, worst = U[self.dtype], 0.0
+        for b, (n, t) in enumerate(zip(self.lens, self.counts)):
+            rows = slice(self.off[b], self.off[b + 1])
+            sees = O.sees_of(n, t, None if self.visible is None else self.visible[rows].view(np.uint64))
+            for h in range(self.heads):
+                kvh = h // (self.heads // self.kv_heads)
+                ref, ref_lse, spread, top = O.attend_sequence(self.q[rows, h], self.keys[b][:, kvh], self.values[b][:, kvh],
+                                                              sees, scale)
+                L = n + t
+                e = (self.dim + 4) * 2.0 ** -24 * top + 2.0 ** -17
+                tol = (2 * e + u + 2 * (L + 64) * 2.0 ** -24)[:, None] * spread + u * np.abs(ref) + 1e-30
+                got = out[rows, h]
+                assert np.array_equal(np.isnan(got), np.isnan(ref)), (b, h)
+                assert np.array_equal(np.isinf(got), np.isinf(ref)), (b, h)
+                fine = np.isfinite(ref)
+                err = np.abs(got - ref)[fine]
+                assert np.all(err <= tol[fine]), (b, h, float((err / tol[fine]).max()))
+                worst = max(worst, float((err / tol[fine]).max(initial=0.0)))
+                g, w = lse[rows, h], ref_lse
+                ok = np.isfinite(w)
+                assert np.array_equal(np.isnan(g), np.isnan(w)) and np.array_equal(g[~ok & ~np.isnan(w)], w[~ok & ~np.isnan(w)])
+                assert np.all(np.abs(g[ok] - w[ok]) <= (e + (L + 64) * 2.0 ** -24)[ok] + 2.0 ** -22 * (1 + np.abs(w[ok])))
+        return worst
+
+    def run(self, **change):
+        import torch
+
+        d = {**self.device(), **change}
+        lse = torch.full((self.N, self.heads), 7.0, device="cuda")
+        out = tree_attention(**d, lse=lse)
+        return out, lse
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,ps", [(4, 4, 64, 16), (8, 2, 128, 16), (3, 1, 8, 16), (14, 2, 80, 32),
+                                                   (8, 1, 256, 16), (2, 2, 40, 64), (6, 3, 96, 16), (4, 2, 136, 128),
+                                                   (32, 4, 128, 1024), (5, 1, 192, 32)])
+def test_lengths_and_trees(heads, kv_heads, dim, ps, dtype):
+    """Lengths around tiles, blocks, rounds and pages; trees from one node to 64."""
+    g = np.random.default_rng(dim + heads)
+    lens = [0, 1, 15, 16, 17, 31, 33, 63, 64, 100, 127, 128, 129, 200, 255, 300]
+    sizes = [1, 64, 2, 17, 3, 1, 33, 5, 16, 31, 1, 7, 12, 2, 48, 63]
+    c = Case(dim, lens, [_tree(g, n, 6) for n in sizes], heads, kv_heads, dim, ps, dtype, spare_rows=3)
+    print(f"[attend] trees {heads}/{kv_heads} x {dim} page {ps} {dtype}", flush=True)
+    out, lse = c.run()
+    print("  of the tolerance:", c.check(out, lse))
+    assert (lse[-3:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 1, 128), (2, 2, 64), (3, 3, 256)])
+def test_chains(heads, kv_heads, dim, dtype):
+    """Single tokens, chains and chunks of prompts, sequences without rows."""
+    lens = [0, 0, 5, 1000, 129, 40, 64, 17, 700]
+    sizes = [1, 100, 1, 1, 70, 300, 64, 0, 9]
+    c = Case(heads, lens, [DraftTree(np.zeros(n)) if n else None for n in sizes], heads, kv_heads, dim, 16, dtype)
+    out, lse = c.run()
+    print("  of the tolerance:", c.check(out, lse))
+
+
+@pytest.mark.parametrize("B,n,T,heads,kv_heads", [(1, 20000, 1, 8, 1), (1, 20000, 24, 8, 8), (2, 9000, 3, 4, 2),
+                                                  (1, 4097, 64, 16, 2), (300, 60, 1, 2, 1)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_long_contexts_in_chunks(B, n, T, heads, kv_heads, dtype):
+    g = np.random.default_rng(n)
+    lens = [n - (b * 37) % (n // 2) for b in range(B)]
+    c = Case(n, lens, [_tree(g, T, 3) for _ in lens], heads, kv_heads, 64, 16, dtype)
+    out, lse = c.run()
+    print("  of the tolerance:", c.check(out, lse))
+    # a bound that is too small changes the plan alone; one too large as well
+    for most in (1, n // 3, 8 * n):
+        c.check(*c.run(max_len=most))
+
+
+def test_rows_that_see_nothing_or_little():
+    import torch
+
+    g = np.random.default_rng(3)
+    c = Case(1, [0, 0, 40], [_tree(g, 9, 3), _tree(g, 64, 4), _tree(g, 5, 2)], 4, 2, 64, 16, "bfloat16")
+    v = c.visible.view(np.uint64)
+    v[:] = 0
+    v[3] = 1 << 8           # a node ahead of it, of its own tree
+    v[4] = (1 << 64) - 1    # nodes that the tree does not have
+    v[9 + 63] = 1 << 63
+    c.visible = v.view(np.int64)
+    out, lse = c.run()
+    c.check(out, lse)
+    assert not out[0].any() and torch.isneginf(lse[0]).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_unseen_infinities_and_nan(dtype):
+    """Keys and values of nodes outside a row's path may be anything."""
+    g = np.random.default_rng(4)
+    import torch
+
+    for at in ("k", "v", "both"):
+        c = Case(2, [40, 0, 129], [DraftTree([0] * 6, [-1, 0, 0, 1, 2, 2]), DraftTree([0] * 4, [-1, 0, 0, 0]),
+                                   _tree(g, 40, 4)], 6, 2, 64, 16, dtype)
+        bad = [(0, 41, np.nan), (0, 43, np.inf), (1, 2, -np.inf), (2, 129 + 7, np.nan), (2, 129 + 20, np.inf)]
+        for b, x, val in bad:
+            page = c.table[b, x // 16]
+            if at != "v":
+                c.keys[b][x, 0, 3] = c.k[page, 0, x % 16, 3] = val
+            if at != "k":
+                c.values[b][x, :, 5] = c.v[page, :, x % 16, 5] = val
+                c.values[b][x, 1, 60] = c.v[page, 1, x % 16, 60] = -val
+        out, lse = c.run()
+        c.check(out, lse)
+        assert torch.isfinite(out).any()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_large_scores(dtype):
+    """Scores of hundreds, rising and falling along the context: the running maximum moves."""
+    c = Case(5, [600, 130], [DraftTree([0] * 5, [-1, 0, 0, 1, 1]), DraftTree([0] * 3)], 4, 2, 64, 16, dtype)
+    c.visible = np.array([1, 3, 5, 11, 19, 1, 3, 7], dtype=np.int64)
+    out, lse = c.run(scale=20.0)
+    c.check(out, lse, 20.0)
+    for b in range(2):  # in ascending and descending order of a row's scores
+        order = np.argsort(c.keys[b][:c.lens[b], 0] @ c.q[c.off[b], 0])
+        for o in (order, order[::-1]):
+            k, v = c.keys[b].copy(), c.values[b].copy()
+            c.keys[b][:c.lens[b]], c.values[b][:c.lens[b]] = k[o], v[o]
+            for x in range(c.lens[b]):
+                c.k[c.table[b, x // 16], :, x % 16], c.v[c.table[b, x // 16], :, x % 16] = c.keys[b][x], c.values[b][x]
+            c.check(*c.run(scale=20.0), 20.0)
+
+
+def test_strides_and_rows_of_others():
+    """q out of one product's rows, out into a wider buffer; rows past the last
+    sequence and columns beside the rows stay as they were."""
+    import torch
+
+    c = Case(6, [50, 3, 77], [DraftTree([0] * 7), DraftTree([0]), DraftTree([0] * 2)], 4, 2, 80, 16, "bfloat16", spare_rows=4)
+    d = c.device()
+    qkv = torch.zeros((c.N, 8 * 80 + 6), dtype=torch.bfloat16, device="cuda")
+    q = qkv[:, 2:2 + 320].view(c.N, 4, 80)
+    q.copy_(d["q"])
+    wide = torch.full((c.N, 400), 9.0, dtype=torch.bfloat16, device="cuda")
+    out = wide[:, 34:354].view(c.N, 4, 80)
+    lse = torch.full((c.N, 4), 7.0, device="cuda")
+    res = tree_attention(**{**d, "q": q}, out=out, lse=lse)
+    assert res.data_ptr() == out.data_ptr()
+    c.check(out, lse)
+    assert (wide[-4:] == 9).all() and (wide[:, :34] == 9).all() and (wide[:, 354:] == 9).all() and (lse[-4:] == 7).all()
+    again = tree_attention(**d)
+    assert torch.equal(again[:-4], out[:-4])
+    table = torch.full((3, 40), 10**6, dtype=torch.int32, device="cuda")
+    table[:, 3:3 + d["page_table"].shape[1]] = d["page_table"]
+    assert torch.equal(tree_attention(**{**d, "page_table": table[:, 3:3 + d["page_table"].shape[1]]})[:-4], out[:-4])
+
+
+def test_pages_outside_the_pool_hold_nothing():
+    """Entries of the table that name no page, ahead and behind: as if the tokens
+    of these pages were not there."""
+    import torch
+
+    for n, dtype in [(100, "bfloat16"), (2000, "float32")]:
+        c = Case(7, [n, 64], [DraftTree([0] * 3), DraftTree([0] * 2)], 4, 2, 64, 16, dtype)
+        d = c.device()
+        for bad in (-1, c.k.shape[0], 2**31 - 1, -2**31):
+            t = c.table.copy()
+            t[0, [1, 4]] = bad
+            keep = np.ones(n + 3, dtype=bool)
+            keep[16:32] = keep[64:80] = False
+            lse = torch.empty((c.N, 4), device="cuda")
+            out = tree_attention(**{**d, "page_table": torch.from_numpy(t).cuda()}, lse=lse).double().cpu().numpy()
+            for h in range(4):
+                ref, *_ = O.attend_sequence(c.q[:3, h], c.keys[0][keep][:, h // 2], c.values[0][keep][:, h // 2],
+                                            O.sees_of(n, 3)[:, keep], 64 ** -0.5)
+                assert np.abs(out[:3, h] - ref).max() < 0.05 if dtype == "bfloat16" else 1e-4
+
+
+def test_tables_shorter_than_the_lengths():
+    """Tokens past a row of the table are not there."""
+    import torch
+
+    c = Case(8, [100], [DraftTree([0] * 2)], 2, 1, 64, 16, "float32")
+    d = c.device()
+    out = tree_attention(**{**d, "page_table": d["page_table"][:, :3].contiguous()}).double().cpu().numpy()
+    for h in range(2):
+        ref, *_ = O.attend_sequence(c.q[:, h], c.keys[0][:48, 0], c.values[0][:48, 0], np.ones((2, 48), bool), 64 ** -0.5)
+        assert np.abs(out[:, h] - ref).max() < 1e-4
+    # broken offsets and lengths: no row of a sequence, or no key of it
+    for lens, off in [([-5], [0, 2]), ([100], [0, -3]), ([100], [5, 2]), ([100], [-4, 1])]:
+        o = torch.zeros_like(d["q"])
+        tree_attention(**{**d, "lens": torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                          "node_off": torch.tensor(off, dtype=torch.int32, device="cuda")}, out=o)
+        torch.cuda.synchronize()
+
+
+def test_places_past_32_bits():
+    """Pages whose elements lie past 2^31 (and bytes past 2^32)."""
+    import torch
+
+    ps, hkv, dim = 64, 8, 128
+    pages = (2**31 + 2**28) // (hkv * ps * dim)
+    k = torch.empty((pages, hkv, ps, dim), dtype=torch.bfloat16, device="cuda")
+    v = torch.empty_like(k)
+    c = Case(9, [150, 70], [DraftTree([0] * 4, [-1, 0, 0, 1]), DraftTree([0] * 2)], 8, 8, dim, ps, "bfloat16", extra_pages=0)
+    n = c.k.shape[0]
+    d = c.device()
+    k[-n:], v[-n:] = d["k_pages"], d["v_pages"]
+    table = torch.where(d["page_table"] < 0, d["page_table"], d["page_table"] + (pages - n))
+    lse = torch.empty((c.N, 8), device="cuda")
+    out = tree_attention(**{**d, "k_pages": k, "v_pages": v, "page_table": table}, lse=lse)
+    c.check(out, lse)
+
+
+def test_equal_calls_give_equal_bits():
+    import torch
+
+    g = np.random.default_rng(10)
+    c = Case(10, [3000, 100, 800], [_tree(g, 30, 3), _tree(g, 64, 8), _tree(g, 1, 1)], 8, 2, 128, 16, "bfloat16")
+    d = c.device()
+    first = tree_attention(**d)
+    for _ in range(5):
+        assert torch.equal(tree_attention(**d), first)
+
+
+def test_streams_and_graphs():
+    """Calls on a side stream; a call captured, replayed over lengths that grow,
+    with eager calls between."""
+    import torch
+
+    c = Case(11, [2000, 300], [DraftTree([0]), DraftTree([0])], 8, 2, 64, 16, "float16")
+    d = c.device()
+    want = tree_attention(**d)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = tree_attention(**d)
+    side.synchronize()
+    assert torch.equal(got, want)
+    d["max_len"] = 4096
+    out = torch.empty_like(d["q"])
+    tree_attention(**d, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tree_attention(**d, out=out)
+    lens = d["lens"].clone()
+    for step in (0, 1, 700, 1500, 20):
+        d["lens"].copy_(torch.clamp(lens - step, min=0))
+        out.zero_()
+        graph.replay()
+        eager = tree_attention(**d)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+
+
+def test_a_call_for_nothing():
+    import torch
+
+    c = Case(12, [5], [DraftTree([0])], 2, 1, 64, 16, "bfloat16")
+    d = c.device()
+    none = tree_attention(**{**d, "q": d["q"][:0], "node_off": torch.zeros(2, dtype=torch.int32, device="cuda")})
+    assert none.shape == (0, 2, 64)
+    e = tree_attention(**{**d, "page_table": d["page_table"][:0], "lens": d["lens"][:0], "node_off": d["node_off"][:1]})
+    assert e.shape == d["q"].shape
+
+
+def test_refusals_on_the_device():
+    import torch
+
+    c = Case(13, [5], [DraftTree([0])], 2, 1, 64, 16, "bfloat16")
+    d = c.device()
+    with pytest.raises(ValueError):
+        tree_attention(**d, scale=0.0)
+    with pytest.raises(ValueError):
+        tree_attention(**d, scale=float("nan"))
+    with pytest.raises(ValueError):
+        tree_attention(**d, out=d["q"])
+    with pytest.raises(NotImplementedError):
+        tree_attention(**{**d, "q": d["q"].expand(65, 2, 64).contiguous(), "max_nodes": 65,
+                          "visible": torch.zeros(65, dtype=torch.int64, device="cuda")})
+    for dim, ps in [(12, 16), (264, 16), (64, 8), (64, 24), (64, 2048)]:
+        kv = torch.zeros((2, 1, ps, dim), dtype=torch.bfloat16, device="cuda")
+        with pytest.raises(ValueError):
+            tree_attention(**{**d, "q": torch.zeros((1, 2, dim), dtype=torch.bfloat16, device="cuda"), "k_pages": kv, "v_pages": kv})
+    kv = torch.zeros((2, 3, 16, 64), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError):
+        tree_attention(**{**d, "k_pages": kv, "v_pages": kv})
+    with pytest.raises(TypeError):
+        tree_attention(**{**d, "q": d["q"].cpu()})

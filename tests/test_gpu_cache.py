@@ -1,0 +1,366 @@
+"""Rotary positions, page copies and kept nodes, PagedCache (needs an MI355X).
+
+Tolerance of a turned pair (a, b): its angle is formed in float64 and its rest, at
+most half a turn, rounded to float32 (2^-24 of pi), sine and cosine are right to 2^-23,
+three float32 operations follow and one rounding to the type (u): 4 * 2^-22 of
+factor * (|a| + |b|), plus u of the result (u = 2^-24, 2^-8, 2^-11).  What is not turned
+keeps its bits."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from oracle import tree as O
+from pagellm_amd.cache import PagedCache, Rotary, copy_pages, keep_nodes, rotary_append
+from pagellm_amd.tree import DraftTree
+
+pytestmark = pytest.mark.gpu
+
+U = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}
+
+
+def _rand(shape, dtype, seed=0):
+    import torch
+
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randn(shape, generator=g, device="cuda").to(getattr(torch, dtype))
+
+
+def _close(got, x, pos, freq, interleaved, factor, dtype):
+    ref = O.rotate(x, pos, freq, interleaved, factor)
+    R = len(freq)
+    first, second = (slice(0, 2 * R, 2), slice(1, 2 * R, 2)) if interleaved else (slice(0, R), slice(R, 2 * R))
+    size = np.abs(x[..., first]) + np.abs(x[..., second])
+    tol = np.zeros_like(ref)
+    tol[..., first] = tol[..., second] = 4 * 2.0 ** -22 * factor * size
+    tol[..., :2 * R] += U[dtype] * np.abs(ref[..., :2 * R]) + 1e-30
+    # a result below the type's normal range is rounded by steps of its smallest
+    tol[..., :2 * R] += {"float32": 2.0 ** -149, "bfloat16": 2.0 ** -133, "float16": 2.0 ** -24}[dtype]
+    assert np.all(np.abs(got - ref) <= tol), float((np.abs(got - ref) / (tol + 1e-300)).max())
+
+
+def _np(x):
+    return x.double().cpu().numpy()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("N,heads,kv_heads,dim,part,layout,ps", [
+    (1, 1, 1, 8, 8, "half", 16), (5, 8, 2, 128, 128, "half", 16), (33, 4, 4, 64, 64, "interleaved", 32),
+    (17, 6, 3, 80, 40, "half", 16), (9, 3, 1, 96, 24, "interleaved", 64), (4, 2, 1, 7, 4, "half", 16),
+    (6, 2, 2, 13, 6, "interleaved", 16), (3, 1, 1, 2, 2, "half", 16), (700, 7, 1, 256, 64, "half", 16),
+    (2, 2, 1, 64, 20, "half", 16), (3, 2, 1, 20, 12, "interleaved", 16),
+])
+def test_rotary_append(N, heads, kv_heads, dim, part, layout, ps, dtype):
+    import torch
+
+    print(f"[rotary] {N} x {heads}/{kv_heads} x {dim} part {part} {layout} {dtype}", flush=True)
+    g = np.random.default_rng(N + dim)
+    rot = Rotary(dim, part=part, layout=layout, factor=1.25)
+    freq = _np(rot.inv_freq)
+    qkv = _rand((N, (heads + 2 * kv_heads) * dim + 3), dtype, N)
+    q = qkv[:, 1:1 + heads * dim].view(N, heads, dim)
+    k = qkv[:, 1 + heads * dim:1 + (heads + kv_heads) * dim].view(N, kv_heads, dim)
+    v = qkv[:, 1 + (heads + kv_heads) * dim:-2].view(N, kv_heads, dim)
+    pos = g.integers(0, 2**20, N)
+    pos[0], pos[-1] = 0, 2**20
+    pages = -(-N // ps) + 2
+    slots = g.permutation(pages * ps)[:N]
+    if N > 3:
+        slots[1], slots[2] = -1, pages * ps  # written nowhere
+    kp, vp = _rand((pages, kv_heads, ps, dim), dtype, 1), _rand((pages, kv_heads, ps, dim), dtype, 2)
+    kw, vw = _np(kp), _np(vp)
+    out = rotary_append(q, k, v, pos, slots, kp, vp, rot)
+    _close(_np(out), _np(q), pos, freq, layout == "interleaved", 1.25, dtype)
+    ok = (slots >= 0) & (slots < pages * ps)
+    _close(_np(kp)[slots[ok] // ps, :, slots[ok] % ps], _np(k)[ok], pos[ok], freq, layout == "interleaved", 1.25, dtype)
+    vw[slots[ok] // ps, :, slots[ok] % ps] = _np(v)[ok]
+    assert np.array_equal(_np(vp), vw)
+    hit = np.zeros((pages, ps), dtype=bool)
+    hit[slots[ok] // ps, slots[ok] % ps] = True
+    assert np.array_equal(_np(kp).transpose(0, 2, 1, 3)[~hit], kw.transpose(0, 2, 1, 3)[~hit])
+    # in place, queries alone, keys and values alone, nothing turned
+    first = out.clone()
+    mine = qkv.clone()
+    inplace = mine[:, 1:1 + heads * dim].view(N, heads, dim)
+    got = rotary_append(inplace, None, None, torch.from_numpy(pos).cuda(), None, None, None, rot, q_out=inplace)
+    assert torch.equal(got, first) and torch.equal(mine[:, 1 + heads * dim:], qkv[:, 1 + heads * dim:])
+    k2, v2 = torch.zeros_like(kp), torch.zeros_like(vp)
+    assert rotary_append(None, k, v, pos, slots, k2, v2, rot) is None
+    at = torch.from_numpy(slots[ok]).cuda()
+    assert torch.equal(k2[at // ps, :, at % ps], kp[at // ps, :, at % ps])
+    assert torch.equal(rotary_append(q, k, v, None, slots, k2, v2, None), q)
+    assert torch.equal(k2[at // ps, :, at % ps], k[torch.from_numpy(ok).cuda()])
+
+
+def test_far_positions():
+    """Angles of millions of radians keep their place on the circle."""
+    import torch
+
+    pos = np.array([2**20 + 1, 2**24 + 3, 2**30 + 7, 2**31 + 11, 2**40])
+    x = np.ones((5, 1, 8))
+    rot = Rotary(inv_freq=[1.0, 0.5, 0.123456789, 1e-4])
+    got = _np(rotary_append(torch.ones((5, 1, 8), device="cuda"), None, None, pos, None, None, None, rot))
+    f = np.asarray([1.0, 0.5, 0.123456789, 1e-4], dtype=np.longdouble)
+    a = pos.astype(np.longdouble)[:, None] * f
+    for i in range(5):
+        # the product's own rounding in float64: 2^-53 of the angle, twice
+        tol = 2.0 ** -20 + float(pos[i]) * 2.0 ** -51
+        c, s = np.cos(a[i]).astype(float), np.sin(a[i]).astype(float)
+        assert np.all(np.abs(got[i, 0, :4] - (c - s)) < tol) and np.all(np.abs(got[i, 0, 4:] - (c + s)) < tol)
+    assert x.shape == got.shape
+
+
+def test_empty_rows_and_refusals():
+    import torch
+
+    kp = torch.zeros((2, 1, 16, 8), device="cuda")
+    e = torch.zeros((0, 1, 8), device="cuda")
+    none = torch.zeros(0, dtype=torch.int64, device="cuda")
+    assert rotary_append(e, e, e, none, none, kp, kp.clone(), Rotary(8)).shape == (0, 1, 8)
+    q = torch.zeros((4, 1, 8), device="cuda")
+    buf = torch.zeros(40, device="cuda")
+    with pytest.raises(ValueError):  # overlaps q without being it
+        rotary_append(buf[:32].view(4, 1, 8), None, None, [0] * 4, None, None, None, Rotary(8), q_out=buf[4:36].view(4, 1, 8))
+    with pytest.raises(ValueError):
+        rotary_append(q, q, q, [0] * 4, [0] * 4, torch.zeros((2, 1, 24, 8), device="cuda"),
+                      torch.zeros((2, 1, 24, 8), device="cuda"), Rotary(8))
+    with pytest.raises(ValueError):
+        Rotary(8, layout="other")
+    with pytest.raises(ValueError):
+        Rotary(8, part=10)
+    with pytest.raises(ValueError):
+        Rotary()
+    with pytest.raises(TypeError):
+        rotary_append(q.cpu(), None, None, [0] * 4, None, None, None, Rotary(8))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("layers,pages,heads,ps,dim,n", [(1, 2, 1, 16, 8, 1), (3, 40, 2, 16, 64, 17), (2, 9, 5, 32, 80, 4),
+                                                          (1, 300, 1, 16, 128, 150), (5, 3, 8, 128, 256, 1)])
+def test_copy_pages(layers, pages, heads, ps, dim, n, dtype):
+    import torch
+
+    g = np.random.default_rng(pages)
+    wide = _rand((layers, 2, pages, heads, ps, dim), dtype, 3)
+    k, v = wide[:, 0], wide[:, 1]  # layers of one buffer, keys and values by turns
+    want = wide.clone()
+    at = g.permutation(pages)
+    src, dst = at[:n].copy(), at[pages - n:].copy()
+    if n > 1:
+        src[1] = src[0]  # one page to two
+    src[np.isin(src, dst)] = at[0]
+    for s, d in zip(src, dst):
+        if s != d:
+            want[:, :, d] = wide[:, :, s]
+    if np.intersect1d(src, dst).size:
+        return
+    copy_pages(k, v, list(src), dst)
+    assert torch.equal(wide, want)
+    # on the device: pages outside the pool do nothing
+    bad = torch.tensor([-1, pages, int(src[0]), 2**31 - 1], dtype=torch.int32, device="cuda")
+    to = torch.tensor([int(dst[0]), int(dst[0]), -3, pages], dtype=torch.int32, device="cuda")
+    copy_pages(k, v, bad, to)
+    assert torch.equal(wide, want)
+    copy_pages(k, v, [], [])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("layers,heads,dim,ps,T", [(1, 1, 8, 16, 4), (3, 2, 64, 16, 33), (2, 5, 80, 32, 64), (2, 3, 128, 16, 150)])
+def test_keep_nodes(layers, heads, dim, ps, T, dtype):
+    import torch
+
+    g = np.random.default_rng(T)
+    lens = np.array([0, 1, 15, 16, 17, 40, 100, 5, 9])
+    B = lens.size
+    each = -(-(100 + T) // ps)
+    table = g.permutation(B * each + 2)[:B * each].reshape(B, each).astype(np.int32)
+    k = _rand((layers, B * each + 2, heads, ps, dim), dtype, 4)
+    v = _rand((layers, B * each + 2, heads, ps, dim), dtype, 5)
+    n = np.array([0, T - 1, 1, min(3, T - 1), T // 2, 2, min(10, T - 1), -1, T - 2])
+    path = np.full((B, T), -1, dtype=np.int32)
+    for b in range(B):
+        if n[b] >= 0:
+            path[b, :n[b] + 1] = [0, *sorted(g.choice(np.arange(1, T), n[b], replace=False))]
+    kw, vw = k.clone(), v.clone()
+    for b in range(B):
+        for j in range(1, n[b] + 1):
+            a, z = int(lens[b] + path[b, j]), int(lens[b] + j)
+            kw[:, table[b, z // ps], :, z % ps] = k[:, table[b, a // ps], :, a % ps]
+            vw[:, table[b, z // ps], :, z % ps] = v[:, table[b, a // ps], :, a % ps]
+    kept = k.clone()
+    keep_nodes(k, v, torch.from_numpy(table).cuda(), lens, path, n)
+    assert torch.equal(k, kw) and torch.equal(v, vw)
+    # tables with pages outside the pool, paths past the table or descending: nothing out of place
+    k.copy_(kept)
+    bad = table.copy()
+    bad[0], bad[1, 0] = 10**6, -7
+    path[2, 1:3] = [T + 10**6, 1]
+    path[3, 1] = -2**31
+    keep_nodes(k, v, torch.from_numpy(bad).cuda(), lens, path, np.minimum(n, 2))
+    free = np.setdiff1d(np.arange(B * each + 2), table)
+    assert torch.equal(k[:, free], kept[:, free])
+
+
+def test_page_work_past_32_bits():
+    import torch
+
+    k = torch.zeros((1, 2**31 // (16 * 8 * 128) + 8, 8, 16, 128), dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    last = k.shape[1] - 1
+    k[0, 3], v[0, last] = 5.0, 6.0
+    copy_pages(k, v, [3, last], [last - 1, 4])
+    assert (k[0, last - 1] == 5).all() and (v[0, 4] == 6).all() and not k[0, 4].any()
+    rows = _rand((1, 8, 128), "bfloat16", 1)
+    rotary_append(None, rows, rows, None, [last * 16 + 7], k[0], v[0], None)
+    assert torch.equal(k[0, last, :, 7], rows[0]) and torch.equal(v[0, last, :, 7], rows[0])
+    table = torch.tensor([[last]], dtype=torch.int32, device="cuda")
+    keep_nodes(k, v, table, [2], [[0, 5]], [1])
+    assert torch.equal(k[0, last, :, 3], rows[0])
+
+
+def test_page_work_in_a_graph():
+    import torch
+
+    k, v = _rand((2, 6, 2, 16, 32), "float16", 1), _rand((2, 6, 2, 16, 32), "float16", 2)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    src, dst, table, lens, path, n = i32(0), i32(3), i32(3, 4).view(1, 2), i32(14), i32(0, 2, 3).view(1, 3), i32(2)
+    rows, slots = _rand((1, 2, 32), "float16", 3), torch.tensor([3 * 16 + 14], device="cuda")
+    pos, rot = torch.tensor([14], device="cuda"), Rotary(32)
+    out = torch.empty_like(rows)
+
+    def go():
+        copy_pages(k, v, src, dst)
+        rotary_append(rows, rows, rows, pos, slots, k[0], v[0], rot, q_out=out)
+        keep_nodes(k, v, table, lens, path, n)
+
+    go()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        go()
+    for i in range(4):
+        k.copy_(_rand(k.shape, "float16", 10 + i))
+        rows.copy_(_rand(rows.shape, "float16", 20 + i))
+        pos.fill_(100 * i)
+        start = k.clone()
+        graph.replay()
+        got, got_q = k.clone(), out.clone()
+        k.copy_(start)
+        go()
+        assert torch.equal(k, got) and torch.equal(out, got_q)
+
+
+def test_forks_and_steps_of_a_cache():
+    """Sequences fork and step; each one's pages hold its own tokens' keys and
+    values, attention reads them, and all pages come back."""
+    import torch
+
+    layers, heads, kv, dim = 2, 4, 2, 32
+    cache = PagedCache(layers, 40, 16, kv, dim, "float32")
+    rot = Rotary(dim)
+    held = {}  # key -> per layer (keys, values) [tokens, kv, dim]
+    g = np.random.default_rng(3)
+
+    def step(keys, trees, accept):
+        s = cache.step(keys, trees)
+        N = sum(map(len, trees))
+        new = []
+        for layer in range(layers):
+            q, k, v = (_rand((N, h, dim), "float32", int(g.integers(1 << 30))) for h in (heads, kv, kv))
+            o = s.attend(layer, q, k, v, rot)
+            pos = s.positions.cpu().numpy()
+            kt = O.rotate(_np(k), pos, _np(rot.inv_freq))
+            qt = O.rotate(_np(q), pos, _np(rot.inv_freq))
+            new.append((kt, _np(v)))
+            off = 0
+            for key, t in zip(keys, trees):
+                past = held[key][layer]
+                n = past[0].shape[0]
+                kk = np.concatenate([past[0], kt[off:off + len(t)]])
+                vv = np.concatenate([past[1], _np(v)[off:off + len(t)]])
+                sees = O.sees_of(n, len(t), t.visible)
+                for h in range(heads):
+                    ref, *_ = O.attend_sequence(qt[off:off + len(t), h], kk[:, h // 2], vv[:, h // 2], sees, dim ** -0.5)
+                    assert np.abs(_np(o)[off:off + len(t), h] - ref).max() < 1e-4
+                off += len(t)
+        most = max(map(len, trees))
+        path, n_acc = np.full((len(keys), most), -1, dtype=np.int32), np.zeros(len(keys), dtype=np.int32)
+        for b, p in enumerate(accept):
+            path[b, :len(p)], n_acc[b] = p, len(p) - 1
+        cache.commit(s, torch.from_numpy(path).cuda(), torch.from_numpy(n_acc).cuda())
+        off = 0
+        for key, t, p in zip(keys, trees, accept):
+            rows = [off + i for i in p]
+            held[key] = [tuple(np.concatenate([old, x[rows]]) for old, x in zip(held[key][layer], new[layer]))
+                         for layer in range(layers)]
+            off += len(t)
+        for key in held:
+            assert cache.length(key) == held[key][0][0].shape[0]
+            for layer in range(layers):
+                kk, vv = cache.download(key, layer)
+                assert np.abs(_np(kk).transpose(1, 0, 2) - held[key][layer][0]).max(initial=0) < 1e-4
+                assert np.array_equal(_np(vv).transpose(1, 0, 2), held[key][layer][1])
+        with pytest.raises(RuntimeError):
+            cache.commit(s)
+        with pytest.raises(RuntimeError):
+            s.attend(0, q, k, v, rot)
+
+    def add(key):
+        cache.add(key)
+        held[key] = [(np.zeros((0, kv, dim)),) * 2 for _ in range(layers)]
+
+    def fork(key, child):
+        cache.fork(key, child)
+        held[child] = list(held[key])
+
+    add("a")
+    add("b")
+    step(["a", "b"], [DraftTree(range(20)), DraftTree(range(37))], [range(20), range(37)])
+    fork("a", "a1")
+    fork("a", "a2")
+    step(["b", "a1", "a"], [DraftTree([0] * 7, [-1, 0, 0, 1, 1, 2, 5]), DraftTree([0] * 3, [-1, 0, 0]), DraftTree([0])],
+         [[0, 2, 5, 6], [0, 2], [0]])
+    fork("a1", "a3")
+    cache.remove("a1")
+    del held["a1"]
+    step(["a2", "a3", "b"], [DraftTree([0] * 30, [-1] + [0] * 29), DraftTree([0] * 2), DraftTree([0] * 4, [-1, 0, 1, 1])],
+         [[0, 29], [0, 1], [0, 1, 3]])
+    before = cache.length("b")
+    cache.truncate("b", 33)
+    held["b"] = [tuple(x[:33] for x in l) for l in held["b"]]
+    assert before > 33
+    step(["b"], [DraftTree([0] * 17)], [range(17)])
+    for key in list(held):
+        cache.remove(key)
+    assert cache.free_pages == 40 and len(cache) == 0
+    with pytest.raises(RuntimeError):
+        cache.add("x")
+        cache.step(["x"], [DraftTree(range(641))])
+    assert cache.free_pages == 40
+
+
+def test_steps_that_do_not_fit_a_commit():
+    cache = PagedCache(1, 8, 16, 1, 8, "float32")
+    cache.add("a")
+    s = cache.step(["a"], [DraftTree([1, 2])])
+    with pytest.raises(ValueError):
+        cache.commit(s, [[0, 1]])
+    with pytest.raises(ValueError):
+        cache.commit(s, [[0, 1]], [2], accepted=[2])
+    with pytest.raises(ValueError):
+        cache.step([], [])
+    with pytest.raises(ValueError):
+        cache.step(["a"], [])
+    cache.commit(s)
+    assert cache.length("a") == 2
+    s = cache.step(["a"], [DraftTree([1])])
+    cache.truncate("a", 1)
+    with pytest.raises(RuntimeError):
+        cache.commit(s)
+    for bad in [dict(layers=0), dict(page_size=24), dict(head_dim=12), dict(head_dim=264)]:
+        with pytest.raises(ValueError):
+            PagedCache(**{**dict(layers=1, pages=8, page_size=16, kv_heads=1, head_dim=8), **bad})
+    with pytest.raises(TypeError):
+        PagedCache(1, 8, 16, 1, 8, "float64")

@@ -1,0 +1,332 @@
+"""Host side of trees and pages: topology, page books, frequencies, and refusals
+that need no GPU."""
+
+from __future__ import annotations
+
+import math
+from types import SimpleNamespace
+
+import numpy as np
+import pytest
+
+from pagellm_amd import _native, cache, fp8, tree
+from pagellm_amd.cache import _PageBook, rotary_frequencies
+from pagellm_amd.tree import DraftTree
+
+
+def test_trees():
+    t = DraftTree([9, 1, 2, 3, 4], [-1, 0, 0, 1, 3])
+    assert list(t.depths) == [0, 1, 1, 2, 3] and [int(v) for v in t.visible] == [1, 3, 5, 11, 27]
+    assert not t.chain and t.path_to(4) == [1, 3, 4] and t.path_to(0) == [] and len(t) == 5
+    c = DraftTree(range(100))
+    assert c.chain and c.visible is None and list(c.parents[:3]) == [-1, 0, 1]
+    wide = DraftTree([0] * 64, [-1] + [0] * 63)
+    assert int(wide.visible[63]) == (1 << 63) | 1
+    for tokens, parents in [([], None), ([1, 2], [-1]), ([1, 2], [0, 0]), ([1, 2], [-1, 1]), ([1, 2], [-1, -1]),
+                            ([-1], None), ([2**31], None), ([0] * 65, [-1] + [0] * 64)]:
+        with pytest.raises(ValueError):
+            DraftTree(tokens, parents)
+
+
+def test_pages_are_shared_until_written():
+    b = _PageBook(8, 16)
+    b.add("a")
+    assert b.reserve(["a"], [20]) == []
+    b.set_length("a", 20)
+    first = list(b.held["a"])
+    b.fork("a", "b")
+    b.fork("a", "c")
+    assert b.held["b"] == first and b.refs[first[0]] == 3 and len(b.free) == 6
+    copies = b.reserve(["a", "b", "c"], [1, 1, 13])
+    # two of the three take a copy of the half-filled page, the last keeps it; c needs one page more
+    assert [s for s, _ in copies] == [first[1]] * 2 and len({d for _, d in copies}) == 2
+    assert b.held["c"][1] == first[1] and len(b.held["c"]) == 3 and len(b.free) == 3
+    assert len({b.held[k][1] for k in "abc"}) == 3 and all(b.held[k][0] == first[0] for k in "abc")
+    for key in "abc":
+        b.set_length(key, 21)
+    assert len(b.free) == 4
+    b.truncate("a", 16)
+    assert len(b.held["a"]) == 1 and len(b.free) == 5
+    for key in "abc":
+        b.remove(key)
+    assert sorted(b.free) == list(range(8)) and not any(b.refs)
+
+
+def test_a_full_page_is_not_copied():
+    b = _PageBook(4, 16)
+    b.add("a")
+    b.reserve(["a"], [16])
+    b.set_length("a", 16)
+    b.fork("a", "b")
+    assert b.reserve(["a", "b"], [1, 1]) == [] and len(b.free) == 1
+
+
+def test_a_forked_page_past_the_tokens_is_not_copied():
+    b = _PageBook(8, 16)
+    b.add("a")
+    b.reserve(["a"], [40])  # three pages, none of them filled
+    b.fork("a", "b")        # of no tokens: it shares nothing
+    assert b.held["b"] == [] and b.reserve(["b"], [1]) == []
+
+
+def test_reserving_is_all_or_nothing():
+    b = _PageBook(3, 16)
+    b.add("a")
+    b.add("b")
+    b.reserve(["a"], [10])
+    b.set_length("a", 10)
+    b.fork("a", "c")
+    before = (list(b.free), list(b.refs), {k: list(v) for k, v in b.held.items()})
+    with pytest.raises(RuntimeError):
+        b.reserve(["a", "c", "b"], [1, 1, 17])
+    with pytest.raises(ValueError):
+        b.reserve(["a", "a"], [1, 1])
+    with pytest.raises(KeyError):
+        b.reserve(["a", "x"], [1, 1])
+    with pytest.raises(ValueError):
+        b.reserve(["a"], [0])
+    assert before == (list(b.free), list(b.refs), {k: list(v) for k, v in b.held.items()})
+    with pytest.raises(ValueError):
+        b.add("a")
+    with pytest.raises(ValueError):
+        b.fork("a", "b")
+    with pytest.raises(KeyError):
+        b.fork("x", "y")
+    assert "y" not in b.held
+    with pytest.raises(ValueError):
+        b.truncate("a", 11)
+
+
+def test_books_of_random_steps():
+    """Every page is free or held as often as its count says; no two sequences
+    write to one page."""
+    g = np.random.default_rng(0)
+    b = _PageBook(40, 16)
+    nxt = 0
+    for _ in range(3000):
+        keys = list(b.held)
+        act = g.integers(0, 5)
+        if act == 0 or not keys:
+            b.add(nxt)
+            nxt += 1
+        elif act == 1:
+            b.fork(keys[g.integers(len(keys))], nxt)
+            nxt += 1
+        elif act == 2:
+            b.remove(keys[g.integers(len(keys))])
+        elif act == 3:
+            k = keys[g.integers(len(keys))]
+            b.truncate(k, int(g.integers(0, b.length[k] + 1)))
+        else:
+            some = [keys[i] for i in g.permutation(len(keys))[:3]]
+            counts = [int(n) for n in g.integers(1, 40, len(some))]
+            try:
+                copies = b.reserve(some, counts)
+            except RuntimeError:
+                continue
+            assert not {s for s, _ in copies} & {d for _, d in copies}
+            for k, n in zip(some, counts):
+                for i in range(b.length[k] // 16, -(-(b.length[k] + n) // 16)):
+                    assert b.refs[b.held[k][i]] == 1
+                b.set_length(k, b.length[k] + int(g.integers(0, n + 1)))
+        refs = [0] * 40
+        for pages in b.held.values():
+            for p in pages:
+                refs[p] += 1
+        assert refs == b.refs and sorted(b.free) == [p for p in range(40) if refs[p] == 0]
+        assert all(len(b.held[k]) >= -(-b.length[k] // 16) for k in b.held)
+
+
+def test_frequencies():
+    f, m = rotary_frequencies(8, 100.0)
+    assert np.allclose(f, [1, 100 ** -0.25, 0.1, 100 ** -0.75], rtol=1e-15) and m == 1.0
+    assert np.allclose(rotary_frequencies(8, 100.0, {"kind": "linear", "factor": 4})[0], f / 4, rtol=1e-15)
+    n, _ = rotary_frequencies(8, 100.0, {"kind": "ntk", "factor": 4})
+    assert n[0] == 1.0 and np.isclose(n[-1], f[-1] / 4, rtol=1e-14)
+    f, _ = rotary_frequencies(64, 10000.0)
+    y, m = rotary_frequencies(64, 10000.0, {"kind": "yarn", "factor": 8, "original_len": 4096})
+    turns = 4096 * f / (2 * math.pi)
+    assert np.array_equal(y[turns >= 32], f[turns >= 32]) and np.allclose(y[turns <= 1], f[turns <= 1] / 8, rtol=1e-15)
+    ramp = (turns > 1) & (turns < 32)
+    assert ramp.any() and np.all((y[ramp] > f[ramp] / 8) & (y[ramp] < f[ramp])) and np.isclose(m, 0.1 * math.log(8) + 1)
+    for bad in [dict(part=3), dict(part=0), dict(part=8, base=0.0), dict(part=8, scaling={"kind": "x", "factor": 2}),
+                dict(part=8, scaling={"kind": "linear"}), dict(part=8, scaling={"kind": "linear", "factor": 0.5}),
+                dict(part=2, scaling={"kind": "ntk", "factor": 2}), dict(part=8, scaling={"kind": "yarn", "factor": 2}),
+                dict(part=8, scaling={"kind": "linear", "factor": 2, "more": 1})]:
+        with pytest.raises(ValueError):
+            rotary_frequencies(**bad)
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """CPU tensors stand for CUDA ones, in a context that no refused call reaches."""
+    import torch
+
+    for m in (cache, tree, fp8):
+        monkeypatch.setattr(m, "_is_torch_cuda", lambda x: isinstance(x, torch.Tensor))
+    return SimpleNamespace(device=None)
+
+
+def _attend_args():
+    import torch
+
+    return dict(q=torch.zeros(3, 4, 16), k_pages=torch.zeros(5, 2, 16, 16), v_pages=torch.zeros(5, 2, 16, 16),
+                page_table=torch.zeros(2, 3, dtype=torch.int32), lens=torch.zeros(2, dtype=torch.int32),
+                node_off=torch.zeros(3, dtype=torch.int32), max_nodes=2, max_len=20)
+
+
+def test_refusals_of_tree_attention(on_cpu):
+    import torch
+
+    z, i32 = torch.zeros, torch.int32
+    for err, change in [
+        (ValueError, dict(q=z(3, 64))),
+        (ValueError, dict(q=z(3, 4, 32)[..., ::2])),
+        (ValueError, dict(q=z(3, 8, 16)[:, ::2])),
+        (ValueError, dict(q=z(4, 16).expand(3, 4, 16))),
+        (TypeError, dict(q=z(3, 4, 16, dtype=torch.float64))),
+        (TypeError, dict(q=z(3, 4, 16, dtype=torch.bfloat16))),
+        (ValueError, dict(q=z(3, 4, 8))),
+        (ValueError, dict(k_pages=z(5, 2, 16))),
+        (ValueError, dict(v_pages=z(4, 2, 16, 16))),
+        (ValueError, dict(k_pages=z(5, 16, 2, 16).transpose(1, 2))),
+        (TypeError, dict(lens=z(2))),
+        (TypeError, dict(lens=z(2, dtype=torch.int64))),
+        (TypeError, dict(lens=z(4, dtype=i32)[::2])),
+        (ValueError, dict(node_off=z(2, dtype=i32))),
+        (ValueError, dict(page_table=z(3, 3, dtype=i32))),
+        (ValueError, dict(page_table=z(2, 0, dtype=i32))),
+        (TypeError, dict(page_table=z(2, 3, dtype=torch.int64))),
+        (ValueError, dict(page_table=z(2, 6, dtype=i32)[:, ::2])),
+        (ValueError, dict(page_table=z(3, dtype=i32).expand(2, 3))),
+        (TypeError, dict(visible=z(2, dtype=torch.int64))),
+        (TypeError, dict(visible=z(3, dtype=i32))),
+        (ValueError, dict(max_nodes=-1)),
+        (ValueError, dict(max_nodes=2**31)),
+        (ValueError, dict(max_len=2**30 + 1)),
+        (ValueError, dict(out=z(3, 4, 8))),
+        (ValueError, dict(out=z(1, 4, 16).expand(3, 4, 16))),
+        (ValueError, dict(out=z(3, 4, 16, dtype=torch.float16))),
+        (TypeError, dict(lse=z(3, 3))),
+        (TypeError, dict(lse=z(3, 4, dtype=torch.float64))),
+    ]:
+        with pytest.raises(err):
+            print(change)
+            tree.tree_attention(**{**_attend_args(), **change}, ctx=on_cpu)
+
+
+def test_refusals_of_rotary_append(on_cpu):
+    import torch
+
+    z = torch.zeros
+    rot = SimpleNamespace(pairs=4, interleaved=False, factor=1.0, inv_freq=z(4, dtype=torch.float64))
+    i64 = torch.int64
+    good = dict(q=z(3, 4, 16), k=z(3, 2, 16), v=z(3, 2, 16), positions=z(3, dtype=i64), slots=z(3, dtype=i64),
+                k_pages=z(5, 2, 16, 16), v_pages=z(5, 2, 16, 16), rotary=rot)
+    for err, change in [
+        (ValueError, dict(k=None)),
+        (ValueError, dict(q=None, k=None, v=None)),
+        (ValueError, dict(q=z(3, 64))),
+        (ValueError, dict(q=z(3, 4, 24))),
+        (ValueError, dict(k=z(2, 2, 16))),
+        (ValueError, dict(v=z(3, 1, 16))),
+        (TypeError, dict(k=z(3, 2, 16, dtype=torch.float16))),
+        (TypeError, dict(q=z(3, 4, 16, dtype=torch.float64))),
+        (ValueError, dict(k_pages=z(5, 3, 16, 16), v_pages=z(5, 3, 16, 16))),
+        (ValueError, dict(k_pages=z(5, 2, 16, 8), v_pages=z(5, 2, 16, 8))),
+        (ValueError, dict(slots=z(2, dtype=i64))),
+        (TypeError, dict(slots=z(3))),
+        (ValueError, dict(positions=z(4, dtype=i64))),
+        (ValueError, dict(rotary=SimpleNamespace(pairs=9, inv_freq=rot.inv_freq))),
+        (ValueError, dict(q_out=z(3, 4, 8))),
+        (ValueError, dict(q=None, q_out=z(3, 4, 16))),
+    ]:
+        with pytest.raises(err):
+            print(change)
+            cache.rotary_append(**{**good, **change}, ctx=on_cpu)
+
+
+def test_refusals_of_page_work(on_cpu):
+    import torch
+
+    z, i32 = torch.zeros, torch.int32
+    k = z(2, 5, 2, 16, 8)
+    for err, args in [
+        (ValueError, (k[0], k[0], [0], [1])),
+        (ValueError, (k, z(2, 4, 2, 16, 8), [0], [1])),
+        (ValueError, (k.transpose(0, 1), k.transpose(0, 1), [0], [1])),
+        (IndexError, (k, k, [5], [1])),
+        (IndexError, (k, k, [0], [-1])),
+        (ValueError, (k, k, [0, 1], [2, 2])),
+        (ValueError, (k, k, [0, 1], [1, 2])),
+        (ValueError, (k, k, z(2, dtype=i32), z(3, dtype=i32))),
+        (TypeError, (k, k, z(2), z(2))),
+    ]:
+        with pytest.raises(err):
+            cache.copy_pages(*args, ctx=on_cpu)
+    good = [k, k, z(2, 3, dtype=i32), z(2, dtype=i32), z(2, 4, dtype=i32), z(2, dtype=i32)]
+    for err, at, x in [(ValueError, 0, k[0]), (ValueError, 2, z(3, 3, dtype=i32)), (TypeError, 2, z(2, 3)),
+                       (TypeError, 3, z(2)), (ValueError, 4, z(3, 4, dtype=i32)), (ValueError, 4, z(2, dtype=i32)),
+                       (ValueError, 5, z(3, dtype=i32))]:
+        args = list(good)
+        args[at] = x
+        with pytest.raises(err):
+            cache.keep_nodes(*args, ctx=on_cpu)
+
+
+def test_refusals_of_verify_tree_on_the_host():
+    ctx = SimpleNamespace(device=0)
+    p = np.full((3, 4), 0.25)
+    good = dict(p=p, q=p, tokens=[0, 1, 2], parents=[-1, 0, 0], node_off=[0, 3], uniforms=np.zeros((1, 3)))
+    for err, change in [
+        (ValueError, dict(p=p[0])),
+        (ValueError, dict(node_off=[0, 4])),
+        (ValueError, dict(node_off=[0, 0, 3])),
+        (ValueError, dict(node_off=[1, 3])),
+        (ValueError, dict(tokens=[0, 1])),
+        (ValueError, dict(parents=[-1, 0])),
+        (IndexError, dict(tokens=[0, 1, 4])),
+        (IndexError, dict(tokens=[0, -1, 2])),
+        (ValueError, dict(parents=[-1, 0, 2])),
+        (ValueError, dict(parents=[-1, -1, 0])),
+        (ValueError, dict(max_nodes=2)),
+    ]:
+        with pytest.raises(err):
+            tree.verify_tree(**{**good, **change}, ctx=ctx)
+
+
+def test_refusals_of_verify_tree(on_cpu):
+    import torch
+
+    z, i32, f8 = torch.zeros, torch.int32, torch.float64
+    good = dict(p=z(3, 4), q=z(3, 4), tokens=z(3, dtype=i32), parents=z(3, dtype=i32), node_off=z(2, dtype=i32),
+                uniforms=z(1, 3, dtype=f8), max_nodes=3)
+    for err, change in [
+        (TypeError, dict(p=z(3, 4, dtype=torch.float16))),
+        (ValueError, dict(p=z(3, 8)[:, ::2])),
+        (ValueError, dict(q=z(3, 5))),
+        (ValueError, dict(q=z(3, 4, dtype=f8))),
+        (ValueError, dict(q=z(3, 8)[:, :4])),
+        (ValueError, dict(max_nodes=None)),
+        (ValueError, dict(max_nodes=4)),
+        (ValueError, dict(max_nodes=2**31)),
+        (ValueError, dict(tokens=z(2, dtype=i32))),
+        (TypeError, dict(parents=z(3))),
+        (ValueError, dict(uniforms=z(1, 3))),
+        (ValueError, dict(uniforms=z(2, 3, dtype=f8))),
+    ]:
+        with pytest.raises(err):
+            tree.verify_tree(**{**good, **change}, ctx=on_cpu)
+
+
+def test_null_contexts():
+    lib = _native.load_library()
+    n = None
+    assert lib.plh_rotary_append(n, n, 1, 1, n, 1, n, 1, n, 1, 1, 0, 1, 1, n, n, 0, 0, 1.0, n, n, 1, 16, n) == -1
+    assert lib.plh_tree_attention_ws_bytes(n, 0, 1, 1, 1, 8, 1, 1, 1) == -1
+    assert lib.plh_tree_attention(n, n, 0, 8, 1, 1, 1, 8, n, n, 1, 16, n, 1, n, n, 1, n, 1.0, 1, 1, n, 8, n, n, 0) == -1
+    assert lib.plh_verify_tree(n, n, n, 0, 1, 1, 1, n, n, n, 1, 1, n, 1, 0, n, n, n, n) == -1
+    assert lib.plh_copy_pages(n, n, n, 1, 16, 1, 16, n, n, 1) == -1
+    assert lib.plh_keep_nodes(n, n, n, 1, 16, 1, 16, 1, 16, n, 1, n, n, 1, n, 1) == -1
+    header = (_native.LIB_PATH.parents[1] / "include" / "pagellm_hip.h").read_text()
+    assert f"#define PLH_MAX_TREE_NODES {_native.PLH_MAX_TREE_NODES}\n" in header

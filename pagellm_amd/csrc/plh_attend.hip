@@ -46,13 +46,13 @@ __device__ __forceinline__ void wave_lds_fence() { asm volatile("s_waitcnt lgkmc
 
 // Waves a SIMD that the registers of a kernel are cut for: what a lane keeps of
 // queries, sums, keys and values.
-constexpr int attend_waves(int es, int dp, int qt) {
+constexpr int attend_waves(int es, int dp, int qt, bool full) {
   const int tile = dp * 16 * es / 4 / 64;  // registers of a tile of 16
   const int regs = qt * (tile + dp / 4) + (es == 4 ? 1 : 2) * 2 * tile + 44 + 12 * qt;
-  return regs <= 128 ? 4 : regs <= 160 ? 3 : regs <= 256 ? 2 : 1;
+  return regs <= 128 ? 4 : regs <= (full ? 168 : 160) ? 3 : regs <= 256 ? 2 : 1;
 }
 constexpr int kMostKeys = 1 << 30;
-constexpr float kGrow = 8.0f;    // weights stay below 2^8 of the maximum that they are scaled by
+constexpr float kGrow = 1024.0f;  // of a lane's weights in a block
 
 // What a lane holds of a tile of 16 keys or queries and of a tile's values, and
 // the two products, for 16-bit types.  DP: the head's size, padded.
@@ -117,6 +117,18 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
 }
 
+// The weights of 32 keys, and column e of load h of a tile's values, as operands.
+template <typename T>
+__device__ __forceinline__ u32x4 weights_of(const float (&p)[4], const float (&q)[4]) {
+  return u32x4{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(q[0], q[1]), pack2<T>(q[2], q[3])};
+}
+template <typename V, int H>
+__device__ __forceinline__ u32x2 columns(const V (&v)[4][H], int h, int e) {
+  const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+  return u32x2{__builtin_amdgcn_perm(v[1][h][e / 2], v[0][h][e / 2], sel),
+               __builtin_amdgcn_perm(v[3][h][e / 2], v[2][h][e / 2], sel)};
+}
+
 // The largest of the lanes l, l ^ 16, l ^ 32, l ^ 48 (those that share a query), in all of them; and the sum.
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16));
@@ -158,6 +170,8 @@ struct State {
   typename G::Piece q[QT][G::kSteps];
   f32x4 o[QT][G::kH][G::kE];
   float m[QT], l[QT];  // l: over the lane's own keys
+  float base[QT];      // m, or 0 before the first key
+  float most[QT];      // sums past this move m: kGrow, -1 before the first key
   uint64_t bits[QT];   // nodes that the row sees
   int last[QT];        // chains: the last key that it sees
 };
@@ -213,43 +227,58 @@ __device__ __forceinline__ void attend_out(const AttendArgs& a, int64_t row, int
   if (a.lse != nullptr && d == 0) a.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
 }
 
-// Rows of a sequence and key head: row = node * group + place in the group.
-template <typename T, int DP, int QT, bool FULL>
-__global__ __launch_bounds__(kAttThreads, attend_waves(sizeof(T), DP, QT)) void k_attend(AttendArgs a) {
-  using G = Geo<T, DP>;
-  constexpr int NT = G::kTiles, kKeys = 16 * NT;
-  constexpr int kRows = 16 * QT, kLd = DP + 4;
-  __shared__ __align__(16) float sm_o[kAttWaves][kRows][kLd];
-  __shared__ float sm_m[kAttWaves][kRows], sm_l[kAttWaves][kRows];
-  const int w = uniform(wave()), n = lane() & 15, g = lane() >> 4;
-  // blocks of rows of one unit lie 8 apart: on one XCD, whose L2 then holds the unit's keys
+// What a workgroup works on: rows r0 .. of a sequence and key head (row = node *
+// group + place in the group) over keys from .. to.  Blocks of rows of one unit lie
+// 8 apart in the grid: on one XCD, whose L2 then holds the unit's keys.
+struct Unit {
+  int kvh, b, c, start, nodes, len, r0, seq_end, from, to;
+  bool any;
+};
+
+// One past the last key that row r may see.
+__device__ __forceinline__ int row_end(const AttendArgs& a, const Unit& u, int r) {
+  return a.visible == nullptr ? u.len + min(r / a.group, u.nodes - 1) + 1 : u.len + u.nodes;
+}
+__device__ __forceinline__ Unit unit_of(const AttendArgs& a, int rows) {
+  Unit u{};
   const int rb = (int)(blockIdx.x / 8 % (unsigned)a.row_blocks);
   const int64_t unit = (int64_t)(blockIdx.x / (8u * (unsigned)a.row_blocks)) * 8 + blockIdx.x % 8;
-  if (unit >= (int64_t)a.chunks * a.B * a.kv_heads) return;
-  const int kvh = (int)(unit % a.kv_heads), b = (int)(unit / a.kv_heads % a.B), c = (int)(unit / a.kv_heads / a.B);
-  const int start = max(a.node_off[b], 0);
-  const int nodes = min(min(a.node_off[b + 1], a.N) - start, a.max_nodes);
-  const int r0 = rb * kRows;
-  if (r0 >= nodes * a.group) return;
-  const int ps = 1 << a.page_shift, D = FULL ? DP : a.D;
-  const int len = min(max(a.lens[b], 0), kMostKeys);
+  if (unit >= (int64_t)a.chunks * a.B * a.kv_heads) return u;
+  u.kvh = (int)(unit % a.kv_heads);
+  u.b = (int)(unit / a.kv_heads % a.B);
+  u.c = (int)(unit / a.kv_heads / a.B);
+  u.start = max(a.node_off[u.b], 0);
+  u.nodes = min(min(a.node_off[u.b + 1], a.N) - u.start, a.max_nodes);
+  u.r0 = rb * rows;
+  if (u.r0 >= u.nodes * a.group) return u;
+  u.len = min(max(a.lens[u.b], 0), kMostKeys);
   // 64 bits: a table's pages may hold more than an int counts
-  const int seq_end = (int)min((int64_t)len + nodes, (int64_t)a.ldt << a.page_shift);
+  u.seq_end = (int)min((int64_t)u.len + u.nodes, (int64_t)a.ldt << a.page_shift);
   // the last chunk takes what is left where max_len was too small
-  const int64_t from64 = (int64_t)c * a.chunk;
-  if (c > 0 && from64 >= seq_end) return;
-  // this block's rows: keys that all of them see, and the last one that some do
-  const int node0 = r0 / a.group, node1 = min((r0 + kRows - 1) / a.group, nodes - 1);
-  const int end = min(a.visible == nullptr ? len + node1 + 1 : len + nodes, seq_end);
-  const int all = min(a.visible == nullptr ? len + node0 + 1 : len, seq_end);
-  const int from = (int)from64, to = c + 1 == a.chunks ? end : (int)min(from64 + a.chunk, (int64_t)end);
+  const int64_t from = (int64_t)u.c * a.chunk;
+  if (u.c > 0 && from >= u.seq_end) return u;
+  const int end = min(row_end(a, u, u.r0 + rows - 1), u.seq_end);
+  u.from = (int)from;
+  u.to = u.c + 1 == a.chunks ? end : (int)min(from + a.chunk, (int64_t)end);
+  u.any = true;
+  return u;
+}
 
-  State<T, DP, QT> st;
+// Rows from r0 on see every key ahead of this one.
+__device__ __forceinline__ int row_all(const AttendArgs& a, const Unit& u, int r0) {
+  return min(a.visible == nullptr ? u.len + r0 / a.group + 1 : u.len, u.seq_end);
+}
+
+template <typename T, int DP, int QT, bool FULL>
+__device__ __forceinline__ void first_state(const AttendArgs& a, const Unit& u, int r0, State<T, DP, QT>& st) {
+  using G = Geo<T, DP>;
+  const int n = lane() & 15, g = lane() >> 4, D = FULL ? DP : a.D;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int r = r0 + 16 * t + n, node = r / a.group;
-    const bool in = node < nodes;
-    const T* row = reinterpret_cast<const T*>(a.q) + (int64_t)(start + node) * a.ldq + (int64_t)(kvh * a.group + r % a.group) * D;
+    const bool in = node < u.nodes;
+    const T* row = reinterpret_cast<const T*>(a.q) + (int64_t)(u.start + node) * a.ldq +
+                   (int64_t)(u.kvh * a.group + r % a.group) * D;
 #pragma unroll
     for (int s = 0; s < G::kSteps; ++s) {
       const int d = G::piece_at(s, g);
@@ -259,33 +288,199 @@ __global__ __launch_bounds__(kAttThreads, attend_waves(sizeof(T), DP, QT)) void 
         st.q[t][s] = *reinterpret_cast<const Loose*>(row + d);
       }
     }
-    st.bits[t] = a.visible != nullptr && in ? a.visible[start + node] : 0;
-    if (nodes < 64) st.bits[t] &= (1ull << nodes) - 1;
-    st.last[t] = in ? len + node : -1;
+    // in before the loop: with a load that may be on its way at the loop's head, every
+    // use of the queries would wait for all the keys in flight
+#pragma unroll
+    for (int s = 0; s < G::kSteps; ++s) asm volatile("" : "+v"(st.q[t][s]));
+    st.bits[t] = a.visible != nullptr && in ? a.visible[u.start + node] : 0;
+    asm volatile("" : "+v"(st.bits[t]));
+    if (u.nodes < 64) st.bits[t] &= (1ull << u.nodes) - 1;
+    st.last[t] = in ? u.len + node : -1;
     st.m[t] = -INFINITY;
+    st.base[t] = 0.0f;
+    st.most[t] = -1.0f;
     st.l[t] = 0.0f;
 #pragma unroll
     for (int h = 0; h < G::kH; ++h)
 #pragma unroll
       for (int e = 0; e < G::kE; ++e) st.o[t][h][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
+}
 
-  // the table through the scalar cache: vector loads return in order, and would
-  // wait for the keys in flight
-  typedef const __attribute__((address_space(4))) int32_t* Table;
-  const Table table = (Table)(a.table + (int64_t)b * a.ldt);
-  auto block_at = [&](int key) {
-    Block<NT> blk;
-    blk.key = key;
+// Whether the lane's row of tile c sees key x (of a page that is there).
+template <typename T, int DP, int QT>
+__device__ __forceinline__ bool sees(const AttendArgs& a, const Unit& u, const State<T, DP, QT>& st, int c, int x) {
+  const int node = x - u.len;
+  if (x >= u.to) return false;
+  if (a.visible == nullptr) return x <= st.last[c];
+  return node < 0 || (node < 64 && (st.bits[c] >> (node & 63) & 1) != 0);
+}
+
+template <typename T, int DP, int QT, int NT>
+__device__ __forceinline__ void mask_scores(const AttendArgs& a, const Unit& u, const State<T, DP, QT>& st,
+                                            const Block<NT>& blk, float (&p)[QT][NT][4]) {
+  const int g = lane() >> 4;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int first = key + 16 * t;
-      const int page = first < to ? table[first >> a.page_shift] : -1;
-      blk.there[t] = (unsigned)page < (unsigned)a.num_pages;
-      blk.at[t] = (((size_t)(blk.there[t] ? page : 0) * a.kv_heads + kvh) * ps + (first & (ps - 1))) * D;
+  for (int c = 0; c < QT; ++c)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool see = blk.there[t] && sees(a, u, st, c, blk.key + 16 * t + 4 * g + r);
+        p[c][t][r] = see ? p[c][t][r] : -INFINITY;
+      }
+}
+
+// Scores to weights (2 ^ (scale * score - m)), and their sum.  m follows the row's
+// maximum only where weights grow past kGrow (float32 sums hold 2^10 as well as 1),
+// or at the row's first keys: a block costs no maximum of its own.
+template <typename T, int DP, int QT, int NT>
+__device__ __forceinline__ void weigh(float scale, State<T, DP, QT>& st, float (&p)[QT][NT][4]) {
+  using G = Geo<T, DP>;
+  float w[QT][NT][4], sum[QT];
+  auto weights = [&]() {
+    bool past = false;
+#pragma unroll
+    for (int c = 0; c < QT; ++c) {
+      sum[c] = 0.0f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[c][t][r] = __builtin_amdgcn_exp2f(fmaf(p[c][t][r], scale, -st.base[c]));
+        sum[c] += (w[c][t][0] + w[c][t][1]) + (w[c][t][2] + w[c][t][3]);
+      }
+      past |= !(sum[c] <= st.most[c]);
     }
-    return blk;
+    return __any(past);
   };
+  if (weights()) {
+#pragma unroll
+    for (int c = 0; c < QT; ++c) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        top = fmaxf(top, fmaxf(fmaxf(p[c][t][0], p[c][t][1]), fmaxf(p[c][t][2], p[c][t][3])));
+      const float m = fmaxf(st.m[c], quad_max(top * scale));
+      const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.m[c] - m);
+      st.m[c] = m;
+      st.base[c] = m == -INFINITY ? 0.0f : m;
+      st.most[c] = m == -INFINITY ? -1.0f : kGrow;
+      st.l[c] *= f;
+#pragma unroll
+      for (int h = 0; h < G::kH; ++h)
+#pragma unroll
+        for (int e = 0; e < G::kE; ++e) st.o[c][h][e] *= f;
+    }
+    (void)weights();
+  }
+#pragma unroll
+  for (int c = 0; c < QT; ++c) {
+    st.l[c] += sum[c];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[c][t][r] = w[c][t][r];
+  }
+}
+
+// Rare: the infinities and NaN of a block's values, which the product took as
+// zeros, for the rows that see their keys.  The weights go through 16 x keys
+// floats of LDS of the wave's own (-1: not seen).
+// Column y of accumulator (h, e) in lane group g: interleaved, or in order.
+template <typename T, int DP, bool ORDER>
+__device__ __forceinline__ int column(int h, int e, int g, int y) {
+  using G = Geo<T, DP>;
+  return ORDER ? (h * G::kE + e) * 16 + 4 * g + y : h * 16 * G::kE + (4 * g + y) * G::kE + e;
+}
+
+template <typename T, int DP, int QT, bool FULL, bool ORDER, int NT>
+__device__ __forceinline__ void add_infinite(const AttendArgs& a, const Unit& u, State<T, DP, QT>& st, const Block<NT>& blk,
+                                          const float (&p)[QT][NT][4], float* mine) {
+  using G = Geo<T, DP>;
+  constexpr int kKeys = 16 * NT;
+  const int n = lane() & 15, g = lane() >> 4, D = FULL ? DP : a.D;
+#pragma unroll
+  for (int c = 0; c < QT; ++c) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool see = blk.there[t] && sees(a, u, st, c, blk.key + 16 * t + 4 * g + r);
+        mine[n * kKeys + 16 * t + 4 * g + r] = see ? p[c][t][r] : -1.0f;
+      }
+    wave_lds_fence();
+#pragma unroll 1
+    for (int i = 0; i < kKeys && blk.key + i < u.to; ++i) {
+      const float wt = mine[n * kKeys + i];
+      const bool there = i < 16 ? blk.there[0] : blk.there[NT - 1];
+      if (!there) continue;
+      const T* row = reinterpret_cast<const T*>(a.v) + (i < 16 ? blk.at[0] : blk.at[NT - 1]) + (size_t)(i & 15) * D;
+#pragma unroll
+      for (int h = 0; h < G::kH; ++h)
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int e = 0; e < G::kE; ++e) {
+            const int d = column<T, DP, ORDER>(h, e, g, y);
+            const float x = FULL || d < D ? (float)row[d] : 0.0f;
+            if (!(wt < 0.0f) && !(fabsf(x) < INFINITY)) st.o[c][h][e][y] += wt * x;
+          }
+    }
+    wave_lds_fence();
+  }
+}
+
+// The scalar cache reads the table: vector loads return in order, and would wait
+// for the keys in flight.
+typedef const __attribute__((address_space(4))) int32_t* Table;
+
+template <int NT>
+__device__ __forceinline__ Block<NT> block_at(const AttendArgs& a, const Unit& u, int D, int key) {
+  const Table table = (Table)(a.table + (int64_t)u.b * a.ldt);
+  const int ps = 1 << a.page_shift;
+  Block<NT> blk;
+  blk.key = key;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int first = key + 16 * t;
+    const int page = first < u.to ? table[first >> a.page_shift] : -1;
+    blk.there[t] = (unsigned)page < (unsigned)a.num_pages;
+    blk.at[t] = (((size_t)(blk.there[t] ? page : 0) * a.kv_heads + u.kvh) * ps + (first & (ps - 1))) * D;
+  }
+  return blk;
+}
+
+// A row's result (four columns of it), or its chunk's part.
+template <typename T>
+__device__ __forceinline__ void put_row(const AttendArgs& a, const Unit& u, int r, int d, float m, float l, f32x4 o) {
+  const int head = u.kvh * a.group + r % a.group, n = u.start + r / a.group;
+  const int64_t at = (int64_t)n * a.heads + head;
+  if (a.chunks == 1) {
+    attend_out<T>(a, at, n, head, d, m, l, o);
+    return;
+  }
+  const int64_t part = (int64_t)u.c * a.N * a.heads + at;
+  *reinterpret_cast<f32x4*>(a.part_o + part * a.D + d) = o;
+  if (d == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * part) = f32x2{m, l};
+}
+
+// Few rows: the waves take blocks of keys in turn, straight into registers.  A
+// block's keys are asked for when the last block's are used up, its values alike, so
+// that 16 KB a wave are on their way most of the time; 8 waves a CU at least.
+template <typename T, int DP, int QT, bool FULL>
+__global__ __launch_bounds__(kAttThreads, attend_waves(sizeof(T), DP, QT, FULL)) void k_attend(AttendArgs a) {
+  using G = Geo<T, DP>;
+  constexpr int NT = G::kTiles, kKeys = 16 * NT;
+  constexpr int kRows = 16 * QT, kLd = DP + 4;
+  __shared__ __align__(16) float sm_o[kAttWaves][kRows][kLd];
+  __shared__ float sm_m[kAttWaves][kRows], sm_l[kAttWaves][kRows];
+  static_assert(16 * kKeys <= kRows * kLd, "a wave's weights fit its part");
+  const Unit u = unit_of(a, kRows);
+  if (!u.any) return;
+  const int w = uniform(wave()), n = lane() & 15, g = lane() >> 4, D = FULL ? DP : a.D;
+  const int all = row_all(a, u, u.r0);
+  State<T, DP, QT> st;
+  first_state<T, DP, QT, FULL>(a, u, u.r0, st);
   typename G::Piece k[NT][G::kSteps];
   typename G::V v[NT][4][G::kH];
   auto fetch_keys = [&](const Block<NT>& blk) {
@@ -297,16 +492,18 @@ __global__ __launch_bounds__(kAttThreads, attend_waves(sizeof(T), DP, QT)) void 
     for (int t = 0; t < NT; ++t) load_values<T, DP, FULL>(reinterpret_cast<const T*>(a.v) + blk.at[t], D, v[t]);
   };
 
-  int key = from + w * kKeys;
-  Block<NT> blk = block_at(key);
-  if (key < to) {
+  int key = u.from + w * kKeys;
+  Block<NT> blk = block_at<NT>(a, u, D, key);
+  if (key < u.to) {
     fetch_keys(blk);
     fetch_values(blk);
   }
-  for (; key < to; key += kAttWaves * kKeys) {
+  for (; key < u.to; key += kAttWaves * kKeys) {
+    // after the last block its own is loaded again, from the caches: with a branch
+    // around the loads every wait for keys would be one for the values behind them
     const int after = key + kAttWaves * kKeys;
-    const Block<NT> next = block_at(after);
-    bool whole = key + kKeys <= min(all, to);
+    const Block<NT> next = block_at<NT>(a, u, D, after < u.to ? after : key);
+    bool whole = key + kKeys <= min(all, u.to);
 #pragma unroll
     for (int t = 0; t < NT; ++t) whole = whole && blk.there[t];
     float p[QT][NT][4];
@@ -320,55 +517,16 @@ __global__ __launch_bounds__(kAttThreads, attend_waves(sizeof(T), DP, QT)) void 
 #pragma unroll
         for (int r = 0; r < 4; ++r) p[c][t][r] = s[r];
       }
-    if (after < to) fetch_keys(next);  // the registers are free again
-    if (!whole) {
-#pragma unroll
-      for (int c = 0; c < QT; ++c)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int x = key + 16 * t + 4 * g + r, node = x - len;
-            bool see = blk.there[t] && x < to;
-            if (a.visible == nullptr) see = see && x <= st.last[c];
-            else see = see && (node < 0 || (node < 64 && (st.bits[c] >> (node & 63) & 1) != 0));
-            p[c][t][r] = see ? p[c][t][r] : -INFINITY;
-          }
-    }
-#pragma unroll
-    for (int c = 0; c < QT; ++c) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-        top = fmaxf(top, fmaxf(fmaxf(p[c][t][0], p[c][t][1]), fmaxf(p[c][t][2], p[c][t][3])));
-      top *= a.scale;
-      // the maximum that weights are scaled by moves only where a score would pass
-      // it by kGrow: float32 sums hold 2^8 as well as 1
-      if (__any(top > st.m[c] + kGrow)) {
-        const float m = fmaxf(st.m[c], quad_max(top));
-        const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.m[c] - m);
-        st.m[c] = m;
-        st.l[c] *= f;
-#pragma unroll
-        for (int h = 0; h < G::kH; ++h)
-#pragma unroll
-          for (int e = 0; e < G::kE; ++e) st.o[c][h][e] *= f;
-      }
-      const float base = st.m[c] == -INFINITY ? 0.0f : st.m[c];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) p[c][t][r] = __builtin_amdgcn_exp2f(fmaf(p[c][t][r], a.scale, -base));
-        st.l[c] += (p[c][t][0] + p[c][t][1]) + (p[c][t][2] + p[c][t][3]);
-      }
-    }
+    fetch_keys(next);  // the registers are free again
+    if (!whole) mask_scores(a, u, st, blk, p);
+    weigh(a.scale, st, p);
     bool odd = false;  // some value is infinite or NaN, which a weight of 0 must not meet
     if (!whole) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const bool in = blk.there[t] && key + 16 * t + 4 * g + r < to;
+          const bool in = blk.there[t] && key + 16 * t + 4 * g + r < u.to;
 #pragma unroll
           for (int h = 0; h < G::kH; ++h) {
             if (!in) v[t][r][h] = typename G::V{};
@@ -388,58 +546,18 @@ __global__ __launch_bounds__(kAttThreads, attend_waves(sizeof(T), DP, QT)) void 
             for (int e = 0; e < G::kE; ++e)
               st.o[c][h][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[0][r][h][e], p[c][0][r], st.o[c][h][e], 0, 0, 0);
       } else {
-        const u32x4 x{pack2<T>(p[c][0][0], p[c][0][1]), pack2<T>(p[c][0][2], p[c][0][3]),
-                      pack2<T>(p[c][1][0], p[c][1][1]), pack2<T>(p[c][1][2], p[c][1][3])};
+        const u32x4 x = weights_of<T>(p[c][0], p[c][1]);
 #pragma unroll
         for (int h = 0; h < G::kH; ++h)
 #pragma unroll
           for (int e = 0; e < G::kE; ++e) {
-            auto pair = [&](int t, int r) {
-              return __builtin_amdgcn_perm(v[t][r + 1][h][e / 2], v[t][r][h][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
-            };
-            st.o[c][h][e] = dot<T>(u32x4{pair(0, 0), pair(0, 2), pair(1, 0), pair(1, 2)}, x, st.o[c][h][e]);
+            const u32x2 lo = columns(v[0], h, e), hi = columns(v[1], h, e);
+            st.o[c][h][e] = dot<T>(u32x4{lo[0], lo[1], hi[0], hi[1]}, x, st.o[c][h][e]);
           }
       }
     }
-    if (odd) {
-      // rare: the infinities and NaN, for the rows that see their keys.  The
-      // weights go through the wave's own part of LDS (-1: not seen)
-      float* mine = &sm_o[w][0][0];
-      static_assert(16 * kKeys <= kRows * kLd, "a wave's weights fit its part");
-#pragma unroll
-      for (int c = 0; c < QT; ++c) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int x = key + 16 * t + 4 * g + r, node = x - len;
-            bool see = blk.there[t] && x < to;
-            if (a.visible == nullptr) see = see && x <= st.last[c];
-            else see = see && (node < 0 || (node < 64 && (st.bits[c] >> (node & 63) & 1) != 0));
-            mine[n * kKeys + 16 * t + 4 * g + r] = see ? p[c][t][r] : -1.0f;
-          }
-        wave_lds_fence();
-#pragma unroll 1
-        for (int i = 0; i < kKeys && key + i < to; ++i) {
-          const float wt = mine[n * kKeys + i];
-          const bool there = i < 16 ? blk.there[0] : blk.there[NT - 1];
-          if (!there) continue;
-          const T* row = reinterpret_cast<const T*>(a.v) + (i < 16 ? blk.at[0] : blk.at[NT - 1]) + (size_t)(i & 15) * D;
-#pragma unroll
-          for (int h = 0; h < G::kH; ++h)
-#pragma unroll
-            for (int y = 0; y < 4; ++y)
-#pragma unroll
-              for (int e = 0; e < G::kE; ++e) {
-                const int d = h * 16 * G::kE + (4 * g + y) * G::kE + e;
-                const float x = FULL || d < D ? (float)row[d] : 0.0f;
-                if (!(wt < 0.0f) && !(fabsf(x) < INFINITY)) st.o[c][h][e][y] += wt * x;
-              }
-        }
-        wave_lds_fence();
-      }
-    }
-    if (after < to) fetch_values(next);
+    if (odd) add_infinite<T, DP, QT, FULL, false, NT>(a, u, st, blk, p, &sm_o[w][0][0]);
+    fetch_values(next);
     blk = next;
   }
 
@@ -460,8 +578,8 @@ __global__ __launch_bounds__(kAttThreads, attend_waves(sizeof(T), DP, QT)) void 
   }
   wg_barrier();
   for (int i = threadIdx.x; i < kRows * (DP / 4); i += kAttThreads) {
-    const int row = i / (DP / 4), d = i % (DP / 4) * 4, r = r0 + row, node = r / a.group;
-    if (node >= nodes || d >= D) continue;
+    const int row = i / (DP / 4), d = i % (DP / 4) * 4;
+    if (u.r0 + row >= u.nodes * a.group || d >= D) continue;
     float m = sm_m[0][row];
 #pragma unroll
     for (int x = 1; x < kAttWaves; ++x) m = fmaxf(m, sm_m[x][row]);
@@ -477,65 +595,361 @@ __global__ __launch_bounds__(kAttThreads, attend_waves(sizeof(T), DP, QT)) void 
         o += f * ox;
       }
     }
-    const int head = kvh * a.group + r % a.group;
-    const int64_t at = (int64_t)(start + node) * a.heads + head;
-    if (a.chunks == 1) {
-      attend_out<T>(a, at, start + node, head, d, m, l, o);
-    } else {
-      const int64_t part = (int64_t)c * a.N * a.heads + at;
-      *reinterpret_cast<f32x4*>(a.part_o + part * D + d) = o;
-      if (d == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * part) = f32x2{m, l};
+    put_row<T>(a, u, u.r0 + row, d, m, l, o);
+  }
+}
+
+// Many rows (16-bit types): eight waves, WR groups of 32 rows, each shared by 8 / WR
+// waves that take blocks of 32 keys in turn.  128 keys a step go through LDS once for
+// all of them, straight from memory (16 bytes a lane to consecutive places), a step
+// ahead, in two buffers: one barrier a step.  Rows of keys and values lie in LDS as in
+// memory, their 16-byte pieces exchanged by the row's number so that neither the
+// pieces of 16 keys nor the transposing reads of 16 columns meet on a bank.
+constexpr int kTileWaves = 8;
+constexpr int kTileThreads = kTileWaves * kWave;
+constexpr int kTileKeys = 16 * kTileWaves;  // of a step: a tile a wave
+constexpr int kOdd = 1;     // a tile with infinities or NaN among its values
+constexpr int kAbsent = 2;  // without a page, or past the end
+
+// Which 16-byte piece of row `key` of a tile lies at place p (and the reverse).
+template <int DP>
+__device__ __forceinline__ int key_place(int key, int p) {
+  return DP == 128 ? p ^ (key & 15) : p ^ (key >> 1 & 7);
+}
+template <int DP>
+__device__ __forceinline__ int value_place(int key, int p) {
+  return DP == 128 ? p ^ 2 * (key & 7) : p ^ 2 * (key >> 1 & 3);
+}
+
+// 16 bytes a lane from base + off to LDS at `to` + 16 * lane.  The compiler does not
+// count it among its loads: arrived() waits.
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to) : "memory", "m0");
+}
+__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Four keys of column lane % 16 of 16 columns: lanes 4 e .. 4 e + 3 of a group of 16 name key e's.
+__device__ __forceinline__ u32x2 read_columns(uint32_t at) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4* P;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)at));
+}
+__device__ __forceinline__ u32x4 read_piece(uint32_t at) {
+  typedef const __attribute__((address_space(3))) u32x4* P;
+  return *(P)at;
+}
+
+template <typename T, int DP, int WR, bool FULL>
+__global__ __launch_bounds__(kTileThreads, DP == 64 ? 4 : 2) void k_attend_tiles(AttendArgs a) {
+  using G = Geo<T, DP>;
+  constexpr int QT = 2, kRows = 16 * QT * WR, WK = kTileWaves / WR;
+  constexpr int kRow = DP * 2, kTile = 16 * kRow;       // bytes of a row, of a tile
+  constexpr int kPieces = kRow / 16, kLoads = kTile / 1024;  // of a row; loads of a tile
+  constexpr int kBuffer = 2 * kTileWaves * kTile;       // keys, then values
+  constexpr int DT = DP / 16, kBlocks = kTileWaves / 2 / WK;
+  __shared__ __align__(1024) char sm[2 * kBuffer];
+  __shared__ float sm_w[kTileWaves][16 * 32];
+  __shared__ float sm_ml[kTileWaves][2][16 * QT];
+  __shared__ int sm_flags[2][kTileWaves];  // of each tile
+  const Unit u = unit_of(a, kRows);
+  if (!u.any) return;
+  const int w = uniform(wave()), wr = w % WR, wk = w / WR, ln = lane(), n = ln & 15, g = ln >> 4, D = FULL ? DP : a.D;
+  const int r0 = u.r0 + wr * 16 * QT;
+  const bool work = r0 < u.nodes * a.group;
+  // the wave's own rows may see less than the workgroup's
+  const int all = min(row_all(a, u, r0), u.to), last = min(row_end(a, u, r0 + 16 * QT - 1), u.to);
+  const int wg_all = min(row_all(a, u, u.r0), u.to);
+  State<T, DP, QT> st;
+  first_state<T, DP, QT, FULL>(a, u, r0, st);
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)sm;
+  if constexpr (!FULL) {  // pieces past D are never written again
+    for (int i = threadIdx.x; i < 2 * kBuffer / 16; i += kTileThreads) reinterpret_cast<u32x4*>(sm)[i] = u32x4{0, 0, 0, 0};
+    wg_barrier();
+  }
+
+  // each load of a tile has rows of its own
+  constexpr int kLoadRows = 1024 / kRow;
+  Block<1> mine;
+  auto fetch = [&](int step, int buf) {
+    mine = block_at<1>(a, u, D, u.from + step * kTileKeys + 16 * w);
+    if (mine.key >= u.to) return;
+    const uint32_t to = lds + buf * kBuffer + w * kTile;
+    const T* kb = reinterpret_cast<const T*>(a.k) + mine.at[0];
+    const T* vb = reinterpret_cast<const T*>(a.v) + mine.at[0];
+    int l = ln;
+    asm volatile("" : "+v"(l));  // the places are found anew each step: they are not worth registers in between
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int row = j * kLoadRows + l / kPieces, p = key_place<DP>(row, l % kPieces);
+      if (FULL || p * 8 < D) load_to_lds(kb, (uint32_t)(row * D * 2 + p * 16), to + j * 1024);
+    }
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int row = j * kLoadRows + l / kPieces, p = value_place<DP>(row, l % kPieces);
+      if (FULL || p * 8 < D) load_to_lds(vb, (uint32_t)(row * D * 2 + p * 16), to + kBuffer / 2 + j * 1024);
+    }
+  };
+  // the wave's tile is in; values that no weight may meet become zeros
+  auto settle = [&](int buf) {
+    arrived();
+    bool odd = false;
+    if (mine.key + 16 > wg_all || !mine.there[0]) {
+      u32x4* x = reinterpret_cast<u32x4*>(sm + buf * kBuffer + kBuffer / 2 + w * kTile);
+#pragma unroll 1
+      for (int j = 0; j < kLoads; ++j) {
+        u32x4 v = x[j * kWave + ln];
+        if (!(mine.there[0] && mine.key + j * kLoadRows + ln / kPieces < u.to)) v = u32x4{0, 0, 0, 0};
+        odd |= take_finite<T>(v);
+        x[j * kWave + ln] = v;
+      }
+      odd = __any(odd);
+    }
+    if (ln == 0) sm_flags[buf][w] = (odd ? kOdd : 0) | (mine.there[0] ? 0 : kAbsent);
+  };
+
+  // where the lane reads: its key's pieces of a tile, its columns' of four keys
+  uint32_t k_at[G::kSteps], v_at[DT];
+#pragma unroll
+  for (int s = 0; s < G::kSteps; ++s) k_at[s] = lds + n * kRow + key_place<DP>(n, 4 * s + g) * 16;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) {
+    const int key = 4 * g + n / 4;
+    v_at[d] = lds + kBuffer / 2 + key * kRow + value_place<DP>(key, 2 * d + (n & 3) / 2) * 16 + (n & 1) * 8;
+  }
+
+  const int steps = (u.to - u.from + kTileKeys - 1) / kTileKeys;
+  if (steps > 0) {
+    fetch(0, 0);
+    settle(0);
+  }
+  wg_barrier();
+  for (int i = 0; i < steps; ++i) {
+    const int buf = i & 1;
+    if (i + 1 < steps) fetch(i + 1, buf ^ 1);
+    // a block's pieces are read while the products before them run
+    u32x4 k[2][G::kSteps];
+    auto read_keys = [&](int pair) {
+      const uint32_t at = buf * kBuffer + pair * 2 * kTile;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < G::kSteps; ++j) k[t][j] = read_piece(k_at[j] + at + t * kTile);
+    };
+    read_keys(wk);
+#pragma unroll
+    for (int y = 0; y < kBlocks; ++y) {
+      const int pair = y * WK + wk, key = u.from + i * kTileKeys + 32 * pair;
+      if (!work || key >= last) break;
+      const uint32_t at = buf * kBuffer + pair * 2 * kTile;
+      float p[QT][2][4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x4 s[QT];
+#pragma unroll
+        for (int c = 0; c < QT; ++c) s[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < G::kSteps; ++j)
+#pragma unroll
+          for (int c = 0; c < QT; ++c) s[c] = dot<T>(k[t][j], st.q[c][j], s[c]);
+#pragma unroll
+        for (int c = 0; c < QT; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p[c][t][r] = s[c][r];
+      }
+      u32x4 v[DT];
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const u32x2 lo = read_columns(v_at[d] + at), hi = read_columns(v_at[d] + at + kTile);
+        v[d] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+      }
+      const int f0 = uniform(sm_flags[buf][2 * pair]), f1 = uniform(sm_flags[buf][2 * pair + 1]);
+      if (y + 1 < kBlocks) read_keys(pair + WK);
+      __builtin_amdgcn_sched_barrier(0);
+      if (key + 32 > all || ((f0 | f1) & kAbsent) != 0) {
+        Block<2> blk;
+        blk.key = key;
+        blk.there[0] = (f0 & kAbsent) == 0;
+        blk.there[1] = (f1 & kAbsent) == 0;
+        mask_scores(a, u, st, blk, p);
+      }
+      weigh(a.scale, st, p);
+      u32x4 x[QT];
+#pragma unroll
+      for (int c = 0; c < QT; ++c) x[c] = weights_of<T>(p[c][0], p[c][1]);
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int c = 0; c < QT; ++c) st.o[c][d / G::kE][d % G::kE] = dot<T>(v[d], x[c], st.o[c][d / G::kE][d % G::kE]);
+      if (((f0 | f1) & kOdd) != 0)
+        add_infinite<T, DP, QT, FULL, true, 2>(a, u, st, block_at<2>(a, u, D, key), p, sm_w[w]);
+    }
+    if (i + 1 < steps) settle(buf ^ 1);
+    wg_barrier();
+  }
+
+  if constexpr (WK == 1) {
+    if (!work) return;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const float l = quad_sum(st.l[t]);
+      const int r = r0 + 16 * t + n;
+      if (r >= u.nodes * a.group) continue;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        if (FULL || 16 * d + 4 * g < D) put_row<T>(a, u, r, 16 * d + 4 * g, st.m[t], l, st.o[t][d / G::kE][d % G::kE]);
+    }
+  } else {
+    // the waves of a group of rows joined, 32 rows x DP floats each
+    f32x4* sm_o = reinterpret_cast<f32x4*>(sm);
+    constexpr int kQuads = DP / 4;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const float l = quad_sum(st.l[t]);
+      if (g == 0) {
+        sm_ml[w][0][16 * t + n] = st.m[t];
+        sm_ml[w][1][16 * t + n] = l;
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) sm_o[(w * 16 * QT + 16 * t + n) * kQuads + ((4 * d + g) ^ (n & 7))] = st.o[t][d / G::kE][d % G::kE];
+    }
+    wg_barrier();
+    for (int i = threadIdx.x; i < kRows * kQuads; i += kTileThreads) {
+      const int row = i / kQuads, d = i % kQuads * 4, in = row % (16 * QT), first = row / (16 * QT);
+      if (u.r0 + row >= u.nodes * a.group || d >= D) continue;
+      float m = -INFINITY, l = 0.0f;
+#pragma unroll
+      for (int x = 0; x < WK; ++x) m = fmaxf(m, sm_ml[first + WR * x][0][in]);
+      f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int x = 0; x < WK; ++x) {
+        const float mx = sm_ml[first + WR * x][0][in], lx = sm_ml[first + WR * x][1][in];
+        if (mx == -INFINITY && lx == 0.0f) continue;
+        const float f = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - m);
+        l += f * lx;
+        o += f * sm_o[((first + WR * x) * 16 * QT + in) * kQuads + ((d / 4) ^ (in & 7))];
+      }
+      put_row<T>(a, u, u.r0 + row, d, m, l, o);
     }
   }
 }
 
-// The chunks of a row joined, a wave a row.
+// Chunks of sequence b that have been written.
+__device__ __forceinline__ int chunks_of(const AttendArgs& a, int b, int nodes) {
+  const int64_t end = min((int64_t)min(max(a.lens[b], 0), kMostKeys) + nodes, (int64_t)a.ldt << a.page_shift);
+  return (int)min((int64_t)a.chunks, max((int64_t)1, (end + a.chunk - 1) / a.chunk));
+}
+
+// The parts of a row's few chunks joined: D / 4 threads a row, each with the
+// chunks' maxima and sums for itself.
+constexpr int kFewChunks = 16;
+constexpr int kManyRows = 4096;  // calls of fewer rows take less time with a workgroup a row (2048 rows of 8 chunks: 31 / 28 us the call; 6144 of 2: 63 / 69)
+
+template <typename T>
+__global__ __launch_bounds__(kAttThreads) void k_attend_join_few(AttendArgs a) {
+  const int b = blockIdx.y, width = a.D / 4, rows_here = kAttThreads / width;
+  const int start = max(a.node_off[b], 0);
+  const int nodes = min(min(a.node_off[b + 1], a.N) - start, a.max_nodes);
+  const int64_t i = (int64_t)blockIdx.x * rows_here + threadIdx.x / width;
+  if ((int)threadIdx.x / width >= rows_here || i >= (int64_t)nodes * a.heads) return;
+  const int d = threadIdx.x % width * 4, chunks = chunks_of(a, b, nodes);
+  const int64_t row = (int64_t)start * a.heads + i, rows = (int64_t)a.N * a.heads;
+  const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + row;
+  const float* x = a.part_o + row * a.D + d;
+  float m = -INFINITY;
+  for (int c = 0; c < chunks; ++c) m = fmaxf(m, ml[c * rows][0]);
+  float l = 0.0f;
+  f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int c = 0; c < chunks; ++c) {
+    const f32x2 z = ml[c * rows];
+    const f32x4 part = *reinterpret_cast<const f32x4*>(x + c * rows * a.D);
+    const float f = z[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(z[0] - m);
+    if (z[0] == -INFINITY && z[1] == 0.0f) continue;  // nothing for the row
+    l += f * z[1];
+    o += f * part;
+  }
+  attend_out<T>(a, row, start + (int)(i / a.heads), (int)(i % a.heads), d, m, l, o);
+}
+
+// The chunks of a row joined, a workgroup a row: D / 4 threads a chunk, as many
+// chunks at a time as fit, added in one order.
+constexpr int kMostChunks = 2048;
+
 template <typename T>
 __global__ __launch_bounds__(kAttThreads) void k_attend_join(AttendArgs a) {
+  __shared__ float part[kMostChunks], red[2][kAttWaves];
+  __shared__ f32x4 sum[kAttThreads];
   const int b = blockIdx.y;
   const int start = max(a.node_off[b], 0);
   const int nodes = min(min(a.node_off[b + 1], a.N) - start, a.max_nodes);
-  const int64_t i = (int64_t)blockIdx.x * kAttWaves + wave();
-  if (i >= (int64_t)nodes * a.heads) return;
-  const int64_t end = min((int64_t)min(max(a.lens[b], 0), kMostKeys) + nodes, (int64_t)a.ldt << a.page_shift);
-  const int chunks = (int)min((int64_t)a.chunks, max((int64_t)1, (end + a.chunk - 1) / a.chunk));
-  const int64_t row = (int64_t)start * a.heads + i, rows = (int64_t)a.N * a.heads;
+  if ((int64_t)blockIdx.x >= (int64_t)nodes * a.heads) return;
+  const int chunks = chunks_of(a, b, nodes);
+  const int64_t row = (int64_t)start * a.heads + blockIdx.x, rows = (int64_t)a.N * a.heads;
+  const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + row;
   float m = -INFINITY;
-  for (int c = lane(); c < chunks; c += kWave) m = fmaxf(m, a.part_ml[2 * (c * rows + row)]);
+  for (int c = threadIdx.x; c < chunks; c += kAttThreads) m = fmaxf(m, ml[c * rows][0]);
   m = wave_max(m);
+  if (lane() == 0) red[0][wave()] = m;
+  wg_barrier();
+  m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   float l = 0.0f;
-  f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
-  const int d = lane() * 4;
-  for (int c = 0; c < chunks; ++c) {
-    const float mx = a.part_ml[2 * (c * rows + row)], lx = a.part_ml[2 * (c * rows + row) + 1];
-    if (mx == -INFINITY && lx == 0.0f) continue;  // nothing was written of it
-    const float f = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - m);
-    l += f * lx;
-    if (d < a.D) o += f * *reinterpret_cast<const f32x4*>(a.part_o + (c * rows + row) * a.D + d);
+  for (int c = threadIdx.x; c < chunks; c += kAttThreads) {
+    const f32x2 x = ml[c * rows];
+    const bool none = x[0] == -INFINITY && x[1] == 0.0f;  // the chunk has nothing for the row
+    const float f = x[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[0] - m);
+    if (!none) l += f * x[1];
+    part[c] = none ? -1.0f : f;
   }
-  if (d < a.D) attend_out<T>(a, row, start + (int)(i / a.heads), (int)(i % a.heads), d, m, l, o);
+  l = wave_sum(l);
+  if (lane() == 0) red[1][wave()] = l;
+  wg_barrier();
+  l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  const int width = a.D / 4, groups = kAttThreads / width, group = threadIdx.x / width, d = threadIdx.x % width * 4;
+  f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+  if (group < groups) {
+    const float* x = a.part_o + row * a.D + d;
+#pragma unroll 4
+    for (int c = group; c < chunks; c += groups) {
+      const float f = part[c];
+      if (!(f < 0.0f)) o += f * *reinterpret_cast<const f32x4*>(x + c * rows * a.D);
+    }
+  }
+  sum[threadIdx.x] = o;
+  wg_barrier();
+  if (group != 0) return;
+  for (int y = 1; y < groups; ++y) o += sum[y * width + threadIdx.x];
+  attend_out<T>(a, row, start + (int)(blockIdx.x / a.heads), (int)(blockIdx.x % a.heads), d, m, l, o);
 }
 
 constexpr int kChunkKeys = kAttWaves * 32;  // a chunk is whole rounds of its waves
 
-template <typename T, int DP, int QT, bool FULL>
-hipError_t launch_attend_t(const AttendArgs& a, hipStream_t s) {
-  const int64_t units = (int64_t)a.chunks * a.B * a.kv_heads;
-  const dim3 grid((unsigned)((units + 7) / 8 * 8 * a.row_blocks));
-  hipLaunchKernelGGL((k_attend<T, DP, QT, FULL>), grid, dim3(kAttThreads), 0, s, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.chunks == 1) return e;
-  const dim3 join((unsigned)(((int64_t)a.max_nodes * a.heads + kAttWaves - 1) / kAttWaves), (unsigned)a.B);
-  hipLaunchKernelGGL(k_attend_join<T>, join, dim3(kAttThreads), 0, s, a);
-  return hipGetLastError();
+template <typename T, int DP, bool FULL>
+void start_attend(const AttendArgs& a, dim3 grid, hipStream_t s) {
+  if constexpr (DP < 256 && sizeof(T) == 2) {
+    const dim3 block(kTileThreads);
+    if (a.row_tiles == 16) hipLaunchKernelGGL((k_attend_tiles<T, DP, 8, FULL>), grid, block, 0, s, a);
+    if (a.row_tiles == 8) hipLaunchKernelGGL((k_attend_tiles<T, DP, 4, FULL>), grid, block, 0, s, a);
+    if (a.row_tiles == 4) hipLaunchKernelGGL((k_attend_tiles<T, DP, 2, FULL>), grid, block, 0, s, a);
+  }
+  if constexpr (DP < 256)
+    if (a.row_tiles == 2) hipLaunchKernelGGL((k_attend<T, DP, 2, FULL>), grid, dim3(kAttThreads), 0, s, a);
+  if (a.row_tiles == 1) hipLaunchKernelGGL((k_attend<T, DP, 1, FULL>), grid, dim3(kAttThreads), 0, s, a);
 }
 
 template <typename T, int DP>
 hipError_t launch_attend_d(const AttendArgs& a, hipStream_t s) {
-  if constexpr (DP < 256)
-    if (a.row_tiles == 2)
-      return a.D == DP ? launch_attend_t<T, DP, 2, true>(a, s) : launch_attend_t<T, DP, 2, false>(a, s);
-  return a.D == DP ? launch_attend_t<T, DP, 1, true>(a, s) : launch_attend_t<T, DP, 1, false>(a, s);
+  const int64_t units = (int64_t)a.chunks * a.B * a.kv_heads;
+  const dim3 grid((unsigned)((units + 7) / 8 * 8 * a.row_blocks));
+  if (a.D == DP) start_attend<T, DP, true>(a, grid, s);
+  else start_attend<T, DP, false>(a, grid, s);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.chunks == 1) return e;
+  const int64_t rows = (int64_t)a.max_nodes * a.heads, few = kAttThreads / (a.D / 4);
+  if (a.chunks <= kFewChunks && (int64_t)a.N * a.heads >= kManyRows)
+    hipLaunchKernelGGL(k_attend_join_few<T>, dim3((unsigned)((rows + few - 1) / few), (unsigned)a.B), dim3(kAttThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL(k_attend_join<T>, dim3((unsigned)rows, (unsigned)a.B), dim3(kAttThreads), 0, s, a);
+  return hipGetLastError();
 }
 
 template <typename T>
@@ -547,11 +961,34 @@ hipError_t launch_attend_of(const AttendArgs& a, hipStream_t s) {
 
 size_t plan_attend(AttendArgs& a, int dtype, int num_cu) {
   const int64_t rows = (int64_t)a.max_nodes * a.group;
-  a.row_tiles = rows > 16 && a.D <= 128 ? 2 : 1;
+  a.row_tiles = a.D > 128 || rows <= 16 ? 1 : rows <= 32 || dtype == PLH_F32 ? 2 : rows <= 64 ? 4 : rows <= 128 ? 8 : 16;
   a.row_blocks = (int)((rows + 16 * a.row_tiles - 1) / (16 * a.row_tiles));
   const int64_t units = std::max<int64_t>(1, (int64_t)a.B * a.kv_heads * a.row_blocks);
   const int64_t most = (a.max_len + kChunkKeys - 1) / kChunkKeys;  // rounds of the longest sequence
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(most / 2, (8LL * num_cu + units - 1) / units));
+  int64_t want = 1;
+  if (a.row_tiles <= 2) {
+    // as many workgroups as the chip holds at once; where there are that many
+    // sequences anyway, shorter chunks even out their lengths.  Microseconds at 3 (what it
+    // holds) and 8 a CU: 1 x 65 536 tokens, 8 key heads, 63 / 69; 64 x 8192 307 / 299.
+    const int dp = a.D <= 64 ? 64 : a.D <= 128 ? 128 : 256;
+    const int64_t held = units < num_cu ? attend_waves(dtype == PLH_F32 ? 4 : 2, dp, a.row_tiles, a.D == dp) : 8;
+    want = std::min<int64_t>({most / 2, (held * num_cu + units - 1) / units, kMostChunks});
+  } else {
+    // a workgroup a CU: the number of chunks whose rounds of workgroups (4 us for 128
+    // keys, 5 us each beside them) and partial results (at 5 GB/ms, and a launch) take least
+    double best = 1e300;
+    for (int64_t n = 1; n <= std::min<int64_t>(most / 2, kMostChunks) || n == 1; ++n) {
+      const double rounds = (double)((units * n + num_cu - 1) / num_cu), steps = (double)((most + n - 1) / n);
+      const double parts = n == 1 ? 0.0 : 6.0 + (double)a.N * a.heads * (a.D + 2) * 8.0 * n / 5e6;
+      const double us = rounds * (4.0 * steps + 5.0) + parts;
+      if (us < best) {
+        best = us;
+        want = n;
+      }
+      if (units * n > 8LL * num_cu) break;
+    }
+  }
+  want = std::max<int64_t>(1, want);
   a.chunk = (int)((most + want - 1) / want) * kChunkKeys;
   a.chunks = (int)((most * kChunkKeys + a.chunk - 1) / a.chunk);
   return a.chunks == 1 ? 0 : (size_t)a.chunks * a.N * a.heads * (a.D + 2) * sizeof(float);

@@ -64,6 +64,9 @@ extern "C" {
 /* plh_set_option options */
 #define PLH_OPT_KERNEL_TIMING 1 /* value 1: bracket the fast path's kernels with
                                    HIP events (read by plh_kernel_times) */
+#define PLH_OPT_TREE_LOOKS 2 /* how often a workgroup of plh_verify_tree looks for
+                                another's sums before it computes them itself (64);
+                                the results do not depend on it */
 
 
 typedef struct plh_ctx plh_ctx;
@@ -472,14 +475,19 @@ int plh_tree_attention(plh_ctx* ctx, const void* q, int dtype, int64_t ldq, int 
  *   out_tokens int32 [B, max_nodes]: the accepted nodes' tokens, then the drawn
  *             one, then -1; out_path [B, max_nodes]: 0 and the accepted nodes, then
  *             -1; out_n_acc [B]: how many were accepted; out_n_used [B]: uniforms
+ *   ws        plh_verify_tree_ws_bytes of the same sizes, 256-byte aligned, the
+ *             caller's until the call's kernels have ended (may be NULL for 0 bytes)
  * A sequence without nodes, with more than max_nodes, or whose walk tests a token
  * outside [0, V) gives -1 everywhere and uses no uniform.  max_nodes <= 256, V <=
- * 524288.  A chain gives what plh_verify gives.
+ * 524288.  A chain gives what plh_verify gives.  Rows of more than 8192 tokens are
+ * shared by several workgroups, which exchange sums through ws; with
+ * PLH_OPT_TREE_LOOKS 0 each computes all of them itself (the same results, slower).
  */
 int plh_verify_tree(plh_ctx* ctx, const void* p, const void* q, int dtype, int64_t ld, int N, int V,
                     const int32_t* tokens, const int32_t* parents, const int32_t* node_off, int B, int max_nodes,
                     const double* uniforms, int64_t ldu, int replacement, int32_t* out_tokens, int32_t* out_path,
-                    int32_t* out_n_acc, int32_t* out_n_used);
+                    int32_t* out_n_acc, int32_t* out_n_used, void* ws, int64_t ws_bytes);
+int64_t plh_verify_tree_ws_bytes(plh_ctx* ctx, int B, int V, int max_nodes);
 
 /*
  * Pages src[i] of all layers copied to dst[i] (int32 [n]), keys and values: what a

@@ -33,6 +33,7 @@ PLH_SAMPLE_HIST_SPANS = 2
 PLH_SAMPLE_NUCLEUS = 4
 PLH_SAMPLE_NUCLEUS_ONLY = 8
 PLH_OPT_KERNEL_TIMING = 1
+PLH_OPT_TREE_LOOKS = 2
 
 _c_int, _c_i64, _c_sz, _vp = ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_void_p
 
@@ -106,8 +107,9 @@ SIGNATURES = {
     "plh_verify_tree": (
         _c_int,
         [_vp, _vp, _vp, _c_int, _c_i64, _c_int, _c_int, _vp, _vp, _vp, _c_int, _c_int, _vp, _c_i64, _c_int, _vp, _vp,
-         _vp, _vp],
+         _vp, _vp, _vp, _c_i64],
     ),
+    "plh_verify_tree_ws_bytes": (_c_i64, [_vp, _c_int, _c_int, _c_int]),
     "plh_copy_pages": (_c_int, [_vp, _vp, _vp, _c_int, _c_i64, _c_int, _c_i64, _vp, _vp, _c_int]),
     "plh_keep_nodes": (
         _c_int,
@@ -458,12 +460,18 @@ class Context:
         )
 
     def verify_tree(self, p_ptr, q_ptr, dtype_code, ld, N, V, tokens, parents, node_off, B, max_nodes, uniforms, ldu,
-                    replacement, out_tokens, out_path, out_n_acc, out_n_used) -> None:
+                    replacement, out_tokens, out_path, out_n_acc, out_n_used, ws, ws_bytes) -> None:
         self._check(
             self.lib.plh_verify_tree(self.handle, p_ptr, q_ptr, dtype_code, ld, N, V, tokens, parents, node_off, B,
                                      max_nodes, uniforms, ldu, int(replacement), out_tokens, out_path, out_n_acc,
-                                     out_n_used)
+                                     out_n_used, ws, ws_bytes)
         )
+
+    def verify_tree_ws_bytes(self, B, V, max_nodes) -> int:
+        n = int(self.lib.plh_verify_tree_ws_bytes(self.handle, B, V, max_nodes))
+        if n < 0:
+            self._check(n)
+        return n
 
     def copy_pages(self, k_ptr, v_ptr, layers, layer_bytes, num_pages, page_bytes, src, dst, n) -> None:
         self._check(self.lib.plh_copy_pages(self.handle, k_ptr, v_ptr, layers, layer_bytes, num_pages, page_bytes, src,

@@ -38,6 +38,7 @@ struct plh_ctx {
   bool scratch_open = false;
   // PLH_OPT_KERNEL_TIMING: event triples (start, between, end) per timed call
   bool timing = false;
+  int tree_looks = 64;  // PLH_OPT_TREE_LOOKS
   std::vector<hipEvent_t> ev_free;
   std::vector<std::array<hipEvent_t, 3>> ev_pending;
   // plh_stage: page-locked buffers; `done` closes the last copy from one
@@ -410,6 +411,10 @@ int plh_set_option(plh_ctx* c, int option, int64_t value) {
     case PLH_OPT_KERNEL_TIMING:
       if (value != 0 && value != 1) return fail(c, PLH_ERR_INVALID_ARG, "PLH_OPT_KERNEL_TIMING takes 0 or 1%s");
       c->timing = value != 0;
+      return PLH_OK;
+    case PLH_OPT_TREE_LOOKS:
+      if (value < 0 || value > 1000000) return fail(c, PLH_ERR_INVALID_ARG, "PLH_OPT_TREE_LOOKS takes 0 to 1000000%s");
+      c->tree_looks = (int)value;
       return PLH_OK;
     default:
       return fail(c, PLH_ERR_INVALID_ARG, "unknown option%s");
@@ -1173,17 +1178,27 @@ int plh_keep_nodes(plh_ctx* c, void* k_pages, void* v_pages, int layers, int64_t
   return PLH_OK;
 }
 
+int64_t plh_verify_tree_ws_bytes(plh_ctx* c, int B, int V, int max_nodes) {
+  if (c == nullptr) return PLH_ERR_INVALID_ARG;
+  if (B < 0 || V < 1 || max_nodes < 1)
+    return fail(c, PLH_ERR_INVALID_ARG, "need B >= 0, V >= 1 and max_nodes >= 1%s");
+  if (max_nodes > plh::kTreeNodes) return fail(c, PLH_ERR_UNSUPPORTED, "trees of more than 256 nodes%s");
+  if (V > plh::kTreeV) return fail(c, PLH_ERR_UNSUPPORTED, "rows of more than 524288 tokens%s");
+  if ((int64_t)B * ((V + 8191) / 8192) > INT32_MAX / 64) return fail(c, PLH_ERR_UNSUPPORTED, "more rows than a grid holds%s");
+  return (int64_t)plh::tree_ws_bytes(B, V, max_nodes);
+}
+
 int plh_verify_tree(plh_ctx* c, const void* p, const void* q, int dtype, int64_t ld, int N, int V,
                     const int32_t* tokens, const int32_t* parents, const int32_t* node_off, int B, int max_nodes,
                     const double* uniforms, int64_t ldu, int replacement, int32_t* out_tokens, int32_t* out_path,
-                    int32_t* out_n_acc, int32_t* out_n_used) {
+                    int32_t* out_n_acc, int32_t* out_n_used, void* ws, int64_t ws_bytes) {
   if (c == nullptr) return PLH_ERR_INVALID_ARG;
   if (B < 0 || N < 0 || V < 1 || max_nodes < 1)
     return fail(c, PLH_ERR_INVALID_ARG, "need B >= 0, N >= 0, V >= 1 and max_nodes >= 1%s");
   if (dtype != PLH_F32 && dtype != PLH_F64) return fail(c, PLH_ERR_INVALID_ARG, "dtype must be PLH_F32 or PLH_F64%s");
   if (ld < V || ldu < max_nodes) return fail(c, PLH_ERR_INVALID_ARG, "need ld >= V and ldu >= max_nodes%s");
-  if (max_nodes > plh::kTreeNodes) return fail(c, PLH_ERR_UNSUPPORTED, "trees of more than 256 nodes%s");
-  if (V > plh::kTreeV) return fail(c, PLH_ERR_UNSUPPORTED, "rows of more than 524288 tokens%s");
+  const int64_t need = plh_verify_tree_ws_bytes(c, B, V, max_nodes);
+  if (need < 0) return (int)need;
   if (B == 0) return PLH_OK;
   if (p == nullptr || tokens == nullptr || parents == nullptr || node_off == nullptr || uniforms == nullptr ||
       out_tokens == nullptr || out_path == nullptr || out_n_acc == nullptr || out_n_used == nullptr)
@@ -1193,9 +1208,11 @@ int plh_verify_tree(plh_ctx* c, const void* p, const void* q, int dtype, int64_t
     return fail(c, PLH_ERR_INVALID_ARG, "p and q must be aligned to their element size%s");
   int rc = use_device(c);
   if (rc != PLH_OK) return rc;
-  plh::TreeArgs a{p,  q,     ld, tokens, parents,   node_off,    uniforms,            ldu,       N,
-                  B,  V,     max_nodes,  replacement ? 1 : 0, out_tokens, out_path, out_n_acc, out_n_used};
-  const hipError_t e = plh::launch_verify_tree(a, dtype == PLH_F64, c->stream);
+  if (need > 0 && (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0 || ws_bytes < need))
+    return fail(c, PLH_ERR_INVALID_ARG, "ws must be 256-byte aligned and hold plh_verify_tree_ws_bytes%s");
+  plh::TreeArgs a{p, q, ld, tokens, parents, node_off, uniforms, ldu, N, B, V, max_nodes, replacement ? 1 : 0,
+                  out_tokens, out_path, out_n_acc, out_n_used, c->tree_looks, nullptr, 0};
+  const hipError_t e = plh::launch_verify_tree(a, dtype == PLH_F64, ws, c->stream);
   if (e != hipSuccess) return hip_fail(c, e, "plh_verify_tree launch");
   return PLH_OK;
 }

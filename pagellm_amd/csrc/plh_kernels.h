@@ -278,6 +278,9 @@ struct TreeArgs {
   int32_t* out_path;    // [B, max_nodes]
   int32_t* out_n_acc;
   int32_t* out_n_used;
+  int looks;                  // for another workgroup's sums, before they are computed anew
+  unsigned long long* slots;  // workspace: [B, passes, segments, 2] sums
+  int passes;                 // launch_verify_tree
 };
 constexpr int kTreeNodes = 256;     // of one sequence's tree
 constexpr int kTreeV = 1 << 19;     // tokens of a row: their pieces' sums lie in LDS
@@ -344,7 +347,8 @@ hipError_t launch_attend(AttendArgs a, int dtype, void* ws, hipStream_t s);
 hipError_t launch_rotary(const RotaryArgs& a, int dtype, hipStream_t s);
 hipError_t launch_copy_pages(CopyArgs a, int n, hipStream_t s);
 hipError_t launch_keep(const KeepArgs& a, int B, hipStream_t s);
-hipError_t launch_verify_tree(const TreeArgs& a, bool f64, hipStream_t s);
+size_t tree_ws_bytes(int B, int V, int max_nodes);
+hipError_t launch_verify_tree(TreeArgs a, bool f64, void* ws, hipStream_t s);
 hipError_t launch_append(int32_t* slab, const int64_t* pos, const int32_t* ids, int n, hipStream_t s);
 
 }  // namespace plh

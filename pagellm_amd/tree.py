@@ -232,10 +232,13 @@ def verify_tree(p, q, tokens, parents, node_off, uniforms, *, max_nodes: int | N
         return res
     c.set_stream(_stream_of(p))
     at = out.data_ptr()
+    nbytes = c.verify_tree_ws_bytes(B, V, max_nodes)
+    # torch's allocator orders its reuse on the stream
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=p.device) if nbytes else None
     c.verify_tree(p.data_ptr(), q.data_ptr() if q is not None else None,
                   _native.PLH_F64 if p.dtype == torch.float64 else _native.PLH_F32, ld, N, V, tokens.data_ptr(),
                   parents.data_ptr(), node_off.data_ptr(), B, max_nodes, uniforms.data_ptr(), ldu, replacement, at,
-                  at + 4 * n, at + 8 * n, at + 8 * n + 4 * B)
+                  at + 4 * n, at + 8 * n, at + 8 * n + 4 * B, ws.data_ptr() if nbytes else None, nbytes)
     return res
 
 
@@ -345,9 +348,11 @@ def verify_tree_step(target_logits, q_rows, trees: Sequence[DraftTree], params, 
              probs.data_ptr(), 0)
     out = torch.empty(B * (2 * most + 2), dtype=torch.int32, device=dev)
     n = B * most
+    nbytes = c.verify_tree_ws_bytes(B, V, most)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     c.verify_tree(probs.data_ptr(), None if q_rows is None else q_rows.data_ptr(), _native.PLH_F64, V, N, V, d_tok, d_par,
                   d_node, B, most, d_u, most, replacement, out.data_ptr(), out.data_ptr() + 4 * n, out.data_ptr() + 8 * n,
-                  out.data_ptr() + 8 * n + 4 * B)
+                  out.data_ptr() + 8 * n + 4 * B, ws.data_ptr() if nbytes else None, nbytes)
     verdict = TreeVerdict(out[:n].view(B, most), out[n:2 * n].view(B, most), out[2 * n:2 * n + B], out[2 * n + B:])
     host = out.cpu().numpy().astype(np.int64)
     toks, n_acc, used = host[:n].reshape(B, most), host[2 * n:2 * n + B], host[2 * n + B:]

@@ -203,6 +203,49 @@ def test_strides_streams_and_graphs():
         verify_tree(big, None, [0], [-1], [0, 1], torch.zeros((1, 1), dtype=torch.float64, device="cuda"), max_nodes=1)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("V", [8193, 20000, 70001])
+def test_results_do_not_depend_on_waits(V, dtype):
+    """With no look for another workgroup's sums every workgroup computes all of
+    them itself: the same bits; many sequences, so that some start late."""
+    import torch
+
+    from pagellm_amd import _native
+
+    ctx = _native.Context()
+    for replacement, with_q in ((False, True), (True, True), (False, False)):
+        p, q, tokens, parents, off, u = _case(V, [40, 1, 7, 2] * 3, V, 4, dtype, replacement, near=1.0)
+        many = lambda x: np.concatenate([x] * 8)  # noqa: E731
+        n = off[-1]
+        args = [many(p), many(q) if with_q else None, many(tokens), many(parents),
+                np.concatenate([[0]] + [off[1:] + n * i for i in range(8)]), np.random.default_rng(1).random((96, 40))]
+        up = lambda x, t: None if x is None else torch.from_numpy(np.ascontiguousarray(x)).to("cuda", t)  # noqa: E731
+        dt = getattr(torch, dtype)
+        args = [up(x, t) for x, t in zip(args, (dt, dt, torch.int32, torch.int32, torch.int32, torch.float64))]
+        want = verify_tree(*args, max_nodes=40, replacement=replacement, ctx=ctx)
+        for looks in (0, 1, 64):
+            ctx._check(ctx.lib.plh_set_option(ctx.handle, _native.PLH_OPT_TREE_LOOKS, looks))
+            got = verify_tree(*args, max_nodes=40, replacement=replacement, ctx=ctx)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (looks, replacement, with_q)
+    with pytest.raises(ValueError):
+        ctx._check(ctx.lib.plh_set_option(ctx.handle, _native.PLH_OPT_TREE_LOOKS, -1))
+
+
+def test_more_rejections_than_shared_sums():
+    """A root with 60 children that are all rejected: passes past the shared ones."""
+    V = 9000
+    g = np.random.default_rng(2)
+    q = g.dirichlet(np.ones(V), 61)
+    p = np.zeros((61, V))
+    p[:, 8500:] = 1 / 500
+    kids = g.permutation(8000)[:60]
+    u = g.random((1, 61))
+    args = [p, q, np.concatenate([[0], kids]), np.array([-1] + [0] * 60), np.array([0, 61]), u]
+    res = verify_tree(*args)
+    _check(res, *args, False)
+    assert res.n_used[0] == 61 and res.n_acc[0] == 0 and res.tokens[0, 0] >= 8500
+
+
 @pytest.mark.parametrize("on_gpu", [False, True])
 def test_a_round_from_logits_and_generators(on_gpu):
     """verify_tree_step against the oracle's probs and rule, Generators left where a

@@ -325,8 +325,10 @@ def test_null_contexts():
     assert lib.plh_rotary_append(n, n, 1, 1, n, 1, n, 1, n, 1, 1, 0, 1, 1, n, n, 0, 0, 1.0, n, n, 1, 16, n) == -1
     assert lib.plh_tree_attention_ws_bytes(n, 0, 1, 1, 1, 8, 1, 1, 1) == -1
     assert lib.plh_tree_attention(n, n, 0, 8, 1, 1, 1, 8, n, n, 1, 16, n, 1, n, n, 1, n, 1.0, 1, 1, n, 8, n, n, 0) == -1
-    assert lib.plh_verify_tree(n, n, n, 0, 1, 1, 1, n, n, n, 1, 1, n, 1, 0, n, n, n, n) == -1
+    assert lib.plh_verify_tree(n, n, n, 0, 1, 1, 1, n, n, n, 1, 1, n, 1, 0, n, n, n, n, n, 0) == -1
+    assert lib.plh_verify_tree_ws_bytes(n, 1, 1, 1) == -1
     assert lib.plh_copy_pages(n, n, n, 1, 16, 1, 16, n, n, 1) == -1
     assert lib.plh_keep_nodes(n, n, n, 1, 16, 1, 16, 1, 16, n, 1, n, n, 1, n, 1) == -1
     header = (_native.LIB_PATH.parents[1] / "include" / "pagellm_hip.h").read_text()
-    assert f"#define PLH_MAX_TREE_NODES {_native.PLH_MAX_TREE_NODES}\n" in header
+    for name in ("PLH_MAX_TREE_NODES", "PLH_OPT_TREE_LOOKS"):
+        assert f"#define {name} {getattr(_native, name)}" in header

@@ -27,7 +27,7 @@ from typing import Hashable, Mapping, Sequence
 import numpy as np
 
 from . import _native
-from .fp8 import _check_device, _float_code
+from .fp8 import _float_code
 from .logits import _pack
 from .sampling import _ctx, _is_torch_cuda, _stream_of
 
@@ -121,35 +121,49 @@ def rotary_frequencies(part: int, base: float = 10000.0, scaling: Mapping | None
     return freq, factor
 
 
-def _rows(c, x, name: str, dim: int | None = None):
-    """(heads, D, row stride) of x [N, heads, D], whose heads lie side by side."""
-    _check_device(c, x, name)
+def _on_device(c, x, name: str) -> None:
+    """x is a CUDA tensor on the context's GPU (get_device() builds no object)."""
+    try:
+        d = x.get_device()
+    except AttributeError:
+        raise TypeError(f"{name} must be a torch CUDA tensor") from None
+    if d != c.device:
+        if d < 0:
+            raise TypeError(f"{name} must be a torch CUDA tensor")
+        raise ValueError(f"{name} is on GPU {d}, the context on GPU {c.device}")
+
+
+def _rows(c, x, name: str):
+    """(N, heads, D, row stride) of x [N, heads, D], whose heads lie side by side."""
+    _on_device(c, x, name)
     if x.dim() != 3:
         raise ValueError(f"{name} must be [N, heads, D]")
     n, h, d = x.shape
-    if dim is not None and d != dim:
-        raise ValueError(f"{name} has heads of {d} values, the others of {dim}")
-    s = x.stride()
-    if x.numel() and ((d > 1 and s[2] != 1) or (h > 1 and s[1] != d)):
+    if x.is_contiguous():
+        return n, h, d, h * d
+    ld, step, one = x.stride()
+    if x.numel() and ((d > 1 and one != 1) or (h > 1 and step != d)):
         raise ValueError(f"the heads of a row of {name} must lie side by side")
-    if n > 1 and x.numel() and s[0] < h * d:
+    if n > 1 and x.numel() and ld < h * d:
         raise ValueError(f"rows of {name} must not overlap")
-    return int(h), int(d), int(s[0]) if n > 1 else int(h * d)
+    return n, h, d, ld if n > 1 else h * d
 
 
 def _check_pages(c, k_pages, v_pages, dims: int) -> None:
-    _check_device(c, k_pages, "k_pages")
-    _check_device(c, v_pages, "v_pages")
+    _on_device(c, k_pages, "k_pages")
+    _on_device(c, v_pages, "v_pages")
     if k_pages.dim() != dims:
         raise ValueError("k_pages must be [pages, kv heads, page size, D]" if dims == 4 else
                          "k_pages must be [layers, pages, kv heads, page size, D]")
     if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
         raise ValueError("v_pages must be like k_pages")
-    if dims == 4:
-        if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
-            raise ValueError("pages must be contiguous")
+    if k_pages.is_contiguous() and v_pages.is_contiguous():
+        if k_pages.numel() == 0:
+            raise ValueError("the cache must hold pages")
+    elif dims == 4:
+        raise ValueError("pages must be contiguous")
     elif k_pages.numel() == 0 or not (k_pages[0].is_contiguous() and v_pages[0].is_contiguous()) or \
-            k_pages.stride(0) != v_pages.stride(0):
+            (k_pages.shape[0] > 1 and k_pages.stride(0) != v_pages.stride(0)):
         raise ValueError("each layer's pages must be contiguous, the layers as far apart in both")
 
 
@@ -158,7 +172,9 @@ def _ints(c, x, name: str, dtype, n: int | None = None):
     context's GPU; sequences and arrays go over in a queued copy."""
     import torch
 
-    if not _is_torch_cuda(x):
+    if isinstance(x, torch.Tensor) and x.dtype is dtype and x.get_device() == c.device and x.is_contiguous():
+        pass
+    elif not _is_torch_cuda(x):
         if isinstance(x, torch.Tensor):
             x = x.numpy()
         host = np.asarray(x)
@@ -175,8 +191,7 @@ def _ints(c, x, name: str, dtype, n: int | None = None):
             buf[:] = host.reshape(-1).view(np.uint8)
             c.stage_h2d(x.data_ptr(), buf)
     else:
-        if x.device.index != c.device:
-            raise ValueError(f"{name} is on GPU {x.device.index}, the context on GPU {c.device}")
+        _on_device(c, x, name)
         if x.dtype != dtype:
             if x.dtype not in (torch.int32, torch.int64):
                 raise TypeError(f"{name} must be int32 or int64")
@@ -185,7 +200,7 @@ def _ints(c, x, name: str, dtype, n: int | None = None):
             x = x.to(dtype)
         if not x.is_contiguous():
             x = x.contiguous()
-    if n is not None and tuple(x.shape) != (n,):
+    if n is not None and (x.dim() != 1 or x.shape[0] != n):
         raise ValueError(f"expected {n} {name}, got {list(x.shape)}")
     return x
 
@@ -211,56 +226,58 @@ def rotary_append(q, k, v, positions, slots, k_pages, v_pages, rotary: Rotary | 
     if some is None:
         raise ValueError("need q, or k and v")
     heads = kv_heads = ldq = ldqo = ldk = ldv = pages = page_size = 0
-    dim = None
+    code = _float_code(some, "q" if q is not None else "k")
+    dt = some.dtype
     if q is not None:
-        heads, dim, ldq = _rows(c, q, "q")
+        N, heads, dim, ldq = _rows(c, q, "q")
     elif q_out is not None:
         raise ValueError("q_out given without q")
-    code = _float_code(some, "q" if q is not None else "k")
-    N = int(some.shape[0])
-    if N > 2**31 - 1:  # ctypes would wrap it
-        raise ValueError("at most 2^31 - 1 rows")
     if k is not None:
-        kv_heads, dim, ldk = _rows(c, k, "k", dim)
-        v_heads, _, ldv = _rows(c, v, "v", dim)
-        if v_heads != kv_heads or k.shape[0] != N or v.shape[0] != N:
-            raise ValueError("q, k and v must have as many rows, k and v as many heads")
+        n, kv_heads, d, ldk = _rows(c, k, "k")
+        if q is None:
+            N, dim = n, d
+        nv, v_heads, dv, ldv = _rows(c, v, "v")
+        if n != N or nv != N or v_heads != kv_heads or d != dim or dv != dim:
+            raise ValueError("q, k and v must have as many rows and heads as long, k and v as many heads")
         _check_pages(c, k_pages, v_pages, 4)
-        if k.dtype != some.dtype or v.dtype != some.dtype or k_pages.dtype != some.dtype:
+        if k.dtype is not dt or v.dtype is not dt or k_pages.dtype is not dt:
             raise TypeError("q, k, v and the pages must have one type")
-        pages, page_heads, page_size, page_dim = map(int, k_pages.shape)
+        pages, page_heads, page_size, page_dim = k_pages.shape
         if page_heads != kv_heads or page_dim != dim:
             raise ValueError(f"the pages hold {page_heads} heads of {page_dim} values, k {kv_heads} of {dim}")
         slots = _ints(c, slots, "slots", torch.int64, N)
+    if N > 2**31 - 1:  # ctypes would wrap it
+        raise ValueError("at most 2^31 - 1 rows")
     pairs = 0
     if rotary is not None:
         pairs = rotary.pairs
         if 2 * pairs > dim:
             raise ValueError(f"{pairs} pairs do not fit heads of {dim} values")
-        _check_device(c, rotary.inv_freq, "inv_freq")
+        _on_device(c, rotary.inv_freq, "inv_freq")
         positions = _ints(c, positions, "positions", torch.int64, N)
     if q is not None:
         if q_out is None:
-            q_out = torch.empty((N, heads, dim), dtype=q.dtype, device=q.device)
-        elif q_out.dtype != q.dtype or q_out.shape != q.shape:
+            q_out = torch.empty((N, heads, dim), dtype=dt, device=q.device)
+            ldqo = heads * dim
+        elif q_out.dtype is not dt or q_out.shape != q.shape:
             raise ValueError("q_out must be like q")
-        ldqo = _rows(c, q_out, "q_out")[2]
+        else:
+            ldqo = _rows(c, q_out, "q_out")[3]
     if N == 0:
         return q_out
     c.set_stream(_stream_of(some))
-    at = lambda x: x.data_ptr() if x is not None else None  # noqa: E731
-    kv = k is not None
-    c.rotary_append(at(q), ldq, heads, at(q_out), ldqo, at(k), ldk, at(v), ldv, kv_heads, code, N, dim,
+    c.rotary_append(None if q is None else q.data_ptr(), ldq, heads, None if q is None else q_out.data_ptr(), ldqo,
+                    None if k is None else k.data_ptr(), ldk, None if k is None else v.data_ptr(), ldv, kv_heads, code, N, dim,
                     positions.data_ptr() if pairs else None, rotary.inv_freq.data_ptr() if pairs else None, pairs,
-                    int(rotary.interleaved) if pairs else 0, rotary.factor if pairs else 1.0,
-                    k_pages.data_ptr() if kv else None, v_pages.data_ptr() if kv else None, pages, page_size,
-                    slots.data_ptr() if kv else None)
+                    rotary.interleaved if pairs else False, rotary.factor if pairs else 1.0,
+                    None if k is None else k_pages.data_ptr(), None if k is None else v_pages.data_ptr(), pages, page_size,
+                    None if k is None else slots.data_ptr())
     return q_out
 
 
-def _layers(k_pool, v_pool):
-    """(layers, bytes from one to the next) of pools [layers, pages, kv heads, page size, D]."""
-    return int(k_pool.shape[0]), int(k_pool.stride(0)) * k_pool.element_size()
+def _layer_bytes(k_pool) -> int:
+    """From one layer to the next in a pool [layers, pages, kv heads, page size, D]."""
+    return k_pool.stride(0) * k_pool.element_size()
 
 
 def copy_pages(k_pool, v_pool, src, dst, *, ctx: _native.Context | None = None) -> None:
@@ -272,7 +289,7 @@ def copy_pages(k_pool, v_pool, src, dst, *, ctx: _native.Context | None = None) 
 
     c = _ctx(ctx)
     _check_pages(c, k_pool, v_pool, 5)
-    pages = int(k_pool.shape[1])
+    pages = k_pool.shape[1]
     if not _is_torch_cuda(src) and not _is_torch_cuda(dst):
         a, b = (np.asarray(x, dtype=np.int64).reshape(-1) for x in (src, dst))
         for x, name in ((a, "src"), (b, "dst")):
@@ -285,29 +302,26 @@ def copy_pages(k_pool, v_pool, src, dst, *, ctx: _native.Context | None = None) 
     dst = _ints(c, dst, "dst", torch.int32)
     if src.dim() != 1 or src.shape != dst.shape:
         raise ValueError("expected as many src as dst")
-    if src.numel() == 0:
+    n = src.numel()
+    if n == 0:
         return
-    layers, layer_bytes = _layers(k_pool, v_pool)
-    page_bytes = int(k_pool.stride(1)) * k_pool.element_size()
+    _, _, heads, page_size, dim = k_pool.shape
     c.set_stream(_stream_of(k_pool))
-    c.copy_pages(k_pool.data_ptr(), v_pool.data_ptr(), layers, layer_bytes, pages, page_bytes, src.data_ptr(),
-                 dst.data_ptr(), int(src.numel()))
+    c.copy_pages(k_pool.data_ptr(), v_pool.data_ptr(), k_pool.shape[0], _layer_bytes(k_pool), pages,
+                 heads * page_size * dim * k_pool.element_size(), src.data_ptr(), dst.data_ptr(), n)
 
 
-def _table(c, page_table, B: int | None = None):
-    """(page_table, its row stride) of int32 [B, pages]."""
+def _table(c, page_table, B: int):
+    """page_table [B, pages] as contiguous int32."""
     import torch
 
-    _check_device(c, page_table, "page_table")
-    if page_table.dtype != torch.int32:
+    _on_device(c, page_table, "page_table")
+    if page_table.dtype is not torch.int32:
         raise TypeError("page_table must be int32")
-    if page_table.dim() != 2 or (B is not None and page_table.shape[0] != B) or page_table.shape[1] < 1 or \
-            (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise ValueError("page_table must be [sequences, pages] with unit stride")
-    if page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]:
-        raise ValueError("rows of page_table must not overlap")
-    # the kernels read no page past a row's own
-    return page_table, int(page_table.shape[1]), int(page_table.stride(0)) if page_table.shape[0] > 1 else int(page_table.shape[1])
+    if page_table.dim() != 2 or page_table.shape[0] != B or page_table.shape[1] < 1:
+        raise ValueError(f"page_table must be [{B}, pages]")
+    # a row's stride would count as its length
+    return page_table if page_table.is_contiguous() else page_table.contiguous()
 
 
 def keep_nodes(k_pool, v_pool, page_table, lens, path, n_acc, *, ctx: _native.Context | None = None) -> None:
@@ -320,22 +334,19 @@ def keep_nodes(k_pool, v_pool, page_table, lens, path, n_acc, *, ctx: _native.Co
     c = _ctx(ctx)
     _check_pages(c, k_pool, v_pool, 5)
     lens = _ints(c, lens, "lens", torch.int32)
-    B = int(lens.numel())
+    B = lens.numel()
     n_acc = _ints(c, n_acc, "n_acc", torch.int32, B)
     path = _ints(c, path, "path", torch.int32)
     if lens.dim() != 1 or path.dim() != 2 or path.shape[0] != B or path.shape[1] < 1:
         raise ValueError("lens must be [B], path [B, nodes]")
-    table, width, ldt = _table(c, page_table, B)
-    if ldt != width:
-        table, ldt = table.contiguous(), width
+    table = _table(c, page_table, B)
     if B == 0:
         return
-    layers, layer_bytes = _layers(k_pool, v_pool)
-    _, pages, heads, page_size, dim = map(int, k_pool.shape)
+    layers, pages, heads, page_size, dim = k_pool.shape
     c.set_stream(_stream_of(k_pool))
-    c.keep_nodes(k_pool.data_ptr(), v_pool.data_ptr(), layers, layer_bytes, pages, page_size, heads,
-                 dim * k_pool.element_size(), table.data_ptr(), ldt, lens.data_ptr(), path.data_ptr(),
-                 int(path.shape[1]), n_acc.data_ptr(), B)
+    c.keep_nodes(k_pool.data_ptr(), v_pool.data_ptr(), layers, _layer_bytes(k_pool), pages, page_size, heads,
+                 dim * k_pool.element_size(), table.data_ptr(), table.shape[1], lens.data_ptr(), path.data_ptr(),
+                 path.shape[1], n_acc.data_ptr(), B)
 
 
 class CacheStep:

@@ -23,8 +23,8 @@ from typing import Callable, NamedTuple, Sequence
 import numpy as np
 
 from . import _native
-from .cache import CacheStep, PagedCache, _check_pages, _ints, _rows, _table
-from .fp8 import _check_device, _float_code
+from .cache import CacheStep, PagedCache, _check_pages, _ints, _on_device, _rows, _table
+from .fp8 import _float_code
 from .logits import _pack
 from .sampling import _as_float_rows, _ctx, _expand_params, _history_ids, _is_torch_cuda, _pack_params, _stream_of
 
@@ -88,41 +88,42 @@ def tree_attention(q, k_pages, v_pages, page_table, lens, node_off, visible=None
     import torch
 
     c = _ctx(ctx)
-    heads, dim, ldq = _rows(c, q, "q")
+    N, heads, dim, ldq = _rows(c, q, "q")
+    dt = q.dtype
     code = _float_code(q, "q")
     _check_pages(c, k_pages, v_pages, 4)
-    if k_pages.dtype != q.dtype:
+    if k_pages.dtype is not dt:
         raise TypeError("q and the pages must have one type")
-    N, (pages, kv_heads, page_size, page_dim) = int(q.shape[0]), k_pages.shape
+    pages, kv_heads, page_size, page_dim = k_pages.shape
     if page_dim != dim:
         raise ValueError(f"the pages hold heads of {page_dim} values, q of {dim}")
     for x, name in ((lens, "lens"), (node_off, "node_off")):
-        _check_device(c, x, name)
-        if x.dtype != torch.int32 or x.dim() != 1 or not x.is_contiguous():
+        _on_device(c, x, name)
+        if x.dtype is not torch.int32 or x.dim() != 1 or not x.is_contiguous():
             raise TypeError(f"{name} must be contiguous int32, one for each sequence")
-    B = int(lens.shape[0])
+    B = lens.shape[0]
     if node_off.shape[0] != B + 1:
         raise ValueError(f"node_off must have {B + 1} entries")
-    page_table, width, ldt = _table(c, page_table, B)
-    if ldt != width:  # a row's stride would count as its length
-        page_table, ldt = page_table.contiguous(), width
+    page_table = _table(c, page_table, B)
     bits = None
     if visible is not None:
-        _check_device(c, visible, "visible")
-        if visible.dtype not in (torch.int64, torch.uint64) or tuple(visible.shape) != (N,) or not visible.is_contiguous():
+        _on_device(c, visible, "visible")
+        if visible.dtype not in (torch.int64, torch.uint64) or visible.shape != (N,) or not visible.is_contiguous():
             raise TypeError(f"visible must be contiguous int64 or uint64 [{N}]")
         bits = visible.data_ptr()
     max_nodes, max_len = int(max_nodes), int(max_len)
     if not (0 <= max_nodes <= 2**31 - 1 and 0 <= max_len <= 2**30 and N <= 2**31 - 1):  # ctypes would wrap them
         raise ValueError("need 0 <= max_nodes < 2^31, 0 <= max_len <= 2^30 and less than 2^31 rows")
     if out is None:
-        out = torch.empty((N, heads, dim), dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape:
+        out = torch.empty((N, heads, dim), dtype=dt, device=q.device)
+        ldo = heads * dim
+    elif out.dtype is not dt or out.shape != q.shape:
         raise ValueError("out must be like q")
-    ldo = _rows(c, out, "out")[2]
+    else:
+        ldo = _rows(c, out, "out")[3]
     if lse is not None:
-        _check_device(c, lse, "lse")
-        if lse.dtype != torch.float32 or tuple(lse.shape) != (N, heads) or not lse.is_contiguous():
+        _on_device(c, lse, "lse")
+        if lse.dtype is not torch.float32 or lse.shape != (N, heads) or not lse.is_contiguous():
             raise TypeError(f"lse must be contiguous float32 [{N}, {heads}]")
     if N == 0 or B == 0:
         return out
@@ -131,9 +132,9 @@ def tree_attention(q, k_pages, v_pages, page_table, lens, node_off, visible=None
     # torch's allocator orders its reuse on the stream
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     c.tree_attention(q.data_ptr(), code, ldq, N, heads, kv_heads, dim, k_pages.data_ptr(), v_pages.data_ptr(), pages,
-                     page_size, page_table.data_ptr(), ldt, lens.data_ptr(), node_off.data_ptr(), B, bits,
+                     page_size, page_table.data_ptr(), page_table.shape[1], lens.data_ptr(), node_off.data_ptr(), B, bits,
                      dim ** -0.5 if scale is None else float(scale), max_nodes, max_len, out.data_ptr(), ldo,
-                     lse.data_ptr() if lse is not None else None, ws.data_ptr() if nbytes else None, nbytes)
+                     None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     return out
 
 
@@ -194,21 +195,26 @@ def verify_tree(p, q, tokens, parents, node_off, uniforms, *, max_nodes: int | N
         got = verify_tree(up(p.astype(dt, copy=False)), None if q is None else up(q.astype(dt, copy=False)), up(tok), up(par),
                           up(off), up(u), max_nodes=max_nodes or most, replacement=replacement, ctx=c)
         return TreeVerdict(*(x.cpu().numpy().astype(np.int64) for x in got))
-    _check_device(c, p, "p")
-    if p.dtype not in (torch.float32, torch.float64):
+    _on_device(c, p, "p")
+    dt = p.dtype
+    if dt is not torch.float32 and dt is not torch.float64:
         raise TypeError("p must be float32 or float64")
-    if p.dim() != 2 or p.shape[1] < 1 or (p.shape[1] > 1 and p.stride(1) != 1):
-        raise ValueError("p must be [N, V] with unit stride in the vocabulary dimension")
-    N, V = int(p.shape[0]), int(p.shape[1])
+    if p.dim() != 2 or p.shape[1] < 1:
+        raise ValueError("p must be [N, V]")
+    N, V = p.shape
+    ld, one = p.stride()
+    if V > 1 and one != 1:
+        raise ValueError("p must have unit stride in the vocabulary dimension")
+    if N < 2:
+        ld = V
     if q is not None:
-        _check_device(c, q, "q")
-        if q.dtype != p.dtype or q.shape != p.shape or (V > 1 and q.stride(1) != 1):
+        _on_device(c, q, "q")
+        if q.dtype is not dt or q.shape != p.shape or (V > 1 and q.stride(1) != 1):
             raise ValueError("q must be like p")
-        if N > 1 and q.stride(0) != p.stride(0):
+        if N > 1 and q.stride(0) != ld:
             raise ValueError("rows of p and q must lie as far apart")
     if max_nodes is None:
         raise ValueError("CUDA tensors need max_nodes")
-    ld = int(p.stride(0)) if N > 1 else V
     max_nodes = int(max_nodes)
     if max(N, V, max_nodes) > 2**31 - 1:  # ctypes would wrap them
         raise ValueError("at most 2^31 - 1 rows, tokens and nodes")
@@ -217,28 +223,26 @@ def verify_tree(p, q, tokens, parents, node_off, uniforms, *, max_nodes: int | N
     node_off = _ints(c, node_off, "node_off", torch.int32)
     if node_off.dim() != 1 or node_off.shape[0] < 1:
         raise ValueError("node_off must be [B + 1]")
-    B = int(node_off.shape[0]) - 1
-    _check_device(c, uniforms, "uniforms")
-    if uniforms.dtype != torch.float64 or uniforms.dim() != 2 or uniforms.shape[0] != B or uniforms.shape[1] < max_nodes or \
-            (uniforms.shape[1] > 1 and uniforms.stride(1) != 1):
-        raise ValueError(f"uniforms must be float64 [{B}, >= {max_nodes}] with unit stride")
-    ldu = int(uniforms.stride(0)) if B > 1 else int(uniforms.shape[1])
-    if B > 1 and ldu < max_nodes:
-        uniforms, ldu = uniforms.contiguous(), int(uniforms.shape[1])
-    out = torch.empty(B * (2 * max_nodes + 2), dtype=torch.int32, device=p.device)
-    n = B * max_nodes
-    res = TreeVerdict(out[:n].view(B, max_nodes), out[n:2 * n].view(B, max_nodes), out[2 * n:2 * n + B], out[2 * n + B:])
+    B = node_off.shape[0] - 1
+    _on_device(c, uniforms, "uniforms")
+    if uniforms.dtype is not torch.float64 or uniforms.dim() != 2 or uniforms.shape[0] != B or uniforms.shape[1] < max_nodes:
+        raise ValueError(f"uniforms must be float64 [{B}, >= {max_nodes}]")
+    if not uniforms.is_contiguous():
+        uniforms = uniforms.contiguous()
+    rows = torch.empty((2, B, max_nodes), dtype=torch.int32, device=p.device)
+    counts = torch.empty((2, B), dtype=torch.int32, device=p.device)
+    res = TreeVerdict(*rows.unbind(), *counts.unbind())
     if B == 0:
         return res
     c.set_stream(_stream_of(p))
-    at = out.data_ptr()
     nbytes = c.verify_tree_ws_bytes(B, V, max_nodes)
     # torch's allocator orders its reuse on the stream
     ws = torch.empty(nbytes, dtype=torch.uint8, device=p.device) if nbytes else None
-    c.verify_tree(p.data_ptr(), q.data_ptr() if q is not None else None,
-                  _native.PLH_F64 if p.dtype == torch.float64 else _native.PLH_F32, ld, N, V, tokens.data_ptr(),
-                  parents.data_ptr(), node_off.data_ptr(), B, max_nodes, uniforms.data_ptr(), ldu, replacement, at,
-                  at + 4 * n, at + 8 * n, at + 8 * n + 4 * B, ws.data_ptr() if nbytes else None, nbytes)
+    at, n = rows.data_ptr(), counts.data_ptr()
+    c.verify_tree(p.data_ptr(), None if q is None else q.data_ptr(),
+                  _native.PLH_F64 if dt is torch.float64 else _native.PLH_F32, ld, N, V, tokens.data_ptr(),
+                  parents.data_ptr(), node_off.data_ptr(), B, max_nodes, uniforms.data_ptr(), uniforms.shape[1], replacement,
+                  at, at + 4 * B * max_nodes, n, n + 4 * B, None if ws is None else ws.data_ptr(), nbytes)
     return res
 
 
@@ -297,7 +301,7 @@ def verify_tree_step(target_logits, q_rows, trees: Sequence[DraftTree], params, 
     x = target_logits
     if not _is_torch_cuda(x):
         x = torch.from_numpy(_as_float_rows(x)).to(dev)
-    _check_device(c, x, "target_logits")
+    _on_device(c, x, "target_logits")
     if x.dtype not in (torch.float32, torch.float64):
         raise TypeError("target_logits must be float32 or float64")
     if x.dim() != 2 or x.shape[0] != sum(counts) or x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):

@@ -9,7 +9,7 @@ from types import SimpleNamespace
 import numpy as np
 import pytest
 
-from pagellm_amd import _native, cache, fp8, tree
+from pagellm_amd import _native, cache, tree
 from pagellm_amd.cache import _PageBook, rotary_frequencies
 from pagellm_amd.tree import DraftTree
 
@@ -162,9 +162,9 @@ def on_cpu(monkeypatch):
     """CPU tensors stand for CUDA ones, in a context that no refused call reaches."""
     import torch
 
-    for m in (cache, tree, fp8):
+    for m in (cache, tree):
         monkeypatch.setattr(m, "_is_torch_cuda", lambda x: isinstance(x, torch.Tensor))
-    return SimpleNamespace(device=None)
+    return SimpleNamespace(device=-1)  # what CPU tensors say
 
 
 def _attend_args():
@@ -197,8 +197,9 @@ def test_refusals_of_tree_attention(on_cpu):
         (ValueError, dict(page_table=z(3, 3, dtype=i32))),
         (ValueError, dict(page_table=z(2, 0, dtype=i32))),
         (TypeError, dict(page_table=z(2, 3, dtype=torch.int64))),
-        (ValueError, dict(page_table=z(2, 6, dtype=i32)[:, ::2])),
-        (ValueError, dict(page_table=z(3, dtype=i32).expand(2, 3))),
+        (ValueError, dict(page_table=z(6, dtype=i32))),
+        (TypeError, dict(page_table=np.zeros((2, 3), np.int32))),
+        (ValueError, dict(k_pages=z(0, 2, 16, 16), v_pages=z(0, 2, 16, 16))),
         (TypeError, dict(visible=z(2, dtype=torch.int64))),
         (TypeError, dict(visible=z(3, dtype=i32))),
         (ValueError, dict(max_nodes=-1)),

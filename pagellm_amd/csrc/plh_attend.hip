@@ -176,7 +176,16 @@ struct State {
   int last[QT];        // chains: the last key that it sees
 };
 
-template <typename T, int DP, bool FULL>
+// ONCE: a key head's rows fit one block, so its keys and values are read once and need
+// not stay in the caches: 64 x 8192 299 -> 292 us.  With several blocks of rows that
+// would cost: 32 rows of 4 heads each of 256 values 320 -> 372.
+template <bool ONCE, typename V>
+__device__ __forceinline__ V load_of(const V* p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
+template <typename T, int DP, bool FULL, bool ONCE>
 __device__ __forceinline__ void load_keys(const T* base, int D, typename Geo<T, DP>::Piece (&k)[Geo<T, DP>::kSteps]) {
   using G = Geo<T, DP>;
   const int n = lane() & 15, g = lane() >> 4;
@@ -184,13 +193,13 @@ __device__ __forceinline__ void load_keys(const T* base, int D, typename Geo<T, 
 #pragma unroll
   for (int s = 0; s < G::kSteps; ++s) {
     const int d = G::piece_at(s, g);
-    if (FULL || d < D) k[s] = *reinterpret_cast<const typename G::Piece*>(row + d);
+    if (FULL || d < D) k[s] = load_of<ONCE>(reinterpret_cast<const typename G::Piece*>(row + d));
     else k[s] = typename G::Piece{};
   }
 }
 
 // The lane's four keys (4 g + r) of a tile.
-template <typename T, int DP, bool FULL>
+template <typename T, int DP, bool FULL, bool ONCE>
 __device__ __forceinline__ void load_values(const T* base, int D, typename Geo<T, DP>::V (&v)[4][Geo<T, DP>::kH]) {
   using G = Geo<T, DP>;
   const int n = lane() & 15, g = lane() >> 4;
@@ -200,7 +209,8 @@ __device__ __forceinline__ void load_values(const T* base, int D, typename Geo<T
 #pragma unroll
     for (int h = 0; h < G::kH; ++h) {
       const int at = h * 16 * G::kE;
-      if (FULL || at + n * G::kE < D) v[r][h] = *reinterpret_cast<const typename G::V*>(row + r * (FULL ? DP : D) + at);
+      if (FULL || at + n * G::kE < D)
+        v[r][h] = load_of<ONCE>(reinterpret_cast<const typename G::V*>(row + r * (FULL ? DP : D) + at));
       else v[r][h] = typename G::V{};
     }
 }
@@ -467,7 +477,7 @@ __device__ __forceinline__ void put_row(const AttendArgs& a, const Unit& u, int 
 // Few rows: the waves take blocks of keys in turn, straight into registers.  A
 // block's keys are asked for when the last block's are used up, its values alike, so
 // that 16 KB a wave are on their way most of the time; 8 waves a CU at least.
-template <typename T, int DP, int QT, bool FULL>
+template <typename T, int DP, int QT, bool FULL, bool ONCE>
 __global__ __launch_bounds__(kAttThreads, attend_waves(sizeof(T), DP, QT, FULL)) void k_attend(AttendArgs a) {
   using G = Geo<T, DP>;
   constexpr int NT = G::kTiles, kKeys = 16 * NT;
@@ -485,11 +495,11 @@ __global__ __launch_bounds__(kAttThreads, attend_waves(sizeof(T), DP, QT, FULL))
   typename G::V v[NT][4][G::kH];
   auto fetch_keys = [&](const Block<NT>& blk) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) load_keys<T, DP, FULL>(reinterpret_cast<const T*>(a.k) + blk.at[t], D, k[t]);
+    for (int t = 0; t < NT; ++t) load_keys<T, DP, FULL, ONCE>(reinterpret_cast<const T*>(a.k) + blk.at[t], D, k[t]);
   };
   auto fetch_values = [&](const Block<NT>& blk) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) load_values<T, DP, FULL>(reinterpret_cast<const T*>(a.v) + blk.at[t], D, v[t]);
+    for (int t = 0; t < NT; ++t) load_values<T, DP, FULL, ONCE>(reinterpret_cast<const T*>(a.v) + blk.at[t], D, v[t]);
   };
 
   int key = u.from + w * kKeys;
@@ -842,7 +852,9 @@ __device__ __forceinline__ int chunks_of(const AttendArgs& a, int b, int nodes) 
 // The parts of a row's few chunks joined: D / 4 threads a row, each with the
 // chunks' maxima and sums for itself.
 constexpr int kFewChunks = 16;
-constexpr int kManyRows = 4096;  // calls of fewer rows take less time with a workgroup a row (2048 rows of 8 chunks: 31 / 28 us the call; 6144 of 2: 63 / 69)
+// calls of fewer rows take less time with a workgroup a row (2048 rows of 8 chunks:
+// 31 / 28 us the call; 6144 of 2: 63 / 69)
+constexpr int kManyRows = 4096;
 
 template <typename T>
 __global__ __launch_bounds__(kAttThreads) void k_attend_join_few(AttendArgs a) {
@@ -926,14 +938,20 @@ constexpr int kChunkKeys = kAttWaves * 32;  // a chunk is whole rounds of its wa
 template <typename T, int DP, bool FULL>
 void start_attend(const AttendArgs& a, dim3 grid, hipStream_t s) {
   if constexpr (DP < 256 && sizeof(T) == 2) {
-    const dim3 block(kTileThreads);
-    if (a.row_tiles == 16) hipLaunchKernelGGL((k_attend_tiles<T, DP, 8, FULL>), grid, block, 0, s, a);
-    if (a.row_tiles == 8) hipLaunchKernelGGL((k_attend_tiles<T, DP, 4, FULL>), grid, block, 0, s, a);
-    if (a.row_tiles == 4) hipLaunchKernelGGL((k_attend_tiles<T, DP, 2, FULL>), grid, block, 0, s, a);
+    const dim3 tile(kTileThreads);
+    if (a.row_tiles == 16) hipLaunchKernelGGL((k_attend_tiles<T, DP, 8, FULL>), grid, tile, 0, s, a);
+    if (a.row_tiles == 8) hipLaunchKernelGGL((k_attend_tiles<T, DP, 4, FULL>), grid, tile, 0, s, a);
+    if (a.row_tiles == 4) hipLaunchKernelGGL((k_attend_tiles<T, DP, 2, FULL>), grid, tile, 0, s, a);
   }
-  if constexpr (DP < 256)
-    if (a.row_tiles == 2) hipLaunchKernelGGL((k_attend<T, DP, 2, FULL>), grid, dim3(kAttThreads), 0, s, a);
-  if (a.row_tiles == 1) hipLaunchKernelGGL((k_attend<T, DP, 1, FULL>), grid, dim3(kAttThreads), 0, s, a);
+  constexpr bool kBlocks = sizeof(T) == 4 || DP == 256;  // more rows than a block's are theirs too
+  const dim3 block(kAttThreads);
+  const bool once = !kBlocks || a.row_blocks == 1;
+  if constexpr (DP < 256) {
+    if (a.row_tiles == 2 && once) hipLaunchKernelGGL((k_attend<T, DP, 2, FULL, true>), grid, block, 0, s, a);
+    if (a.row_tiles == 2 && !once) hipLaunchKernelGGL((k_attend<T, DP, 2, FULL, !kBlocks>), grid, block, 0, s, a);
+  }
+  if (a.row_tiles == 1 && once) hipLaunchKernelGGL((k_attend<T, DP, 1, FULL, true>), grid, block, 0, s, a);
+  if (a.row_tiles == 1 && !once) hipLaunchKernelGGL((k_attend<T, DP, 1, FULL, !kBlocks>), grid, block, 0, s, a);
 }
 
 template <typename T, int DP>

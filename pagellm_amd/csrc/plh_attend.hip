@@ -655,9 +655,9 @@ __global__ __launch_bounds__(kTileThreads, DP == 64 ? 4 : 2) void k_attend_tiles
   constexpr int QT = 2, kRows = 16 * QT * WR, WK = kTileWaves / WR;
   constexpr int kRow = DP * 2, kTile = 16 * kRow;       // bytes of a row, of a tile
   constexpr int kPieces = kRow / 16, kLoads = kTile / 1024;  // of a row; loads of a tile
-  constexpr int kBuffer = 2 * kTileWaves * kTile;       // keys, then values
+  constexpr int kBuffer = kTileWaves * kTile;           // two of keys, then two of values
   constexpr int DT = DP / 16, kBlocks = kTileWaves / 2 / WK;
-  __shared__ __align__(1024) char sm[2 * kBuffer];
+  __shared__ __align__(1024) char sm[4 * kBuffer];
   __shared__ float sm_w[kTileWaves][16 * 32];
   __shared__ float sm_ml[kTileWaves][2][16 * QT];
   __shared__ int sm_flags[2][kTileWaves];  // of each tile
@@ -673,7 +673,7 @@ __global__ __launch_bounds__(kTileThreads, DP == 64 ? 4 : 2) void k_attend_tiles
   first_state<T, DP, QT, FULL>(a, u, r0, st);
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)sm;
   if constexpr (!FULL) {  // pieces past D are never written again
-    for (int i = threadIdx.x; i < 2 * kBuffer / 16; i += kTileThreads) reinterpret_cast<u32x4*>(sm)[i] = u32x4{0, 0, 0, 0};
+    for (int i = threadIdx.x; i < 4 * kBuffer / 16; i += kTileThreads) reinterpret_cast<u32x4*>(sm)[i] = u32x4{0, 0, 0, 0};
     wg_barrier();
   }
 
@@ -696,7 +696,7 @@ __global__ __launch_bounds__(kTileThreads, DP == 64 ? 4 : 2) void k_attend_tiles
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int row = j * kLoadRows + l / kPieces, p = value_place<DP>(row, l % kPieces);
-      if (FULL || p * 8 < D) load_to_lds(vb, (uint32_t)(row * D * 2 + p * 16), to + kBuffer / 2 + j * 1024);
+      if (FULL || p * 8 < D) load_to_lds(vb, (uint32_t)(row * D * 2 + p * 16), to + 2 * kBuffer + j * 1024);
     }
   };
   // the wave's tile is in; values that no weight may meet become zeros
@@ -704,7 +704,7 @@ __global__ __launch_bounds__(kTileThreads, DP == 64 ? 4 : 2) void k_attend_tiles
     arrived();
     bool odd = false;
     if (mine.key + 16 > wg_all || !mine.there[0]) {
-      u32x4* x = reinterpret_cast<u32x4*>(sm + buf * kBuffer + kBuffer / 2 + w * kTile);
+      u32x4* x = reinterpret_cast<u32x4*>(sm + (2 + buf) * kBuffer + w * kTile);
 #pragma unroll 1
       for (int j = 0; j < kLoads; ++j) {
         u32x4 v = x[j * kWave + ln];
@@ -720,11 +720,11 @@ __global__ __launch_bounds__(kTileThreads, DP == 64 ? 4 : 2) void k_attend_tiles
   // where the lane reads: its key's pieces of a tile, its columns' of four keys
   uint32_t k_at[G::kSteps], v_at[DT];
 #pragma unroll
-  for (int s = 0; s < G::kSteps; ++s) k_at[s] = lds + n * kRow + key_place<DP>(n, 4 * s + g) * 16;
+  for (int s = 0; s < G::kSteps; ++s) k_at[s] = lds + wk * 2 * kTile + n * kRow + key_place<DP>(n, 4 * s + g) * 16;
 #pragma unroll
   for (int d = 0; d < DT; ++d) {
     const int key = 4 * g + n / 4;
-    v_at[d] = lds + kBuffer / 2 + key * kRow + value_place<DP>(key, 2 * d + (n & 3) / 2) * 16 + (n & 1) * 8;
+    v_at[d] = lds + 2 * kBuffer + wk * 2 * kTile + key * kRow + value_place<DP>(key, 2 * d + (n & 3) / 2) * 16 + (n & 1) * 8;
   }
 
   const int steps = (u.to - u.from + kTileKeys - 1) / kTileKeys;
@@ -736,22 +736,26 @@ __global__ __launch_bounds__(kTileThreads, DP == 64 ? 4 : 2) void k_attend_tiles
   for (int i = 0; i < steps; ++i) {
     const int buf = i & 1;
     if (i + 1 < steps) fetch(i + 1, buf ^ 1);
-    // a block's pieces are read while the products before them run
+    // The wave with products goes first, so that the other's exponentials run beside
+    // them: 4 trees of 64 x 32 768, 64 heads, 296 -> 286 us.  (A wave's own next
+    // products among its exponentials gained nothing, 288 - 292.)  A block's pieces
+    // are read while the products before them run.
     u32x4 k[2][G::kSteps];
-    auto read_keys = [&](int pair) {
-      const uint32_t at = buf * kBuffer + pair * 2 * kTile;
+    auto read_keys = [&](int y) {
+      const uint32_t at = y * WK * 2 * kTile;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int j = 0; j < G::kSteps; ++j) k[t][j] = read_piece(k_at[j] + at + t * kTile);
     };
-    read_keys(wk);
+    read_keys(0);
 #pragma unroll
     for (int y = 0; y < kBlocks; ++y) {
       const int pair = y * WK + wk, key = u.from + i * kTileKeys + 32 * pair;
       if (!work || key >= last) break;
-      const uint32_t at = buf * kBuffer + pair * 2 * kTile;
+      const uint32_t at = y * WK * 2 * kTile;
       float p[QT][2][4];
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         f32x4 s[QT];
@@ -773,7 +777,7 @@ __global__ __launch_bounds__(kTileThreads, DP == 64 ? 4 : 2) void k_attend_tiles
         v[d] = u32x4{lo[0], lo[1], hi[0], hi[1]};
       }
       const int f0 = uniform(sm_flags[buf][2 * pair]), f1 = uniform(sm_flags[buf][2 * pair + 1]);
-      if (y + 1 < kBlocks) read_keys(pair + WK);
+      if (y + 1 < kBlocks) read_keys(y + 1);
       __builtin_amdgcn_sched_barrier(0);
       if (key + 32 > all || ((f0 | f1) & kAbsent) != 0) {
         Block<2> blk;
@@ -782,7 +786,9 @@ __global__ __launch_bounds__(kTileThreads, DP == 64 ? 4 : 2) void k_attend_tiles
         blk.there[1] = (f1 & kAbsent) == 0;
         mask_scores(a, u, st, blk, p);
       }
+      __builtin_amdgcn_s_setprio(0);
       weigh(a.scale, st, p);
+      __builtin_amdgcn_s_setprio(1);
       u32x4 x[QT];
 #pragma unroll
       for (int c = 0; c < QT; ++c) x[c] = weights_of<T>(p[c][0], p[c][1]);
@@ -793,7 +799,14 @@ __global__ __launch_bounds__(kTileThreads, DP == 64 ? 4 : 2) void k_attend_tiles
       if (((f0 | f1) & kOdd) != 0)
         add_infinite<T, DP, QT, FULL, true, 2>(a, u, st, block_at<2>(a, u, D, key), p, sm_w[w]);
     }
+    __builtin_amdgcn_s_setprio(0);
     if (i + 1 < steps) settle(buf ^ 1);
+    // on to the other buffer
+    const int next = buf == 0 ? kBuffer : -kBuffer;
+#pragma unroll
+    for (int j = 0; j < G::kSteps; ++j) k_at[j] += next;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) v_at[d] += next;
     wg_barrier();
   }
 

@@ -176,9 +176,7 @@ struct State {
   int last[QT];        // chains: the last key that it sees
 };
 
-// ONCE: a key head's rows fit one block, so its keys and values are read once and need
-// not stay in the caches: 64 x 8192 299 -> 292 us.  With several blocks of rows that
-// would cost: 32 rows of 4 heads each of 256 values 320 -> 372.
+// ONCE: keys and values pass the caches without being kept there (see plan_attend).
 template <bool ONCE, typename V>
 __device__ __forceinline__ V load_of(const V* p) {
   if constexpr (ONCE) return __builtin_nontemporal_load(p);
@@ -633,8 +631,12 @@ __device__ __forceinline__ int value_place(int key, int p) {
 
 // 16 bytes a lane from base + off to LDS at `to` + 16 * lane.  The compiler does not
 // count it among its loads: arrived() waits.
+template <bool ONCE>
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to) : "memory", "m0");
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "s"(to) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to) : "memory", "m0");
 }
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -649,7 +651,7 @@ __device__ __forceinline__ u32x4 read_piece(uint32_t at) {
   return *(P)at;
 }
 
-template <typename T, int DP, int WR, bool FULL>
+template <typename T, int DP, int WR, bool FULL, bool ONCE>
 __global__ __launch_bounds__(kTileThreads, DP == 64 ? 4 : 2) void k_attend_tiles(AttendArgs a) {
   using G = Geo<T, DP>;
   constexpr int QT = 2, kRows = 16 * QT * WR, WK = kTileWaves / WR;
@@ -691,12 +693,12 @@ __global__ __launch_bounds__(kTileThreads, DP == 64 ? 4 : 2) void k_attend_tiles
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int row = j * kLoadRows + l / kPieces, p = key_place<DP>(row, l % kPieces);
-      if (FULL || p * 8 < D) load_to_lds(kb, (uint32_t)(row * D * 2 + p * 16), to + j * 1024);
+      if (FULL || p * 8 < D) load_to_lds<ONCE>(kb, (uint32_t)(row * D * 2 + p * 16), to + j * 1024);
     }
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int row = j * kLoadRows + l / kPieces, p = value_place<DP>(row, l % kPieces);
-      if (FULL || p * 8 < D) load_to_lds(vb, (uint32_t)(row * D * 2 + p * 16), to + 2 * kBuffer + j * 1024);
+      if (FULL || p * 8 < D) load_to_lds<ONCE>(vb, (uint32_t)(row * D * 2 + p * 16), to + 2 * kBuffer + j * 1024);
     }
   };
   // the wave's tile is in; values that no weight may meet become zeros
@@ -948,31 +950,28 @@ __global__ __launch_bounds__(kAttThreads) void k_attend_join(AttendArgs a) {
 
 constexpr int kChunkKeys = kAttWaves * 32;  // a chunk is whole rounds of its waves
 
-template <typename T, int DP, bool FULL>
+template <typename T, int DP, bool FULL, bool ONCE>
 void start_attend(const AttendArgs& a, dim3 grid, hipStream_t s) {
   if constexpr (DP < 256 && sizeof(T) == 2) {
     const dim3 tile(kTileThreads);
-    if (a.row_tiles == 16) hipLaunchKernelGGL((k_attend_tiles<T, DP, 8, FULL>), grid, tile, 0, s, a);
-    if (a.row_tiles == 8) hipLaunchKernelGGL((k_attend_tiles<T, DP, 4, FULL>), grid, tile, 0, s, a);
-    if (a.row_tiles == 4) hipLaunchKernelGGL((k_attend_tiles<T, DP, 2, FULL>), grid, tile, 0, s, a);
+    if (a.row_tiles == 16) hipLaunchKernelGGL((k_attend_tiles<T, DP, 8, FULL, ONCE>), grid, tile, 0, s, a);
+    if (a.row_tiles == 8) hipLaunchKernelGGL((k_attend_tiles<T, DP, 4, FULL, ONCE>), grid, tile, 0, s, a);
+    if (a.row_tiles == 4) hipLaunchKernelGGL((k_attend_tiles<T, DP, 2, FULL, ONCE>), grid, tile, 0, s, a);
   }
-  constexpr bool kBlocks = sizeof(T) == 4 || DP == 256;  // more rows than a block's are theirs too
   const dim3 block(kAttThreads);
-  const bool once = !kBlocks || a.row_blocks == 1;
-  if constexpr (DP < 256) {
-    if (a.row_tiles == 2 && once) hipLaunchKernelGGL((k_attend<T, DP, 2, FULL, true>), grid, block, 0, s, a);
-    if (a.row_tiles == 2 && !once) hipLaunchKernelGGL((k_attend<T, DP, 2, FULL, !kBlocks>), grid, block, 0, s, a);
-  }
-  if (a.row_tiles == 1 && once) hipLaunchKernelGGL((k_attend<T, DP, 1, FULL, true>), grid, block, 0, s, a);
-  if (a.row_tiles == 1 && !once) hipLaunchKernelGGL((k_attend<T, DP, 1, FULL, !kBlocks>), grid, block, 0, s, a);
+  if constexpr (DP < 256)
+    if (a.row_tiles == 2) hipLaunchKernelGGL((k_attend<T, DP, 2, FULL, ONCE>), grid, block, 0, s, a);
+  if (a.row_tiles == 1) hipLaunchKernelGGL((k_attend<T, DP, 1, FULL, ONCE>), grid, block, 0, s, a);
 }
 
 template <typename T, int DP>
 hipError_t launch_attend_d(const AttendArgs& a, hipStream_t s) {
   const int64_t units = (int64_t)a.chunks * a.B * a.kv_heads;
   const dim3 grid((unsigned)((units + 7) / 8 * 8 * a.row_blocks));
-  if (a.D == DP) start_attend<T, DP, true>(a, grid, s);
-  else start_attend<T, DP, false>(a, grid, s);
+  if (a.D == DP && a.once) start_attend<T, DP, true, true>(a, grid, s);
+  else if (a.D == DP) start_attend<T, DP, true, false>(a, grid, s);
+  else if (a.once) start_attend<T, DP, false, true>(a, grid, s);
+  else start_attend<T, DP, false, false>(a, grid, s);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.chunks == 1) return e;
   const int64_t rows = (int64_t)a.max_nodes * a.heads, few = kAttThreads / (a.D / 4);
@@ -996,6 +995,12 @@ size_t plan_attend(AttendArgs& a, int dtype, int num_cu) {
   a.row_blocks = (int)((rows + 16 * a.row_tiles - 1) / (16 * a.row_tiles));
   const int64_t units = std::max<int64_t>(1, (int64_t)a.B * a.kv_heads * a.row_blocks);
   const int64_t most = (a.max_len + kChunkKeys - 1) / kChunkKeys;  // rounds of the longest sequence
+  // Keys and values that the last cache (256 MB) cannot keep for the next call need not
+  // pass through it.  Microseconds with it and without: few rows 32 x 4096 (0.5 GB) 88 / 92,
+  // 64 x 8192 (2.1 GB) 299 / 292; many rows 16 x 2048 (0.13 GB) 46 / 47, 16 x 4096 63 / 57,
+  // 32 x 4096 96 / 88.  Few rows in several blocks read them several times: with it.
+  const double bytes = 2.0 * a.B * a.max_len * a.kv_heads * a.D * (dtype == PLH_F32 ? 4 : 2);
+  a.once = a.row_tiles > 2 ? bytes > 0.25e9 : a.row_blocks == 1 && bytes > 1e9;
   int64_t want = 1;
   if (a.row_tiles <= 2) {
     // as many workgroups as the chip holds at once; where there are that many

@@ -225,6 +225,7 @@ struct AttendArgs {
   int max_nodes;
   int64_t max_len;
   int row_tiles, row_blocks, chunk, chunks;  // plan_attend
+  bool once;
 };
 
 struct RotaryArgs {

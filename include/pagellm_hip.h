@@ -408,8 +408,8 @@ int plh_fp8_linear(plh_ctx* ctx, const void* x, int dtype, int64_t ldx, int N, i
  * x[i + pairs]), or with `interleaved` (x[2 i], x[2 i + 1]); a head's values from
  * 2 * pairs on, and v, stay as they are.
  *   q       [N, ldq], q_heads heads of D values each; q_out [N, ldqo] takes it
- *           turned: q itself (ldqo = ldq), or rows that meet none of it.  Both
- *           NULL: no queries
+ *           turned: q itself (ldqo = ldq), or rows that meet none of it; none of
+ *           k's and v's in either case.  Both NULL: no queries
  *   k, v    [N, ldk] and [N, ldv], kv_heads heads; written to the layer's pages
  *           at slots[n] = page * page_size + place (int64).  Rows with a slot
  *           outside the pages write nothing; of rows with the same slot one wins,

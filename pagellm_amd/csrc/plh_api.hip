@@ -132,23 +132,26 @@ int timing_begin(plh_ctx* c, std::array<hipEvent_t, 3>& ev) {
   return PLH_OK;
 }
 
-// Whether some row of x [B, ld] and some row of out [B, out_ld], V elements of
-// es bytes each, share memory.
-bool rows_overlap(const void* x, int64_t ld, const void* out, int64_t out_ld, int B, int V, size_t es) {
+// Whether some row of x [B, ld] and some row of out [B, out_ld], V and out_V elements
+// of es bytes each, share memory.
+bool rows_meet(const void* x, int64_t ld, int V, const void* out, int64_t out_ld, int out_V, int B, size_t es) {
   const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), o0 = reinterpret_cast<uintptr_t>(out);
   const uintptr_t x1 = x0 + ((size_t)(B - 1) * (size_t)ld + (size_t)V) * es;
-  const uintptr_t o1 = o0 + ((size_t)(B - 1) * (size_t)out_ld + (size_t)V) * es;
+  const uintptr_t o1 = o0 + ((size_t)(B - 1) * (size_t)out_ld + (size_t)out_V) * es;
   if (!(x0 < o1 && o0 < x1)) return false;
   if (ld != out_ld) return true;
   // interleaved rows (x = buf[:, :V], out = buf[:, V:2V]) never touch:
-  // row b' of out meets row b of x iff |d + (b' - b) * L| < V * es, with
-  // d = o0 - x0 and L the row pitch; only the two m = b' - b nearest
-  // -d / L can satisfy it
-  const int64_t d = (int64_t)(o0 - x0), L = ld * (int64_t)es, w = (int64_t)V * (int64_t)es;
+  // row b' of out meets row b of x iff -out_V * es < d + (b' - b) * L < V * es, with
+  // d = o0 - x0 and L the row pitch, no row longer than that; only the two
+  // m = b' - b nearest -d / L can satisfy it
+  const int64_t d = (int64_t)(o0 - x0), L = ld * (int64_t)es, w = (int64_t)V * (int64_t)es, ow = (int64_t)out_V * (int64_t)es;
   const int64_t q = d >= 0 ? -(d / L) - 1 : (-d) / L;  // floor(-d / L) or one below it
   for (int64_t m = q - 1; m <= q + 2; ++m)
-    if (m > -(int64_t)B && m < (int64_t)B && d + m * L < w && d + m * L > -w) return true;
+    if (m > -(int64_t)B && m < (int64_t)B && d + m * L < w && d + m * L > -ow) return true;
   return false;
+}
+bool rows_overlap(const void* x, int64_t ld, const void* out, int64_t out_ld, int B, int V, size_t es) {
+  return rows_meet(x, ld, V, out, out_ld, V, B, es);
 }
 
 int page_shift_of(int page_size) { return __builtin_ctz((unsigned)page_size); }
@@ -1077,6 +1080,10 @@ int plh_rotary_append(plh_ctx* c, const void* q, int64_t ldq, int q_heads, void*
       return fail(c, PLH_ERR_INVALID_ARG, "rows and pages must be aligned to their element size%s");
   if (has_q && (q == q_out ? ldq != ldqo : rows_overlap(q, ldq, q_out, ldqo, N, q_heads * D, es)))
     return fail(c, PLH_ERR_INVALID_ARG, "q_out must be q itself (ldqo = ldq) or rows that meet none of it%s");
+  if (has_q && has_kv)
+    for (int i = 0; i < 2; ++i)
+      if (rows_meet(i == 0 ? k : v, i == 0 ? ldk : ldv, kv_heads * D, q_out, ldqo, q_heads * D, N, es))
+        return fail(c, PLH_ERR_INVALID_ARG, "q_out must meet no row of k or v%s");
   int rc = use_device(c);
   if (rc != PLH_OK) return rc;
   plh::RotaryArgs a{};

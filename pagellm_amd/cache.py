@@ -211,7 +211,7 @@ def rotary_append(q, k, v, positions, slots, k_pages, v_pages, rotary: Rotary | 
     ``positions`` [N] and writes the keys and the values ``v`` to ``slots`` [N] (page *
     page size + place) of one layer's pages [pages, kv heads, page size, D].  Returns
     the turned queries, in ``q_out`` (a new tensor when None; ``q`` itself turns them
-    in place).
+    in place; else rows that meet none of ``q``, ``k`` and ``v``).
 
     Rows may be views of a wider buffer (one product's q, k and v).  Without ``q``
     keys and values are written alone, without ``k`` and ``v`` queries turned alone;
@@ -368,7 +368,7 @@ class CacheStep:
         from .tree import tree_attention
 
         if not self.open:
-            raise RuntimeError("the step has been committed")
+            raise RuntimeError("the step has ended")
         cache = self.cache
         q = rotary_append(q, k, v, self.positions, self.slots, cache.k[layer], cache.v[layer], rotary, ctx=cache.ctx)
         return tree_attention(q, cache.k[layer], cache.v[layer], self.page_table, self.lens, self.node_off, self.visible,
@@ -385,7 +385,8 @@ class PagedCache:
         cache.fork(key, child); cache.truncate(key, n); cache.remove(key)
 
     Forked sequences share their pages; the first that writes to a shared page gets
-    its own copy (``step`` copies all of a batch's in one launch)."""
+    its own copy (``step`` copies all of a batch's in one launch).  A sequence has one
+    open step at most: another one, ``truncate`` and ``remove`` end it."""
 
     def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: str = "bfloat16", *,
                  ctx: _native.Context | None = None):
@@ -407,6 +408,7 @@ class PagedCache:
         self.k = torch.empty(shape, dtype=types[dtype], device=device)
         self.v = torch.empty(shape, dtype=types[dtype], device=device)
         self._book = _PageBook(int(pages), self.page_size)
+        self._steps: dict[Hashable, CacheStep] = {}  # open ones
 
     def __contains__(self, key) -> bool:
         return key in self._book.held
@@ -432,10 +434,17 @@ class PagedCache:
     def truncate(self, key, n: int) -> None:
         """The sequence keeps its first ``n`` tokens."""
         self._book.truncate(key, n)
+        self._end_step(key)
 
     def remove(self, key) -> None:
         """A finished or aborted sequence gives its pages back."""
         self._book.remove(key)
+        self._end_step(key)
+
+    def _end_step(self, key) -> None:
+        step = self._steps.pop(key, None)
+        if step is not None:
+            step.open = False
 
     def step(self, keys: Sequence[Hashable], trees: Sequence) -> CacheStep:
         """Room for a step of ``trees[b]`` (:class:`pagellm_amd.tree.DraftTree`) behind
@@ -451,6 +460,8 @@ class PagedCache:
         if not chains and max(counts) > _native.PLH_MAX_TREE_NODES:
             raise ValueError(f"trees have at most {_native.PLH_MAX_TREE_NODES} nodes (chains have any number)")
         copies = self._book.reserve(keys, counts)
+        for key in keys:
+            self._end_step(key)
         c = self.ctx
         if copies:
             copy_pages(self.k, self.v, [a for a, _ in copies], [b for _, b in copies], ctx=c)
@@ -488,6 +499,8 @@ class PagedCache:
         (step.slots, step.positions, step.visible, step.tokens, step.parents, step.node_off, step.lens,
          step.page_table) = views
         step.max_nodes, step.max_len = max(counts), max(n + t for n, t in zip(lens, counts))
+        for key in keys:
+            self._steps[key] = step
         return step
 
     def commit(self, step: CacheStep, path=None, n_acc=None, *, accepted: Sequence[int] | None = None) -> None:
@@ -496,9 +509,7 @@ class PagedCache:
         pages behind them back; ``accepted`` is ``n_acc`` where the host has it (else
         it is downloaded).  -1 keeps nothing.  Without ``path`` every node stays."""
         if not step.open or step.cache is not self:
-            raise RuntimeError("not an open step of this cache")
-        if any(self._book.length.get(key) != n for key, n in zip(step.keys, step.host_lens)):
-            raise RuntimeError("a sequence of the step has changed since")
+            raise RuntimeError("not an open step of this cache (another one, truncate or remove ended it, or commit)")
         if path is None:
             kept = [len(t.tokens) for t in step.trees]
         else:
@@ -510,8 +521,8 @@ class PagedCache:
             if len(kept) != len(step.keys) or any(not 0 <= n <= len(t.tokens) for n, t in zip(kept, step.trees)):
                 raise ValueError("n_acc must be in [-1, nodes) for each sequence")
             keep_nodes(self.k, self.v, step.page_table, step.lens, path, n_acc, ctx=self.ctx)
-        step.open = False
         for key, n, m in zip(step.keys, step.host_lens, kept):
+            self._end_step(key)
             self._book.set_length(key, n + m)
 
     def download(self, key, layer: int):

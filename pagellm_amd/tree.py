@@ -52,12 +52,14 @@ class DraftTree:
         self.chain = bool(np.array_equal(p, np.arange(-1, t.size - 1)))
         if not self.chain and t.size > _native.PLH_MAX_TREE_NODES:
             raise ValueError(f"a tree has at most {_native.PLH_MAX_TREE_NODES} nodes")
+        if t.size > 64:
+            self.depths, self.visible = np.arange(t.size, dtype=np.int64), None
+            return
         depths, bits = [], []
         for i, up in enumerate(p.tolist()):
             depths.append(depths[up] + 1 if i else 0)
             bits.append((bits[up] if i else 0) | 1 << i)
-        self.depths = np.asarray(depths, dtype=np.int64)
-        self.visible = np.array(bits, dtype=np.uint64) if t.size <= 64 else None
+        self.depths, self.visible = np.asarray(depths, dtype=np.int64), np.array(bits, dtype=np.uint64)
 
     def __len__(self) -> int:
         return int(self.tokens.size)
@@ -282,8 +284,9 @@ def verify_tree_step(target_logits, q_rows, trees: Sequence[DraftTree], params, 
     :func:`pagellm_amd.speculative.verify_step` is for chains: ``p[n] =
     probs(target_logits[n], params_b, contexts[b] + the drafts on the way to n)``
     (``speculative.py:125-127``; contexts end with the roots), then
-    :func:`verify_tree` with the uniforms of ``rngs[b]``, which ends where a loop that
-    draws one for each test and one for the token leaves it.
+    :func:`verify_tree` with the uniforms of ``rngs[b]`` (a Generator of its own for each
+    sequence), which ends where a loop that draws one for each test and one for the
+    token leaves it.
 
     ``target_logits`` [N, V] are the rows of the trees one after the other, numpy or a
     CUDA tensor (read in place on torch's current stream); ``q_rows`` float64 [N, V],
@@ -297,6 +300,8 @@ def verify_tree_step(target_logits, q_rows, trees: Sequence[DraftTree], params, 
     contexts = [()] * B if contexts is None else contexts
     if len(contexts) != B or len(rngs) != B:
         raise ValueError(f"expected {B} contexts and Generators")
+    if len({id(g.bit_generator) for g in rngs}) != B:
+        raise ValueError("each sequence needs a Generator of its own")
     dev = torch.device("cuda", c.device)
     x = target_logits
     if not _is_torch_cuda(x):
@@ -387,10 +392,11 @@ class TreeDecoder:
         self.cache, self.forward = cache, forward
 
     def prefill(self, keys: Sequence, prompts: Sequence[Sequence[int]]) -> None:
-        """New sequences whose prompts but their last tokens go into the cache."""
+        """New sequences whose prompts but their last tokens go into the cache.  None of
+        them stays where that fails."""
         keys, prompts = list(keys), [list(p) for p in prompts]
-        if len(keys) != len(prompts) or any(len(p) < 1 for p in prompts):
-            raise ValueError("expected a prompt of at least one token for each sequence")
+        if len(keys) != len(prompts) or any(len(p) < 1 for p in prompts) or len(set(keys)) != len(keys):
+            raise ValueError("expected a prompt of at least one token for each of different sequences")
         for key in keys:
             if key in self.cache:
                 raise ValueError(f"sequence {key!r} is in the cache already")
@@ -400,12 +406,12 @@ class TreeDecoder:
         if some:
             try:
                 step = self.cache.step([key for key, _ in some], [DraftTree(p[:-1]) for _, p in some])
+                self.forward(step)
+                self.cache.commit(step)
             except Exception:
                 for key in keys:
                     self.cache.remove(key)
                 raise
-            self.forward(step)
-            self.cache.commit(step)
 
     def round(self, keys: Sequence, trees: Sequence[DraftTree], params, rngs, contexts=None, *, q_rows=None,
               replacement: bool = False) -> TreeRound:

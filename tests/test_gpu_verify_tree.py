@@ -390,6 +390,29 @@ def test_greedy_rounds_give_what_single_steps_give():
     assert cache.free_pages == 64
 
 
+def test_a_failed_prefill_leaves_no_sequence():
+    cache = PagedCache(1, 4, 16, 1, 8, "float32")
+
+    def forward(step):
+        raise OverflowError("no logits")
+
+    dec = TreeDecoder(cache, forward)
+    cache.add("old")
+    for keys, prompts, error in [(["a", "b"], [[1, 2], [3]], OverflowError), (["a"], [range(100)], RuntimeError),
+                                 (["a", "a"], [[1], [2]], ValueError), (["a", "old"], [[1], [2]], ValueError)]:
+        with pytest.raises(error):
+            dec.prefill(keys, prompts)
+        assert len(cache) == 1 and cache.free_pages == 4
+
+
+def test_sequences_have_generators_of_their_own():
+    rng = make_rng(1, 0)
+    trees = [DraftTree([1, 2]), DraftTree([3])]
+    logits = np.random.default_rng(0).standard_normal((3, 8))
+    with pytest.raises(ValueError):
+        verify_tree_step(logits, None, trees, SamplingParams(), [rng, rng])
+
+
 def test_sampled_rounds_run_with_penalties():
     model = Model(seed=3)
     cache = PagedCache(model.layers, 64, 16, model.kv_heads, model.dim, "float32")

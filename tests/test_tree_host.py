@@ -20,6 +20,8 @@ def test_trees():
     assert not t.chain and t.path_to(4) == [1, 3, 4] and t.path_to(0) == [] and len(t) == 5
     c = DraftTree(range(100))
     assert c.chain and c.visible is None and list(c.parents[:3]) == [-1, 0, 1]
+    long = DraftTree(np.zeros(300_000))  # a prompt: no masks of as many bits
+    assert long.visible is None and int(long.depths[-1]) == 299_999
     wide = DraftTree([0] * 64, [-1] + [0] * 63)
     assert int(wide.visible[63]) == (1 << 63) | 1
     for tokens, parents in [([], None), ([1, 2], [-1]), ([1, 2], [0, 0]), ([1, 2], [-1, 1]), ([1, 2], [-1, -1]),

@@ -9,11 +9,16 @@
 // share).  Keys and values go from HBM to registers in whole rows; nothing of the
 // loop passes through LDS.
 //
-//   k_attend        (chunk of keys, sequence, key head, block of rows): running
-//                   maximum and sum, four waves that take blocks of keys in turn,
-//                   joined through LDS
-//   k_attend_join   (row): the chunks' partial results joined, where there are
-//                   several
+//   k_attend        (chunk of keys, sequence, key head, block of up to 32 rows):
+//                   running maximum and sum, four waves that take blocks of keys in
+//                   turn, joined through LDS.  float32, heads of more than 128
+//                   values, and up to 32 rows a key head.  Bound by the read: 64 x
+//                   8192 tokens, 8 key heads of 128 bf16, 286 us, 5.6 TB/s
+//   k_attend_tiles  16-bit types, more rows: keys and values through LDS for up to
+//                   256 rows.  32 trees of 32 x 4096 100-112 us with the call, 3.6 TB/s;
+//                   4 of 64 x 32 768, 64 heads on 8, 282, 0.55 PFLOP/s
+//   k_attend_join, k_attend_join_few  (row): the chunks' partial results joined,
+//                   where there are several: 6 to 8 us
 //
 // Values are the rows of the second product.  The matrix instruction wants eight
 // keys of one column in a lane; a lane loads 8 columns of 8 keys and pairs their

@@ -128,7 +128,8 @@ __global__ __launch_bounds__(kCacheThreads) void k_rotary(RotaryArgs a) {
   }
 }
 
-// 16 KB of one page of one layer, four 16-byte loads a thread.
+// 16 KB of one page of one layer, four 16-byte loads a thread: 512 pairs of 32 KB in
+// 16 layers, keys and values, 204 us, 5.3 TB/s (a large copy's rate); 8 pairs 4.6 us.
 constexpr int kCopyLoads = 4;
 constexpr int kCopyBytes = kCopyLoads * kCacheThreads * 16;
 
@@ -155,7 +156,8 @@ __global__ __launch_bounds__(kCacheThreads) void k_copy(CopyArgs a) {
 
 // 16 bytes of a token's row of one layer, pool and head: a thread walks the path.
 // Place j takes node path[j] >= j, so a later node's place is never written before
-// it is read: eight loads, then their eight stores.
+// it is read: eight loads, then their eight stores.  64 sequences x 32 layers, 8 heads
+// of 128: 10 us, a launch and two rounds of loads and stores; 8 x 16 layers 4.1 us.
 constexpr int kKeepNodes = 64;  // of the path at a time
 constexpr int kKeepLoads = 8;
 

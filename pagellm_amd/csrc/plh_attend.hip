@@ -657,7 +657,7 @@ __device__ __forceinline__ u32x4 read_piece(uint32_t at) {
 }
 
 template <typename T, int DP, int WR, bool FULL, bool ONCE>
-__global__ __launch_bounds__(kTileThreads, DP == 64 ? 4 : 2) void k_attend_tiles(AttendArgs a) {
+__global__ __launch_bounds__(kTileThreads, 2) void k_attend_tiles(AttendArgs a) {
   using G = Geo<T, DP>;
   constexpr int QT = 2, kRows = 16 * QT * WR, WK = kTileWaves / WR;
   constexpr int kRow = DP * 2, kTile = 16 * kRow;       // bytes of a row, of a tile

@@ -11,9 +11,10 @@
 //
 //   k_attend        (chunk of keys, sequence, key head, block of up to 32 rows):
 //                   running maximum and sum, four waves that take blocks of keys in
-//                   turn, joined through LDS.  float32, heads of more than 128
-//                   values, and up to 32 rows a key head.  Bound by the read: 64 x
-//                   8192 tokens, 8 key heads of 128 bf16, 286 us, 5.6 TB/s
+//                   turn, joined through LDS.  float32, and up to 32 rows a key
+//                   head (16 of heads past 128 values).  Bound by the read: 64 x
+//                   8192 tokens, 8 key heads of 128 bf16, 286 us, 5.6 TB/s; float32
+//                   trees of 64 x 8192, 64 heads on 8, 510 us, half of its products' rate
 //   k_attend_tiles  16-bit types, more rows: keys and values through LDS for up to
 //                   256 rows.  32 trees of 32 x 4096 100-112 us with the call, 3.6 TB/s;
 //                   4 of 64 x 32 768, 64 heads on 8, 282, 0.55 PFLOP/s
@@ -612,26 +613,25 @@ __global__ __launch_bounds__(kAttThreads, attend_waves(sizeof(T), DP, QT, FULL))
   }
 }
 
-// Many rows (16-bit types): eight waves, WR groups of 32 rows, each shared by 8 / WR
-// waves that take blocks of 32 keys in turn.  128 keys a step go through LDS once for
-// all of them, straight from memory (16 bytes a lane to consecutive places), a step
+// Many rows (16-bit types): eight waves, WR groups of 32 rows (16 of heads past 128
+// values), each shared by 8 / WR waves that take blocks of 32 keys in turn.  128 keys (64)
+// a step go through LDS once for all of them, straight from memory (16 bytes a lane to consecutive places), a step
 // ahead, in two buffers: one barrier a step.  Rows of keys and values lie in LDS as in
 // memory, their 16-byte pieces exchanged by the row's number so that neither the
 // pieces of 16 keys nor the transposing reads of 16 columns meet on a bank.
 constexpr int kTileWaves = 8;
 constexpr int kTileThreads = kTileWaves * kWave;
-constexpr int kTileKeys = 16 * kTileWaves;  // of a step: a tile a wave
 constexpr int kOdd = 1;     // a tile with infinities or NaN among its values
 constexpr int kAbsent = 2;  // without a page, or past the end
 
 // Which 16-byte piece of row `key` of a tile lies at place p (and the reverse).
 template <int DP>
 __device__ __forceinline__ int key_place(int key, int p) {
-  return DP == 128 ? p ^ (key & 15) : p ^ (key >> 1 & 7);
+  return DP >= 128 ? p ^ (key & 15) : p ^ (key >> 1 & 7);
 }
 template <int DP>
 __device__ __forceinline__ int value_place(int key, int p) {
-  return DP == 128 ? p ^ 2 * (key & 7) : p ^ 2 * (key >> 1 & 3);
+  return DP >= 128 ? p ^ 2 * (key & 7) : p ^ 2 * (key >> 1 & 3);
 }
 
 // 16 bytes a lane from base + off to LDS at `to` + 16 * lane.  The compiler does not
@@ -659,15 +659,20 @@ __device__ __forceinline__ u32x4 read_piece(uint32_t at) {
 template <typename T, int DP, int WR, bool FULL, bool ONCE>
 __global__ __launch_bounds__(kTileThreads, 2) void k_attend_tiles(AttendArgs a) {
   using G = Geo<T, DP>;
-  constexpr int QT = 2, kRows = 16 * QT * WR, WK = kTileWaves / WR;
-  constexpr int kRow = DP * 2, kTile = 16 * kRow;       // bytes of a row, of a tile
-  constexpr int kPieces = kRow / 16, kLoads = kTile / 1024;  // of a row; loads of a tile
-  constexpr int kBuffer = kTileWaves * kTile;           // two of keys, then two of values
-  constexpr int DT = DP / 16, kBlocks = kTileWaves / 2 / WK;
+  constexpr int QT = DP == 256 ? 1 : 2, kRows = 16 * QT * WR, WK = kTileWaves / WR;
+  constexpr int kTileKeys = DP == 256 ? 64 : 128, kTiles = kTileKeys / 16, kBlocks = kTiles / 2 / WK;  // of a step
+  static_assert(kBlocks >= 1, "a block of 32 keys a wave");
+  constexpr int kMine = kTileKeys / kTileWaves, kEach = kTileWaves / kTiles;  // keys that a wave loads; waves a tile
+  constexpr int kRow = DP * 2, kTile = 16 * kRow;  // bytes of a row, of a tile
+  constexpr int kPieces = kRow / 16, kLoads = kMine * kRow / 1024;  // of a row; of a wave's keys
+  constexpr int kBuffer = kTileKeys * kRow;  // two of keys, then two of values
+  constexpr int DT = DP / 16;
+  // places of 16 rows repeat after 256 bytes
+  constexpr int KP = G::kSteps < 4 ? G::kSteps : 4, VP = DT < 8 ? DT : 8;
   __shared__ __align__(1024) char sm[4 * kBuffer];
   __shared__ float sm_w[kTileWaves][16 * 32];
   __shared__ float sm_ml[kTileWaves][2][16 * QT];
-  __shared__ int sm_flags[2][kTileWaves];  // of each tile
+  __shared__ int sm_flags[2][kTileWaves];  // of each wave's keys
   const Unit u = unit_of(a, kRows);
   if (!u.any) return;
   const int w = uniform(wave()), wr = w % WR, wk = w / WR, ln = lane(), n = ln & 15, g = ln >> 4, D = FULL ? DP : a.D;
@@ -686,36 +691,37 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_attend_tiles(AttendArgs a) 
 
   // each load of a tile has rows of its own
   constexpr int kLoadRows = 1024 / kRow;
+  const int my_tile = w / kEach, my_row = w % kEach * kMine;
   Block<1> mine;
   auto fetch = [&](int step, int buf) {
-    mine = block_at<1>(a, u, D, u.from + step * kTileKeys + 16 * w);
+    mine = block_at<1>(a, u, D, u.from + step * kTileKeys + 16 * my_tile);
     if (mine.key >= u.to) return;
-    const uint32_t to = lds + buf * kBuffer + w * kTile;
+    const uint32_t to = lds + buf * kBuffer + w * kMine * kRow;
     const T* kb = reinterpret_cast<const T*>(a.k) + mine.at[0];
     const T* vb = reinterpret_cast<const T*>(a.v) + mine.at[0];
     int l = ln;
     asm volatile("" : "+v"(l));  // the places are found anew each step: they are not worth registers in between
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
-      const int row = j * kLoadRows + l / kPieces, p = key_place<DP>(row, l % kPieces);
+      const int row = my_row + j * kLoadRows + l / kPieces, p = key_place<DP>(row, l % kPieces);
       if (FULL || p * 8 < D) load_to_lds<ONCE>(kb, (uint32_t)(row * D * 2 + p * 16), to + j * 1024);
     }
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
-      const int row = j * kLoadRows + l / kPieces, p = value_place<DP>(row, l % kPieces);
+      const int row = my_row + j * kLoadRows + l / kPieces, p = value_place<DP>(row, l % kPieces);
       if (FULL || p * 8 < D) load_to_lds<ONCE>(vb, (uint32_t)(row * D * 2 + p * 16), to + 2 * kBuffer + j * 1024);
     }
   };
-  // the wave's tile is in; values that no weight may meet become zeros
+  // the wave's keys are in; values that no weight may meet become zeros
   auto settle = [&](int buf) {
     arrived();
     bool odd = false;
     if (mine.key + 16 > wg_all || !mine.there[0]) {
-      u32x4* x = reinterpret_cast<u32x4*>(sm + (2 + buf) * kBuffer + w * kTile);
+      u32x4* x = reinterpret_cast<u32x4*>(sm + (2 + buf) * kBuffer + w * kMine * kRow);
 #pragma unroll 1
       for (int j = 0; j < kLoads; ++j) {
         u32x4 v = x[j * kWave + ln];
-        if (!(mine.there[0] && mine.key + j * kLoadRows + ln / kPieces < u.to)) v = u32x4{0, 0, 0, 0};
+        if (!(mine.there[0] && mine.key + my_row + j * kLoadRows + ln / kPieces < u.to)) v = u32x4{0, 0, 0, 0};
         odd |= take_finite<T>(v);
         x[j * kWave + ln] = v;
       }
@@ -725,11 +731,11 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_attend_tiles(AttendArgs a) 
   };
 
   // where the lane reads: its key's pieces of a tile, its columns' of four keys
-  uint32_t k_at[G::kSteps], v_at[DT];
+  uint32_t k_at[KP], v_at[VP];
 #pragma unroll
-  for (int s = 0; s < G::kSteps; ++s) k_at[s] = lds + wk * 2 * kTile + n * kRow + key_place<DP>(n, 4 * s + g) * 16;
+  for (int s = 0; s < KP; ++s) k_at[s] = lds + wk * 2 * kTile + n * kRow + key_place<DP>(n, 4 * s + g) * 16;
 #pragma unroll
-  for (int d = 0; d < DT; ++d) {
+  for (int d = 0; d < VP; ++d) {
     const int key = 4 * g + n / 4;
     v_at[d] = lds + 2 * kBuffer + wk * 2 * kTile + key * kRow + value_place<DP>(key, 2 * d + (n & 3) / 2) * 16 + (n & 1) * 8;
   }
@@ -753,7 +759,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_attend_tiles(AttendArgs a) 
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int j = 0; j < G::kSteps; ++j) k[t][j] = read_piece(k_at[j] + at + t * kTile);
+        for (int j = 0; j < G::kSteps; ++j) k[t][j] = read_piece(k_at[j % KP] + at + t * kTile + j / KP * 256);
     };
     read_keys(0);
 #pragma unroll
@@ -777,13 +783,17 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_attend_tiles(AttendArgs a) 
 #pragma unroll
           for (int r = 0; r < 4; ++r) p[c][t][r] = s[c][r];
       }
-      u32x4 v[DT];
+      u32x4 v[VP];
+      auto read_values = [&](int h) {
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const u32x2 lo = read_columns(v_at[d] + at), hi = read_columns(v_at[d] + at + kTile);
-        v[d] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-      }
-      const int f0 = uniform(sm_flags[buf][2 * pair]), f1 = uniform(sm_flags[buf][2 * pair + 1]);
+        for (int d = 0; d < VP; ++d) {
+          const u32x2 lo = read_columns(v_at[d] + at + h * 256), hi = read_columns(v_at[d] + at + kTile + h * 256);
+          v[d] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
+      };
+      read_values(0);
+      const int* flags = sm_flags[buf] + 2 * kEach * pair;
+      const int f0 = uniform(flags[0] | flags[kEach - 1]), f1 = uniform(flags[kEach] | flags[2 * kEach - 1]);
       if (y + 1 < kBlocks) read_keys(y + 1);
       __builtin_amdgcn_sched_barrier(0);
       if (key + 32 > all || ((f0 | f1) & kAbsent) != 0) {
@@ -800,9 +810,13 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_attend_tiles(AttendArgs a) 
 #pragma unroll
       for (int c = 0; c < QT; ++c) x[c] = weights_of<T>(p[c][0], p[c][1]);
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+      for (int h = 0; h < DT / VP; ++h) {
+        if (h > 0) read_values(h);
 #pragma unroll
-        for (int c = 0; c < QT; ++c) st.o[c][d / G::kE][d % G::kE] = dot<T>(v[d], x[c], st.o[c][d / G::kE][d % G::kE]);
+        for (int d = h * VP; d < (h + 1) * VP; ++d)
+#pragma unroll
+          for (int c = 0; c < QT; ++c) st.o[c][d / G::kE][d % G::kE] = dot<T>(v[d % VP], x[c], st.o[c][d / G::kE][d % G::kE]);
+      }
       if (((f0 | f1) & kOdd) != 0)
         add_infinite<T, DP, QT, FULL, true, 2>(a, u, st, block_at<2>(a, u, D, key), p, sm_w[w]);
     }
@@ -811,9 +825,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_attend_tiles(AttendArgs a) 
     // on to the other buffer
     const int next = buf == 0 ? kBuffer : -kBuffer;
 #pragma unroll
-    for (int j = 0; j < G::kSteps; ++j) k_at[j] += next;
+    for (int j = 0; j < KP; ++j) k_at[j] += next;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) v_at[d] += next;
+    for (int d = 0; d < VP; ++d) v_at[d] += next;
     wg_barrier();
   }
 
@@ -957,11 +971,13 @@ constexpr int kChunkKeys = kAttWaves * 32;  // a chunk is whole rounds of its wa
 
 template <typename T, int DP, bool FULL, bool ONCE>
 void start_attend(const AttendArgs& a, dim3 grid, hipStream_t s) {
-  if constexpr (DP < 256 && sizeof(T) == 2) {
+  if constexpr (sizeof(T) == 2) {
     const dim3 tile(kTileThreads);
-    if (a.row_tiles == 16) hipLaunchKernelGGL((k_attend_tiles<T, DP, 8, FULL, ONCE>), grid, tile, 0, s, a);
-    if (a.row_tiles == 8) hipLaunchKernelGGL((k_attend_tiles<T, DP, 4, FULL, ONCE>), grid, tile, 0, s, a);
-    if (a.row_tiles == 4) hipLaunchKernelGGL((k_attend_tiles<T, DP, 2, FULL, ONCE>), grid, tile, 0, s, a);
+    constexpr int kGroup = DP == 256 ? 1 : 2;  // tiles of rows a wave
+    if (a.row_tiles == 8 * kGroup) hipLaunchKernelGGL((k_attend_tiles<T, DP, 8, FULL, ONCE>), grid, tile, 0, s, a);
+    if (a.row_tiles == 4 * kGroup) hipLaunchKernelGGL((k_attend_tiles<T, DP, 4, FULL, ONCE>), grid, tile, 0, s, a);
+    if constexpr (DP < 256)
+      if (a.row_tiles == 4) hipLaunchKernelGGL((k_attend_tiles<T, DP, 2, FULL, ONCE>), grid, tile, 0, s, a);
   }
   const dim3 block(kAttThreads);
   if constexpr (DP < 256)
@@ -996,7 +1012,14 @@ hipError_t launch_attend_of(const AttendArgs& a, hipStream_t s) {
 
 size_t plan_attend(AttendArgs& a, int dtype, int num_cu) {
   const int64_t rows = (int64_t)a.max_nodes * a.group;
-  a.row_tiles = a.D > 128 || rows <= 16 ? 1 : rows <= 32 || dtype == PLH_F32 ? 2 : rows <= 64 ? 4 : rows <= 128 ? 8 : 16;
+  // Heads past 128 values: a wave holds 16 rows, and many rows begin there (24 rows of
+  // 32 x 4096 keys, two blocks of 16 / tiles: 150 / 97 us; 1 x 16 384 27 / 30).
+  const bool wide = a.D > 128;
+  a.row_tiles = rows <= 16 || (wide && dtype == PLH_F32)    ? 1
+                : (rows <= 32 && !wide) || dtype == PLH_F32 ? 2
+                : rows <= 64                                ? 4
+                : rows <= 128 || wide                       ? 8
+                                                            : 16;
   a.row_blocks = (int)((rows + 16 * a.row_tiles - 1) / (16 * a.row_tiles));
   const int64_t units = std::max<int64_t>(1, (int64_t)a.B * a.kv_heads * a.row_blocks);
   const int64_t most = (a.max_len + kChunkKeys - 1) / kChunkKeys;  // rounds of the longest sequence
@@ -1016,12 +1039,12 @@ size_t plan_attend(AttendArgs& a, int dtype, int num_cu) {
     want = std::min<int64_t>({most / 2, (held * num_cu + units - 1) / units, kMostChunks});
   } else {
     // a workgroup a CU: the number of chunks whose rounds of workgroups (4 us for 128
-    // keys, 5 us each beside them) and partial results (at 5 GB/ms, and a launch) take least
+    // keys, 8 of heads past 128 values, 5 us each beside them) and partial results (at 5 GB/ms, and a launch) take least
     double best = 1e300;
     for (int64_t n = 1; n <= std::min<int64_t>(most / 2, kMostChunks) || n == 1; ++n) {
       const double rounds = (double)((units * n + num_cu - 1) / num_cu), steps = (double)((most + n - 1) / n);
       const double parts = n == 1 ? 0.0 : 6.0 + (double)a.N * a.heads * (a.D + 2) * 8.0 * n / 5e6;
-      const double us = rounds * (4.0 * steps + 5.0) + parts;
+      const double us = rounds * ((wide ? 8.0 : 4.0) * steps + 5.0) + parts;
       if (us < best) {
         best = us;
         want = n;

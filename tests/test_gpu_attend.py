@@ -156,6 +156,17 @@ def test_long_contexts_in_chunks(B, n, T, heads, kv_heads, dtype):
         c.check(*c.run(max_len=most))
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,T,n", [(4, 1, 256, 5, 4000), (2, 2, 256, 64, 70), (4, 2, 200, 33, 900),
+                                                    (12, 3, 136, 64, 2000), (3, 3, 256, 300, 200)])
+def test_wide_heads_of_many_rows(heads, kv_heads, dim, T, n, dtype):
+    g = np.random.default_rng(T)
+    trees = [DraftTree(np.zeros(m)) if T > 64 else _tree(g, m, 3) for m in (T, 1, T - T // 3)]
+    c = Case(T + 1, [n, n // 2, 0], trees, heads, kv_heads, dim, 32, dtype)
+    out, lse = c.run()
+    print("  of the tolerance:", c.check(out, lse))
+
+
 def test_rows_that_see_nothing_or_little():
     import torch
 
@@ -173,14 +184,15 @@ def test_rows_that_see_nothing_or_little():
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
-def test_unseen_infinities_and_nan(dtype):
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_unseen_infinities_and_nan(dim, dtype):
     """Keys and values of nodes outside a row's path may be anything."""
     g = np.random.default_rng(4)
     import torch
 
     for at in ("k", "v", "both"):
         c = Case(2, [40, 0, 129], [DraftTree([0] * 6, [-1, 0, 0, 1, 2, 2]), DraftTree([0] * 4, [-1, 0, 0, 0]),
-                                   _tree(g, 40, 4)], 6, 2, 64, 16, dtype)
+                                   _tree(g, 40, 4)], 6, 2, dim, 16, dtype)
         bad = [(0, 41, np.nan), (0, 43, np.inf), (1, 2, -np.inf), (2, 129 + 7, np.nan), (2, 129 + 20, np.inf)]
         for b, x, val in bad:
             page = c.table[b, x // 16]
@@ -188,7 +200,7 @@ def test_unseen_infinities_and_nan(dtype):
                 c.keys[b][x, 0, 3] = c.k[page, 0, x % 16, 3] = val
             if at != "k":
                 c.values[b][x, :, 5] = c.v[page, :, x % 16, 5] = val
-                c.values[b][x, 1, 60] = c.v[page, 1, x % 16, 60] = -val
+                c.values[b][x, 1, dim - 4] = c.v[page, 1, x % 16, dim - 4] = -val
         out, lse = c.run()
         c.check(out, lse)
         assert torch.isfinite(out).any()

@@ -163,6 +163,8 @@ int check_page_size(plh_ctx* c, int page_size) {
 }
 
 // The sizes of a tree attention call, checked, in the plan's arguments.
+constexpr int64_t kMostThreads = UINT32_MAX;  // of a grid
+
 int attend_sizes(plh_ctx* c, plh::AttendArgs& a, int dtype, int N, int q_heads, int kv_heads, int D, int B,
                  int max_nodes, int64_t max_len) {
   if (dtype != PLH_F32 && dtype != PLH_BF16 && dtype != PLH_F16)
@@ -181,8 +183,10 @@ int attend_sizes(plh_ctx* c, plh::AttendArgs& a, int dtype, int N, int q_heads, 
   a.B = B;
   a.max_nodes = max_nodes < N ? max_nodes : N;
   a.max_len = max_len > 0 ? max_len : 1;
-  // rows, workgroups and the workspace's floats are counted in 64 bits up to here
-  if ((int64_t)N * q_heads > INT32_MAX || (int64_t)B * kv_heads * (((int64_t)a.max_nodes * a.group + 15) / 16) > INT32_MAX / 16)
+  // rows, workgroups and the workspace's floats are counted in 64 bits up to here; a block of
+  // 16 rows takes 256 threads at most, units lie in eights
+  const int64_t units = ((int64_t)B * kv_heads + 7) / 8 * 8;
+  if ((int64_t)N * q_heads > INT32_MAX || units * (((int64_t)a.max_nodes * a.group + 15) / 16) > kMostThreads / 256)
     return fail(c, PLH_ERR_UNSUPPORTED, "more rows than a grid holds%s");
   return PLH_OK;
 }
@@ -1069,6 +1073,7 @@ int plh_rotary_append(plh_ctx* c, const void* q, int64_t ldq, int q_heads, void*
   }
   if (has_q && (ldq < (int64_t)q_heads * D || ldqo < (int64_t)q_heads * D))
     return fail(c, PLH_ERR_INVALID_ARG, "need ldq and ldqo >= q_heads * D%s");
+  if (N > kMostThreads / 256) return fail(c, PLH_ERR_UNSUPPORTED, "more rows than a grid holds%s");
   if (N == 0 || (!has_q && !has_kv)) return PLH_OK;
   if ((has_q && (q == nullptr || q_out == nullptr)) ||
       (has_kv && (k == nullptr || v == nullptr || k_pages == nullptr || v_pages == nullptr || slots == nullptr)) ||
@@ -1125,7 +1130,7 @@ int plh_copy_pages(plh_ctx* c, void* k_pages, void* v_pages, int layers, int64_t
       (layers > 1 && layer_bytes < (int64_t)num_pages * page_bytes))
     return fail(c, PLH_ERR_INVALID_ARG,
                 "page_bytes (< 2^31) and layer_bytes must be multiples of 16, and layers must not overlap%s");
-  if (n > 0 && (int64_t)n * ((page_bytes + 16383) / 16384) > INT32_MAX)
+  if (n > 0 && (int64_t)n * ((page_bytes + 16383) / 16384) > kMostThreads / 256)
     return fail(c, PLH_ERR_UNSUPPORTED, "more pages than a grid holds%s");
   if (n == 0) return PLH_OK;
   if (k_pages == nullptr || v_pages == nullptr || src == nullptr || dst == nullptr)
@@ -1191,7 +1196,7 @@ int64_t plh_verify_tree_ws_bytes(plh_ctx* c, int B, int V, int max_nodes) {
     return fail(c, PLH_ERR_INVALID_ARG, "need B >= 0, V >= 1 and max_nodes >= 1%s");
   if (max_nodes > plh::kTreeNodes) return fail(c, PLH_ERR_UNSUPPORTED, "trees of more than 256 nodes%s");
   if (V > plh::kTreeV) return fail(c, PLH_ERR_UNSUPPORTED, "rows of more than 524288 tokens%s");
-  if ((int64_t)B * ((V + 8191) / 8192) > INT32_MAX / 64) return fail(c, PLH_ERR_UNSUPPORTED, "more rows than a grid holds%s");
+  if ((int64_t)B * ((V + 8191) / 8192) > kMostThreads / 512) return fail(c, PLH_ERR_UNSUPPORTED, "more rows than a grid holds%s");
   return (int64_t)plh::tree_ws_bytes(B, V, max_nodes);
 }
 

@@ -18,6 +18,8 @@ import numpy as np
 import pytest
 
 from oracle import tree as O
+from pagellm_amd import _native
+from pagellm_amd.sampling import _ctx
 from pagellm_amd.tree import DraftTree, tree_attention
 
 pytestmark = pytest.mark.gpu
@@ -375,6 +377,12 @@ def test_refusals_on_the_device():
         kv = torch.zeros((2, 1, ps, dim), dtype=torch.bfloat16, device="cuda")
         with pytest.raises(ValueError):
             tree_attention(**{**d, "q": torch.zeros((1, 2, dim), dtype=torch.bfloat16, device="cuda"), "k_pages": kv, "v_pages": kv})
+    c = _ctx(None)
+    assert c.tree_attention_ws_bytes(_native.PLH_BF16, 1 << 20, 8, 8, 64, 65535, 16, 100) >= 0
+    with pytest.raises(NotImplementedError):  # more workgroups than a grid holds
+        c.tree_attention_ws_bytes(_native.PLH_BF16, 1 << 26, 8, 8, 64, 65535, 1024, 1100)
+    with pytest.raises(NotImplementedError):
+        c.verify_tree_ws_bytes(10_000_000, 1, 4)
     kv = torch.zeros((2, 3, 16, 64), dtype=torch.bfloat16, device="cuda")
     with pytest.raises(ValueError):
         tree_attention(**{**d, "k_pages": kv, "v_pages": kv})

@@ -139,9 +139,11 @@ def _rows(c, x, name: str):
     if x.dim() != 3:
         raise ValueError(f"{name} must be [N, heads, D]")
     n, h, d = x.shape
-    if x.is_contiguous():
-        return n, h, d, h * d
     ld, step, one = x.stride()
+    if one == 1 and step == d and n > 1 and ld >= h * d:
+        return n, h, d, ld
+    if x.is_contiguous():  # strides of dimensions of one may be anything
+        return n, h, d, h * d
     if x.numel() and ((d > 1 and one != 1) or (h > 1 and step != d)):
         raise ValueError(f"the heads of a row of {name} must lie side by side")
     if n > 1 and x.numel() and ld < h * d:

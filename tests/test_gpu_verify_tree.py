@@ -15,7 +15,7 @@ from oracle import tree as O
 from pagellm_amd.cache import PagedCache, Rotary
 from pagellm_amd.params import SamplingParams, make_rng
 from pagellm_amd.speculative import verify_batch
-from pagellm_amd.tree import DraftTree, TreeDecoder, verify_tree, verify_tree_step
+from pagellm_amd.tree import DraftTree, TreeDecoder, tree_attention, verify_tree, verify_tree_step
 
 pytestmark = pytest.mark.gpu
 
@@ -436,3 +436,43 @@ def test_sampled_rounds_run_with_penalties():
             if emitted[b] != toks:
                 return
             ctx[b] += toks
+
+
+def test_two_graphs_at_once():
+    """Captured calls with workspaces of their own, replayed on two streams together."""
+    import torch
+
+    def verdicts(seed):
+        p, q, tokens, parents, off, u = (torch.from_numpy(np.ascontiguousarray(x)).cuda()
+                                         for x in _case(seed, [9, 16, 3], 20_000, 3, "float64", False))
+        return lambda: verify_tree(p, q, tokens, parents, off, u, max_nodes=16)
+
+    def outputs(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        k, v = (torch.randn(300, 2, 16, 128, generator=g, device="cuda").half() for _ in range(2))
+        x = torch.randn(50, 8, 128, generator=g, device="cuda").half()
+        table = torch.arange(300, dtype=torch.int32, device="cuda").view(2, 150)
+        lens, off = (torch.tensor(n, dtype=torch.int32, device="cuda") for n in ([2000 + seed, 40], [0, 20, 50]))
+        return lambda: (tree_attention(x, k, v, table, lens, off, max_nodes=30, max_len=2100),)
+
+    for make in (verdicts, outputs):
+        calls = [make(1), make(2)]
+        want = [[x.clone() for x in call()] for call in calls]
+        torch.cuda.synchronize()
+        streams, graphs, got = [torch.cuda.Stream() for _ in calls], [], []
+        for call, s in zip(calls, streams):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=s):
+                got.append(call())
+        for _ in range(5):
+            for graph, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(got, want):
+                assert all(torch.equal(x, y) for x, y in zip(a, b))
+                for x in a:
+                    x.fill_(3)
+            for call, b in zip(calls, want):  # eager calls in between
+                assert all(torch.equal(x, y) for x, y in zip(call(), b))
+            torch.cuda.synchronize()
